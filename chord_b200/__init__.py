@@ -29,6 +29,14 @@ _EXPORTS = {
     "check_status": "chord_b200.indexed_gemm",
     "indexed_gate_up_silu": "chord_b200.indexed_gemm",
     "set_option": "chord_b200._lib",
+    "gemv": "chord_b200.gemv_op",
+    "KVCache": "chord_b200.attention",
+    "kv_cache": "chord_b200.attention",
+    "cache_read": "chord_b200.attention",
+    "cache_write": "chord_b200.attention",
+    "paged_attention": "chord_b200.attention",
+    "qk_norm_rope": "chord_b200.attention",
+    "qk_norm_rope_write": "chord_b200.attention",
 }
 
 

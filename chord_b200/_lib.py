@@ -29,6 +29,7 @@ _LIB_PATH = Path(__file__).resolve().parent / "libchord_b200.so"
 _i64 = ctypes.c_int64
 _ptr = ctypes.c_void_p
 _int = ctypes.c_int
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/chord_b200.h one to one.
 SIGNATURES = {
@@ -75,7 +76,26 @@ SIGNATURES = {
                                    _ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr]),
     "chord_b200_ep_combine_signal": (_int, [_ptr, _i64, _i64, _i64, _ptr]),
     "chord_b200_ep_combine_wait": (_int, [_ptr, _i64, _i64, _ptr]),
+    "chord_b200_gemv": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _ptr]),
+    "chord_b200_qk_norm_rope": (_int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _int, _ptr,
+                                       _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _f64, _ptr]),
+    "chord_b200_qk_norm_rope_write": (_int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr,
+                                             _i64, _i64, _int, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _f64, _ptr]),
+    "chord_b200_cache_write": (_int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr, _ptr]),
+    "chord_b200_cache_read": (_int, [_ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr, _i64, _ptr, _ptr]),
+    "chord_b200_paged_attention": (_int, [_ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64,
+                                          _ptr, _i64, _ptr, _i64, _i64, _i64, _f64, _ptr]),
+    "chord_b200_paged_attention_lock_words": (_int, []),
+    "chord_b200_paged_attention_workspace_bytes": (_i64, [_i64]),
 }
+
+
+class KVCacheDescriptor(ctypes.Structure):
+    """``chord_b200_kv_cache`` of include/chord_b200.h."""
+
+    _fields_ = [(name, _ptr) for name in ("k", "v", "k_scale", "v_scale")] + [
+        (name, _i64) for name in ("num_pages", "page_size", "heads", "head_dim", "stride_page", "stride_head",
+                                  "stride_token", "scale_stride_page", "scale_stride_head", "scale_stride_token")]
 
 
 def library_path() -> Path:
@@ -105,8 +125,8 @@ def load() -> ctypes.CDLL:
 
 
 def native():
-    """The entry points for calls with plain integer arguments (addresses included; None is
-    the null pointer): through
+    """The entry points for calls with plain arguments (integers, addresses, where None is the
+    null pointer, and at most one double): through
     the ``_call`` extension module where it was built, otherwise the ctypes functions of
     :func:`load`.  ctypes spends 4.5 us on converting the 21 arguments of ``indexed``, the
     module less than 1 us; a pass of four calls on a small layer goes from 71 to 47 us with this and
@@ -118,7 +138,7 @@ def native():
         for name, (restype, argtypes) in SIGNATURES.items():
             fn = getattr(lib, name)
             if _call is not None and restype is _int and ctypes.c_char_p not in argtypes:
-                signature = "".join("p" if t is _ptr else "i" for t in argtypes)
+                signature = "".join("p" if t is _ptr else "d" if t is _f64 else "i" for t in argtypes)
                 fn = functools.partial(_call.call, ctypes.cast(fn, ctypes.c_void_p).value, signature)
             functions[name] = fn
         _NATIVE = SimpleNamespace(**functions)

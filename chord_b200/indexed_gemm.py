@@ -20,6 +20,7 @@ _STATUS: dict[int, torch.Tensor] = {}
 
 _STATUS_BITS = {1: "producer wait", 2: "MMA-issuer wait", 4: "dequantisation wait",
                 8: "epilogue wait", 16: "stream-K lock wait"}
+_INDEX_BIT = 32  # an index outside a cache, a block table or a table of positions
 
 
 def _device_index(device: torch.device) -> int:
@@ -50,8 +51,8 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 def check_status(device=None) -> None:
     """Synchronise ``device`` and raise ``RuntimeError`` if any kernel since the last
-    check gave up on a bounded wait (its output is then not to be trusted).  Clears the
-    word.  After a stream-K lock timeout the caller's ``locks`` tensor must be zeroed
+    check gave up on a bounded wait or met an index outside a cache, a block table or a table
+    of positions (its output is then not to be trusted).  Clears the word.  After a stream-K lock timeout the caller's ``locks`` tensor must be zeroed
     again before it is reused."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     word = _STATUS.get(_device_index(device))
@@ -61,13 +62,16 @@ def check_status(device=None) -> None:
     bits = int(word.item())
     if bits:
         word.zero_()
+        if bits == _INDEX_BIT:
+            raise RuntimeError("a chord_b200 kernel met an index outside a cache, a block table or a table of "
+                               f"positions (status {bits})")
         names = [name for bit, name in _STATUS_BITS.items() if bits & bit]
         raise RuntimeError(f"a chord_b200 kernel gave up on a bounded wait ({', '.join(names)}; "
                            f"status {bits})")
 
 
 def default_locks(device: torch.device) -> torch.Tensor:
-    key = (_device_index(device), torch.cuda.current_stream(device).cuda_stream)
+    key = (_device_index(device), _lib.stream_handle(device))
     locks = _DEFAULT_LOCKS.get(key)
     if locks is None:
         _refuse_allocation_in_capture(device, "the default locks buffer (locks=None)")

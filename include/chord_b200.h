@@ -367,6 +367,112 @@ int chord_b200_ep_combine_signal(void* const* peer_state, int64_t world, int64_t
                                  void* stream);
 int chord_b200_ep_combine_wait(void* state, int64_t world, int64_t epoch, void* stream);
 
+/* ---- products of a few rows -----------------------------------------------------------
+ * No counterpart in the reference, whose operators all take routing blocks.  With
+ * expert_ids null (one expert's weight, rows <= 16):
+ *   out[r, :] = x[r, :] . dequant(W[0])^T
+ * with expert_ids int32 [rows] (rows <= 65535):
+ *   out[r, :] = x[r / top_k, :] . dequant(W[expert_ids[r] - expert_base])^T
+ * and zeros where expert_ids[r] lies outside [expert_base, expert_base + num_experts), an
+ * expert that another GPU holds.  dequant(W) = (code - 8) * scale, not rounded to BF16: sums
+ * and scales are FP32, the result is rounded once.  x is bf16, its rows x_stride elements apart
+ * (even); out is bf16 [rows, n].  No scratch, no locks; the same inputs give the same bits. */
+int chord_b200_gemv(const void* x, int64_t x_stride, const int32_t* packed, const void* scale,
+                    const int32_t* expert_ids, void* out, int64_t rows, int64_t n, int64_t k,
+                    int64_t num_experts, int64_t top_k, int64_t expert_base, void* stream);
+
+/* ---- paged key-value cache ------------------------------------------------------------
+ * No counterpart in the reference, nor for what follows below.  Keys and values lie in pages of
+ * page_size tokens.  A row is what one head keeps of one token: head_dim BF16 values
+ * (k_scale == v_scale == null), or head_dim bytes of codes with an FP32 scale per row,
+ *   value = (code - 128) * scale,   scale = max |x| / 127,   code = round(x / scale) + 128.
+ * head_dim is a multiple of 16, at most 256.  Strides are in elements and the same for keys and
+ * values; every row starts on a 16-byte boundary.  A slot is page * page_size + place in the page.
+ * An index outside its range is never followed: the row counts as zeros, or is not written, and
+ * bit 32 is ORed into `status`. */
+typedef struct chord_b200_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_pages, page_size, heads, head_dim;
+  int64_t stride_page, stride_head, stride_token;
+  int64_t scale_stride_page, scale_stride_head, scale_stride_token;
+} chord_b200_kv_cache;
+
+/* Norms of queries and keys for each head, and the position rotation:
+ *   h = x / sqrt(mean(x^2) + eps) * weight
+ * then the first rotary_dim elements of h are turned by the angles of the token's position: element
+ * i with element i + rotary_dim / 2, or (interleaved != 0) 2 i with 2 i + 1,
+ *   a' = a cos_i - b sin_i,  b' = b cos_i + a sin_i.
+ *  q, k       bf16 [tokens, heads / kv_heads, head_dim], strides of tokens and heads in elements
+ *             (multiples of 8)
+ *  weights    bf16 [head_dim];  cos_sin fp32 [max_positions, rotary_dim]: cosines, then sines
+ *  positions  int32 [tokens]; a token at a position outside the table gets zeros and status bit 32
+ *  q_out, k_out  bf16 [tokens, heads / kv_heads, head_dim], contiguous
+ * All in FP32 with one rounding at the end. */
+int chord_b200_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* k,
+                            int64_t k_token, int64_t k_head, const void* q_weight,
+                            const void* k_weight, const float* cos_sin, int64_t max_positions,
+                            int64_t rotary_dim, int interleaved, const int32_t* positions,
+                            void* q_out, void* k_out, int64_t tokens, int64_t heads,
+                            int64_t kv_heads, int64_t head_dim, int32_t* status, double eps,
+                            void* stream);
+
+/* The same with the keys, and the values as they are, written into the cache: token t at slot
+ * slots[t], nowhere where that is negative.  Keys are quantised from FP32.  Two tokens with one
+ * slot leave either's row. */
+int chord_b200_qk_norm_rope_write(const void* q, int64_t q_token, int64_t q_head, const void* k,
+                                  int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
+                                  int64_t v_head, const void* q_weight, const void* k_weight,
+                                  const float* cos_sin, int64_t max_positions, int64_t rotary_dim,
+                                  int interleaved, const int32_t* positions, void* q_out,
+                                  const chord_b200_kv_cache* cache, const int32_t* slots,
+                                  int64_t tokens, int64_t heads, int32_t* status, double eps,
+                                  void* stream);
+
+/* Keys and values bf16 [tokens, kv_heads, head_dim] into the cache, as above.  A row that holds an
+ * infinity or a NaN reads back as NaN from an 8-bit cache. */
+int chord_b200_cache_write(const void* k, int64_t k_token, int64_t k_head, const void* v,
+                           int64_t v_token, int64_t v_head, const chord_b200_kv_cache* cache,
+                           const int32_t* slots, int64_t tokens, int32_t* status, void* stream);
+
+/* The tokens of `batch` sequences out of the cache, one sequence after another: token t of
+ * sequence b, offsets[b] <= offsets[b] + t < offsets[b + 1], becomes row offsets[b] + t of k_out and
+ * v_out, bf16 [total, kv_heads, head_dim].  tables int32 [batch, max_pages] holds each sequence's
+ * pages, rows table_stride apart; offsets int32 [batch + 1] never falls.  Rows of no sequence are
+ * zeros. */
+int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* tables,
+                          int64_t table_stride, int64_t max_pages, const int32_t* offsets,
+                          int64_t batch, void* k_out, void* v_out, int64_t total, int32_t* status,
+                          void* stream);
+
+/* ---- attention of one new token over the paged cache ----------------------------------
+ *   out[b, h] = sum_t p_t v_t,  p = softmax_t(scale * q[b, h] . k_t)
+ * over the last min(window, lengths[b]) tokens of sequence b (window 0: all), with the keys and
+ * values of head h / (heads / kv_heads).  lse[b, h] (optional) = log sum_t exp(scale * q . k_t).
+ * A sequence without tokens, or whose scores are all minus infinity, gets zeros and an lse of minus
+ * infinity.
+ *  q        bf16 [batch, heads, head_dim], strides in elements (multiples of 8)
+ *  cache    head_dim 64, 96, 128, 192 or 256; heads % cache->heads == 0
+ *  tables, table_stride, max_pages  as above; lengths int32 [batch], at most
+ *           max_pages * page_size (more: cut, status bit 32)
+ *  out      bf16 [batch, heads, head_dim];  lse fp32 [batch, heads]
+ *  locks    int32, chord_b200_paged_attention_lock_words() words, zero on entry and on exit
+ *  workspace  chord_b200_paged_attention_workspace_bytes(head_dim) bytes, 16-byte aligned
+ *  scale    finite; head_dim ^ -0.5 as a rule
+ * Work is dealt out over the device by tokens, whatever the lengths; parts of a sequence are joined
+ * in their order, so the same inputs give the same bits.  No kernel waits for another CTA. */
+int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head,
+                               const chord_b200_kv_cache* cache, const int32_t* tables,
+                               int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                               void* out, float* lse, int32_t* locks, int64_t num_locks,
+                               void* workspace, int64_t workspace_bytes, int32_t* status,
+                               int64_t batch, int64_t heads, int64_t window, double scale,
+                               void* stream);
+int chord_b200_paged_attention_lock_words(void);
+int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim);
+
 #ifdef __cplusplus
 }
 #endif
