@@ -86,7 +86,7 @@ SIGNATURES = {
     "chord_b200_paged_attention": (_int, [_ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64,
                                           _ptr, _i64, _ptr, _i64, _i64, _i64, _f64, _ptr]),
     "chord_b200_paged_attention_lock_words": (_int, []),
-    "chord_b200_paged_attention_workspace_bytes": (_i64, [_i64]),
+    "chord_b200_paged_attention_workspace_bytes": (_i64, [_i64, _i64]),
 }
 
 

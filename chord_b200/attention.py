@@ -257,11 +257,12 @@ def cache_read(cache: KVCache, block_tables: torch.Tensor, offsets: torch.Tensor
 
 
 @functools.lru_cache(maxsize=64)
-def _attention_scratch(device_index: int, head_dim: int):
-    """(lock words, workspace bytes), asked of the library once per device and width."""
+def _attention_scratch(device_index: int, head_dim: int, group: int):
+    """(lock words, workspace bytes), asked of the library once per device and shape."""
     del device_index  # a cache key only (the current device must be it)
     lib = _lib.load()
-    words, size = lib.chord_b200_paged_attention_lock_words(), lib.chord_b200_paged_attention_workspace_bytes(head_dim)
+    words = lib.chord_b200_paged_attention_lock_words()
+    size = lib.chord_b200_paged_attention_workspace_bytes(head_dim, group)
     if words < 0 or size < 0:
         raise RuntimeError(_lib.last_error())
     return words, size
@@ -316,7 +317,7 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     if batch == 0:
         return outputs
     with _lib.on_device(device):
-        words, size = _attention_scratch(_device_index(device), dim)
+        words, size = _attention_scratch(_device_index(device), dim, heads // cache.heads)
         if locks is None:
             locks = default_locks(device)
         else:

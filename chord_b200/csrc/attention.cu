@@ -13,8 +13,13 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxCtasPerSm = 2;
-constexpr int kMaxParts = 1024;  // CTAs of a launch at most
+constexpr int kMaxCtasPerSm = 3;
+constexpr int kMaxCtas = 480;      // of a launch: three on each of 160 SMs
+constexpr int kFan = 48;           // parts of a row that are joined at once
+// A lot's lock word: arrivals of its row's CTAs (11 bits), of the first kFan of them, and of the kFan
+// neighbours that the lot is the first of (6 bits each).
+constexpr int kRowShift = 0, kFirstShift = 11, kFanShift = 17;
+static_assert(kMaxCtas < (1 << 11) && kFan < (1 << 6), "the fields' widths");
 
 struct AttentionParams {
   Cache cache;
@@ -28,42 +33,59 @@ struct AttentionParams {
   int32_t* status;
   int64_t q_batch, q_head, table_stride;
   int32_t batch, heads, group, head_blocks, capacity, window;
-  float scale;  // of the scores, with log2(e)
+  float scale;  // of the scores, with log2(e) and, for codes, 2^53
+  bool whole_groups;
 };
 
 // What follows from the head's width and the cache's type.  A warp takes kStep tokens at a time, whose
-// keys and values are some 5 to 16 KB; kStages of them are on their way or in use.
-template <int kDim, bool kCodes>
+// keys and values are some 5 to 18 KB; kStages of them are on their way or in use.
+template <int kDim, bool kCodes, int kTiles>
 struct Layout {
   static constexpr int kRow = kDim * (kCodes ? 1 : 2);  // bytes of a row
   static constexpr int kPitch = kRow + 16;              // an odd number of 16-byte pieces: no bank conflicts
-  static constexpr int kStep = kRow < 128 ? 32 : 16;
-  static constexpr int kUnit = kStep * kWarps;          // tokens of a CTA's step
+  static constexpr int kStep = kCodes || kRow < 128 ? 32 : 16;
   static constexpr int kScaleBytes = kCodes ? 2 * kStep * 4 : 0;
   static constexpr int kStageBytes = 2 * kStep * kPitch + kScaleBytes;
-  static constexpr int kCtas = kDim > 128 ? 1 : kMaxCtasPerSm;
-  static constexpr int kFit = (kCtas == 1 ? 220 : 110) * 1024 / (kWarps * kStageBytes);
+  static constexpr int kCtas = kDim > 128 ? 1 : kDim == 64 && kTiles == 1 ? 3 : 2;  // of an SM
+  static constexpr int kFit = (kCtas == 1 ? 220 : kCtas == 2 ? 111 : 74) * 1024 / (kWarps * kStageBytes);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
-  static constexpr int kHeads = 16;                     // query heads of a CTA
-  static_assert(kStages >= 2 && kSmem >= kWarps * kHeads * kDim * 4, "the partial sums of the warps take the ring's place");
+  static_assert(kStages >= 2 && kStages * kStageBytes >= 8 * kTiles * (kDim + 2) * 4, "a warp's part takes its ring's place");
 };
 
-__host__ __device__ constexpr int64_t partial_floats(int dim) { return 16 * dim + 32; }
+// Part of a row: [dims, in the products' order][heads] values, the heads' maxima and their sums.
+__host__ __device__ constexpr int64_t part_floats(int dim, int heads) { return heads * (dim + 2); }
 
-template <bool kCodes>
-__device__ __forceinline__ void codes_to_bf16(uint32_t four, uint32_t select_a, uint32_t select_b, uint32_t& a, uint32_t& b) {
+// Floats of workspace: kSlots parts for each lot, one for each warp.
+constexpr int kSlots = 3;
+constexpr int64_t workspace_floats(int64_t ctas, int dim, int heads) {
+  return ctas * (kSlots + kWarps) * part_floats(dim, heads);
+}
+
+// Two of four codes as BF16 pairs, (code - 128) / 64, exact.
+__device__ __forceinline__ uint32_t two_codes(uint32_t four, uint32_t select) {
   constexpr uint32_t kOffset = 0xC000C000u;  // -128 / 64, twice
-  a = bf16x2_fma(__byte_perm(four, 0, select_a), kTwo127, kOffset);
-  b = bf16x2_fma(__byte_perm(four, 0, select_b), kTwo127, kOffset);
+  return bf16x2_fma(__byte_perm(four, 0, select), kTwo127, kOffset);
 }
 
 __device__ __forceinline__ void ldmatrix_x4_at(uint32_t addr, uint32_t (&r)[4]) { ptx::ldmatrix_x4<0>(addr, r); }
+
+__device__ __forceinline__ void cp_async_16_all(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid) {
   const uint32_t bytes = valid ? 4u : 0u;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+
+// What a warp has of a row that does not lie in its share alone.
+struct Part {
+  float* at;
+  int32_t b, row;
+  int32_t first_lot, lots;  // that have parts of the row
+  bool there, began;        // began: in an earlier share
+};
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -71,59 +93,248 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// The logarithm of a sum, kept relative to 2^top.
+__device__ __forceinline__ float lse_of(float top, float sum) {
+  return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+}
+
+__device__ __forceinline__ void add_weighted(float4& v, const float4& weight, const float4& x) {
+  v.x = fmaf(weight.x, x.x, v.x);
+  v.y = fmaf(weight.y, x.y, v.y);
+  v.z = fmaf(weight.z, x.z, v.z);
+  v.w = fmaf(weight.w, x.w, v.w);
+}
+
+// Reads of parts, in shared memory or written by another CTA.
+__device__ __forceinline__ float4 read_part4(const float* p) {
+  float4 v;
+  asm volatile("ld.relaxed.gpu.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ int32_t atomic_add_acq_rel(int32_t* p, int32_t v) {
+  int32_t before;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(before) : "l"(p), "r"(v) : "memory");
+  return before;
+}
+
+// n / d, in 32 bits where they do.
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+  if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+
+__device__ __forceinline__ float rate_of(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+
+// An 8x8 matrix of 16-bit elements, a row in four lanes, to its transpose.
+__device__ __forceinline__ uint32_t transposed(uint32_t pair) {
+  uint32_t t;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(pair));
+  return t;
+}
+
+// The query heads of a row of work, and its results.
+struct Row {
+  int64_t head0;  // of the batch's heads
+  int32_t heads;
+  __device__ __forceinline__ Row(const AttentionParams& p, int32_t b, int32_t row) {
+    const int32_t kv_head = row / p.head_blocks, head_block = row % p.head_blocks;
+    heads = min(p.group - head_block * 16, 16);
+    head0 = static_cast<int64_t>(b) * p.heads + kv_head * p.group + head_block * 16;
+  }
+  // Four heads' values of one dim, the `place`-th of the products' order: with codes a 16-byte piece has
+  // its even dims first.
+  template <int kDim, bool kCodes>
+  __device__ __forceinline__ void finish(const AttentionParams& p, int head, int place, const float4& v, const float4& all,
+                                         const float4& most) const {
+    const int dim = kCodes ? place / 16 * 16 + place % 8 * 2 + place % 16 / 8 : place;
+    const float value[4] = {v.x, v.y, v.z, v.w}, sum[4] = {all.x, all.y, all.z, all.w}, top[4] = {most.x, most.y, most.z, most.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (head + i >= heads) break;
+      p.out[(head0 + head + i) * kDim + dim] = __float2bfloat16(value[i] * rate_of(sum[i]));
+      if (place == 0 && p.lse != nullptr) p.lse[head0 + head + i] = lse_of(top[i], sum[i]);
+    }
+  }
+};
+
+// A thread's values while a row's parts are joined: four heads' values of kItems dims, with the heads'
+// maxima and sums.  Every thread keeps its own, so that nothing but the parts themselves is waited for,
+// once for kBatch of them: a round trip to what other SMs have just written takes 1.1 us.
+template <int kDim, int kHeads>
+struct Joined {
+  static constexpr int kQuads = kHeads / 4;
+  static constexpr int kItems = (kDim * kQuads + kThreads - 1) / kThreads;  // (dims, kThreads / kQuads apart)
+  static constexpr int kBatch = kItems <= 2 ? 8 : kItems == 3 ? 6 : kItems == 4 ? 4 : 2;
+  static constexpr bool kWhole = kDim * kQuads % kThreads == 0;  // every thread has all its items
+  static __device__ __forceinline__ bool mine(int i) { return kWhole || threadIdx.x + i * kThreads < kDim * kQuads; }
+  float4 value[kItems], top, sum;
+  __device__ __forceinline__ Joined() {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) value[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    top = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  }
+  // The first `count` of kBatch parts; all are read before any is used.
+  __device__ __forceinline__ void add(const float* const (&list)[kBatch], int32_t count) {
+    float4 m[kBatch], l[kBatch], v[kBatch][kItems];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      m[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      l[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) v[j][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (j < count) {
+        const float* const from = list[j] + threadIdx.x % kQuads * 4;
+        m[j] = read_part4(from + kDim * kHeads);
+        l[j] = read_part4(from + (kDim + 1) * kHeads);
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          if (mine(i)) v[j][i] = read_part4(list[j] + 4 * (threadIdx.x + i * kThreads));
+        }
+      }
+    }
+    float4 next = top;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      next.x = fmaxf(next.x, m[j].x);
+      next.y = fmaxf(next.y, m[j].y);
+      next.z = fmaxf(next.z, m[j].z);
+      next.w = fmaxf(next.w, m[j].w);
+    }
+    const float4 old = factors(top, next);
+    sum = make_float4(sum.x * old.x, sum.y * old.y, sum.z * old.z, sum.w * old.w);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      value[i] = make_float4(value[i].x * old.x, value[i].y * old.y, value[i].z * old.z, value[i].w * old.w);
+    }
+    top = next;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const float4 weight = factors(m[j], top);
+      add_weighted(sum, weight, l[j]);
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) add_weighted(value[i], weight, v[j][i]);
+    }
+  }
+  static __device__ __forceinline__ float factor(float from, float to) { return to == -INFINITY ? 0.0f : exp2_approx(from - to); }
+  static __device__ __forceinline__ float4 factors(const float4& from, const float4& to) {
+    return make_float4(factor(from.x, to.x), factor(from.y, to.y), factor(from.z, to.z), factor(from.w, to.w));
+  }
+  // To a part, or to the results (to == null).
+  template <bool kCodes>
+  __device__ __forceinline__ void give(const AttentionParams& p, const Row& of, float* to) const {
+    const int32_t head = threadIdx.x % kQuads * 4;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (!mine(i)) break;
+      const int32_t index = threadIdx.x + i * kThreads;
+      if (to == nullptr) {
+        of.template finish<kDim, kCodes>(p, head, index / kQuads, value[i], sum, top);
+      } else {
+        __stcg(reinterpret_cast<float4*>(to + 4 * index), value[i]);
+      }
+    }
+    if (to != nullptr && threadIdx.x < kQuads) {
+      __stcg(reinterpret_cast<float4*>(to + kDim * kHeads + head), top);
+      __stcg(reinterpret_cast<float4*>(to + (kDim + 1) * kHeads + head), sum);
+    }
+  }
+};
+
 // One row of work is a sequence, one of its key-value heads and a block of up to 16 of the query heads
-// that share it; the rows' tokens, in units of kUnit, are numbered through and dealt out to the CTAs in
-// equal shares, so that lengths need not be alike.  A CTA's share is cut into segments at the rows'
-// ends.  The four warps of a CTA take every fourth step of a segment, each with its own ring of
-// cp.async stages, running maximum, sum and output, and meet only at its end.
+// that share it; a step is kStep of its tokens.  A lot is a CTA's work.  Where there are few rows, each is
+// cut into lots of its own; else the steps of all rows are numbered through and cut into equal lots, so
+// that lengths need not be alike.  A warp goes through its quarter of a lot on its own: a ring of
+// cp.async stages that runs ahead across the rows' ends, and a running maximum, sum and output.  Rows
+// that lie in one quarter are finished by their warp; the others' parts are joined within the CTA once
+// all its warps are done, and then, through memory, by the last CTA of a row to arrive (with more than
+// kFan parts by the last of each kFan neighbours, and the last of these).
 //
-// Products: scores S[heads 16, tokens] = Q K^T and O[heads, dim] += P V on mma.m16n8k16, whose score
-// fragment is the operand fragment of P.  P is multiplied as the sum of two BF16 numbers (16 bits of
-// it); with up to eight heads the second part travels in the operand's idle rows 8-15 and costs
-// nothing (kWide == false).  Codes are exact in BF16, (code - 128) / 64; the keys' scales are applied
-// to the scores, the values' to P.
-template <int kDim, bool kCodes, bool kWide>
-__global__ void __launch_bounds__(kThreads, (Layout<kDim, kCodes>::kCtas))
+// Products on mma.m16n8k16, keys and values as the 16-row operand, the heads (eight for each of kTiles)
+// as columns: S[tokens, heads] = K Q^T and O[dims, heads] += V^T P, P by movmatrix from the score
+// fragments.  (With the heads as rows, half of every product was idle with up to eight of them: 890
+// instead of 500 instructions per 32 tokens of codes.)  P is multiplied as the sum of two BF16 numbers, 16 bits of it.
+// Codes are exact in BF16; the keys' scales are applied to the scores, the values' to P.  The codes of
+// values become (code - 128) / 64.  Those of keys are multiplied as they stand, as the BF16 numbers
+// code * 2^-133, with queries times 2^80: the scores start from minus 128 times the query's sum, which
+// saves a multiply-add for every two codes.
+//
+// The running maximum is raised, and the sums are scaled, only where a score passes it by more than
+// 2^kSlack; until then P is up to 2^kSlack, which costs no precision, and no lane needs another's scores.
+template <int kDim, bool kCodes, int kTiles>
+__global__ void __launch_bounds__(kThreads, (Layout<kDim, kCodes, kTiles>::kCtas))
 paged_attention_kernel(const AttentionParams p) {
-  using L = Layout<kDim, kCodes>;
-  constexpr int kTiles = L::kStep / 8;      // score tiles of eight tokens
-  constexpr int kOut = kDim / 8;            // output tiles of eight dims
+  using L = Layout<kDim, kCodes, kTiles>;
   constexpr int kChunks = kDim / 16;
+  constexpr int kGroups = L::kStep / 16;  // of 16 tokens
+  constexpr int kHeads = 8 * kTiles;
+  constexpr float kSlack = 8.0f;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float warp_max[kWarps][16], warp_sum[kWarps][16];
-  __shared__ int64_t found[2];
-  __shared__ int64_t scan[kWarps];
-  __shared__ int32_t last_arrival;
+  __shared__ int32_t answer[2];
+  // Parts 2 w and 2 w + 1: what warp w holds of the row that its share begins inside of, and of the one
+  // that its share ends inside of (the latter where both are one).
+  __shared__ Part parts[2 * kWarps];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q4 = lane & 3, r8 = lane >> 2;
+  constexpr int64_t kPartFloats = part_floats(kDim, kHeads);
+  using Join = Joined<kDim, kHeads>;
+  if (lane < 2) parts[2 * warp + lane].there = false;
   ptx::grid_dependency_wait();
 
   const int32_t rows_per_sequence = p.cache.heads * p.head_blocks;
-  // Tokens of sequence b that are read, and the first of them.
+  // The tokens of sequence b that are seen, from `begin` to the one returned; steps count from a
+  // multiple of kStep.
   auto extent = [&](int32_t b, int32_t& begin) {
-    int32_t length = __ldg(p.lengths + b);
-    length = max(0, min(length, p.capacity));
+    const int32_t length = max(0, min(__ldg(p.lengths + b), p.capacity));
     begin = p.window > 0 && length > p.window ? length - p.window : 0;
-    return length - begin;
+    return length;
   };
-  auto units_of = [&](int32_t b) {
+  auto steps_between = [&](int32_t begin, int32_t end) { return (end - begin / L::kStep * L::kStep + L::kStep - 1) / L::kStep; };
+  auto steps_of = [&](int32_t b) {
     int32_t begin;
-    return (extent(b, begin) + L::kUnit - 1) / L::kUnit;
+    const int32_t end = extent(b, begin);
+    return steps_between(begin, end);
   };
 
-  // Where the shares begin: a scan over the sequences' units.
-  const int32_t per_thread = (p.batch + kThreads - 1) / kThreads;
-  const int32_t b0 = min(p.batch, static_cast<int32_t>(threadIdx.x) * per_thread), b1 = min(p.batch, b0 + per_thread);
+  // Where the warp's share begins: a scan over the sequences' steps, each warp for itself (with barriers
+  // between four of them it took twice the time).
+  const int32_t per_lane = (p.batch + 31) / 32;
+  const int32_t b0 = min(p.batch, lane * per_lane), b1 = min(p.batch, b0 + per_lane);
+  auto sum_up = [&](int64_t value) {  // inclusive
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t below = __shfl_up_sync(0xffffffffu, value, d);
+      if (lane >= d) value += below;
+    }
+    return value;
+  };
   int64_t mine = 0;
-  for (int32_t b = b0; b < b1; ++b) {
-    const int32_t units = units_of(b);
-    mine += static_cast<int64_t>(units) * rows_per_sequence;
-    if (blockIdx.x == 0 && p.status != nullptr && __ldg(p.lengths + b) > p.capacity) atomicOr(p.status, kStatusIndex);
+  for (int32_t b = b0; b < b1; ++b) mine += static_cast<int64_t>(steps_of(b)) * rows_per_sequence;
+  int64_t upto = sum_up(mine);
+  const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+  const int64_t share = max(quotient(total + gridDim.x * kWarps - 1, gridDim.x * kWarps), static_cast<int64_t>(1));
+  const int32_t piece = static_cast<int32_t>(min(share * kWarps, static_cast<int64_t>(1) << 30));  // a lot's steps
+  int64_t lots = quotient(total + piece - 1, piece);
+  auto pieces_of = [&](int32_t b) { return (steps_of(b) + piece - 1) / piece; };
+  bool aligned = static_cast<int64_t>(p.batch) * rows_per_sequence <= gridDim.x;
+  if (aligned) {
+    int64_t pieces = 0;
+    for (int32_t b = b0; b < b1; ++b) pieces += static_cast<int64_t>(pieces_of(b)) * rows_per_sequence;
+    const int64_t pieces_upto = sum_up(pieces), all = __shfl_sync(0xffffffffu, pieces_upto, 31);
+    aligned = all <= gridDim.x;
+    if (aligned) {
+      mine = pieces;
+      upto = pieces_upto;
+      lots = all;
+    }
   }
-  // Sequences with nothing to attend to.
+
+  // Sequences with nothing to attend to, and lengths that the table cannot hold.
   for (int32_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (units_of(b) != 0) continue;
+    if (threadIdx.x == 0 && p.status != nullptr && __ldg(p.lengths + b) > p.capacity) atomicOr(p.status, kStatusIndex);
+    if (steps_of(b) != 0) continue;
     const int64_t row = static_cast<int64_t>(b) * p.heads;
     for (int32_t i = threadIdx.x; i < p.heads * (kDim / 8); i += kThreads) {
       *reinterpret_cast<uint4*>(p.out + row * kDim + 8 * static_cast<int64_t>(i)) = make_uint4(0, 0, 0, 0);
@@ -132,430 +343,530 @@ paged_attention_kernel(const AttentionParams p) {
       for (int32_t h = threadIdx.x; h < p.heads; h += kThreads) p.lse[row + h] = -INFINITY;
     }
   }
-  int64_t inclusive = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t below = __shfl_up_sync(0xffffffffu, inclusive, d);
-    if (lane >= d) inclusive += below;
-  }
-  if (lane == 31) scan[warp] = inclusive;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) inclusive += scan[w];
-    total += scan[w];
-  }
-  const int64_t share = max((total + gridDim.x - 1) / static_cast<int64_t>(gridDim.x), static_cast<int64_t>(1));
-  int64_t unit = blockIdx.x * share;
-  const int64_t unit_end = min(unit + share, total);
-  if (unit >= unit_end) return;
-  if (unit >= inclusive - mine && unit < inclusive) {
-    int64_t base = inclusive - mine;
-    for (int32_t b = b0; b < b1; ++b) {
-      const int64_t units = static_cast<int64_t>(units_of(b)) * rows_per_sequence;
-      if (unit < base + units) {
-        found[0] = b;
-        found[1] = base;
-        break;
-      }
-      base += units;
-    }
-  }
-  __syncthreads();
-  int32_t b = static_cast<int32_t>(found[0]);
-  int64_t base = found[1];  // of sequence b
+  const int32_t lot = blockIdx.x;
+  if (lot >= lots) return;
 
   uint8_t* const ring = smem + warp * (L::kStages * L::kStageBytes);
   const uint32_t ring_addr = ptx::smem_u32(ring);
+  float* const stash = p.partials + (kSlots * static_cast<int64_t>(gridDim.x) + blockIdx.x * kWarps + warp) * kPartFloats;
 
-  while (unit < unit_end) {
-    int32_t begin;
-    int32_t tokens = extent(b, begin);
-    int32_t units = (tokens + L::kUnit - 1) / L::kUnit;
-    while (unit >= base + static_cast<int64_t>(units) * rows_per_sequence) {  // on to the next sequence with tokens
-      base += static_cast<int64_t>(units) * rows_per_sequence;
-      ++b;
-      tokens = extent(b, begin);
-      units = (tokens + L::kUnit - 1) / L::kUnit;
+  // A place in the numbering: a row, its tokens and the next of its steps.
+  struct Cursor {
+    int32_t b, row, begin, end, token, left;
+  };
+  Cursor at;
+  int32_t steps, row_first_lot = 0, row_lots = 0;
+  const int64_t first_step = lot * static_cast<int64_t>(piece) + warp * share;
+  {
+    // (the warp's first step or, aligned, the lot)
+    const int64_t wanted = aligned ? lot : min(first_step, total - 1);
+    int32_t b = 0;
+    int64_t base = upto - mine;
+    const bool here = wanted >= base && wanted < upto;
+    if (here) {
+      for (b = b0; b < b1; ++b) {
+        const int64_t count = static_cast<int64_t>(aligned ? pieces_of(b) : steps_of(b)) * rows_per_sequence;
+        if (wanted < base + count) break;
+        base += count;
+      }
     }
-    const int32_t row = static_cast<int32_t>((unit - base) / units);
-    const int64_t row_first = base + static_cast<int64_t>(row) * units;
-    const int32_t first_unit = static_cast<int32_t>(unit - row_first);
-    const int32_t steps = static_cast<int32_t>(min(unit_end, row_first + units) - unit);
-    const int32_t kv_head = row / p.head_blocks;
-    const int32_t head_block = row % p.head_blocks;
-    const int32_t heads = min(p.group - head_block * 16, 16);
-    const int32_t head0 = kv_head * p.group + head_block * 16;
-    const int32_t end = begin + tokens;
+    const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    at.b = __shfl_sync(0xffffffffu, b, from);
+    base = __shfl_sync(0xffffffffu, base, from);
+    at.end = extent(at.b, at.begin);
+    const int32_t per_row = steps_between(at.begin, at.end);
+    int32_t done;
+    if (aligned) {
+      row_lots = (per_row + piece - 1) / piece;
+      const int32_t inside = static_cast<int32_t>(wanted - base);
+      at.row = inside / row_lots;
+      row_first_lot = lot - inside % row_lots;
+      done = (inside % row_lots) * piece + warp * static_cast<int32_t>(share);
+      steps = max(0, min(static_cast<int32_t>(share), per_row - done));
+    } else {
+      at.row = static_cast<int32_t>(quotient(wanted - base, per_row));
+      done = static_cast<int32_t>(wanted - base - static_cast<int64_t>(at.row) * per_row);
+      steps = static_cast<int32_t>(max(static_cast<int64_t>(0), min(share, total - first_step)));
+    }
+    at.token = (at.begin / L::kStep + done) * L::kStep;
+    at.left = per_row - done;
+  }
+  if (steps > 0) {
+    auto enter = [&](Cursor& c) {  // the first step of row c.row of sequence c.b, or of the next with tokens
+      if (c.row == rows_per_sequence) {
+        c.row = 0;
+        do {
+          c.end = extent(++c.b, c.begin);
+        } while (c.end == 0);
+      }
+      c.token = c.begin / L::kStep * L::kStep;
+      c.left = (c.end - c.token + L::kStep - 1) / L::kStep;
+    };
+    Cursor ahead = at;  // of the loads
+    int32_t to_load = steps;
+    int32_t load_stage = 0;
 
-    const int32_t* table = p.tables + static_cast<int64_t>(b) * p.table_stride;
-    const uint8_t* k_head = p.cache.k + kv_head * p.cache.head;
-    const uint8_t* v_head = p.cache.v + kv_head * p.cache.head;
-
-    // The page of each of a step's tokens, a lane's own, looked up a step before it is needed; place -1:
-    // no token.
-    int32_t ref_page = 0, ref_place = -1;
-    auto look_up = [&](int32_t step) {
-      const int32_t token = begin + (first_unit + step) * L::kUnit + warp * L::kStep + lane % L::kStep;
+    // Pages are looked up a step before they are needed: that of a lane's own token or, where pages hold
+    // whole groups of 16 tokens (p.whole_groups), of the first token of its group.
+    constexpr int kPieces = L::kRow / 16;
+    constexpr int kCopies = L::kStep * kPieces / 32;
+    static_assert(16 * kPieces % 32 == 0, "whole warps");
+    const int32_t own = lane % L::kStep;
+    int32_t ref_page = 0, ref_place = -1;  // place -1: no token
+    auto look_up = [&]() {
+      if (to_load == 0) return;
+      const int32_t token = ahead.token + (p.whole_groups ? own / 16 * 16 : own);
       ref_place = -1;
-      if (step < steps && token < end) {
+      if (token < ahead.end && token + (p.whole_groups ? 15 : 0) >= ahead.begin) {
         const uint32_t index = p.cache.page_size.div(token);
         ref_place = token - index * p.cache.page_size.d;
-        ref_page = __ldg(table + index);
+        ref_page = __ldg(p.tables + ahead.b * p.table_stride + index);
       }
     };
-    auto load = [&](int32_t step) {
-      if (step >= steps) return;
-      const uint32_t stage = ring_addr + (step % L::kStages) * L::kStageBytes;
-      if (static_cast<uint32_t>(ref_page) >= static_cast<uint32_t>(p.cache.num_pages) && ref_place >= 0) {
-        if (p.status != nullptr) atomicOr(p.status, kStatusIndex);
-        ref_place = -1;
-      }
-      constexpr int kPieces = L::kRow / 16;
-      static_assert(L::kStep * kPieces % 32 == 0, "whole warps");
+    auto load = [&]() {
+      if (to_load == 0) return;
+      const uint32_t stage = ring_addr + load_stage * L::kStageBytes;
+      load_stage = load_stage + 1 == L::kStages ? 0 : load_stage + 1;
+      const bool there = ref_place >= 0 && static_cast<uint32_t>(ref_page) < static_cast<uint32_t>(p.cache.num_pages);
+      if (ref_place >= 0 && !there && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+      const int32_t kv_head = p.head_blocks == 1 ? ahead.row : ahead.row / p.head_blocks;
+      const int64_t offset = there ? kv_head * p.cache.head + ref_page * p.cache.page + ref_place * p.cache.token : -1;
+      const bool full = ahead.token >= ahead.begin && ahead.token + L::kStep <= ahead.end && __all_sync(0xffffffffu, there);
+      if (p.whole_groups && full && p.cache.token == L::kRow) {
+        // rows of a group follow one another
 #pragma unroll
-      for (int i = 0; i < L::kStep * kPieces / 32; ++i) {
-        const int piece = i * 32 + lane, at = piece / kPieces, column = piece % kPieces;
-        const int32_t page = __shfl_sync(0xffffffffu, ref_page, at);
-        const int32_t place = __shfl_sync(0xffffffffu, ref_place, at);
-        const bool there = place >= 0;
-        const int64_t offset = there ? page * p.cache.page + place * p.cache.token + column * 16 : 0;
-        const uint32_t dst = stage + at * L::kPitch + column * 16;
-        ptx::cp_async_16(dst, k_head + offset, there);
-        ptx::cp_async_16(dst + L::kStep * L::kPitch, v_head + offset, there);
+        for (int g = 0; g < L::kStep / 16; ++g) {
+          const int64_t from = L::kStep == 16 ? offset : __shfl_sync(0xffffffffu, offset, 16 * g);
+          const uint8_t* k = p.cache.k + from + lane * 16;
+          const uint8_t* v = p.cache.v + from + lane * 16;
+#pragma unroll
+          for (int i = 0; i < kPieces / 2; ++i) {
+            const int at_piece = i * 32 + lane, row = 16 * g + at_piece / kPieces, column = at_piece % kPieces;
+            const uint32_t dst = stage + row * L::kPitch + column * 16;
+            cp_async_16_all(dst, k + i * 512);
+            cp_async_16_all(dst + L::kStep * L::kPitch, v + i * 512);
+          }
+        }
+      } else {
+        const int32_t stride = static_cast<int32_t>(p.cache.token);  // (in groups: fits)
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int at_piece = i * 32 + lane, row = at_piece / kPieces, column = at_piece % kPieces;
+          int64_t from = __shfl_sync(0xffffffffu, offset, p.whole_groups ? row / 16 * 16 : row);
+          const bool seen = from >= 0 && ahead.token + row >= ahead.begin && ahead.token + row < ahead.end;
+          if (p.whole_groups) from += static_cast<int64_t>(row % 16) * stride;
+          from = seen ? from + column * 16 : 0;
+          const uint32_t dst = stage + row * L::kPitch + column * 16;
+          ptx::cp_async_16(dst, p.cache.k + from, seen);
+          ptx::cp_async_16(dst + L::kStep * L::kPitch, p.cache.v + from, seen);
+        }
       }
       if constexpr (kCodes) {
-        const bool there = ref_place >= 0;
-        const int64_t offset = there ? ref_page * p.cache.scale_page + kv_head * p.cache.scale_head + ref_place * p.cache.scale_token : 0;
-        const uint32_t dst = stage + 2 * L::kStep * L::kPitch + (lane % L::kStep) * 4;
+        const bool seen = there && ahead.token + own >= ahead.begin && ahead.token + own < ahead.end;
+        const int64_t from = seen ? kv_head * p.cache.scale_head + ref_page * p.cache.scale_page +
+                                        (ref_place + (p.whole_groups ? own % 16 : 0)) * p.cache.scale_token
+                                  : 0;
+        const uint32_t dst = stage + 2 * L::kStep * L::kPitch + own * 4;
         if (lane < L::kStep) {
-          cp_async_4(dst, p.cache.k_scale + offset, there);
-          cp_async_4(dst + L::kStep * 4, p.cache.v_scale + offset, there);
+          cp_async_4(dst, p.cache.k_scale + from, seen);
+          cp_async_4(dst + L::kStep * 4, p.cache.v_scale + from, seen);
         }
+      }
+      --to_load;
+      ahead.token += L::kStep;
+      if (--ahead.left == 0 && to_load > 0) {
+        ++ahead.row;
+        enter(ahead);
       }
     };
 
-    look_up(0);
+    look_up();
 #pragma unroll
     for (int s = 0; s < L::kStages - 1; ++s) {
-      load(s);
-      look_up(s + 1);
+      load();
+      look_up();
       ptx::cp_async_commit();
     }
 
-    // The queries' fragments: rows r8 (and r8 + 8) of the block's heads; codes want the dims of a
-    // 16-byte piece in the order in which its bytes lie in the lanes.
-    uint32_t qf[kChunks][kWide ? 4 : 2];
-    {
-      const __nv_bfloat16* q = p.q + b * p.q_batch + static_cast<int64_t>(head0) * p.q_head;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-        for (int i = 0; i < (kWide ? 4 : 2); ++i) {
-          const int head = kWide ? r8 + 8 * (i & 1) : r8;
-          const int part = kWide ? i >> 1 : i;
-          const int dim = 16 * c + (kCodes ? 4 * q4 + 2 * part : 2 * q4 + 8 * part);
-          qf[c][i] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + head * p.q_head + dim)) : 0u;
-        }
-      }
-    }
-
-    float out[kOut][4] = {};
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    uint32_t qf[kChunks][kTiles][2];
+    float start[kTiles][2] = {};
+    // A lane's heads are 8 n + 2 q4 and the next; of the dims it has rows r8 and r8 + 8 of each chunk.
+    float out[kChunks][kTiles][4], top[kTiles][2], sum[kTiles][2];
+    bool began = at.token > at.begin;  // in an earlier share
+    bool fresh = true;
+    int32_t stage_index = 0;
 
     for (int32_t step = 0; step < steps; ++step) {
-      ptx::cp_async_wait_group<L::kStages - 2>();
-      __syncwarp();
-      load(step + L::kStages - 1);
-      look_up(step + L::kStages);
-      ptx::cp_async_commit();
-
-      const int32_t token0 = begin + (first_unit + step) * L::kUnit + warp * L::kStep;
-      if (token0 >= end) continue;  // (the whole warp)
-      const uint32_t stage = ring_addr + (step % L::kStages) * L::kStageBytes;
-      float s[kTiles][4] = {};
+      if (fresh) {
+        // The queries' fragments: head 8 n + r8; codes want the dims of a 16-byte piece in the order in
+        // which its bytes lie in the lanes.
+        fresh = false;
+        const Row of(p, at.b, at.row);
+        const int32_t heads = of.heads;
+        const __nv_bfloat16* q = p.q + at.b * p.q_batch + (of.head0 - static_cast<int64_t>(at.b) * p.heads) * p.q_head;
 #pragma unroll
-      for (int j = 0; j < L::kStep / 16; ++j) {
-        if constexpr (!kCodes) {
-          const uint32_t at = stage + (j * 16 + (lane & 7) + ((lane >> 4) << 3)) * L::kPitch + ((lane >> 3) & 1) * 16;
+        for (int n = 0; n < kTiles; ++n) {
+          const int head = 8 * n + r8;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
-            uint32_t kf[4];
-            ldmatrix_x4_at(at + c * 32, kf);
-            const uint32_t a[4] = {qf[c][0], kWide ? qf[c][1] : 0u, qf[c][kWide ? 2 : 1], kWide ? qf[c][kWide ? 3 : 0] : 0u};
-            ptx::mma_m16n8k16(s[2 * j], a, kf[0], kf[1]);
-            ptx::mma_m16n8k16(s[2 * j + 1], a, kf[2], kf[3]);
-          }
-        } else {
-          const uint32_t at = stage + (j * 16 + (lane & 7) + ((lane >> 4) << 3)) * L::kPitch + ((lane >> 3) & 1) * 16;
-#pragma unroll
-          for (int c = 0; c < kChunks; c += 2) {
-            uint32_t kf[4];
-            ldmatrix_x4_at(at + c * 16, kf);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int cc = c + (i & 1);
-              uint32_t lo, hi;
-              codes_to_bf16<kCodes>(kf[i], 0x4140, 0x4342, lo, hi);
-              const uint32_t a[4] = {qf[cc][0], kWide ? qf[cc][1] : 0u, qf[cc][kWide ? 2 : 1], kWide ? qf[cc][kWide ? 3 : 0] : 0u};
-              ptx::mma_m16n8k16(s[2 * j + (i >> 1)], a, lo, hi);
-            }
-          }
-        }
-      }
-      // Scores times the scale and log2(e); minus infinity behind the last token.
-      float high[2] = {-INFINITY, -INFINITY};
-      float value_scale[kCodes ? kTiles : 1][2];
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        float f[2] = {p.scale, p.scale};
-        if constexpr (kCodes) {
-          const float2 ks = *reinterpret_cast<const float2*>(ring + (step % L::kStages) * L::kStageBytes + 2 * L::kStep * L::kPitch + (8 * t + 2 * q4) * 4);
-          const float2 vs = *reinterpret_cast<const float2*>(ring + (step % L::kStages) * L::kStageBytes + 2 * L::kStep * L::kPitch + L::kStep * 4 + (8 * t + 2 * q4) * 4);
-          f[0] *= 64.0f * ks.x;
-          f[1] *= 64.0f * ks.y;
-          value_scale[t][0] = 64.0f * vs.x;
-          value_scale[t][1] = 64.0f * vs.y;
-        }
-        const bool seen[2] = {token0 + 8 * t + 2 * q4 < end, token0 + 8 * t + 2 * q4 + 1 < end};
-#pragma unroll
-        for (int i = 0; i < (kWide ? 4 : 2); ++i) {
-          s[t][i] = seen[i & 1] ? s[t][i] * f[i & 1] : -INFINITY;
-          high[i >> 1] = fmaxf(high[i >> 1], s[t][i]);
-        }
-      }
-      bool rises = false;
-#pragma unroll
-      for (int i = 0; i < (kWide ? 2 : 1); ++i) {
-        high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], 1));
-        high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], 2));
-        rises |= high[i] > top[i];
-      }
-      if (__any_sync(0xffffffffu, rises)) {
-        float factor[2] = {1.0f, 1.0f};
-#pragma unroll
-        for (int i = 0; i < (kWide ? 2 : 1); ++i) {
-          const float next = fmaxf(top[i], high[i]);
-          factor[i] = next == -INFINITY ? 1.0f : exp2_approx(top[i] - next);
-          top[i] = next;
-          sum[i] *= factor[i];
-        }
-        if constexpr (!kWide) factor[1] = factor[0];
-#pragma unroll
-        for (int t = 0; t < kOut; ++t) {
-          out[t][0] *= factor[0];
-          out[t][1] *= factor[0];
-          out[t][2] *= factor[1];
-          out[t][3] *= factor[1];
-        }
-      }
-      const float from[2] = {top[0] == -INFINITY ? 0.0f : top[0], top[1] == -INFINITY ? 0.0f : top[1]};
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-        for (int i = 0; i < (kWide ? 4 : 2); ++i) {
-          s[t][i] = exp2_approx(s[t][i] - from[i >> 1]);
-          sum[i >> 1] += s[t][i];
-          if constexpr (kCodes) s[t][i] *= value_scale[t][i & 1];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < L::kStep / 16; ++j) {
-        // P of these 16 tokens in two parts
-        uint32_t part[2][kWide ? 4 : 2];
-#pragma unroll
-        for (int i = 0; i < (kWide ? 4 : 2); ++i) {
-          const float* pair = &s[2 * j + (kWide ? i >> 1 : i)][kWide ? 2 * (i & 1) : 0];
-          part[0][i] = pack_bf16(pair[0], pair[1]);
-          part[1][i] = pack_bf16(pair[0] - bf16_lo(part[0][i]), pair[1] - bf16_hi(part[0][i]));
-        }
-        auto multiply = [&](float (&o)[4], uint32_t v0, uint32_t v1) {
-          if constexpr (kWide) {
-            ptx::mma_m16n8k16(o, {part[0][0], part[0][1], part[0][2], part[0][3]}, v0, v1);
-            ptx::mma_m16n8k16(o, {part[1][0], part[1][1], part[1][2], part[1][3]}, v0, v1);
-          } else {
-            ptx::mma_m16n8k16(o, {part[0][0], part[1][0], part[0][1], part[1][1]}, v0, v1);
-          }
-        };
-        const uint32_t at = stage + L::kStep * L::kPitch + (j * 16 + (lane & 15)) * L::kPitch + (lane >> 4) * 16;
-        if constexpr (!kCodes) {
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            uint32_t vf[4];
-            ldmatrix_x4_trans(at + c * 32, vf);
-            multiply(out[2 * c], vf[0], vf[1]);
-            multiply(out[2 * c + 1], vf[2], vf[3]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kChunks; c += 2) {
-            uint32_t vf[4];
-            ldmatrix_x4_trans(at + c * 16, vf);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              uint32_t even[2], odd[2];
-              codes_to_bf16<kCodes>(vf[2 * i], 0x4240, 0x4341, even[0], odd[0]);
-              codes_to_bf16<kCodes>(vf[2 * i + 1], 0x4240, 0x4341, even[1], odd[1]);
-              multiply(out[2 * (c + i)], even[0], even[1]);
-              multiply(out[2 * (c + i) + 1], odd[0], odd[1]);
+              const int dim = 16 * c + (kCodes ? 4 * q4 + 2 * i : 2 * q4 + 8 * i);
+              qf[c][n][i] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + head * p.q_head + dim)) : 0u;
             }
           }
+          if constexpr (kCodes) {
+            // queries times 2^80, and what the scores start from
+            float all = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                all += bf16_lo(qf[c][n][i]) + bf16_hi(qf[c][n][i]);
+                qf[c][n][i] = bf16x2_fma(qf[c][n][i], 0x67806780u, 0x80008000u);  // times 2^80, minus zero
+              }
+            }
+            all += __shfl_xor_sync(0xffffffffu, all, 1);
+            all += __shfl_xor_sync(0xffffffffu, all, 2);
+            all *= -128.0f * 0x1p-53f;
+            start[n][0] = __shfl_sync(0xffffffffu, all, 8 * q4);
+            start[n][1] = __shfl_sync(0xffffffffu, all, 8 * q4 + 4);
+          }
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) out[c][n][0] = out[c][n][1] = out[c][n][2] = out[c][n][3] = 0.0f;
+          top[n][0] = top[n][1] = -INFINITY;
+          sum[n][0] = sum[n][1] = 0.0f;
         }
       }
-    }
-    ptx::cp_async_wait_group<0>();
 
-    // The warps' results into one: the ring is free.
+      ptx::cp_async_wait_group<L::kStages - 2>();
+      __syncwarp();
+      load();
+      look_up();
+      ptx::cp_async_commit();
+
+      const uint32_t stage = ring_addr + stage_index * L::kStageBytes;
+      const float* const scales = reinterpret_cast<const float*>(ring + stage_index * L::kStageBytes + 2 * L::kStep * L::kPitch);
+      stage_index = stage_index + 1 == L::kStages ? 0 : stage_index + 1;
+      float s[kGroups][kTiles][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-      if (q4 == 0 && (kWide || i == 0)) {
-        warp_max[warp][r8 + 8 * i] = top[i];
-        warp_sum[warp][r8 + 8 * i] = sum[i];
-      }
-    }
-    __syncthreads();
-    constexpr int kRows = kWide ? 16 : 8;
-    float* const shared_out = reinterpret_cast<float*>(smem);  // [kWarps][kRows][kDim]
+      for (int j = 0; j < kGroups; ++j) {
 #pragma unroll
-    for (int i = 0; i < (kWide ? 2 : 1); ++i) {
-      const int head = r8 + 8 * i;
-      float most = warp_max[0][head];
+        for (int n = 0; n < kTiles; ++n) s[j][n][0] = s[j][n][2] = start[n][0], s[j][n][1] = s[j][n][3] = start[n][1];
+        const uint32_t k_at = stage + (j * 16 + (lane & 15)) * L::kPitch + (lane >> 4) * 16;
+        if constexpr (!kCodes) {
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) most = fmaxf(most, warp_max[w][head]);
-      const float factor = most == -INFINITY ? 0.0f : exp2_approx(top[i] - most);
-      float* to = shared_out + (warp * kRows + head) * kDim;
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t a[4];
+            ldmatrix_x4_at(k_at + c * 32, a);
 #pragma unroll
-      for (int t = 0; t < kOut; ++t) {
-        float v0 = out[t][2 * i], v1 = out[t][2 * i + 1];
-        if constexpr (!kWide) v0 += out[t][2], v1 += out[t][3];
-        // even and odd dims of a 16-byte piece of codes are two tiles
-        const int d0 = kCodes ? 16 * (t / 2) + 4 * q4 + t % 2 : 8 * t + 2 * q4;
-        to[d0] = v0 * factor;
-        to[d0 + (kCodes ? 2 : 1)] = v1 * factor;
-      }
-    }
-    __syncthreads();
-    const int64_t first_cta = row_first / share, last_cta = (row_first + units - 1) / share;
-    const bool whole = first_cta == last_cta;
-    float* slot = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (blockIdx.x == first_cta ? 1 : 0)) * partial_floats(kDim);
-    auto head_state = [&](int head, float& most, float& all) {
-      most = warp_max[0][head];
+            for (int n = 0; n < kTiles; ++n) ptx::mma_m16n8k16(s[j][n], a, qf[c][n][0], qf[c][n][1]);
+          }
+        } else {
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) most = fmaxf(most, warp_max[w][head]);
-      all = 0.0f;
+          for (int c = 0; c < kChunks; c += 2) {
+            uint32_t kf[4];
+            ldmatrix_x4_at(k_at + c * 16, kf);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) all += most == -INFINITY ? 0.0f * warp_sum[w][head] : warp_sum[w][head] * exp2_approx(warp_max[w][head] - most);
-    };
-    auto finish = [&](int head, int dim, const float (&v)[4], float all) {
-      const float rate = all == 0.0f ? 0.0f : 1.0f / all;
-      __nv_bfloat16* to = p.out + (static_cast<int64_t>(b) * p.heads + head0 + head) * kDim + dim;
-      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(v[0] * rate, v[1] * rate), pack_bf16(v[2] * rate, v[3] * rate));
-    };
-    auto finish_lse = [&](int head, float most, float all) {
-      if (p.lse != nullptr) p.lse[static_cast<int64_t>(b) * p.heads + head0 + head] = all == 0.0f ? -INFINITY : (most + log2f(all)) * 0.693147180559945309f;
-    };
-    for (int i = threadIdx.x; i < heads * (kDim / 4); i += kThreads) {
-      const int head = i / (kDim / 4), dim = i % (kDim / 4) * 4;
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a[4] = {__byte_perm(kf[2 * i], 0, 0x4140), __byte_perm(kf[2 * i + 1], 0, 0x4140),
+                                     __byte_perm(kf[2 * i], 0, 0x4342), __byte_perm(kf[2 * i + 1], 0, 0x4342)};
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float4 x = *reinterpret_cast<const float4*>(shared_out + (w * kRows + head) * kDim + dim);
-        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-      }
-      float most, all;
-      head_state(head, most, all);
-      if (whole) {
-        finish(head, dim, v, all);
-        if (dim == 0) finish_lse(head, most, all);
-      } else {
-        __stcg(reinterpret_cast<float4*>(slot + head * kDim + dim), make_float4(v[0], v[1], v[2], v[3]));
-        if (dim == 0) {
-          __stcg(slot + 16 * kDim + head, most);
-          __stcg(slot + 16 * kDim + 16 + head, all);
+              for (int n = 0; n < kTiles; ++n) ptx::mma_m16n8k16(s[j][n], a, qf[c + i][n][0], qf[c + i][n][1]);
+            }
+          }
         }
       }
-    }
-    if (!whole) {
-      // The last CTA of the row to arrive joins the parts, in their order.  The count goes back to zero.
-      __threadfence();
-      __syncthreads();
-      const int32_t parts = static_cast<int32_t>(last_cta - first_cta) + 1;
-      if (threadIdx.x == 0) {
-        const int32_t before = atomicAdd(p.locks + first_cta, 1);
-        last_arrival = before == parts - 1;
-        if (last_arrival) p.locks[first_cta] = 0;
-      }
-      __syncthreads();
-      if (last_arrival) {
-        __threadfence();
-        auto part_at = [&](int32_t part) {
-          return p.partials + (2 * (first_cta + part) + (part == 0 ? 1 : 0)) * partial_floats(kDim);
-        };
-        float* weights = reinterpret_cast<float*>(smem);  // [parts][16]
-        {
-          const int head = threadIdx.x >> 3, sub = threadIdx.x & 7;
-          float most = -INFINITY;
-          if (head < heads) {
-            for (int32_t i = sub; i < parts; i += 8) most = fmaxf(most, __ldcg(part_at(i) + 16 * kDim + head));
+      // Scores times the scale and log2(e); minus infinity before the first and behind the last token.
+      // A lane's tokens are r8 and r8 + 8 of each 16.
+      float value_scale[kCodes ? kGroups : 1][2];
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float f = p.scale;
+          if constexpr (kCodes) {
+            f *= scales[16 * j + 8 * i + r8];
+            value_scale[j][i] = 64.0f * scales[L::kStep + 16 * j + 8 * i + r8];
           }
 #pragma unroll
-          for (int d = 1; d < 8; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-          float all = 0.0f;
-          if (head < heads) {
-            for (int32_t i = sub; i < parts; i += 8) {
-              const float high = __ldcg(part_at(i) + 16 * kDim + head);
-              const float weight = most == -INFINITY ? 0.0f : exp2_approx(high - most);
-              weights[i * 16 + head] = weight;
-              all += weight * __ldcg(part_at(i) + 16 * kDim + 16 + head);
+          for (int n = 0; n < kTiles; ++n) s[j][n][2 * i] *= f, s[j][n][2 * i + 1] *= f;
+        }
+      }
+      if (at.token < at.begin || at.token + L::kStep > at.end) {
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int32_t token = at.token + 16 * j + 8 * i + r8;
+            if (token < at.begin || token >= at.end) {
+#pragma unroll
+              for (int n = 0; n < kTiles; ++n) s[j][n][2 * i] = s[j][n][2 * i + 1] = -INFINITY;
+            }
+          }
+        }
+      }
+      float high[kTiles][2];
+      bool rises = false;
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          high[n][i] = fmaxf(s[0][n][i], s[0][n][2 + i]);
+#pragma unroll
+          for (int j = 1; j < kGroups; ++j) high[n][i] = fmaxf(high[n][i], fmaxf(s[j][n][i], s[j][n][2 + i]));
+          rises |= high[n][i] > top[n][i] + kSlack;
+        }
+      }
+      if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          float factor[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) high[n][i] = fmaxf(high[n][i], __shfl_xor_sync(0xffffffffu, high[n][i], d));
+            const float next = fmaxf(top[n][i], high[n][i]);
+            factor[i] = next == -INFINITY ? 1.0f : exp2_approx(top[n][i] - next);
+            top[n][i] = next;
+            sum[n][i] *= factor[i];
+          }
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[c][n][i] *= factor[i & 1];
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        const float from[2] = {top[n][0] == -INFINITY ? 0.0f : top[n][0], top[n][1] == -INFINITY ? 0.0f : top[n][1]};
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[j][n][i] = exp2_approx(s[j][n][i] - from[i & 1]);
+            sum[n][i & 1] += s[j][n][i];
+            if constexpr (kCodes) s[j][n][i] *= value_scale[j][i >> 1];
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        // P of these 16 tokens in two parts, tokens along the lane's registers
+        uint32_t two[2][kTiles][2];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float x = s[j][n][2 * i], y = s[j][n][2 * i + 1];
+            const uint32_t coarse = pack_bf16(x, y);
+            two[0][n][i] = transposed(coarse);
+            two[1][n][i] = transposed(pack_bf16(x - bf16_lo(coarse), y - bf16_hi(coarse)));
+          }
+        }
+        auto multiply = [&](int c, const uint32_t (&a)[4]) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            ptx::mma_m16n8k16(out[c][n], a, two[0][n][0], two[0][n][1]);
+            ptx::mma_m16n8k16(out[c][n], a, two[1][n][0], two[1][n][1]);
+          }
+        };
+        const uint32_t v_at = stage + L::kStep * L::kPitch + (j * 16 + (lane & 7) + ((lane >> 4) << 3)) * L::kPitch + ((lane >> 3) & 1) * 16;
+        if constexpr (!kCodes) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t a[4];
+            ldmatrix_x4_trans(v_at + c * 32, a);
+            multiply(c, a);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kChunks; c += 2) {
+            uint32_t vf[4];
+            ldmatrix_x4_trans(v_at + c * 16, vf);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              // even dims of the piece, then the odd ones
+              multiply(c + i, {two_codes(vf[i], 0x4240), two_codes(vf[i], 0x4341), two_codes(vf[2 + i], 0x4240),
+                               two_codes(vf[2 + i], 0x4341)});
+            }
+          }
+        }
+      }
+
+      at.token += L::kStep;
+      --at.left;
+      if (at.left != 0 && step + 1 < steps) continue;
+
+      // The end of the row, or of the share.
+      const bool ended = at.left == 0;
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) sum[n][i] += __shfl_xor_sync(0xffffffffu, sum[n][i], d);
+        }
+      }
+      if (ended && !began) {
+        const Row of(p, at.b, at.row);
+        const int32_t heads = of.heads;
+        const int64_t head0 = of.head0;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          const float rate[2] = {rate_of(sum[n][0]), rate_of(sum[n][1])};
+          __nv_bfloat16* to = p.out + (head0 + 8 * n + r8) * kDim;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            // dims 2 q4 and 2 q4 + 1 of head r8, of each half of the chunk
+            const uint32_t a = transposed(pack_bf16(out[c][n][0] * rate[0], out[c][n][1] * rate[1]));
+            const uint32_t b = transposed(pack_bf16(out[c][n][2] * rate[0], out[c][n][3] * rate[1]));
+            if (8 * n + r8 < heads) {
+              if constexpr (!kCodes) {
+                *reinterpret_cast<uint32_t*>(to + 16 * c + 2 * q4) = a;
+                *reinterpret_cast<uint32_t*>(to + 16 * c + 2 * q4 + 8) = b;
+              } else {
+                *reinterpret_cast<uint2*>(to + 16 * c + 4 * q4) = make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+              }
             }
           }
 #pragma unroll
-          for (int d = 1; d < 8; d <<= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-          if (sub == 0 && head < heads) {
-            warp_sum[0][head] = all;
-            finish_lse(head, most, all);
+          for (int i = 0; i < 2; ++i) {
+            const int head = 8 * n + 2 * q4 + i;
+            if (p.lse != nullptr && r8 == 0 && head < heads) p.lse[head0 + head] = lse_of(top[n][i], sum[n][i]);
           }
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < heads * (kDim / 4); i += kThreads) {
-          const int head = i / (kDim / 4), dim = i % (kDim / 4) * 4;
-          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-          for (int32_t part = 0; part < parts; ++part) {
-            const float weight = weights[part * 16 + head];
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(part_at(part) + head * kDim + dim));
-            v[0] = fmaf(weight, x.x, v[0]);
-            v[1] = fmaf(weight, x.y, v[1]);
-            v[2] = fmaf(weight, x.z, v[2]);
-            v[3] = fmaf(weight, x.w, v[3]);
+      } else {
+        // (the ring is free where the share ends)
+        if (!ended) ptx::cp_async_wait_group<0>();
+        __syncwarp();
+        float* const part = ended ? stash : reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              *reinterpret_cast<float2*>(part + (16 * c + 8 * i + r8) * kHeads + 8 * n + 2 * q4) = make_float2(out[c][n][2 * i], out[c][n][2 * i + 1]);
+            }
           }
-          finish(head, dim, v, warp_sum[0][head]);
+          if (r8 == 0) {
+            *reinterpret_cast<float2*>(part + kDim * kHeads + 8 * n + 2 * q4) = make_float2(top[n][0], top[n][1]);
+            *reinterpret_cast<float2*>(part + (kDim + 1) * kHeads + 8 * n + 2 * q4) = make_float2(sum[n][0], sum[n][1]);
+          }
+        }
+        if (lane == 0) {
+          Part part_of = {part, at.b, at.row, row_first_lot, row_lots, true, began};
+          if (!aligned) {
+            const int32_t per_row = steps_between(at.begin, at.end);
+            const int64_t row_first = first_step + step + 1 - (per_row - at.left);
+            part_of.first_lot = static_cast<int32_t>(quotient(row_first, piece));
+            part_of.lots = static_cast<int32_t>(quotient(row_first + per_row - 1, piece)) - part_of.first_lot + 1;
+          }
+          parts[2 * warp + (ended ? 0 : 1)] = part_of;
         }
       }
+      began = false;
+      fresh = true;
+      if (step + 1 < steps) {
+        ++at.row;
+        enter(at);
+      }
     }
-    __syncthreads();  // the shared memory is free again
-    unit += steps;
+  }
+  __syncthreads();
+
+  // Joins.  First the lot's own: parts of one row are neighbours, and a part at an even place ends its row.
+  // A lot's slots: for the row that it begins inside of, for the one that it ends inside of, and for the join
+  // of kFan neighbours.
+  auto slot_of = [&](int32_t of_lot, int which) { return p.partials + (kSlots * static_cast<int64_t>(of_lot) + which) * kPartFloats; };
+  int32_t pending[2] = {0, 0}, waiting = 0;
+  for (int32_t i = 0; i < 2 * kWarps;) {
+    if (!parts[i].there) {
+      ++i;
+      continue;
+    }
+    const int32_t first = i;
+    const float* all[kWarps] = {};  // (a warp has one part of a row at most)
+    int32_t count = 0;
+    bool ended = false;
+#pragma unroll
+    for (int32_t j = 0; j < 2 * kWarps; ++j) {
+      if (j < first || ended || !parts[j].there) continue;
+      ended = j % 2 == 0;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        if (k == count) all[k] = parts[j].at;
+      }
+      ++count;
+      i = j + 1;
+    }
+    const bool began = parts[first].began, whole = ended && !began;
+    float* const to = whole ? nullptr : slot_of(lot, began ? 0 : 1);
+    if (!whole) pending[waiting++] = first;
+    const Row of(p, parts[first].b, parts[first].row);
+    Join joined;
+#pragma unroll
+    for (int j0 = 0; j0 < kWarps; j0 += Join::kBatch) {
+      const float* list[Join::kBatch] = {};
+#pragma unroll
+      for (int j = 0; j < Join::kBatch && j0 + j < kWarps; ++j) list[j] = all[j0 + j];
+      joined.add(list, count - j0);
+    }
+    joined.template give<kCodes>(p, of, to);
+  }
+  if (waiting == 0) return;
+
+  // Then with other lots' parts, by the last CTA to arrive, in the parts' order; it leaves the counts at
+  // zero.  (The barrier and the release order the parts before the count.)
+  for (; waiting > 0; --waiting) {
+    const Part part = parts[pending[waiting - 1]];
+    const bool twice = part.lots > kFan;
+    const Row of(p, part.b, part.row);
+    for (int level = twice ? 0 : 1; level < 2; ++level) {
+      const int32_t from = level == 0 ? (lot - part.first_lot) / kFan * kFan : 0, stride = level == 1 && twice ? kFan : 1;
+      const int32_t count = level == 0 ? min(kFan, part.lots - from) : (part.lots + stride - 1) / stride;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int shift = level == 1 ? kRowShift : from == 0 ? kFirstShift : kFanShift;
+        int32_t* const word = p.locks + part.first_lot + from;
+        const int32_t before = atomic_add_acq_rel(word, 1 << shift) >> shift & (level == 1 ? (1 << 11) - 1 : (1 << 6) - 1);
+        answer[level] = before == count - 1;
+        if (before == count - 1) atomicSub(word, count << shift);
+      }
+      __syncthreads();
+      if (!answer[level]) break;
+      float* const to = level == 0 ? slot_of(part.first_lot + from, 2) : nullptr;
+      Join joined;
+      for (int32_t j0 = 0; j0 < count; j0 += Join::kBatch) {
+        const float* list[Join::kBatch];
+#pragma unroll
+        for (int j = 0; j < Join::kBatch; ++j) {
+          list[j] = slot_of(part.first_lot + from + (j0 + j) * stride, stride > 1 ? 2 : from + j0 + j == 0 ? 1 : 0);
+        }
+        joined.add(list, count - j0);
+      }
+      joined.template give<kCodes>(p, of, to);
+    }
   }
 }
 
 struct Variant {
   void (*kernel)(AttentionParams);
-  int smem, unit, ctas;
+  int smem, step, ctas;
 };
 
-template <int kDim, bool kCodes, bool kWide>
+template <int kDim, bool kCodes, int kTiles>
 Variant variant() {
-  using L = Layout<kDim, kCodes>;
-  return {paged_attention_kernel<kDim, kCodes, kWide>, L::kSmem, L::kUnit, L::kCtas};
+  using L = Layout<kDim, kCodes, kTiles>;
+  return {paged_attention_kernel<kDim, kCodes, kTiles>, L::kSmem, L::kStep, L::kCtas};
 }
 
 template <int kDim>
 Variant variant_of(bool codes, bool wide) {
-  if (codes) return wide ? variant<kDim, true, true>() : variant<kDim, true, false>();
-  return wide ? variant<kDim, false, true>() : variant<kDim, false, false>();
+  if (codes) return wide ? variant<kDim, true, 2>() : variant<kDim, true, 1>();
+  return wide ? variant<kDim, false, 2>() : variant<kDim, false, 1>();
 }
 
 bool variant_for(int64_t dim, bool codes, bool wide, Variant* out) {
@@ -589,14 +900,18 @@ extern "C" {
 int chord_b200_paged_attention_lock_words(void) {
   chord::DeviceInfo device;
   if (chord::current_device_info(&device)) return -1;
-  return device.sm_count * chord::kMaxCtasPerSm;
+  const int ctas = device.sm_count * chord::kMaxCtasPerSm;
+  return ctas < chord::kMaxCtas ? ctas : chord::kMaxCtas;
 }
 
-int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim) {
-  chord::DeviceInfo device;
-  if (chord::current_device_info(&device)) return -1;
-  if (head_dim <= 0 || head_dim > 256) return chord::fail(chord::kInvalidArgument, "head_dim out of range"), -1;
-  return 2ll * device.sm_count * chord::kMaxCtasPerSm * chord::partial_floats(static_cast<int>(head_dim)) * 4;
+int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t group) {
+  using namespace chord;
+  DeviceInfo device;
+  if (current_device_info(&device)) return -1;
+  Variant v;
+  if (!variant_for(head_dim, false, group > 8, &v)) return fail(kInvalidArgument, "head_dim must be 64, 96, 128, 192 or 256"), -1;
+  const int ctas = device.sm_count * v.ctas;
+  return 4 * workspace_floats(ctas < kMaxCtas ? ctas : kMaxCtas, static_cast<int>(head_dim), group > 8 ? 16 : 8);
 }
 
 int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, const chord_b200_kv_cache* cache,
@@ -633,16 +948,17 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, c
   if (int rc = require_blackwell(device)) return rc;
   if (int rc = allow_smem(v, cache->head_dim, codes, wide, device.device)) return rc;
   const int64_t head_blocks = (group + 15) / 16;
-  // No more CTAs than there can be units of work.
+  // No more CTAs than there can be shares.
   // (token numbers, those of the steps loaded ahead too, fit 32 bits)
   int64_t capacity = max_pages * cache->page_size;
   if (capacity > (1ll << 31) - 65536) capacity = (1ll << 31) - 65536;
   const int64_t longest = window > 0 && window < capacity ? window : capacity;
-  const int64_t most = batch * cache->heads * head_blocks * ((longest + v.unit - 1) / v.unit);
+  const int64_t most = batch * cache->heads * head_blocks * (((longest + v.step - 1) / v.step + kWarps) / kWarps);
   int64_t ctas = static_cast<int64_t>(device.sm_count) * v.ctas;
+  if (ctas > kMaxCtas) ctas = kMaxCtas;
   if (ctas > most) ctas = most;
-  const int64_t need = 2 * ctas * partial_floats(static_cast<int>(cache->head_dim)) * 4;
-  CHORD_REQUIRE(num_locks >= ctas && ctas <= kMaxParts, "locks has %lld lock words, this launch needs %lld",
+  const int64_t need = 4 * workspace_floats(ctas, static_cast<int>(cache->head_dim), wide ? 16 : 8);
+  CHORD_REQUIRE(num_locks >= ctas, "locks has %lld lock words, this launch needs %lld",
                 static_cast<long long>(num_locks), static_cast<long long>(ctas));
   CHORD_REQUIRE(workspace_bytes >= need, "the workspace has %lld bytes, this launch needs %lld",
                 static_cast<long long>(workspace_bytes), static_cast<long long>(need));
@@ -663,7 +979,8 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, c
   p.group = static_cast<int32_t>(group);
   p.head_blocks = static_cast<int32_t>(head_blocks);
   p.window = static_cast<int32_t>(window);
-  p.scale = static_cast<float>(scale * 1.4426950408889634074);
+  p.scale = static_cast<float>(scale * 1.4426950408889634074 * (codes ? 0x1p53 : 1.0));
+  p.whole_groups = cache->page_size % 16 == 0 && p.cache.token < (1ll << 31);
   OptionsReadLock guard(options_mutex());
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), v.smem,
                            static_cast<cudaStream_t>(stream), options().pdl != 0, p));

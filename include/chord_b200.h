@@ -459,7 +459,8 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
  *           max_pages * page_size (more: cut, status bit 32)
  *  out      bf16 [batch, heads, head_dim];  lse fp32 [batch, heads]
  *  locks    int32, chord_b200_paged_attention_lock_words() words, zero on entry and on exit
- *  workspace  chord_b200_paged_attention_workspace_bytes(head_dim) bytes, 16-byte aligned
+ *  workspace  chord_b200_paged_attention_workspace_bytes(head_dim, heads / cache->heads) bytes,
+ *           16-byte aligned
  *  scale    finite; head_dim ^ -0.5 as a rule
  * Work is dealt out over the device by tokens, whatever the lengths; parts of a sequence are joined
  * in their order, so the same inputs give the same bits.  No kernel waits for another CTA. */
@@ -471,7 +472,7 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head,
                                int64_t batch, int64_t heads, int64_t window, double scale,
                                void* stream);
 int chord_b200_paged_attention_lock_words(void);
-int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim);
+int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t group);
 
 #ifdef __cplusplus
 }
