@@ -74,11 +74,6 @@ __device__ __forceinline__ void cp_async_16_all(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid) {
-  const uint32_t bytes = valid ? 4u : 0u;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 // What a warp has of a row that does not lie in its share alone.
 struct Part {
   float* at;

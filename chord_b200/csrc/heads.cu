@@ -20,9 +20,10 @@ struct HeadsParams {
   const int32_t* slots;
   int32_t* status;
   Cache cache;
-  int64_t items;
-  int32_t q_heads, k_heads, v_heads, dim, rotary, max_positions, items_per_token;
-  float eps;
+  int32_t items, q_heads, k_heads, v_heads, dim, rotary, max_positions;
+  int32_t q_items, k_items;  // items of a token: its queries', keys' and
+  Divisor items_per_token;   // all
+  float eps, share;          // share: 1 / dim
   bool interleaved;
 };
 
@@ -39,35 +40,59 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
 }
 
-// Eight codes round(x / scale) + 128 of a row whose largest |x| is `top`, scale = top / 127.
-__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float top) {
-  // (rows below 2^-100 are taken times 2^100, so that 127 / top stays finite)
-  const float lift = top < 0x1p-100f ? 0x1p100f : 1.0f;
-  const float rate = top > 0.0f ? 127.0f / (top * lift) : 0.0f;
-  uint32_t w[2] = {0, 0};
+// The larger magnitude; a NaN where there is one.
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return c;
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// Eight codes round(x / scale) + 128 of a row whose largest |x| is `top`, scale = top / 127.  Adding 1.5 * 2^23
+// + 128 rounds to a whole number and leaves the code in the sum's low byte.
+__device__ __forceinline__ uint2 quantise8(float (&x)[8], float top) {
+  if (top < 0x1p-100f) {  // (127 / top has to stay finite)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t code = static_cast<uint32_t>(__float2int_rn(x[i] * lift * rate) + 128);
-    w[i / 4] |= (code & 0xFFu) << (8 * (i % 4));
+    for (int i = 0; i < 8; ++i) x[i] *= 0x1p100f;
+    top *= 0x1p100f;
   }
-  return make_uint2(w[0], w[1]);
+  const float rate = top > 0.0f ? __fdividef(127.0f, top) : 0.0f;
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(fmaf(x[i], rate, 12583040.0f));
+  return make_uint2(low_bytes(w[0], w[1], w[2], w[3]), low_bytes(w[4], w[5], w[6], w[7]));
 }
 
 // kLanes lanes hold a row of up to 8 kLanes elements, 16 bytes each, so a warp works on 32 / kLanes
 // rows at a time and on kRows of those sets, whose loads are all in flight at once.  An item is the
-// rows of a warp; all belong to one token, so the angles are read once.  Everything between the load
-// and the store is FP32; the result is rounded once, to BF16 or to the codes.
+// rows of a warp: rows of one token, all queries, keys or values.  What an item's rows have in common is
+// worked out once: with x' the element that x turns with, a result is rate * (A x + B x'), where A and B
+// hold the norm's weights and the angles, and x' comes from its lane as the bits that were loaded.
+// Everything between the load and the store is FP32; the result is rounded once, to BF16 or to the codes.
 template <int kLanes, int kRows, bool kRotate, bool kWrite>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 heads_kernel(const HeadsParams p) {
   constexpr int kSide = 32 / kLanes;
   const int lane = threadIdx.x & 31, chunk = lane % kLanes, side = lane / kLanes;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (item >= p.items) return;
-  const int32_t token = static_cast<int32_t>(item / p.items_per_token);
-  const int32_t first = static_cast<int32_t>(item % p.items_per_token) * (kSide * kRows) + side;
-  const int32_t rows = p.q_heads + p.k_heads + p.v_heads;
+  const int32_t token = p.items_per_token.div(item);
+  int32_t group = item - token * p.items_per_token.d;
+  // Which of the three, and the first of the item's rows.
+  const bool is_q = kRotate && group < p.q_items;
+  if (!is_q) group -= p.q_items;
+  const bool is_v = kWrite && !is_q && group >= p.k_items;
+  if (is_v) group -= p.k_items;
+  const int32_t rows = is_q ? p.q_heads : p.k_heads;
+  const int32_t first = group * (kSide * kRows) + side;
   const bool inside = 8 * chunk < p.dim;
+  const __nv_bfloat16* from = (is_q ? p.q + token * p.q_token : is_v ? p.v + token * p.v_token : p.k + token * p.k_token) + 8 * chunk;
+  const int64_t stride = is_q ? p.q_head : is_v ? p.v_head : p.k_head;
+  from += first * stride;
   ptx::grid_dependency_wait();
 
   // (the results may take the inputs' place)
@@ -75,62 +100,59 @@ heads_kernel(const HeadsParams p) {
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int32_t row = first + i * kSide;
-    const __nv_bfloat16* at = p.q + token * p.q_token + row * p.q_head;
-    if (row >= p.q_heads) at = p.k + token * p.k_token + (row - p.q_heads) * p.k_head;
-    if (kWrite && row >= p.q_heads + p.k_heads) at = p.v + token * p.v_token + (row - p.q_heads - p.k_heads) * p.v_head;
-    raw[i] = row < rows && inside ? load_once_coherent(at + 8 * chunk) : make_uint4(0, 0, 0, 0);
+    raw[i] = row < rows && inside ? load_once_coherent(from) : make_uint4(0, 0, 0, 0);
+    from += kSide * stride;
   }
 
-  float cos[8], sin[8];
-  bool turned = false, lost = false;
+  float own[8], other[8];  // A, B
   int partner = lane;
-  float sign = 0.0f;
-  uint4 q_weight, k_weight;
+  bool lost = false;
   if constexpr (kRotate) {
-    q_weight = k_weight = make_uint4(0, 0, 0, 0);
-    if (inside) {
-      q_weight = __ldg(reinterpret_cast<const uint4*>(p.q_weight) + chunk);
-      k_weight = __ldg(reinterpret_cast<const uint4*>(p.k_weight) + chunk);
-    }
-    const int32_t position = __ldg(p.positions + token);
-    lost = position < 0 || position >= p.max_positions;
-    if (lost && p.status != nullptr && lane == 0) atomicOr(p.status, kStatusIndex);
-    turned = 8 * chunk < p.rotary && !lost;
-    const int32_t half = p.rotary / 2;
-    const bool upper = 8 * chunk >= half;
+    if (!is_v) {
+      const uint4* const weight = reinterpret_cast<const uint4*>(is_q ? p.q_weight : p.k_weight);
+      const int32_t position = __ldg(p.positions + token), half = p.rotary / 2;
+      lost = position < 0 || position >= p.max_positions;
+      if (lost && p.status != nullptr && lane == 0) atomicOr(p.status, kStatusIndex);
+      const bool turned = 8 * chunk < p.rotary, upper = 8 * chunk >= half;
+      float w[8];
+      unpack8(inside ? __ldg(weight + chunk) : make_uint4(0, 0, 0, 0), w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cos[i] = 1.0f, sin[i] = 0.0f;
-    if (turned) {
-      const float* at = p.cos_sin + static_cast<int64_t>(position) * p.rotary +
-                        (p.interleaved ? 4 * chunk : 8 * chunk - (upper ? half : 0));
-      float4 c[2], s[2];
-      c[0] = __ldg(reinterpret_cast<const float4*>(at));
-      s[0] = __ldg(reinterpret_cast<const float4*>(at + half));
-      c[1] = c[0];
-      s[1] = s[0];
-      if (!p.interleaved) {
-        c[1] = __ldg(reinterpret_cast<const float4*>(at) + 1);
-        s[1] = __ldg(reinterpret_cast<const float4*>(at + half) + 1);
-        partner = upper ? lane - half / 8 : lane + half / 8;
-        sign = upper ? 1.0f : -1.0f;
-      }
+      for (int j = 0; j < 8; ++j) own[j] = w[j], other[j] = 0.0f;
+      if (turned && !lost) {
+        const float* const at = p.cos_sin + static_cast<int64_t>(position) * p.rotary + (p.interleaved ? 4 * chunk : 8 * chunk - (upper ? half : 0));
+        const float4 c0 = __ldg(reinterpret_cast<const float4*>(at)), s0 = __ldg(reinterpret_cast<const float4*>(at + half));
+        if (p.interleaved) {
+          const float c[4] = {c0.x, c0.y, c0.z, c0.w}, s[4] = {s0.x, s0.y, s0.z, s0.w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        cos[4 * i] = c[i].x, cos[4 * i + 1] = c[i].y, cos[4 * i + 2] = c[i].z, cos[4 * i + 3] = c[i].w;
-        sin[4 * i] = s[i].x, sin[4 * i + 1] = s[i].y, sin[4 * i + 2] = s[i].z, sin[4 * i + 3] = s[i].w;
+          for (int j = 0; j < 4; ++j) {
+            own[2 * j] *= c[j], own[2 * j + 1] *= c[j];
+            other[2 * j] = -s[j] * w[2 * j + 1], other[2 * j + 1] = s[j] * w[2 * j];
+          }
+        } else {
+          const float4 c1 = __ldg(reinterpret_cast<const float4*>(at) + 1), s1 = __ldg(reinterpret_cast<const float4*>(at + half) + 1);
+          const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+          const int away = upper ? -half / 8 : half / 8;
+          partner = lane + away;
+          unpack8(__ldg(weight + chunk + away), w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            own[j] *= c[j];
+            other[j] = (upper ? s[j] : -s[j]) * w[j];
+          }
+        }
       }
     }
   }
   int64_t page_offset = -1, scale_offset = 0;
   if constexpr (kWrite) {
-    const int32_t slot = __ldg(p.slots + token);
-    if (slot >= 0) {
-      const uint32_t page = p.cache.page_size.div(static_cast<uint32_t>(slot));
+    if (!is_q) {
+      const int32_t slot = __ldg(p.slots + token);
+      const uint32_t page = slot >= 0 ? p.cache.page_size.div(static_cast<uint32_t>(slot)) : 0;
       const uint32_t in_page = static_cast<uint32_t>(slot) - page * p.cache.page_size.d;
-      if (page < static_cast<uint32_t>(p.cache.num_pages)) {
+      if (slot >= 0 && page < static_cast<uint32_t>(p.cache.num_pages)) {
         page_offset = page * p.cache.page + in_page * p.cache.token;
         scale_offset = page * p.cache.scale_page + in_page * p.cache.scale_token;
-      } else if (p.status != nullptr && lane == 0) {
+      } else if (slot >= 0 && p.status != nullptr && lane == 0) {
         atomicOr(p.status, kStatusIndex);
       }
     }
@@ -140,66 +162,52 @@ heads_kernel(const HeadsParams p) {
   for (int i = 0; i < kRows; ++i) {
     const int32_t row = first + i * kSide;
     if (row - side >= rows) break;  // (the whole warp)
+    const bool mine = row < rows && inside;
     float x[8];
     unpack8(raw[i], x);
-    const bool is_q = row < p.q_heads, is_v = kWrite && row >= p.q_heads + p.k_heads;
-    if constexpr (kRotate) {
+    if (kRotate && !is_v) {
       float square = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) square = fmaf(x[j], x[j], square);
 #pragma unroll
       for (int d = kLanes / 2; d > 0; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
-      const float rate = rsqrtf(square / static_cast<float>(p.dim) + p.eps);
-      float w[8], y[8];
-      unpack8(is_q ? q_weight : k_weight, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = x[j] * rate * w[j];
+      const float rate = rsqrtf(fmaf(square, p.share, p.eps));
+      uint4 turn = raw[i];
       if (p.interleaved) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = y[2 * j], b = y[2 * j + 1];
-          y[2 * j] = a * cos[j] - b * sin[j];
-          y[2 * j + 1] = b * cos[j] + a * sin[j];
-        }
+        turn.x = __byte_perm(turn.x, 0, 0x1032);
+        turn.y = __byte_perm(turn.y, 0, 0x1032);
+        turn.z = __byte_perm(turn.z, 0, 0x1032);
+        turn.w = __byte_perm(turn.w, 0, 0x1032);
       } else {
+        turn.x = __shfl_sync(0xffffffffu, turn.x, partner);
+        turn.y = __shfl_sync(0xffffffffu, turn.y, partner);
+        turn.z = __shfl_sync(0xffffffffu, turn.z, partner);
+        turn.w = __shfl_sync(0xffffffffu, turn.w, partner);
+      }
+      float y[8];
+      unpack8(turn, y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float other = __shfl_sync(0xffffffffu, y[j], partner);
-          y[j] = turned ? y[j] * cos[j] + sign * other * sin[j] : y[j];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = is_v ? x[j] : lost ? 0.0f : y[j];
+      for (int j = 0; j < 8; ++j) x[j] = lost ? 0.0f : rate * fmaf(x[j], own[j], y[j] * other[j]);
     }
-    if (kRotate && is_q) {
-      if (inside) {
-        *reinterpret_cast<uint4*>(p.q_out + (static_cast<int64_t>(token) * p.q_heads + row) * p.dim + 8 * chunk) = pack8(x);
-      }
-    }
-    if constexpr (!kWrite) {
-      if (!is_q && row < rows && inside) {
-        const int32_t head = row - p.q_heads;
-        *reinterpret_cast<uint4*>(p.k_out + (static_cast<int64_t>(token) * p.k_heads + head) * p.dim + 8 * chunk) = pack8(x);
-      }
-    } else {
-      const int32_t head = row - p.q_heads - (is_v ? p.k_heads : 0);
-      const bool keep = !is_q && row < rows && inside && page_offset >= 0;
-      uint8_t* at = (is_v ? p.cache.v : p.cache.k) + page_offset + head * p.cache.head;
+    if (is_q || !kWrite) {
+      __nv_bfloat16* const to = is_q ? p.q_out : p.k_out;
+      if (mine) *reinterpret_cast<uint4*>(to + (static_cast<int64_t>(token) * rows + row) * p.dim + 8 * chunk) = pack8(x);
+    } else if constexpr (kWrite) {
+      const bool keep = mine && page_offset >= 0;
+      uint8_t* const at = (is_v ? p.cache.v : p.cache.k) + page_offset + row * p.cache.head;
       if (p.cache.k_scale == nullptr) {
-        if (keep) *reinterpret_cast<uint4*>(at + 16 * chunk) = pack8(x);
+        if (keep) *reinterpret_cast<uint4*>(at + 16 * chunk) = kRotate && !is_v ? pack8(x) : raw[i];
       } else {
-        // The largest |x| by its bits: infinities and NaNs come out on top, and such a row gets a scale
-        // of NaN, so that it reads back as NaN.
-        uint32_t bits = 0;
+        float top = max_magnitude(max_magnitude(max_magnitude(x[0], x[1]), max_magnitude(x[2], x[3])),
+                                  max_magnitude(max_magnitude(x[4], x[5]), max_magnitude(x[6], x[7])));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-#pragma unroll
-        for (int d = kLanes / 2; d > 0; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
-        const bool finite = bits < 0x7F800000u;
-        const float top = __uint_as_float(finite ? bits : 0x7FC00000u);
+        for (int d = kLanes / 2; d > 0; d >>= 1) top = max_magnitude(top, __shfl_xor_sync(0xffffffffu, top, d));
+        // A row with an infinity or a NaN gets a scale of NaN, so that it reads back as NaN.
+        const bool finite = top < INFINITY;
         if (keep) {
+          const float scale = finite ? top * (1.0f / 127.0f) : __uint_as_float(0x7FC00000u);
           *reinterpret_cast<uint2*>(at + 8 * chunk) = finite ? quantise8(x, top) : make_uint2(0x80808080u, 0x80808080u);
-          if (chunk == 0) (is_v ? p.cache.v_scale : p.cache.k_scale)[scale_offset + head * p.cache.scale_head] = top / 127.0f;
+          if (chunk == 0) (is_v ? p.cache.v_scale : p.cache.k_scale)[scale_offset + row * p.cache.scale_head] = scale;
         }
       }
     }
@@ -212,20 +220,21 @@ struct ReadParams {
   const int32_t* offsets;
   __nv_bfloat16 *k_out, *v_out;  // [total, heads, dim]
   int32_t* status;
-  int64_t table_stride, items;
-  int32_t batch, max_pages, total, dim, items_per_token;
+  int64_t table_stride;
+  int32_t items, batch, max_pages, total, dim;
+  Divisor items_per_token;
 };
 
 // As heads_kernel: a warp reads rows of one token, its keys' heads and then its values'.
 template <int kLanes, int kRows>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 cache_read_kernel(const ReadParams p) {
   constexpr int kSide = 32 / kLanes;
   const int lane = threadIdx.x & 31, chunk = lane % kLanes, side = lane / kLanes;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (item >= p.items) return;
-  const int32_t token = static_cast<int32_t>(item / p.items_per_token);
-  const int32_t first = static_cast<int32_t>(item % p.items_per_token) * (kSide * kRows) + side;
+  const int32_t token = p.items_per_token.div(item);
+  const int32_t first = (item - token * static_cast<int32_t>(p.items_per_token.d)) * (kSide * kRows) + side;
   const int32_t rows = 2 * p.cache.heads;
   ptx::grid_dependency_wait();
 
@@ -281,13 +290,13 @@ cache_read_kernel(const ReadParams p) {
     const int32_t head = is_v ? row - p.cache.heads : row;
     uint4 value = raw[i];
     if (p.cache.k_scale != nullptr) {
+      // (a byte as the low one of 2^23 + 128 + it)
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t code = ((j < 4 ? raw[i].x : raw[i].y) >> (8 * (j % 4))) & 0xFFu;
-        x[j] = page_offset < 0 ? 0.0f : static_cast<float>(static_cast<int32_t>(code) - 128) * scale[i];
+        x[j] = (__uint_as_float(__byte_perm(j < 4 ? raw[i].x : raw[i].y, 0x4B000000u, 0x7440 | j % 4)) - 8388736.0f) * scale[i];
       }
-      value = pack8(x);
+      value = page_offset < 0 ? make_uint4(0, 0, 0, 0) : pack8(x);
     }
     *reinterpret_cast<uint4*>((is_v ? p.v_out : p.k_out) + (static_cast<int64_t>(token) * p.cache.heads + head) * p.dim + 8 * chunk) = value;
   }
@@ -309,14 +318,19 @@ int launch_heads(HeadsParams p, int64_t tokens, cudaStream_t stream) {
   const int64_t rows = p.q_heads + p.k_heads + p.v_heads;
   const bool wide = many(tokens, rows, lanes, device.sm_count);
   const int64_t per_item = 32 / lanes * (wide ? 4 : 1);
-  p.items_per_token = static_cast<int32_t>((rows + per_item - 1) / per_item);
-  p.items = tokens * p.items_per_token;
+  const auto items = [&](int32_t heads) { return static_cast<int32_t>((heads + per_item - 1) / per_item); };
+  p.q_items = items(p.q_heads);
+  p.k_items = items(p.k_heads);
+  const int64_t of_token = p.q_items + p.k_items + items(p.v_heads);
+  CHORD_REQUIRE(tokens * of_token < (1ll << 31), "too many rows");
+  p.items_per_token = Divisor(static_cast<uint32_t>(of_token));
+  p.items = static_cast<int32_t>(tokens * of_token);
+  p.share = 1.0f / static_cast<float>(p.dim);
   using Fn = void (*)(HeadsParams);
   static const Fn kernels[3][2] = {{heads_kernel<8, 1, kRotate, kWrite>, heads_kernel<8, 4, kRotate, kWrite>},
                                    {heads_kernel<16, 1, kRotate, kWrite>, heads_kernel<16, 4, kRotate, kWrite>},
                                    {heads_kernel<32, 1, kRotate, kWrite>, heads_kernel<32, 4, kRotate, kWrite>}};
-  const int64_t blocks = (p.items + 7) / 8;
-  CHORD_REQUIRE(blocks < (1ll << 31), "too many rows");
+  const int64_t blocks = (p.items + 7ll) / 8;
   OptionsReadLock guard(options_mutex());
   CHORD_CUDA(launch_kernel(kernels[lanes / 16][wide], dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
                            options().pdl != 0, p));
@@ -468,14 +482,15 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
   const int64_t rows = 2 * cache->heads;
   const bool wide = many(total, rows, lanes, device.sm_count);
   const int64_t per_item = 32 / lanes * (wide ? 4 : 1);
-  p.items_per_token = static_cast<int32_t>((rows + per_item - 1) / per_item);
-  p.items = total * p.items_per_token;
+  const int64_t of_token = (rows + per_item - 1) / per_item;
+  CHORD_REQUIRE(total * of_token < (1ll << 31), "too many rows");
+  p.items_per_token = Divisor(static_cast<uint32_t>(of_token));
+  p.items = static_cast<int32_t>(total * of_token);
   using Fn = void (*)(ReadParams);
   static const Fn kernels[3][2] = {{cache_read_kernel<8, 1>, cache_read_kernel<8, 4>},
                                    {cache_read_kernel<16, 1>, cache_read_kernel<16, 4>},
                                    {cache_read_kernel<32, 1>, cache_read_kernel<32, 4>}};
-  const int64_t blocks = (p.items + 7) / 8;
-  CHORD_REQUIRE(blocks < (1ll << 31), "too many rows");
+  const int64_t blocks = (p.items + 7ll) / 8;
   OptionsReadLock guard(options_mutex());
   CHORD_CUDA(launch_kernel(kernels[lanes / 16][wide], dim3(static_cast<unsigned>(blocks)), dim3(256), 0,
                            static_cast<cudaStream_t>(stream), options().pdl != 0, p));

@@ -53,6 +53,18 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
   return v;
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four bytes to shared memory, zeros where there are none.
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, bool valid) {
+  const uint32_t bytes = valid ? 4u : 0u;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 // Four 8x8 matrices of 16-bit elements, each transposed: lane l receives, of matrix i, rows
 // 2 (l % 4) and 2 (l % 4) + 1 of column l / 4 in r[i].
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
