@@ -22,6 +22,11 @@ try:  # built next to the library where Python's headers are installed
 except ImportError:
     _call = None
 
+try:  # the same, where torch's headers are
+    from . import _torch_call
+except ImportError:
+    _torch_call = None
+
 _LIB = None
 _NATIVE = None
 _LIB_PATH = Path(__file__).resolve().parent / "libchord_b200.so"
@@ -143,6 +148,19 @@ def native():
             functions[name] = fn
         _NATIVE = SimpleNamespace(**functions)
     return _NATIVE
+
+
+@functools.lru_cache(maxsize=1)
+def direct():
+    """The ``_torch_call`` module with the library's entry points, or None where it was not built.  Its
+    functions answer None to a call that they leave to the wrapper."""
+    if _torch_call is None:
+        return None
+    names = ("gemv", "qk_norm_rope", "qk_norm_rope_write", "cache_write", "cache_read", "paged_attention",
+             "paged_attention_workspace_bytes")
+    lib = load()
+    known = _torch_call.entries(*(ctypes.cast(getattr(lib, "chord_b200_" + name), ctypes.c_void_p).value for name in names))
+    return _torch_call if known else None
 
 
 def _apply_env_options(lib: ctypes.CDLL) -> None:

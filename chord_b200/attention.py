@@ -27,7 +27,7 @@ class KVCache:
     ``head_dim`` is a multiple of 16 up to 256.  :func:`kv_cache` allocates one."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "num_pages", "heads", "page_size", "head_dim", "device", "address",
-                 "_descriptor")
+                 "index", "scale", "_descriptor")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
@@ -57,7 +57,7 @@ class KVCache:
             scale_strides = k_scale.stride()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.heads, self.page_size, self.head_dim = num_pages, heads, page_size, head_dim
-        self.device = k.device
+        self.device, self.index, self.scale = k.device, _device_index(k.device), head_dim ** -0.5
         self._descriptor = _lib.KVCacheDescriptor(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if coded else None, v_scale.data_ptr() if coded else None,
             num_pages, page_size, heads, head_dim, *k.stride()[:3], *scale_strides)
@@ -179,6 +179,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     ``positions`` is int32 ``[tokens]``; a position outside the table gives zeros and is reported by
     :func:`chord_b200.check_status`.  Returns BF16 ``(q_out, k_out)``, contiguous; contiguous inputs may be
     given as their own outputs."""
+    direct = _lib.direct()
+    if direct is not None and q_out is None and k_out is None:
+        result = direct.qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved)
+        if result is not None:
+            return result
     device, tokens, heads, dim, q_rows, k_rows, rest = _rotation(q, k, q_weight, k_weight, cos_sin, positions, eps,
                                                                  interleaved, None)
     q_out = _bf16_like("q_out", q_out, q.shape, device)
@@ -198,6 +203,12 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
     ``t`` at slot ``slots[t]`` (int32, page * page_size + place; negative: not kept).  Keys are
     quantised from FP32.  Returns the queries."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None and q_out is None:
+        result = direct.qk_norm_rope_write(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, v,
+                                           cache.address, cache.index, slots)
+        if result is not None:
+            return result
     device, tokens, heads, dim, q_rows, k_rows, rest = _rotation(q, k, q_weight, k_weight, cos_sin, positions, eps,
                                                                  interleaved, cache.heads)
     if dim != cache.head_dim or device != cache.device:
@@ -218,6 +229,9 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, cache: KVCache, slots: torch.T
     not written and is reported by :func:`chord_b200.check_status`.  A row that holds an infinity or a
     NaN reads back as NaN from an 8-bit cache."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None and direct.cache_write(k, v, cache.address, cache.index, slots):
+        return
     device = cache.device
     if not isinstance(k, torch.Tensor) or k.ndim != 3:
         raise TypeError("k must be a 3D torch.bfloat16 tensor")
@@ -239,6 +253,11 @@ def cache_read(cache: KVCache, block_tables: torch.Tensor, offsets: torch.Tensor
     never falls; rows of no sequence are zeros, as are tokens whose page the table or the cache does
     not have, which :func:`chord_b200.check_status` reports."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None and k_out is None and v_out is None:
+        result = direct.cache_read(cache.address, cache.index, block_tables, offsets, total)
+        if result is not None:
+            return result
     device = cache.device
     _checks.supported_gpu(device)
     _checks.integer("total", total, minimum=0)
@@ -287,6 +306,12 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     int32, left zeroed, one buffer per launches that may overlap; with ``None`` a per-stream buffer of
     the library's.  The same inputs give the same bits."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None and outputs is None and locks is None and window != 0:
+        result = direct.paged_attention(q, cache.address, cache.index, block_tables, lengths, lse,
+                                        0 if window is None else window, cache.scale if scale is None else scale)
+        if result is not None:
+            return result
     if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype is not torch.bfloat16:
         raise TypeError("q must be a 3D torch.bfloat16 tensor")
     device, dim = cache.device, cache.head_dim

@@ -9,6 +9,7 @@ once, in-tree, and linked into one C-ABI shared library.  Run as
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -32,13 +33,14 @@ def _nvcc() -> str:
 
 
 def _newest_source_mtime() -> float:
-    files = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list(CSRC.glob("*.c"))
+    files = [f for kind in ("cu", "cuh", "h", "c") for f in CSRC.glob("*." + kind)]
     files.append(PACKAGE_DIR.parent / "include" / "chord_b200.h")
     return max(f.stat().st_mtime for f in files if f.exists())
 
 
 def is_fresh() -> bool:
-    return LIB_PATH.exists() and LIB_PATH.stat().st_mtime >= _newest_source_mtime() and _call_module_is_fresh()
+    return (LIB_PATH.exists() and LIB_PATH.stat().st_mtime >= _newest_source_mtime() and _call_module_is_fresh()
+            and _torch_module_is_fresh())
 
 
 def _call_module_path() -> Path:
@@ -93,6 +95,55 @@ def _build_call_module() -> None:
     warnings.warn(f"chord_b200._call was not built, calls go through ctypes (some 4 us each): {reason}")
 
 
+def _torch_module_path() -> Path:
+    return PACKAGE_DIR / ("_torch_call" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def _torch_compiler() -> list[str] | None:
+    """What compiles the `_torch_call` module, without its source and output, or None where that
+    cannot be done here."""
+    spec = importlib.util.find_spec("torch")
+    gxx = shutil.which(os.environ.get("CXX", "g++"))
+    if spec is None or spec.origin is None or gxx is None:
+        return None
+    torch = Path(spec.origin).parent
+    cuda = Path(_nvcc()).resolve().parents[1] / "include"
+    headers = [Path(sysconfig.get_paths()["include"]), torch / "include", torch / "include/torch/csrc/api/include", cuda]
+    if not all((headers[i] / name).exists() for i, name in ((0, "Python.h"), (1, "ATen/cuda/EmptyTensor.h"),
+                                                            (3, "cuda_runtime_api.h"))):
+        return None
+    libraries = ["torch_python", "torch_cuda", "torch_cpu", "c10_cuda", "c10"]
+    return [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{h}" for h in headers), f"-L{torch / 'lib'}",
+            *(f"-l{name}" for name in libraries)]
+
+
+def _torch_module_is_fresh() -> bool:
+    """Up to date, or not to be had here (the wrappers then do all of it in Python)."""
+    path = _torch_module_path()
+    if path.exists():
+        sources = (CSRC / "torch_call.cpp", PACKAGE_DIR.parent / "include" / "chord_b200.h")
+        return path.stat().st_mtime >= max(f.stat().st_mtime for f in sources)
+    return _torch_compiler() is None
+
+
+def _build_torch_module() -> None:
+    """The optional ``_torch_call`` extension module (csrc/torch_call.cpp): short ways through the
+    wrappers of the operators that are called once per layer and token."""
+    out = _torch_module_path()
+    compiler = _torch_compiler()
+    reason = "no C++ compiler or no headers of Python, torch and CUDA"
+    if compiler is not None:
+        tmp = out.with_suffix(".tmp")
+        proc = subprocess.run([*compiler[:5], str(CSRC / "torch_call.cpp"), "-o", str(tmp), *compiler[5:]],
+                              capture_output=True, text=True)
+        if proc.returncode == 0:
+            os.replace(tmp, out)
+            return
+        reason = proc.stderr
+    out.unlink(missing_ok=True)  # not one of another version
+    warnings.warn(f"chord_b200._torch_call was not built, the wrappers take 5 to 20 us longer: {reason}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the CUDA sources for sm_100a and link ``libchord_b200.so`` in-tree."""
     if not force and is_fresh():
@@ -100,8 +151,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     nvcc = _nvcc()
     obj_dir = PACKAGE_DIR / "build"
     obj_dir.mkdir(exist_ok=True)
-    with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as pool:
+        torch_module = pool.submit(_build_torch_module)
         objs = list(pool.map(lambda s: _compile(nvcc, s, obj_dir, verbose), SOURCES))
+        torch_module.result()
     _build_call_module()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objs)]

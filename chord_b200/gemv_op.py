@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from . import _checks, _lib
+from .indexed_gemm import status_word
 from .packing import PreparedWeight
 
 MAX_ROWS = 16           # rows that share one weight
@@ -31,6 +32,12 @@ def gemv(x: torch.Tensor, weight: PreparedWeight, *, expert_ids: torch.Tensor | 
     The rows of ``x`` may be a view with a row stride.  Weights are ``(code - 8) * scale`` without a
     rounding to BF16; sums are FP32, the result is rounded once.
     """
+    direct = _lib.direct()
+    if direct is not None and outputs is None and type(weight) is PreparedWeight:
+        result = direct.gemv(x, weight.packed, weight.scale, weight.n, weight.k, weight.num_experts, expert_ids, top_k,
+                             expert_base)
+        if result is not None:
+            return result
     if not isinstance(x, torch.Tensor) or x.ndim != 2 or x.dtype != torch.bfloat16:
         raise TypeError("x must be a 2D torch.bfloat16 tensor")
     if not x.is_cuda:
@@ -69,6 +76,7 @@ def gemv(x: torch.Tensor, weight: PreparedWeight, *, expert_ids: torch.Tensor | 
         _checks.bf16_output(outputs, (rows, shape_n), device, exact_shape=True)
     if rows == 0:
         return outputs
+    status_word(device)  # (the short way above goes to devices that have one)
     with _lib.on_device(device):
         _lib.check(_lib.native().chord_b200_gemv(
             x.data_ptr(), stride, packed.data_ptr(), scale.data_ptr(), ids, outputs.data_ptr(), rows, shape_n,

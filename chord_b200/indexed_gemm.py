@@ -46,6 +46,8 @@ def status_word(device: torch.device) -> torch.Tensor:
         _refuse_allocation_in_capture(device, "the status word")
         word = torch.zeros(1, dtype=torch.int32, device=device)
         _STATUS[index] = word
+        if _lib.direct() is not None:
+            _lib.direct().device(index, word.data_ptr())
     return word
 
 
@@ -77,6 +79,8 @@ def default_locks(device: torch.device) -> torch.Tensor:
         _refuse_allocation_in_capture(device, "the default locks buffer (locks=None)")
         locks = torch.zeros(1024, dtype=torch.int32, device=device)
         _DEFAULT_LOCKS[key] = locks
+        if _lib.direct() is not None:
+            _lib.direct().locks(*key, locks.data_ptr(), locks.numel())
     return locks
 
 
