@@ -15,9 +15,11 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCtasPerSm = 3;
 constexpr int kMaxCtas = 480;      // of a launch: three on each of 160 SMs
-constexpr int kFan = 48;           // parts of a row that are joined at once
-// A lot's lock word: arrivals of its row's CTAs (11 bits), of the first kFan of them, and of the kFan
-// neighbours that the lot is the first of (6 bits each).
+// Parts of a row that one CTA joins at once: up to kAtOnce of them; more than that by groups of half as many
+// neighbours or, where that would leave more than as many groups, of kFan.
+constexpr int kAtOnce = 16, kFan = 24;
+// A lot's lock word: arrivals of its row's CTAs or groups (11 bits), of its row's first group, and of the
+// group that the lot is the first of (6 bits each).
 constexpr int kRowShift = 0, kFirstShift = 11, kFanShift = 17;
 static_assert(kMaxCtas < (1 << 11) && kFan < (1 << 6), "the fields' widths");
 
@@ -154,13 +156,11 @@ struct Row {
 };
 
 // A thread's values while a row's parts are joined: four heads' values of kItems dims, with the heads'
-// maxima and sums.  Every thread keeps its own, so that nothing but the parts themselves is waited for,
-// once for kBatch of them: a round trip to what other SMs have just written takes 1.1 us.
+// maxima and sums.
 template <int kDim, int kHeads>
 struct Joined {
   static constexpr int kQuads = kHeads / 4;
   static constexpr int kItems = (kDim * kQuads + kThreads - 1) / kThreads;  // (dims, kThreads / kQuads apart)
-  static constexpr int kBatch = kItems <= 2 ? 8 : kItems == 3 ? 6 : kItems == 4 ? 4 : 2;
   static constexpr bool kWhole = kDim * kQuads % kThreads == 0;  // every thread has all its items
   static __device__ __forceinline__ bool mine(int i) { return kWhole || threadIdx.x + i * kThreads < kDim * kQuads; }
   float4 value[kItems], top, sum;
@@ -170,46 +170,21 @@ struct Joined {
     sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     top = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
   }
-  // The first `count` of kBatch parts; all are read before any is used.
-  __device__ __forceinline__ void add(const float* const (&list)[kBatch], int32_t count) {
-    float4 m[kBatch], l[kBatch], v[kBatch][kItems];
+  __device__ __forceinline__ void add(const float* from) {
+    const int32_t quad = threadIdx.x % kQuads * 4;
+    const float4 m = read_part4(from + kDim * kHeads + quad), l = read_part4(from + (kDim + 1) * kHeads + quad);
+    float4 v[kItems];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      m[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      l[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) v[j][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (j < count) {
-        const float* const from = list[j] + threadIdx.x % kQuads * 4;
-        m[j] = read_part4(from + kDim * kHeads);
-        l[j] = read_part4(from + (kDim + 1) * kHeads);
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-          if (mine(i)) v[j][i] = read_part4(list[j] + 4 * (threadIdx.x + i * kThreads));
-        }
-      }
-    }
-    float4 next = top;
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      next.x = fmaxf(next.x, m[j].x);
-      next.y = fmaxf(next.y, m[j].y);
-      next.z = fmaxf(next.z, m[j].z);
-      next.w = fmaxf(next.w, m[j].w);
-    }
-    const float4 old = factors(top, next);
+    for (int i = 0; i < kItems; ++i) v[i] = mine(i) ? read_part4(from + 4 * (threadIdx.x + i * kThreads)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 next = make_float4(fmaxf(top.x, m.x), fmaxf(top.y, m.y), fmaxf(top.z, m.z), fmaxf(top.w, m.w));
+    const float4 old = factors(top, next), weight = factors(m, next);
+    top = next;
     sum = make_float4(sum.x * old.x, sum.y * old.y, sum.z * old.z, sum.w * old.w);
+    add_weighted(sum, weight, l);
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       value[i] = make_float4(value[i].x * old.x, value[i].y * old.y, value[i].z * old.z, value[i].w * old.w);
-    }
-    top = next;
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const float4 weight = factors(m[j], top);
-      add_weighted(sum, weight, l[j]);
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) add_weighted(value[i], weight, v[j][i]);
+      add_weighted(value[i], weight, v[i]);
     }
   }
   static __device__ __forceinline__ float factor(float from, float to) { return to == -INFINITY ? 0.0f : exp2_approx(from - to); }
@@ -236,6 +211,82 @@ struct Joined {
     }
   }
 };
+
+// Joins `count` (at most kFan) parts that other CTAs have written, source(j) the j-th of them, into a part or
+// the results.  What they hold comes into shared memory by cp.async, all of it at once where there is room;
+// the weights are worked out while the values are on their way, by every warp for itself.
+template <int kDim, bool kCodes, int kHeads, int kSmem, typename Source>
+__device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& of, uint8_t* smem, int32_t count, float* to, Source source) {
+  using Join = Joined<kDim, kHeads>;
+  constexpr int kStats = 2 * kHeads * 4, kValues = kDim * kHeads * 4;  // bytes of a part
+  constexpr int kRound = (kSmem - kFan * (kStats + kHeads * 4) - 2 * kHeads * 4) / kValues;
+  static_assert(kRound >= 4 && kValues % 512 == 0, "room for some parts; whole pieces for a warp");
+  float* const stats = reinterpret_cast<float*>(smem);           // [count][maxima, sums][heads]
+  float* const weights = stats + kFan * 2 * kHeads;              // [count][heads]
+  float* const result = weights + kFan * kHeads;                 // maxima, sums
+  float* const values = result + 2 * kHeads;                     // [kRound][dims][heads]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+#pragma unroll 1
+  for (int32_t e = threadIdx.x; e < count * (kStats / 16); e += kThreads) {
+    const int32_t j = e / (kStats / 16), piece = e % (kStats / 16);
+    cp_async_16_all(ptx::smem_u32(stats) + e * 16, source(j) + kDim * kHeads + piece * 4);
+  }
+  ptx::cp_async_commit();
+  Join joined;
+#pragma unroll 1
+  for (int32_t j0 = 0; j0 < count; j0 += kRound) {
+    const int32_t here = min(kRound, count - j0);
+    if (j0 != 0) __syncthreads();
+#pragma unroll 1
+    for (int32_t j = warp; j < here; j += kWarps) {
+      const float* const from = source(j0 + j) + lane * 4;
+      const uint32_t dst = ptx::smem_u32(values) + j * kValues + lane * 16;
+#pragma unroll
+      for (int i = 0; i < kValues / 512; ++i) cp_async_16_all(dst + i * 512, from + i * 128);
+    }
+    ptx::cp_async_commit();
+    if (j0 == 0) {
+      ptx::cp_async_wait_group<1>();
+      __syncthreads();
+      constexpr int kSides = 32 / kHeads;
+      const int head = lane % kHeads, side = lane / kHeads;
+      float most = -INFINITY, all = 0.0f;
+#pragma unroll 1
+      for (int32_t j = side; j < count; j += kSides) most = fmaxf(most, stats[2 * j * kHeads + head]);
+#pragma unroll
+      for (int d = kHeads; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+#pragma unroll 1
+      for (int32_t j = side; j < count; j += kSides) {
+        const float weight = Join::factor(stats[2 * j * kHeads + head], most);
+        weights[j * kHeads + head] = weight;  // (the same from every warp)
+        all = fmaf(weight, stats[(2 * j + 1) * kHeads + head], all);
+      }
+#pragma unroll
+      for (int d = kHeads; d < 32; d <<= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+      if (side == 0) {
+        result[head] = most;
+        result[kHeads + head] = all;
+      }
+    }
+    ptx::cp_async_wait_group<0>();
+    __syncthreads();
+    const int quad = threadIdx.x % Join::kQuads * 4;
+#pragma unroll 4
+    for (int32_t j = 0; j < here; ++j) {
+      const float4 weight = *reinterpret_cast<const float4*>(weights + (j0 + j) * kHeads + quad);
+#pragma unroll
+      for (int i = 0; i < Join::kItems; ++i) {
+        if (Join::mine(i)) {
+          add_weighted(joined.value[i], weight, *reinterpret_cast<const float4*>(values + j * (kDim * kHeads) + 4 * (threadIdx.x + i * kThreads)));
+        }
+      }
+    }
+  }
+  joined.top = *reinterpret_cast<const float4*>(result + threadIdx.x % Join::kQuads * 4);
+  joined.sum = *reinterpret_cast<const float4*>(result + kHeads + threadIdx.x % Join::kQuads * 4);
+  joined.template give<kCodes>(p, of, to);
+}
 
 // One row of work is a sequence, one of its key-value heads and a block of up to 16 of the query heads
 // that share it; a step is kStep of its tokens.  A lot is a CTA's work.  Where there are few rows, each is
@@ -306,6 +357,7 @@ paged_attention_kernel(const AttentionParams p) {
     return value;
   };
   int64_t mine = 0;
+#pragma unroll 1
   for (int32_t b = b0; b < b1; ++b) mine += static_cast<int64_t>(steps_of(b)) * rows_per_sequence;
   int64_t upto = sum_up(mine);
   const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
@@ -316,6 +368,7 @@ paged_attention_kernel(const AttentionParams p) {
   bool aligned = static_cast<int64_t>(p.batch) * rows_per_sequence <= gridDim.x;
   if (aligned) {
     int64_t pieces = 0;
+#pragma unroll 1
     for (int32_t b = b0; b < b1; ++b) pieces += static_cast<int64_t>(pieces_of(b)) * rows_per_sequence;
     const int64_t pieces_upto = sum_up(pieces), all = __shfl_sync(0xffffffffu, pieces_upto, 31);
     aligned = all <= gridDim.x;
@@ -327,14 +380,17 @@ paged_attention_kernel(const AttentionParams p) {
   }
 
   // Sequences with nothing to attend to, and lengths that the table cannot hold.
+#pragma unroll 1
   for (int32_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
     if (threadIdx.x == 0 && p.status != nullptr && __ldg(p.lengths + b) > p.capacity) atomicOr(p.status, kStatusIndex);
     if (steps_of(b) != 0) continue;
     const int64_t row = static_cast<int64_t>(b) * p.heads;
+#pragma unroll 1
     for (int32_t i = threadIdx.x; i < p.heads * (kDim / 8); i += kThreads) {
       *reinterpret_cast<uint4*>(p.out + row * kDim + 8 * static_cast<int64_t>(i)) = make_uint4(0, 0, 0, 0);
     }
     if (p.lse != nullptr) {
+#pragma unroll 1
       for (int32_t h = threadIdx.x; h < p.heads; h += kThreads) p.lse[row + h] = -INFINITY;
     }
   }
@@ -359,6 +415,7 @@ paged_attention_kernel(const AttentionParams p) {
     int64_t base = upto - mine;
     const bool here = wanted >= base && wanted < upto;
     if (here) {
+#pragma unroll 1
       for (b = b0; b < b1; ++b) {
         const int64_t count = static_cast<int64_t>(aligned ? pieces_of(b) : steps_of(b)) * rows_per_sequence;
         if (wanted < base + count) break;
@@ -777,51 +834,40 @@ paged_attention_kernel(const AttentionParams p) {
   // of kFan neighbours.
   auto slot_of = [&](int32_t of_lot, int which) { return p.partials + (kSlots * static_cast<int64_t>(of_lot) + which) * kPartFloats; };
   int32_t pending[2] = {0, 0}, waiting = 0;
-  for (int32_t i = 0; i < 2 * kWarps;) {
-    if (!parts[i].there) {
-      ++i;
-      continue;
-    }
-    const int32_t first = i;
-    const float* all[kWarps] = {};  // (a warp has one part of a row at most)
-    int32_t count = 0;
+  uint32_t there = 0;
+#pragma unroll
+  for (int32_t j = 0; j < 2 * kWarps; ++j) there |= static_cast<uint32_t>(parts[j].there) << j;
+#pragma unroll 1
+  while (there != 0) {
+    const int32_t first = __ffs(there) - 1;
     bool ended = false;
-#pragma unroll
-    for (int32_t j = 0; j < 2 * kWarps; ++j) {
-      if (j < first || ended || !parts[j].there) continue;
+    Join joined;
+#pragma unroll 1
+    while (there != 0 && !ended) {
+      const int32_t j = __ffs(there) - 1;
+      joined.add(parts[j].at);
       ended = j % 2 == 0;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        if (k == count) all[k] = parts[j].at;
-      }
-      ++count;
-      i = j + 1;
+      there &= there - 1;
     }
     const bool began = parts[first].began, whole = ended && !began;
-    float* const to = whole ? nullptr : slot_of(lot, began ? 0 : 1);
     if (!whole) pending[waiting++] = first;
     const Row of(p, parts[first].b, parts[first].row);
-    Join joined;
-#pragma unroll
-    for (int j0 = 0; j0 < kWarps; j0 += Join::kBatch) {
-      const float* list[Join::kBatch] = {};
-#pragma unroll
-      for (int j = 0; j < Join::kBatch && j0 + j < kWarps; ++j) list[j] = all[j0 + j];
-      joined.add(list, count - j0);
-    }
-    joined.template give<kCodes>(p, of, to);
+    joined.template give<kCodes>(p, of, whole ? nullptr : slot_of(lot, began ? 0 : 1));
   }
   if (waiting == 0) return;
 
   // Then with other lots' parts, by the last CTA to arrive, in the parts' order; it leaves the counts at
   // zero.  (The barrier and the release order the parts before the count.)
+#pragma unroll 1
   for (; waiting > 0; --waiting) {
     const Part part = parts[pending[waiting - 1]];
-    const bool twice = part.lots > kFan;
+    const bool twice = part.lots > kAtOnce;
+    const int32_t fan = part.lots <= kAtOnce * kAtOnce / 4 ? kAtOnce / 2 : kFan;
     const Row of(p, part.b, part.row);
+#pragma unroll 1
     for (int level = twice ? 0 : 1; level < 2; ++level) {
-      const int32_t from = level == 0 ? (lot - part.first_lot) / kFan * kFan : 0, stride = level == 1 && twice ? kFan : 1;
-      const int32_t count = level == 0 ? min(kFan, part.lots - from) : (part.lots + stride - 1) / stride;
+      const int32_t from = level == 0 ? (lot - part.first_lot) / fan * fan : 0, stride = level == 1 && twice ? fan : 1;
+      const int32_t count = level == 0 ? min(fan, part.lots - from) : (part.lots + stride - 1) / stride;
       __syncthreads();
       if (threadIdx.x == 0) {
         const int shift = level == 1 ? kRowShift : from == 0 ? kFirstShift : kFanShift;
@@ -833,16 +879,9 @@ paged_attention_kernel(const AttentionParams p) {
       __syncthreads();
       if (!answer[level]) break;
       float* const to = level == 0 ? slot_of(part.first_lot + from, 2) : nullptr;
-      Join joined;
-      for (int32_t j0 = 0; j0 < count; j0 += Join::kBatch) {
-        const float* list[Join::kBatch];
-#pragma unroll
-        for (int j = 0; j < Join::kBatch; ++j) {
-          list[j] = slot_of(part.first_lot + from + (j0 + j) * stride, stride > 1 ? 2 : from + j0 + j == 0 ? 1 : 0);
-        }
-        joined.add(list, count - j0);
-      }
-      joined.template give<kCodes>(p, of, to);
+      join_parts<kDim, kCodes, kHeads, L::kSmem>(p, of, smem, count, to, [&](int32_t j) {
+        return slot_of(part.first_lot + from + j * stride, stride > 1 ? 2 : from + j == 0 ? 1 : 0);
+      });
     }
   }
 }
