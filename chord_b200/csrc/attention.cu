@@ -357,15 +357,24 @@ paged_attention_kernel(const AttentionParams p) {
     return value;
   };
   int64_t mine = 0;
+  int32_t most = 0;
 #pragma unroll 1
-  for (int32_t b = b0; b < b1; ++b) mine += static_cast<int64_t>(steps_of(b)) * rows_per_sequence;
+  for (int32_t b = b0; b < b1; ++b) {
+    const int32_t steps = steps_of(b);
+    mine += static_cast<int64_t>(steps) * rows_per_sequence;
+    most = max(most, steps);
+  }
   int64_t upto = sum_up(mine);
   const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
-  const int64_t share = max(quotient(total + gridDim.x * kWarps - 1, gridDim.x * kWarps), static_cast<int64_t>(1));
+  bool aligned = static_cast<int64_t>(p.batch) * rows_per_sequence <= gridDim.x;
+  int64_t share = max(quotient(total + gridDim.x * kWarps - 1, gridDim.x * kWarps), static_cast<int64_t>(1));
+  // Short rows stay in one lot: a join with other lots takes as long as four steps of 16 tokens.
+  const int32_t longest = __reduce_max_sync(0xffffffffu, most);
+  constexpr int32_t kAlone = L::kStep == 16 ? 4 : 3;
+  if (aligned && longest <= kAlone * kWarps) share = max(share, static_cast<int64_t>((longest + kWarps - 1) / kWarps));
   const int32_t piece = static_cast<int32_t>(min(share * kWarps, static_cast<int64_t>(1) << 30));  // a lot's steps
   int64_t lots = quotient(total + piece - 1, piece);
   auto pieces_of = [&](int32_t b) { return (steps_of(b) + piece - 1) / piece; };
-  bool aligned = static_cast<int64_t>(p.batch) * rows_per_sequence <= gridDim.x;
   if (aligned) {
     int64_t pieces = 0;
 #pragma unroll 1
@@ -465,6 +474,15 @@ paged_attention_kernel(const AttentionParams p) {
     static_assert(16 * kPieces % 32 == 0, "whole warps");
     const int32_t own = lane % L::kStep;
     int32_t ref_page = 0, ref_place = -1;  // place -1: no token
+    // What follows from the row: its part of the table and its head's offsets, in units of 16 bytes and in floats.
+    const int32_t* row_table;
+    uint64_t row_offset, row_scale = 0;
+    auto enter_row = [&]() {
+      const uint32_t kv_head = p.head_blocks == 1 ? ahead.row : ahead.row / p.head_blocks;
+      row_table = p.tables + ahead.b * p.table_stride;
+      row_offset = static_cast<uint64_t>(kv_head) * p.cache.head16;
+      if constexpr (kCodes) row_scale = static_cast<uint64_t>(kv_head) * static_cast<uint32_t>(p.cache.scale_head);
+    };
     auto look_up = [&]() {
       if (to_load == 0) return;
       const int32_t token = ahead.token + (p.whole_groups ? own / 16 * 16 : own);
@@ -472,7 +490,7 @@ paged_attention_kernel(const AttentionParams p) {
       if (token < ahead.end && token + (p.whole_groups ? 15 : 0) >= ahead.begin) {
         const uint32_t index = p.cache.page_size.div(token);
         ref_place = token - index * p.cache.page_size.d;
-        ref_page = __ldg(p.tables + ahead.b * p.table_stride + index);
+        ref_page = __ldg(row_table + index);
       }
     };
     auto load = [&]() {
@@ -481,8 +499,8 @@ paged_attention_kernel(const AttentionParams p) {
       load_stage = load_stage + 1 == L::kStages ? 0 : load_stage + 1;
       const bool there = ref_place >= 0 && static_cast<uint32_t>(ref_page) < static_cast<uint32_t>(p.cache.num_pages);
       if (ref_place >= 0 && !there && p.status != nullptr) atomicOr(p.status, kStatusIndex);
-      const int32_t kv_head = p.head_blocks == 1 ? ahead.row : ahead.row / p.head_blocks;
-      const int64_t offset = there ? kv_head * p.cache.head + ref_page * p.cache.page + ref_place * p.cache.token : -1;
+      const uint32_t page = ref_page, place = ref_place;
+      const int64_t offset = there ? static_cast<int64_t>(row_offset + static_cast<uint64_t>(page) * p.cache.page16 + static_cast<uint64_t>(place) * p.cache.token16) << 4 : -1;
       const bool full = ahead.token >= ahead.begin && ahead.token + L::kStep <= ahead.end && __all_sync(0xffffffffu, there);
       if (p.whole_groups && full && p.cache.token == L::kRow) {
         // rows of a group follow one another
@@ -515,9 +533,9 @@ paged_attention_kernel(const AttentionParams p) {
       }
       if constexpr (kCodes) {
         const bool seen = there && ahead.token + own >= ahead.begin && ahead.token + own < ahead.end;
-        const int64_t from = seen ? kv_head * p.cache.scale_head + ref_page * p.cache.scale_page +
-                                        (ref_place + (p.whole_groups ? own % 16 : 0)) * p.cache.scale_token
-                                  : 0;
+        const uint64_t from = seen ? row_scale + static_cast<uint64_t>(page) * static_cast<uint32_t>(p.cache.scale_page) +
+                                         static_cast<uint64_t>(place + (p.whole_groups ? own % 16 : 0)) * static_cast<uint32_t>(p.cache.scale_token)
+                                   : 0;
         const uint32_t dst = stage + 2 * L::kStep * L::kPitch + own * 4;
         if (lane < L::kStep) {
           cp_async_4(dst, p.cache.k_scale + from, seen);
@@ -529,9 +547,11 @@ paged_attention_kernel(const AttentionParams p) {
       if (--ahead.left == 0 && to_load > 0) {
         ++ahead.row;
         enter(ahead);
+        enter_row();
       }
     };
 
+    enter_row();
     look_up();
 #pragma unroll
     for (int s = 0; s < L::kStages - 1; ++s) {
@@ -942,9 +962,11 @@ int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t gro
   using namespace chord;
   DeviceInfo device;
   if (current_device_info(&device)) return -1;
-  Variant v;
-  if (!variant_for(head_dim, false, group > 8, &v)) return fail(kInvalidArgument, "head_dim must be 64, 96, 128, 192 or 256"), -1;
-  const int ctas = device.sm_count * v.ctas;
+  Variant v, w;  // of either type of cache
+  if (!variant_for(head_dim, false, group > 8, &v) || !variant_for(head_dim, true, group > 8, &w)) {
+    return fail(kInvalidArgument, "head_dim must be 64, 96, 128, 192 or 256"), -1;
+  }
+  const int ctas = device.sm_count * (v.ctas > w.ctas ? v.ctas : w.ctas);
   return 4 * workspace_floats(ctas < kMaxCtas ? ctas : kMaxCtas, static_cast<int>(head_dim), group > 8 ? 16 : 8);
 }
 

@@ -33,6 +33,7 @@ struct Cache {
   float* v_scale;
   int64_t page, head, token;                    // strides in bytes, of k and v alike
   int64_t scale_page, scale_head, scale_token;  // strides in floats
+  uint32_t page16, head16, token16;             // strides in units of 16 bytes
   int32_t num_pages, heads;
   Divisor page_size;
 };
@@ -58,9 +59,15 @@ inline int make_cache(const chord_b200_kv_cache* c, Cache* out) {
   CHORD_REQUIRE(c->k_scale == nullptr || (c->scale_stride_page >= 0 && c->scale_stride_head >= 0 &&
                                           c->scale_stride_token >= 0),
                 "the scales' strides must not be negative");
+  constexpr int64_t kMost = 1ll << 32;
+  CHORD_REQUIRE(c->stride_page * size / 16 < kMost && c->stride_head * size / 16 < kMost && c->stride_token * size / 16 < kMost &&
+                    (c->k_scale == nullptr || (c->scale_stride_page < kMost && c->scale_stride_head < kMost && c->scale_stride_token < kMost)),
+                "the cache's strides must be below 2^36 bytes, its scales' below 2^34");
   *out = Cache{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale,
                c->stride_page * size, c->stride_head * size, c->stride_token * size,
                c->scale_stride_page, c->scale_stride_head, c->scale_stride_token,
+               static_cast<uint32_t>(c->stride_page * size / 16), static_cast<uint32_t>(c->stride_head * size / 16),
+               static_cast<uint32_t>(c->stride_token * size / 16),
                static_cast<int32_t>(c->num_pages), static_cast<int32_t>(c->heads),
                Divisor(static_cast<uint32_t>(c->page_size))};
   return kOk;
