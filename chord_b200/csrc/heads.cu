@@ -52,18 +52,29 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Eight codes round(x / scale) + 128 of a row whose largest |x| is `top`, scale = top / 127.  Adding 1.5 * 2^23
-// + 128 rounds to a whole number and leaves the code in the sum's low byte.
+// Eight codes round(x / scale) + 128 of a row whose largest |x| is `top`, scale = top / 127; halves go to the
+// even code.  A half is common (x = top / 2 is 63.5 steps), and x * rate is off by up to 2^-17 there: the first
+// sum rounds to steps of 2^-15, which brings it back, the second (1.5 * 2^23 + 128 in all) to whole numbers, the
+// code in the low byte.
 __device__ __forceinline__ uint2 quantise8(float (&x)[8], float top) {
-  if (top < 0x1p-100f) {  // (127 / top has to stay finite)
+  if (!(top > 0x1p-100f && top < 0x1p100f)) {  // (the reciprocal's range)
+    const float factor = top < 1.0f ? 0x1p100f : 0x1p-64f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= 0x1p100f;
-    top *= 0x1p100f;
+    for (int i = 0; i < 8; ++i) x[i] *= factor;
+    top = top > 0.0f ? top * factor : 1.0f;
   }
-  const float rate = top > 0.0f ? __fdividef(127.0f, top) : 0.0f;
+  const float inverse = __fdividef(1.0f, top);
+  float rate = 127.0f * inverse;
+  rate = fmaf(fmaf(-top, rate, 127.0f), inverse, rate);  // (as good as correctly rounded)
   uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(fmaf(x[i], rate, 12583040.0f));
+  for (int i = 0; i < 8; i += 2) {
+    // Two at a time.
+    asm("{\n .reg .b64 x, r, c;\n mov.b64 x, {%2, %3};\n mov.b64 r, {%4, %4};\n mov.b64 c, {%5, %5};\n fma.rn.f32x2 x, x, r, c;\n"
+        " mov.b64 c, {%6, %6};\n add.rn.f32x2 x, x, c;\n mov.b64 {%0, %1}, x;\n}"
+        : "=r"(w[i]), "=r"(w[i + 1])
+        : "f"(x[i]), "f"(x[i + 1]), "f"(rate), "f"(384.0f), "f"(12583040.0f - 384.0f));
+  }
   return make_uint2(low_bytes(w[0], w[1], w[2], w[3]), low_bytes(w[4], w[5], w[6], w[7]));
 }
 

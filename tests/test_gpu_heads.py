@@ -180,6 +180,32 @@ def test_rows_of_zeros_infinities_and_tiny_values(device):
         check_kept(got[i:i + 1], x[i:i + 1], 8)
 
 
+def test_halves_go_to_the_even_code(device):
+    """A row's largest x is 127 steps, so +-x / 2 is 63.5 steps: 64; for every size of x, the type's largest too.
+    The other columns are n + 1/2 steps where the largest is 127 or 254 of something: all n.  No tolerance."""
+    tops = torch.arange(1 << 7, 0x7F80, dtype=torch.int32, device=device).to(torch.int16).view(torch.bfloat16)
+    tops = tops[tops >= 2.0 ** -120]
+    n = torch.arange(127, device=device).float()
+    rows = torch.stack([tops, tops / 2, -tops / 2] + [torch.zeros_like(tops)] * 253, dim=1)
+    steps = torch.zeros((40, 256), device=device)
+    steps[:, :127], steps[:, 127], steps[:, 128:255] = n + 0.5, 127, -n - 0.5
+    steps *= 2.0 ** torch.arange(-100, 100, 5, device=device).float()[:, None]
+    x = torch.cat([rows, steps.to(torch.bfloat16)])
+    cache = chord_b200.kv_cache(len(x), 1, 1, 256, dtype=torch.uint8, device=device)
+    chord_b200.cache_write(x[:, None], -x[:, None], cache, torch.arange(len(x), dtype=torch.int32, device=device))
+    even = torch.round(n + 0.5)   # (torch rounds halves to even)
+    for codes, sign in ((cache.k[:, 0, 0], 1), (cache.v[:, 0, 0], -1)):
+        codes = sign * (codes.int() - 128)
+        head, tail = codes[:len(rows)], codes[len(rows):]
+        assert bool((head[:, 0] == 127).all()) and bool((head[:, 1] == 64).all()) and bool((head[:, 2] == -64).all())
+        assert bool((head[:, 3:] == 0).all())
+        assert bool((tail[:, :127] == even).all()) and bool((tail[:, 128:255] == -even).all())
+    for scale, x in ((cache.k_scale, x), (cache.v_scale, -x)):
+        want = x.double().abs().amax(1) / 127
+        assert bool(((scale[:, 0, 0].double() - want).abs() <= 4 * A.SINGLE * want).all())
+    chord_b200.check_status(device)
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_a_cache_past_four_gigabytes(device, bits):
     """Offsets of the last pages pass 2^32 bytes."""
