@@ -1037,9 +1037,8 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, c
   p.window = static_cast<int32_t>(window);
   p.scale = static_cast<float>(scale * 1.4426950408889634074 * (codes ? 0x1p53 : 1.0));
   p.whole_groups = cache->page_size % 16 == 0 && p.cache.token < (1ll << 31);
-  OptionsReadLock guard(options_mutex());
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), v.smem,
-                           static_cast<cudaStream_t>(stream), options().pdl != 0, p));
+                           static_cast<cudaStream_t>(stream), kEarlyLaunch, p));
   return kOk;
 }
 

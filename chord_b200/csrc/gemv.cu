@@ -413,9 +413,8 @@ int chord_b200_gemv(const void* x, int64_t x_stride, const int32_t* packed, cons
                              static_cast<int32_t>(top_k), static_cast<int32_t>(expert_base),
                              x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0};
   const dim3 grid(cluster, static_cast<unsigned>(n / 64), static_cast<unsigned>(expert_ids != nullptr ? rows : 1));
-  OptionsReadLock guard(options_mutex());
   CHORD_CUDA(launch_kernel_clusters(v.kernel, cluster, grid, dim3(kGemvWarps * 32), v.smem, static_cast<cudaStream_t>(stream),
-                                    options().pdl != 0, params));
+                                    kEarlyLaunch, params));
   return kOk;
 }
 

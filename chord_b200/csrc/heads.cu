@@ -471,9 +471,8 @@ int launch_heads(HeadsParams p, int64_t tokens, cudaStream_t stream) {
                                    {heads_kernel<16, 1, kRotate, kKeep>, heads_kernel<16, 4, kRotate, kKeep>},
                                    {heads_kernel<32, 1, kRotate, kKeep>, heads_kernel<32, 4, kRotate, kKeep>}};
   const int64_t blocks = (p.items + kWarps - 1ll) / kWarps;
-  OptionsReadLock guard(options_mutex());
   CHORD_CUDA(launch_kernel(kernels[lanes / 16][wide], dim3(static_cast<unsigned>(blocks)), dim3(kWarps * 32), 0, stream,
-                           options().pdl != 0, p));
+                           kEarlyLaunch, p));
   return kOk;
 }
 
@@ -632,9 +631,8 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
                                    {cache_read_kernel<16, 1>, cache_read_kernel<16, 4>},
                                    {cache_read_kernel<32, 1>, cache_read_kernel<32, 4>}};
   const int64_t blocks = (p.items + kWarps - 1ll) / kWarps;
-  OptionsReadLock guard(options_mutex());
   CHORD_CUDA(launch_kernel(kernels[lanes / 16][wide], dim3(static_cast<unsigned>(blocks), wide ? 1 : 2), dim3(kWarps * 32), 0,
-                           static_cast<cudaStream_t>(stream), options().pdl != 0, p));
+                           static_cast<cudaStream_t>(stream), kEarlyLaunch, p));
   return kOk;
 }
 

@@ -9,6 +9,13 @@
 
 namespace chord {
 
+// The operators of a token's way through a layer are launched with the programmatic stream-serialization
+// attribute, whatever the option: they are a few microseconds each, follow one another, and touch no memory before
+// they have waited for what was launched before them.  us of a call among others of its kind, without and with it:
+// one row of 4096 x 7168 8.3 and 6.1, 13 rows of 7168 x 2048 8.2 and 5.7, attention over 333 tokens 10.3 and
+// 8.5.  They do not let the next one in before they end (attention then took 2 % longer, the others as long).
+constexpr bool kEarlyLaunch = true;
+
 // a * b + c on two BF16 numbers, rounded once.  Subnormal operands count in full, which is what
 // turns bits into numbers below: a BF16 pattern under 0x100 is the number pattern * 2^-133, so a code
 // of up to eight bits is a number as it stands, and one multiply-add takes its offset off.

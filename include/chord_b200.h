@@ -368,6 +368,8 @@ int chord_b200_ep_combine_signal(void* const* peer_state, int64_t world, int64_t
 int chord_b200_ep_combine_wait(void* state, int64_t world, int64_t epoch, void* stream);
 
 /* ---- products of a few rows -----------------------------------------------------------
+ * These and the operators below always carry the programmatic stream-serialization attribute (the
+ * option "pdl" is not asked): they touch no memory before all that precedes them in the stream is done.
  * No counterpart in the reference, whose operators all take routing blocks.  With
  * expert_ids null (one expert's weight, rows <= 16):
  *   out[r, :] = x[r, :] . dequant(W[0])^T
@@ -385,7 +387,8 @@ int chord_b200_gemv(const void* x, int64_t x_stride, const int32_t* packed, cons
  * No counterpart in the reference, nor for what follows below.  Keys and values lie in pages of
  * page_size tokens.  A row is what one head keeps of one token: head_dim BF16 values
  * (k_scale == v_scale == null), or head_dim bytes of codes with an FP32 scale per row,
- *   value = (code - 128) * scale,   scale = max |x| / 127,   code = round(x / scale) + 128.
+ *   value = (code - 128) * scale,   scale = max |x| / 127,   code = round(x / scale) + 128,
+ * halves to the even code.
  * head_dim is a multiple of 16, at most 256.  Strides are in elements and the same for keys and
  * values; every row starts on a 16-byte boundary.  A slot is page * page_size + place in the page.
  * An index outside its range is never followed: the row counts as zeros, or is not written, and
