@@ -11,7 +11,7 @@
 namespace chord {
 namespace {
 
-constexpr int kGemvWarps = 8;
+constexpr int kGemvWarps = 8;  // of a CTA; kernels for up to four rows also with half of them
 
 struct GemvParams {
   const __nv_bfloat16* x;
@@ -47,16 +47,16 @@ __device__ __forceinline__ void operand(uint32_t word, uint32_t (&a)[4]) {
 // shared memory, always in the same order.
 
 // Joins what the warps, and the CTAs of a cluster, have of kTokens x 64 results.  `sums`: room for
-// kGemvWarps + 1 times that many; a lane's are v(token, row) for its rows.
-template <int kTokens>
+// kWarps + 1 times that many; a lane's are v(token, row) for its rows.
+template <int kTokens, int kWarps>
 __device__ __forceinline__ void join_and_store(const GemvParams& p, float* sums, int64_t out_row, int rows, int block) {
   const int cluster = gridDim.x, rank = blockIdx.x;
-  float* const part = sums + kGemvWarps * kTokens * 64;
+  float* const part = sums + kWarps * kTokens * 64;
   __syncthreads();
-  for (int i = threadIdx.x; i < kTokens * 64; i += kGemvWarps * 32) {
+  for (int i = threadIdx.x; i < kTokens * 64; i += kWarps * 32) {
     float v = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kGemvWarps; ++j) v += sums[j * (kTokens * 64) + i];
+    for (int j = 0; j < kWarps; ++j) v += sums[j * (kTokens * 64) + i];
     const int token = i / 64;
     if (cluster > 1) {
       part[i] = v;
@@ -67,7 +67,7 @@ __device__ __forceinline__ void join_and_store(const GemvParams& p, float* sums,
   if (cluster > 1) {
     __syncwarp();
     ptx::cluster_sync();
-    for (int i = threadIdx.x * cluster + rank; i < rows * 64; i += kGemvWarps * 32 * cluster) {
+    for (int i = threadIdx.x * cluster + rank; i < rows * 64; i += kWarps * 32 * cluster) {
       const uint32_t addr = ptx::smem_u32(part + i);
       float v = 0.0f;
       for (int j = 0; j < cluster; ++j) v += ld_cluster_f32(ptx::map_to_cta(addr, j));
@@ -96,7 +96,7 @@ struct GemvPlace {
 
 // Up to four rows: words go straight into the registers that the products read, those of kBatch scale
 // groups at a time, all in flight at once.
-template <int kTokens, int kSlots, int kBatch>
+template <int kTokens, int kSlots, int kBatch, int kWarps>
 __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& at, float (&acc)[4][2]) {
   constexpr int kSets = kBatch / kSlots;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -109,7 +109,7 @@ __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& a
   for (int s = 0; s < 4; ++s) acc[s][0] = acc[s][1] = 0.0f;
 
   // Groups past the last are read as the last one, with zero inputs and a zero scale.
-  for (int first = (blockIdx.x * kGemvWarps + warp) * kBatch; first < groups; first += gridDim.x * kGemvWarps * kBatch) {
+  for (int first = (blockIdx.x * kWarps + warp) * kBatch; first < groups; first += gridDim.x * kWarps * kBatch) {
     uint4 w[2 * kBatch], sc[kSets][2];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -127,15 +127,18 @@ __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& a
         if (g >= groups) sc[set][j] = make_uint4(0, 0, 0, 0);
       }
     }
+    // The column's row and groups: 32 inputs of each in fragment order.
+    uint32_t xr[kSets][4];
 #pragma unroll
     for (int set = 0; set < kSets; ++set) {
-      // The column's row and group: its 32 inputs in fragment order.
-      uint32_t xr[4];
       const int g = first + set * kSlots + r % kSlots;
       const bool there = token < at.rows && g < groups;
       const uint32_t* const from = reinterpret_cast<const uint32_t*>(x + (there ? 32 * g : 0));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xr[i] = there ? __ldg(from + 4 * i) : 0u;
+      for (int i = 0; i < 4; ++i) xr[set][i] = there ? __ldg(from + 4 * i) : 0u;
+    }
+#pragma unroll
+    for (int set = 0; set < kSets; ++set) {
       float c[4][4] = {};
 #pragma unroll
       for (int slot = 0; slot < kSlots; ++slot) {
@@ -144,7 +147,7 @@ __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& a
           const uint4& v = w[2 * (set * kSlots + slot) + h];
           const uint32_t word[4] = {v.x, v.y, v.z, v.w};
           const bool mine = r % kSlots == slot;
-          const uint32_t b0 = mine ? xr[2 * h] : 0u, b1 = mine ? xr[2 * h + 1] : 0u;
+          const uint32_t b0 = mine ? xr[set][2 * h] : 0u, b1 = mine ? xr[set][2 * h + 1] : 0u;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             uint32_t a[4];
@@ -164,11 +167,11 @@ __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& a
   }
 }
 
-template <int kTokens, int kSlots, int kBatch>
-__global__ void __launch_bounds__(kGemvWarps * 32, 2)
+template <int kTokens, int kSlots, int kBatch, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
 gemv_few_kernel(const GemvParams p) {
   static_assert(kSlots > 1 && kBatch % kSlots == 0 && kTokens * kSlots <= 8, "a batch holds whole sets");
-  __shared__ float sums[(kGemvWarps + 1) * kTokens * 64];
+  __shared__ float sums[(kWarps + 1) * kTokens * 64];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q = lane & 3, r = lane >> 2;
   const int block = blockIdx.y;
@@ -185,7 +188,7 @@ gemv_few_kernel(const GemvParams p) {
   at.scales = p.scale + static_cast<int64_t>(expert) * (p.k / 32) * p.n + block * 64 + r * 8;
 
   float acc[4][2];  // [16-row tile][upper half]
-  gemv_few<kTokens, kSlots, kBatch>(p, at, acc);
+  gemv_few<kTokens, kSlots, kBatch, kWarps>(p, at, acc);
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
 #pragma unroll
@@ -196,12 +199,12 @@ gemv_few_kernel(const GemvParams p) {
       if (2 * q % kSlots == 0 && 2 * q / kSlots < kTokens) sums[(warp * kTokens + 2 * q / kSlots) * 64 + 16 * s + 8 * rh + r] = v;
     }
   }
-  join_and_store<kTokens>(p, sums, at.out_row, at.rows, block);
+  join_and_store<kTokens, kWarps>(p, sums, at.out_row, at.rows, block);
 }
 
 // Five to sixteen rows: a ring of cp.async stages for each warp, 64 K of 64 weight rows: 2 KB of words, their
 // scales and the rows' inputs, which ldmatrix then reads as operands (with loads of four bytes straight
-// into registers they took most of the time: 16 rows of 14336 x 7168 39.7 us, 27.6 like this).
+// into registers they took most of the time: 16 rows of 14336 x 7168 39.7 us, 23.1 like this).
 template <int kTokens>
 struct GemvLayout {
   static constexpr int kTiles = kTokens > 8 ? 2 : 1;  // products of eight columns
@@ -334,22 +337,23 @@ gemv_rows_kernel(const GemvParams p) {
       to[72] = acc[t][s][3];
     }
   }
-  join_and_store<kTokens>(p, sums, 0, p.rows, blockIdx.y);
+  join_and_store<kTokens, kGemvWarps>(p, sums, 0, p.rows, blockIdx.y);
 }
 
 struct GemvVariant {
   void (*kernel)(GemvParams);
-  int smem, groups, ctas, index;  // groups: that a warp takes at a time; ctas: of an SM
+  int smem, groups, ctas, index, warps;  // groups: that a warp takes at a time; ctas: of an SM
 };
 
 template <int kTokens, int kSlots, int kBatch>
-GemvVariant few() {
-  return {gemv_few_kernel<kTokens, kSlots, kBatch>, 0, kBatch, 2, kTokens};
+GemvVariant few(bool half) {
+  if (half) return {gemv_few_kernel<kTokens, kSlots, kBatch, kGemvWarps / 2>, 0, kBatch, 4, kTokens, kGemvWarps / 2};
+  return {gemv_few_kernel<kTokens, kSlots, kBatch, kGemvWarps>, 0, kBatch, 2, kTokens, kGemvWarps};
 }
 
 template <int kTokens>
 GemvVariant many_rows() {
-  return {gemv_rows_kernel<kTokens>, GemvLayout<kTokens>::kSmem, 2, 1, kTokens};
+  return {gemv_rows_kernel<kTokens>, GemvLayout<kTokens>::kSmem, 2, 1, kTokens, kGemvWarps};
 }
 
 // Allows a kernel its shared memory, once per device.
@@ -392,19 +396,23 @@ int chord_b200_gemv(const void* x, int64_t x_stride, const int32_t* packed, cons
   if (int rc = require_blackwell(device)) return rc;
 
   const int64_t shared = expert_ids != nullptr ? 1 : rows;
-  const GemvVariant v = shared == 1 ? few<1, 8, 8>() : shared == 2 ? few<2, 4, 8>() : shared <= 4 ? few<4, 2, 4>() :
+  const int64_t blocks = n / 64 * (expert_ids != nullptr ? rows : 1);
+  // CTAs of four warps where there are more of them than are resident with eight.  Eight experts of 4096 x 7168
+  // 29.3 us with eight warps, 27.5 with four, of 7168 x 2048 16.5 and 15.1; one row of 28416 x 4096 16.2 and
+  // 14.2; where all are resident eight are better, 14336 x 14336 26.5 and 27.6, 7168 x 2048 3.1 and 3.6.
+  const bool half = blocks > 2ll * device.sm_count;
+  const GemvVariant v = shared == 1 ? few<1, 8, 8>(half) : shared == 2 ? few<2, 4, 8>(half) : shared <= 4 ? few<4, 2, 4>(half) :
                         shared <= 8 ? many_rows<8>() : many_rows<16>();
   if (int rc = allow_smem(v, device.device)) return rc;
-  const int64_t blocks = n / 64 * (expert_ids != nullptr ? rows : 1);
   // CTAs of a cluster: the fewest with which a warp has the least to do, where all CTAs are resident at once.
-  // One row of 4096 x 7168: one CTA for 64 rows of the weight 10.9 us, two 7.6, four 6.3, eight (more than are
-  // resident) 11.3; 7168 x 2048, whose batches of K are as many as the warps of one CTA, 3.5 with one, 5.5 with
-  // two; 14336 x 14336 27.0 with one, 32.2 with two.  13 rows of 7168 x 2048, whose CTAs are best one to an
-  // SM: 6.1 with one, 8.0 with two.
+  // One row of 4096 x 7168: one CTA for 64 rows of the weight 10.7 us, two 7.5, four 6.2, eight (more than are
+  // resident) 11.3; 7168 x 2048, whose batches of K are as many as the warps of one CTA, 3.1 with one, 5.3 with
+  // two; 14336 x 14336 26.5 with one, 32.0 with two.  13 rows of 7168 x 2048, whose CTAs are best one to an
+  // SM: 5.6 with one, 8.0 with two.
   const int64_t batches = (k / 32 + v.groups - 1) / v.groups;
   int cluster = 1;
   for (int c = 2; c <= 8 && blocks * c <= static_cast<int64_t>(v.ctas) * device.sm_count; c *= 2) {
-    const auto turns = [&](int ctas) { return (batches + ctas * kGemvWarps - 1) / (ctas * kGemvWarps); };
+    const auto turns = [&](int ctas) { return (batches + ctas * v.warps - 1) / (ctas * v.warps); };
     if (turns(c) < turns(cluster)) cluster = c;
   }
   const GemvParams params = {static_cast<const __nv_bfloat16*>(x), packed, static_cast<const __nv_bfloat16*>(scale),
@@ -413,7 +421,7 @@ int chord_b200_gemv(const void* x, int64_t x_stride, const int32_t* packed, cons
                              static_cast<int32_t>(top_k), static_cast<int32_t>(expert_base),
                              x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0};
   const dim3 grid(cluster, static_cast<unsigned>(n / 64), static_cast<unsigned>(expert_ids != nullptr ? rows : 1));
-  CHORD_CUDA(launch_kernel_clusters(v.kernel, cluster, grid, dim3(kGemvWarps * 32), v.smem, static_cast<cudaStream_t>(stream),
+  CHORD_CUDA(launch_kernel_clusters(v.kernel, cluster, grid, dim3(v.warps * 32), v.smem, static_cast<cudaStream_t>(stream),
                                     kEarlyLaunch, params));
   return kOk;
 }

@@ -44,6 +44,32 @@ def test_large(device, rows, n, k):
     check(chord_b200.gemv(x, weight), want, size, k)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 4, 7])
+def test_more_blocks_than_are_resident(device, rows):
+    """300 blocks of 64 weight rows: CTAs of four warps, with batches of K left over."""
+    n, k = 19200, 1344
+    codes, scale, weight = weight_of(1, n, k, rows, device)
+    x = torch.randn((rows, k), generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to(device)
+    want, size = A.gemv(x, codes, scale)
+    check(chord_b200.gemv(x, weight), want, size, k)
+
+
+def test_experts_of_more_blocks_than_are_resident(device):
+    experts, n, k, rows = 5, 640, 576, 40
+    codes, scale, weight = weight_of(experts, n, k, 3, device)
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn((rows, k), generator=g).to(torch.bfloat16).to(device)
+    ids = torch.randint(0, 7, (rows,), generator=g, dtype=torch.int32)
+    got = chord_b200.gemv(x, weight, expert_ids=ids.to(device))
+    for e in range(7):
+        mine = (ids == e).nonzero()[:, 0].to(device)
+        if e >= experts:
+            assert bool((got[mine] == 0).all())
+        elif len(mine):
+            want, size = A.gemv(x[mine], codes[e:e + 1], scale[e:e + 1])
+            check(got[mine], want, size, k)
+
+
 @pytest.mark.parametrize("tokens,top_k", [(1, 1), (1, 8), (3, 2), (5, 7)])
 @pytest.mark.parametrize("base", [0, 3])
 def test_experts(device, tokens, top_k, base):
