@@ -299,8 +299,7 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 //
 // Products on mma.m16n8k16, keys and values as the 16-row operand, the heads (eight for each of kTiles)
 // as columns: S[tokens, heads] = K Q^T and O[dims, heads] += V^T P, P by movmatrix from the score
-// fragments.  (With the heads as rows, half of every product was idle with up to eight of them: 890
-// instead of 500 instructions per 32 tokens of codes.)  P is multiplied as the sum of two BF16 numbers, 16 bits of it.
+// fragments.  (With the heads as rows, half of every product was idle with up to eight of them.)  P is multiplied as the sum of two BF16 numbers, 16 bits of it.
 // Codes are exact in BF16; the keys' scales are applied to the scores, the values' to P.  The codes of
 // values become (code - 128) / 64.  Those of keys are multiplied as they stand, as the BF16 numbers
 // code * 2^-133, with queries times 2^80: the scores start from minus 128 times the query's sum, which
@@ -308,6 +307,14 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 //
 // The running maximum is raised, and the sums are scaled, only where a score passes it by more than
 // 2^kSlack; until then P is up to 2^kSlack, which costs no precision, and no lane needs another's scores.
+//
+// Long rows are bounded by memory and by how unequally the SMs are served: 64 sequences of up to 8192 tokens in
+// BF16, 64 + 8 heads of 128, 1.36 GB, 248 us = 5.5 TB/s, 83 % of a plain copy's rate (of 64 x 4096, equal lots, 12
+// SMs were done after 127 us, 96 after 152, 40 after 174; lots by ticket or two and three times as many were no
+// better).  Codes also by instructions, some 600 for 32 tokens: 131072 tokens of one sequence, 277 MB, 58 us =
+// 4.8 TB/s, of which about 8 are the launch, the rings' filling and two joins.  Three CTAs of an SM with steps of 16
+// tokens instead of two with 32 gain 9 % on 64 x 4096 of codes, and lose 10 % on that one and 40 % on 37 x 1000.  Short
+// rows are bounded by latency: 333 tokens of 8 heads 8.4 us, some five dependent round trips to memory and one join.
 template <int kDim, bool kCodes, int kTiles>
 __global__ void __launch_bounds__(kThreads, (Layout<kDim, kCodes, kTiles>::kCtas))
 paged_attention_kernel(const AttentionParams p) {
@@ -368,10 +375,12 @@ paged_attention_kernel(const AttentionParams p) {
   const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
   bool aligned = static_cast<int64_t>(p.batch) * rows_per_sequence <= gridDim.x;
   int64_t share = max(quotient(total + gridDim.x * kWarps - 1, gridDim.x * kWarps), static_cast<int64_t>(1));
-  // Short rows stay in one lot: a join with other lots takes as long as four steps of 16 tokens.
-  const int32_t longest = __reduce_max_sync(0xffffffffu, most);
+  // Where there are few rows they stay in one lot each, if the longest then takes its warps no longer than equal
+  // lots and a join with other lots, which is as long as four steps of 16 tokens.  (37 sequences with a window of 1000
+  // tokens, 12 heads of 64, codes: 32 or 33 steps a row, in equal lots 23.5 us, whole 19.7.)
+  const int32_t longest = __reduce_max_sync(0xffffffffu, most), whole = (longest + kWarps - 1) / kWarps;
   constexpr int32_t kAlone = L::kStep == 16 ? 4 : 3;
-  if (aligned && longest <= kAlone * kWarps) share = max(share, static_cast<int64_t>((longest + kWarps - 1) / kWarps));
+  if (aligned && whole < share + kAlone) share = max(share, static_cast<int64_t>(whole));
   const int32_t piece = static_cast<int32_t>(min(share * kWarps, static_cast<int64_t>(1) << 30));  // a lot's steps
   int64_t lots = quotient(total + piece - 1, piece);
   auto pieces_of = [&](int32_t b) { return (steps_of(b) + piece - 1) / piece; };
