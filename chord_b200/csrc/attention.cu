@@ -45,10 +45,15 @@ template <int kDim, bool kCodes, int kTiles>
 struct Layout {
   static constexpr int kRow = kDim * (kCodes ? 1 : 2);  // bytes of a row
   static constexpr int kPitch = kRow + 16;              // an odd number of 16-byte pieces: no bank conflicts
-  static constexpr int kStep = kCodes || kRow < 128 ? 32 : 16;
+  static constexpr int kStep = kCodes && kDim <= 192 ? 32 : 16;
   static constexpr int kScaleBytes = kCodes ? 2 * kStep * 4 : 0;
   static constexpr int kStageBytes = 2 * kStep * kPitch + kScaleBytes;
-  static constexpr int kCtas = kDim > 128 ? 1 : kDim == 64 && kTiles == 1 ? 3 : 2;  // of an SM
+  // CTAs of an SM: as many as have room for two stages and for their registers.  Heads of 192, 64 x 4096 and 256 x
+  // 256 tokens: codes 111.0 and 44.8 us with two, 113.6 and 55.6 with one, BF16 184.5 and 62.7, 201.5 and 68.0.
+  // Heads of 256, codes, with steps of 16 tokens two: 142.7 and 52.7, with 32 one: 136.2 and 58.9, 37 x 1000 31.4 and 34.0.
+  // Heads of 64, codes: 47.4 and 25.6 with three, 52.9 and 28.2 with two, 46.5 and 24.4 with four, which lose where rows
+  // are few (37 x 1000 of 12 heads 22.6, 18.7 with three).
+  static constexpr int kCtas = kDim > 192 ? (kCodes ? 2 : 1) : kDim == 64 && kTiles == 1 ? 3 : 2;
   static constexpr int kFit = (kCtas == 1 ? 220 : kCtas == 2 ? 111 : 74) * 1024 / (kWarps * kStageBytes);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
@@ -372,28 +377,41 @@ paged_attention_kernel(const AttentionParams p) {
     most = max(most, steps);
   }
   int64_t upto = sum_up(mine);
+  const int64_t before = upto - mine;
   const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
   bool aligned = static_cast<int64_t>(p.batch) * rows_per_sequence <= gridDim.x;
   int64_t share = max(quotient(total + gridDim.x * kWarps - 1, gridDim.x * kWarps), static_cast<int64_t>(1));
   // Where there are few rows they stay in one lot each, if the longest then takes its warps no longer than equal
-  // lots and a join with other lots, which is as long as four steps of 16 tokens.  (37 sequences with a window of 1000
-  // tokens, 12 heads of 64, codes: 32 or 33 steps a row, in equal lots 23.5 us, whole 19.7.)
+  // lots and a join with other lots, which is as long as four steps of 16 tokens.  Else each is cut into lots of its
+  // own, as short as there are CTAs for all of them, or, where they would be kCut steps longer than equal lots, the
+  // steps of all rows are numbered through.  (64 + 8 heads of 128 in BF16, 24 sequences with a window of 1000 tokens: lots
+  // of their own 25.4 us, equal ones 29.3; 20 of them 25.0 and 26.4; 37 of up to 2000 tokens 44.4 and 46.7.  37 with a
+  // window of 1000, 12 heads of 64, codes: whole 19.2, in equal lots 23.5.)
   const int32_t longest = __reduce_max_sync(0xffffffffu, most), whole = (longest + kWarps - 1) / kWarps;
-  constexpr int32_t kAlone = L::kStep == 16 ? 4 : 3;
+  constexpr int32_t kAlone = L::kStep == 16 ? 4 : 3, kCut = L::kStep == 16 ? 16 : 6;
   if (aligned && whole < share + kAlone) share = max(share, static_cast<int64_t>(whole));
-  const int32_t piece = static_cast<int32_t>(min(share * kWarps, static_cast<int64_t>(1) << 30));  // a lot's steps
+  const auto piece_for = [&](int64_t steps) { return static_cast<int32_t>(min(steps * kWarps, static_cast<int64_t>(1) << 30)); };
+  int32_t piece = piece_for(share);  // a lot's steps
   int64_t lots = quotient(total + piece - 1, piece);
   auto pieces_of = [&](int32_t b) { return (steps_of(b) + piece - 1) / piece; };
   if (aligned) {
-    int64_t pieces = 0;
+    int32_t longer = 0;
 #pragma unroll 1
-    for (int32_t b = b0; b < b1; ++b) pieces += static_cast<int64_t>(pieces_of(b)) * rows_per_sequence;
-    const int64_t pieces_upto = sum_up(pieces), all = __shfl_sync(0xffffffffu, pieces_upto, 31);
-    aligned = all <= gridDim.x;
+    do {
+      piece = piece_for(share + longer);
+      mine = 0;
+#pragma unroll 1
+      for (int32_t b = b0; b < b1; ++b) mine += static_cast<int64_t>(pieces_of(b)) * rows_per_sequence;
+      lots = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(mine));
+    } while (lots > gridDim.x && ++longer < kCut);
+    aligned = lots <= gridDim.x;
     if (aligned) {
-      mine = pieces;
-      upto = pieces_upto;
-      lots = all;
+      share += longer;
+      upto = sum_up(mine);
+    } else {
+      mine = upto - before;
+      piece = piece_for(share);
+      lots = quotient(total + piece - 1, piece);
     }
   }
 
