@@ -70,6 +70,21 @@ def test_experts_of_more_blocks_than_are_resident(device):
             check(got[mine], want, size, k)
 
 
+@pytest.mark.parametrize("rows", [2, 6])
+def test_results_at_an_odd_element(device, rows):
+    """A result needs no more alignment than its type; rows of experts held elsewhere are zeros there too."""
+    n, k = 256, 320
+    codes, scale, weight = weight_of(2, n, k, 8, device)
+    x = torch.randn((rows, k), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(device)
+    ids = torch.tensor([1, 5] * (rows // 2), dtype=torch.int32, device=device)
+    room = torch.full((rows * n + 2,), 7.0, dtype=torch.bfloat16, device=device)
+    out = room[1:-1].view(rows, n)
+    chord_b200.gemv(x, weight, expert_ids=ids, outputs=out)
+    want, size = A.gemv(x[::2], codes[1:], scale[1:])
+    check(out[::2], want, size, k)
+    assert bool((out[1::2] == 0).all()) and float(room[0]) == float(room[-1]) == 7.0
+
+
 @pytest.mark.parametrize("tokens,top_k", [(1, 1), (1, 8), (3, 2), (5, 7)])
 @pytest.mark.parametrize("base", [0, 3])
 def test_experts(device, tokens, top_k, base):
