@@ -95,7 +95,10 @@ struct GemvPlace {
 };
 
 // Up to four rows: words go straight into the registers that the products read, those of kBatch scale
-// groups at a time, all in flight at once.
+// groups at a time, all in flight at once.  A warp's loads and products take turns, and instructions (14.6 for a
+// word) fill half of an SM's issue slots: eight experts of 4096 x 7168, 132 MB, 27.5 us = 4.8 TB/s, 74 % of a plain
+// copy's rate; one row of 14336 x 14336, whose 224 CTAs are two on some SMs and one on others, 26.5 us = 4.4 TB/s.  One
+// row of 4096 x 7168, 16.5 MB, 5.6 us: a launch, one turn and the join of a cluster.
 template <int kTokens, int kSlots, int kBatch, int kWarps>
 __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& at, float (&acc)[4][2]) {
   constexpr int kSets = kBatch / kSlots;
@@ -202,9 +205,11 @@ gemv_few_kernel(const GemvParams p) {
   join_and_store<kTokens, kWarps>(p, sums, at.out_row, at.rows, block);
 }
 
-// Five to sixteen rows: a ring of cp.async stages for each warp, 64 K of 64 weight rows: 2 KB of words, their
+// More rows, up to sixteen: a ring of cp.async stages for each warp, 64 K of 64 weight rows: 2 KB of words, their
 // scales and the rows' inputs, which ldmatrix then reads as operands (with loads of four bytes straight
-// into registers they took most of the time: 16 rows of 14336 x 7168 39.7 us, 23.1 like this).
+// into registers they took most of the time: 16 rows of 14336 x 7168 39.7 us, 23.1 like this).  Instructions bound it,
+// 18 for a word with one product and 26 with two, 83 and 72 % of the busiest SM's issue slots: eight rows of 14336 x
+// 14336 27.6 us = 4.2 TB/s, 16 of 14336 x 7168 23.1 us = 2.5 TB/s.
 template <int kTokens>
 struct GemvLayout {
   static constexpr int kTiles = kTokens > 8 ? 2 : 1;  // products of eight columns
@@ -401,7 +406,11 @@ int chord_b200_gemv(const void* x, int64_t x_stride, const int32_t* packed, cons
   // 29.3 us with eight warps, 27.5 with four, of 7168 x 2048 16.5 and 15.1; one row of 28416 x 4096 16.2 and
   // 14.2; where all are resident eight are better, 14336 x 14336 26.5 and 27.6, 7168 x 2048 3.1 and 3.6.
   const bool half = blocks > 2ll * device.sm_count;
-  const GemvVariant v = shared == 1 ? few<1, 8, 8>(half) : shared == 2 ? few<2, 4, 8>(half) : shared <= 4 ? few<4, 2, 4>(half) :
+  // Three and four rows take the ring where a warp has a long way to go: 4096 x 7168 7.0 us without and 6.8 with it,
+  // 8192 x 8192 11.4 and 10.1, 14336 x 14336 30.6 and 27.2; 28416 x 4096 16.7 and 18.2, 14336 x 2048 5.9 and 6.2, 1024 x 512
+  // 1.9 and 2.3.  Two rows 4096 x 7168 6.4 and 6.9.
+  const GemvVariant v = shared == 1 ? few<1, 8, 8>(half) : shared == 2 ? few<2, 4, 8>(half) :
+                        shared <= 4 && k <= 4096 ? few<4, 2, 4>(half) :
                         shared <= 8 ? many_rows<8>() : many_rows<16>();
   if (int rc = allow_smem(v, device.device)) return rc;
   // CTAs of a cluster: the fewest with which a warp has the least to do, where all CTAs are resident at once.
