@@ -5,6 +5,7 @@
 
 #include "../../include/chord_b200.h"
 #include "common.h"
+#include "join_plan.h"
 #include "kv_cache.cuh"
 #include "warp_ops.cuh"
 
@@ -15,12 +16,9 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCtasPerSm = 3;
 constexpr int kMaxCtas = 480;      // of a launch: three on each of 160 SMs
-// Parts of a row that one CTA joins at once: up to kAtOnce of them; more than that by groups of half as many
-// neighbours or, where that would leave more than as many groups, of kFan.
-constexpr int kAtOnce = 16, kFan = 24;
-// A lot's lock word: arrivals of its row's CTAs or groups (11 bits), of its row's first group, and of the
-// group that the lot is the first of (6 bits each).
-constexpr int kRowShift = 0, kFirstShift = 11, kFanShift = 17;
+// A lot's lock word: arrivals at the last join of the row that it is the first lot of (11 bits), and at the join of
+// the group that it is the first of (6 bits).
+constexpr int kRowShift = 0, kGroupShift = 11;
 static_assert(kMaxCtas < (1 << 11) && kFan < (1 << 6), "the fields' widths");
 
 struct AttentionParams {
@@ -64,7 +62,6 @@ struct Layout {
 __host__ __device__ constexpr int64_t part_floats(int dim, int heads) { return heads * (dim + 2); }
 
 // Floats of workspace: kSlots parts for each lot, one for each warp.
-constexpr int kSlots = 3;
 constexpr int64_t workspace_floats(int64_t ctas, int dim, int heads) {
   return ctas * (kSlots + kWarps) * part_floats(dim, heads);
 }
@@ -300,7 +297,7 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 // cp.async stages that runs ahead across the rows' ends, and a running maximum, sum and output.  Rows
 // that lie in one quarter are finished by their warp; the others' parts are joined within the CTA once
 // all its warps are done, and then, through memory, by the last CTA of a row to arrive (with more than
-// kFan parts by the last of each kFan neighbours, and the last of these).
+// kAtOnce parts by the last of each group of 8 or 24 neighbours, and the last of these).
 //
 // Products on mma.m16n8k16, keys and values as the 16-row operand, the heads (eight for each of kTiles)
 // as columns: S[tokens, heads] = K Q^T and O[dims, heads] += V^T P, P by movmatrix from the score
@@ -877,9 +874,7 @@ paged_attention_kernel(const AttentionParams p) {
   __syncthreads();
 
   // Joins.  First the lot's own: parts of one row are neighbours, and a part at an even place ends its row.
-  // A lot's slots: for the row that it begins inside of, for the one that it ends inside of, and for the join
-  // of kFan neighbours.
-  auto slot_of = [&](int32_t of_lot, int which) { return p.partials + (kSlots * static_cast<int64_t>(of_lot) + which) * kPartFloats; };
+  auto slot_of = [&](int32_t of_lot, int32_t which) { return p.partials + (kSlots * static_cast<int64_t>(of_lot) + which) * kPartFloats; };
   int32_t pending[2] = {0, 0}, waiting = 0;
   uint32_t there = 0;
 #pragma unroll
@@ -899,7 +894,7 @@ paged_attention_kernel(const AttentionParams p) {
     const bool began = parts[first].began, whole = ended && !began;
     if (!whole) pending[waiting++] = first;
     const Row of(p, parts[first].b, parts[first].row);
-    joined.template give<kCodes>(p, of, whole ? nullptr : slot_of(lot, began ? 0 : 1));
+    joined.template give<kCodes>(p, of, whole ? nullptr : slot_of(lot, began ? kSlotInside : kSlotFirst));
   }
   if (waiting == 0) return;
 
@@ -908,26 +903,26 @@ paged_attention_kernel(const AttentionParams p) {
 #pragma unroll 1
   for (; waiting > 0; --waiting) {
     const Part part = parts[pending[waiting - 1]];
-    const bool twice = part.lots > kAtOnce;
-    const int32_t fan = part.lots <= kAtOnce * kAtOnce / 4 ? kAtOnce / 2 : kFan;
+    const RowJoin join(part.first_lot, part.lots);
+    const int32_t begin = join.group_of(lot), of_group = join.group_lots(begin);
     const Row of(p, part.b, part.row);
 #pragma unroll 1
-    for (int level = twice ? 0 : 1; level < 2; ++level) {
-      const int32_t from = level == 0 ? (lot - part.first_lot) / fan * fan : 0, stride = level == 1 && twice ? fan : 1;
-      const int32_t count = level == 0 ? min(fan, part.lots - from) : (part.lots + stride - 1) / stride;
+    for (int level = of_group > 1 ? 0 : 1; level < 2; ++level) {
+      const int32_t count = level == 0 ? of_group : join.groups();
       __syncthreads();
       if (threadIdx.x == 0) {
-        const int shift = level == 1 ? kRowShift : from == 0 ? kFirstShift : kFanShift;
-        int32_t* const word = p.locks + part.first_lot + from;
+        const int shift = level == 1 ? kRowShift : kGroupShift;
+        int32_t* const word = p.locks + part.first_lot + (level == 0 ? begin : 0);
         const int32_t before = atomic_add_acq_rel(word, 1 << shift) >> shift & (level == 1 ? (1 << 11) - 1 : (1 << 6) - 1);
         answer[level] = before == count - 1;
         if (before == count - 1) atomicSub(word, count << shift);
       }
       __syncthreads();
       if (!answer[level]) break;
-      float* const to = level == 0 ? slot_of(part.first_lot + from, 2) : nullptr;
+      float* const to = level == 0 ? slot_of(part.first_lot + begin, kSlotGroup) : nullptr;
       join_parts<kDim, kCodes, kHeads, L::kSmem>(p, of, smem, count, to, [&](int32_t j) {
-        return slot_of(part.first_lot + from + j * stride, stride > 1 ? 2 : from + j == 0 ? 1 : 0);
+        const PartPlace at_part = level == 0 ? join.part(begin, j) : join.joined(j);
+        return slot_of(at_part.lot, at_part.slot);
       });
     }
   }
