@@ -36,6 +36,23 @@ class Shape:
 
 
 FEW_TOKENS = 4  # up to here every token's experts are read for it alone
+MAX_BATCH = 16  # rows of a gemv
+
+
+def slots_for(tables: torch.Tensor, positions: torch.Tensor, page: int) -> torch.Tensor:
+    """Where each sequence's token at its position is kept; nowhere (-1) past the last page of its table, so that
+    a sequence that has outgrown its pages is reported by check_status and touches nothing."""
+    pages = tables.shape[1]
+    index = positions // page
+    slots = tables.gather(1, index.clamp(0, pages - 1).long()[:, None])[:, 0] * page + positions % page
+    return torch.where((index >= 0) & (index < pages), slots, -1).to(torch.int32)
+
+
+def _check_sizes(shape: Shape, batch: int, steps: int) -> None:
+    if not 1 <= batch <= MAX_BATCH:
+        raise ValueError(f"batch must be from 1 to {MAX_BATCH}, got {batch}")
+    if not 1 <= steps <= shape.max_tokens - 4:
+        raise ValueError(f"steps must be from 1 to {shape.max_tokens - 4}, got {steps}")
 
 
 def _packed(experts, n, k, g, keep):
@@ -76,8 +93,7 @@ class DecodeLayer:
     def attention(self, x: torch.Tensor) -> torch.Tensor:
         s = self.shape
         positions = self.lengths.clone()
-        page = self.tables.gather(1, (positions // s.page).long()[:, None])[:, 0]
-        slots = page * s.page + positions % s.page
+        slots = slots_for(self.tables, positions, s.page)
         qkv = chord_b200.gemv(x, self.qkv).view(self.batch, s.heads + 2 * s.kv_heads, s.head_dim)
         q, k, v = qkv.split([s.heads, s.kv_heads, s.kv_heads], dim=1)
         q = chord_b200.qk_norm_rope_write(q, k, v, self.q_weight, self.k_weight, self.cos_sin, positions, self.cache,
@@ -151,6 +167,7 @@ class PlainLayer:
 
 def compare(shape: Shape, batch: int, steps: int, bits: int, seed: int = 0) -> float:
     """Relative distance (2-norm) of the layer's outputs from the plain layer's, over all steps."""
+    _check_sizes(shape, batch, steps)
     layer = DecodeLayer(shape, batch, bits, seed)
     plain = PlainLayer(layer)
     g = torch.Generator(device="cuda").manual_seed(seed + 1)
@@ -166,6 +183,7 @@ def compare(shape: Shape, batch: int, steps: int, bits: int, seed: int = 0) -> f
 
 def time_step(shape: Shape, batch: int, steps: int, bits: int) -> float:
     """Microseconds of a step, replayed from a CUDA graph."""
+    _check_sizes(shape, batch, steps)
     layer = DecodeLayer(shape, batch, bits)
     x = torch.randn((batch, shape.hidden), device="cuda").to(torch.bfloat16)
     for _ in range(2):
@@ -191,6 +209,10 @@ def main():
     ap.add_argument("--steps", type=int, default=64)
     ap.add_argument("--bits", type=int, default=8, choices=[8, 16])
     a = ap.parse_args()
+    try:
+        _check_sizes(Shape(), a.batch, a.steps)
+    except ValueError as e:
+        ap.error(str(e))
     print(f"relative distance from FP32 over {a.steps} tokens: {compare(Shape(), a.batch, a.steps, a.bits):.2e}")
     print(f"a step: {time_step(Shape(), a.batch, a.steps, a.bits):.1f} us")
 
