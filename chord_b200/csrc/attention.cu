@@ -104,6 +104,15 @@ __device__ __forceinline__ void add_weighted(float4& v, const float4& weight, co
   v.w = fmaf(weight.w, x.w, v.w);
 }
 
+// Two numbers of at least zero as sums of two BF16 numbers each, to 2^-16.  Both parts of a number above zero are
+// above zero (its last bit is set, the first part is cut off and not rounded), so that an infinity times the
+// number is an infinity and not the difference of two, or zero times one.
+__device__ __forceinline__ void positive_parts(float x, float y, uint32_t& coarse, uint32_t& fine) {
+  const uint32_t a = __float_as_uint(x) | 1u, b = __float_as_uint(y) | 1u;
+  coarse = __byte_perm(a, b, 0x7632);
+  fine = pack_bf16(__uint_as_float(a) - __uint_as_float(a & 0xFFFF0000u), __uint_as_float(b) - __uint_as_float(b & 0xFFFF0000u));
+}
+
 // Reads of parts, in shared memory or written by another CTA.
 __device__ __forceinline__ float4 read_part4(const float* p) {
   float4 v;
@@ -301,7 +310,8 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 //
 // Products on mma.m16n8k16, keys and values as the 16-row operand, the heads (eight for each of kTiles)
 // as columns: S[tokens, heads] = K Q^T and O[dims, heads] += V^T P, P by movmatrix from the score
-// fragments.  (With the heads as rows, half of every product was idle with up to eight of them.)  P is multiplied as the sum of two BF16 numbers, 16 bits of it.
+// fragments.  (With the heads as rows, half of every product was idle with up to eight of them.)  P is multiplied
+// as the sum of two BF16 numbers, 16 bits of it.
 // Codes are exact in BF16; the keys' scales are applied to the scores, the values' to P.  The codes of
 // values become (code - 128) / 64.  Those of keys are multiplied as they stand, as the BF16 numbers
 // code * 2^-133, with queries times 2^80: the scores start from minus 128 times the query's sum, which
@@ -756,9 +766,15 @@ paged_attention_kernel(const AttentionParams p) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float x = s[j][n][2 * i], y = s[j][n][2 * i + 1];
-            const uint32_t coarse = pack_bf16(x, y);
+            uint32_t coarse, fine;
+            if constexpr (kCodes) {
+              coarse = pack_bf16(x, y);
+              fine = pack_bf16(x - bf16_lo(coarse), y - bf16_hi(coarse));
+            } else {
+              positive_parts(x, y, coarse, fine);
+            }
             two[0][n][i] = transposed(coarse);
-            two[1][n][i] = transposed(pack_bf16(x - bf16_lo(coarse), y - bf16_hi(coarse)));
+            two[1][n][i] = transposed(fine);
           }
         }
         auto multiply = [&](int c, const uint32_t (&a)[4]) {
