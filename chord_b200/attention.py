@@ -299,7 +299,8 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     are written first.  ``window`` keeps the last so many tokens.  ``scale`` is ``head_dim ** -0.5``
     where it is not given.  Returns BF16 ``[batch, heads, head_dim]``; ``lse``, if given, FP32 ``[batch,
     heads]``, receives the logarithm of each softmax's sum, with which results over parts of a
-    sequence can be joined.  A sequence of length zero gives zeros and minus infinity.
+    sequence can be joined.  A sequence of length zero gives zeros and minus infinity; a head whose query
+    holds an infinity gives NaN over an 8-bit cache.
 
     Page ids outside the cache count as keys and values of zero and, like lengths beyond the
     table, are reported by :func:`chord_b200.check_status`.  ``locks`` is as for ``indexed``: zeroed

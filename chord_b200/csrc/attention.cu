@@ -33,7 +33,7 @@ struct AttentionParams {
   int32_t* status;
   int64_t q_batch, q_head, table_stride;
   int32_t batch, heads, group, head_blocks, capacity, window;
-  float scale;  // of the scores, with log2(e) and, for codes, 2^53
+  float scale;  // of the scores, with log2(e)
   bool whole_groups;
 };
 
@@ -132,7 +132,11 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
   return n / d;
 }
 
-__device__ __forceinline__ float rate_of(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+// What outputs are multiplied with: those of codes are 64ths.
+template <bool kCodes>
+__device__ __forceinline__ float rate_of(float sum) { return sum == 0.0f ? 0.0f : (kCodes ? 64.0f : 1.0f) / sum; }
+
+__device__ __forceinline__ float power_of_two(int32_t exponent) { return __int_as_float((exponent + 127) << 23); }
 
 // An 8x8 matrix of 16-bit elements, a row in four lanes, to its transpose.
 __device__ __forceinline__ uint32_t transposed(uint32_t pair) {
@@ -160,7 +164,7 @@ struct Row {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (head + i >= heads) break;
-      p.out[(head0 + head + i) * kDim + dim] = __float2bfloat16(value[i] * rate_of(sum[i]));
+      p.out[(head0 + head + i) * kDim + dim] = __float2bfloat16(value[i] * rate_of<kCodes>(sum[i]));
       if (place == 0 && p.lse != nullptr) p.lse[head0 + head + i] = lse_of(top[i], sum[i]);
     }
   }
@@ -314,8 +318,8 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 // as the sum of two BF16 numbers, 16 bits of it.
 // Codes are exact in BF16; the keys' scales are applied to the scores, the values' to P.  The codes of
 // values become (code - 128) / 64.  Those of keys are multiplied as they stand, as the BF16 numbers
-// code * 2^-133, with queries times 2^80: the scores start from minus 128 times the query's sum, which
-// saves a multiply-add for every two codes.
+// code * 2^-133, with queries times a power of two that takes the row's largest (finite) one to 2^111 or just
+// above: the scores start from minus 128 times the query's sum, which saves a multiply-add for every two codes.
 //
 // The running maximum is raised, and the sums are scaled, only where a score passes it by more than
 // 2^kSlack; until then P is up to 2^kSlack, which costs no precision, and no lane needs another's scores.
@@ -596,6 +600,7 @@ paged_attention_kernel(const AttentionParams p) {
 
     uint32_t qf[kChunks][kTiles][2];
     float start[kTiles][2] = {};
+    float of_scores = p.scale, of_codes = 1.0f;  // factors of the scores
     // A lane's heads are 8 n + 2 q4 and the next; of the dims it has rows r8 and r8 + 8 of each chunk.
     float out[kChunks][kTiles][4], top[kTiles][2], sum[kTiles][2];
     bool began = at.token > at.begin;  // in an earlier share
@@ -621,27 +626,64 @@ paged_attention_kernel(const AttentionParams p) {
               qf[c][n][i] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + head * p.q_head + dim)) : 0u;
             }
           }
-          if constexpr (kCodes) {
-            // queries times 2^80, and what the scores start from
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) out[c][n][0] = out[c][n][1] = out[c][n][2] = out[c][n][3] = 0.0f;
+          top[n][0] = top[n][1] = -INFINITY;
+          sum[n][0] = sum[n][1] = 0.0f;
+        }
+        if constexpr (kCodes) {
+          // The largest magnitude among the row's heads, infinities and NaN left out (their heads are NaN).
+          uint32_t most_of_two = 0;
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) most_of_two = __vmaxu2(most_of_two, qf[c][n][i] & 0x7FFF7FFFu);
+            }
+          }
+          uint32_t largest = __reduce_max_sync(0xffffffffu, max(most_of_two & 0xFFFFu, most_of_two >> 16));
+          if (largest >= 0x7F80u) {
+            largest = 0;
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+              for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const uint32_t low = qf[c][n][i] & 0x7FFFu, high = qf[c][n][i] >> 16 & 0x7FFFu;
+                  largest = max(largest, max(low < 0x7F80u ? low : 0u, high < 0x7F80u ? high : 0u));
+                }
+              }
+            }
+            largest = __reduce_max_sync(0xffffffffu, largest);
+          }
+          // It lies below 2^(biased exponent - 126).  The queries' factor is 2^up, in two where one BF16 number does
+          // not hold it; that of the scores 2^(133 - up), in two that FP32 holds whatever it is.
+          const int32_t up = 238 - max(static_cast<int32_t>(largest >> 7), 1), rest = 133 - up;
+          const uint32_t factor = static_cast<uint32_t>(min(up, 127) + 127) * 0x00800080u;
+          const uint32_t factor2 = static_cast<uint32_t>(max(up - 127, 0) + 127) * 0x00800080u;
+          of_codes = power_of_two(rest >> 1);
+          of_scores = p.scale * power_of_two(rest - (rest >> 1));
+          constexpr uint32_t kMinusZero = 0x80008000u;
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
             float all = 0.0f;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
+                qf[c][n][i] = bf16x2_fma(qf[c][n][i], factor, kMinusZero);
+                if (up > 127) qf[c][n][i] = bf16x2_fma(qf[c][n][i], factor2, kMinusZero);
                 all += bf16_lo(qf[c][n][i]) + bf16_hi(qf[c][n][i]);
-                qf[c][n][i] = bf16x2_fma(qf[c][n][i], 0x67806780u, 0x80008000u);  // times 2^80, minus zero
               }
             }
             all += __shfl_xor_sync(0xffffffffu, all, 1);
             all += __shfl_xor_sync(0xffffffffu, all, 2);
-            all *= -128.0f * 0x1p-53f;
+            all *= -0x1p-126f;  // -128 codes
             start[n][0] = __shfl_sync(0xffffffffu, all, 8 * q4);
             start[n][1] = __shfl_sync(0xffffffffu, all, 8 * q4 + 4);
           }
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) out[c][n][0] = out[c][n][1] = out[c][n][2] = out[c][n][3] = 0.0f;
-          top[n][0] = top[n][1] = -INFINITY;
-          sum[n][0] = sum[n][1] = 0.0f;
         }
       }
 
@@ -690,10 +732,10 @@ paged_attention_kernel(const AttentionParams p) {
       for (int j = 0; j < kGroups; ++j) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float f = p.scale;
+          float f = of_scores;
           if constexpr (kCodes) {
-            f *= scales[16 * j + 8 * i + r8];
-            value_scale[j][i] = 64.0f * scales[L::kStep + 16 * j + 8 * i + r8];
+            f = f * scales[16 * j + 8 * i + r8] * of_codes;
+            value_scale[j][i] = scales[L::kStep + 16 * j + 8 * i + r8];
           }
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) s[j][n][2 * i] *= f, s[j][n][2 * i + 1] *= f;
@@ -827,7 +869,7 @@ paged_attention_kernel(const AttentionParams p) {
         const int64_t head0 = of.head0;
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
-          const float rate[2] = {rate_of(sum[n][0]), rate_of(sum[n][1])};
+          const float rate[2] = {rate_of<kCodes>(sum[n][0]), rate_of<kCodes>(sum[n][1])};
           __nv_bfloat16* to = p.out + (head0 + 8 * n + r8) * kDim;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
@@ -1073,7 +1115,7 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, c
   p.group = static_cast<int32_t>(group);
   p.head_blocks = static_cast<int32_t>(head_blocks);
   p.window = static_cast<int32_t>(window);
-  p.scale = static_cast<float>(scale * 1.4426950408889634074 * (codes ? 0x1p53 : 1.0));
+  p.scale = static_cast<float>(scale * 1.4426950408889634074);
   p.whole_groups = cache->page_size % 16 == 0 && p.cache.token < (1ll << 31);
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), v.smem,
                            static_cast<cudaStream_t>(stream), kEarlyLaunch, p));

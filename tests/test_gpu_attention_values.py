@@ -36,3 +36,41 @@ def test_infinite_values(device, dim, heads, kv_heads, length):
         out[:, :, name] = 0
     check(q, cache, table, lengths, out, lse)
     assert torch.equal(torch.isfinite(want[1]), torch.isfinite(lse))
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (128, 16, 2), (192, 12, 1), (256, 8, 8)])
+@pytest.mark.parametrize("power", [-100, -60, -20, 20, 47, 50, 80, 112])
+def test_queries_of_every_size_over_codes(device, power, dim, heads, kv_heads):
+    """Queries times 2^power and keys' scales divided by it: the scores are as they were."""
+    q, cache, table, lengths = make(device, [700, 33, 1], heads, kv_heads, dim, 16, 8, seed=dim + power)
+    q = (q.double() * 2.0 ** power).to(torch.bfloat16)
+    cache.k_scale.copy_((cache.k_scale.double() * 2.0 ** -power).float())
+    out, lse = run(q, cache, table, lengths)
+    check(q, cache, table, lengths, out, lse)
+
+
+def test_heads_of_unlike_sizes_over_codes(device):
+    """Heads that share keys, their queries 2^80 apart: the small ones' scores are near zero, not lost; a head with an
+    infinity or a NaN is NaN and changes no other."""
+    q, cache, table, lengths = make(device, [500, 80], 8, 1, 128, 16, 8, seed=4)
+    q[:, 1] = (q[:, 1].double() * 2.0 ** 60).to(torch.bfloat16)
+    q[:, 2] = (q[:, 2].double() * 2.0 ** -20).to(torch.bfloat16)
+    q[:, 3] = 0
+    out, lse = run(q, cache, table, lengths)
+    check(q, cache, table, lengths, out, lse)
+    for value in (math.inf, -math.inf, math.nan):
+        odd = q.clone()
+        odd[0, 5, 7] = value
+        got, got_lse = run(odd, cache, table, lengths)
+        assert bool(torch.isnan(got[0, 5]).all()) and bool(torch.isnan(got_lse[0, 5]))
+        keep = torch.ones((2, 8), dtype=torch.bool, device=device)
+        keep[0, 5] = False
+        assert torch.equal(got[keep], out[keep]) and torch.equal(got_lse[keep], lse[keep])
+
+
+@pytest.mark.parametrize("power", [-80, -20, 40, 100, 118])
+def test_values_of_every_size_over_codes(device, power):
+    q, cache, table, lengths = make(device, [900, 20], 8, 2, 128, 16, 8, seed=power + 200)
+    cache.v_scale.copy_((cache.v_scale.double() * 2.0 ** power).float())
+    out, lse = run(q, cache, table, lengths)
+    check(q, cache, table, lengths, out, lse)
