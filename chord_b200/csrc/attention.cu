@@ -320,6 +320,8 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 // values become (code - 128) / 64.  Those of keys are multiplied as they stand, as the BF16 numbers
 // code * 2^-133, with queries times a power of two that takes the row's largest (finite) one to 2^111 or just
 // above: the scores start from minus 128 times the query's sum, which saves a multiply-add for every two codes.
+// Their additions are then off by FP32's roundings of up to 383 sum |q| steps (dim / 16 + 4 times 2^-22 of it), where the keys'
+// own codes are off by up to half a step: under half a percent of that, however close to 128 the codes lie.
 //
 // The running maximum is raised, and the sums are scaled, only where a score passes it by more than
 // 2^kSlack; until then P is up to 2^kSlack, which costs no precision, and no lane needs another's scores.

@@ -456,6 +456,8 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
  * values of head h / (heads / kv_heads).  lse[b, h] (optional) = log sum_t exp(scale * q . k_t).
  * A sequence without tokens, or whose scores are all minus infinity, gets zeros and an lse of minus
  * infinity; a head whose query holds an infinity gets NaN over an 8-bit cache.
+ * Scores over an 8-bit cache are exact to (head_dim / 16 + 4) 2^-22 383 |scale| k_scale sum |q|, half a percent of
+ * what the keys' rounding to codes may cost; over BF16 to (head_dim / 16 + 4) 2^-22 |scale| sum |q k|.
  *  q        bf16 [batch, heads, head_dim], strides in elements (multiples of 8)
  *  cache    head_dim 64, 96, 128, 192 or 256; heads % cache->heads == 0
  *  tables, table_stride, max_pages  as above; lengths int32 [batch], at most

@@ -74,3 +74,24 @@ def test_values_of_every_size_over_codes(device, power):
     cache.v_scale.copy_((cache.v_scale.double() * 2.0 ** power).float())
     out, lse = run(q, cache, table, lengths)
     check(q, cache, table, lengths, out, lse)
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (128, 64, 8), (256, 12, 1)])
+def test_codes_near_the_middle(device, dim, heads, kv_heads):
+    """Keys with one large element each, whose other codes lie about 128: sums of codes times queries are far larger
+    than the scores.  Each of dim / 16 + 4 additions is off by up to 2^-22 of (255 + 128) sum |q| steps, under half a percent
+    of the half step that a code may be off itself."""
+    q, cache, table, lengths = make(device, [1500, 40], heads, kv_heads, dim, 16, 8, seed=dim)
+    g = torch.Generator(device=device).manual_seed(dim)
+    cache.k.copy_(torch.randint(125, 132, cache.k.shape, generator=g, device=device, dtype=torch.int32))
+    cache.k[..., 17] = torch.where(torch.rand(cache.k.shape[:3], generator=g, device=device) < 0.5, 1, 255).to(torch.uint8)
+    cache.k_scale.mul_(40)   # (as large as with elements of about 50)
+    q.abs_()
+    out, lse = run(q, cache, table, lengths)
+    want, want_lse, value_size, _ = A.attention(q, *A.stored(cache), table, lengths, 16)
+    steps = cache.k_scale.double().amax() * q.double().abs().sum(-1) * dim ** -0.5
+    score = (dim / 16 + 4) * A.SINGLE * (255 + 128) * steps + 2.0 ** -20 * (1 + want_lse.abs())
+    assert float((score - 2.0 ** -20 * (1 + want_lse.abs())).max()) < 0.005 * float((0.5 * steps).max())
+    assert bool(((lse.double() - want_lse).abs() <= score).all())
+    limit = A.HALF * want.abs() + (2.0 ** -16 + 2 * score[..., None]) * value_size * 1.01
+    assert bool(((out.double() - want).abs() <= limit).all())
