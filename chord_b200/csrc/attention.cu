@@ -358,7 +358,7 @@ paged_attention_kernel(const AttentionParams p) {
   // The tokens of sequence b that are seen, from `begin` to the one returned; steps count from a
   // multiple of kStep.
   auto extent = [&](int32_t b, int32_t& begin) {
-    const int32_t length = max(0, min(__ldg(p.lengths + b), p.capacity));
+    const int32_t length = max(0, min(load_arg(p.lengths + b), p.capacity));
     begin = p.window > 0 && length > p.window ? length - p.window : 0;
     return length;
   };
@@ -431,7 +431,7 @@ paged_attention_kernel(const AttentionParams p) {
   // Sequences with nothing to attend to, and lengths that the table cannot hold.
 #pragma unroll 1
   for (int32_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (threadIdx.x == 0 && p.status != nullptr && __ldg(p.lengths + b) > p.capacity) atomicOr(p.status, kStatusIndex);
+    if (threadIdx.x == 0 && p.status != nullptr && load_arg(p.lengths + b) > p.capacity) atomicOr(p.status, kStatusIndex);
     if (steps_of(b) != 0) continue;
     const int64_t row = static_cast<int64_t>(b) * p.heads;
 #pragma unroll 1
@@ -530,7 +530,7 @@ paged_attention_kernel(const AttentionParams p) {
       if (token < ahead.end && token + (p.whole_groups ? 15 : 0) >= ahead.begin) {
         const uint32_t index = p.cache.page_size.div(token);
         ref_place = token - index * p.cache.page_size.d;
-        ref_page = __ldg(row_table + index);
+        ref_page = load_arg(row_table + index);
       }
     };
     auto load = [&]() {
@@ -625,7 +625,7 @@ paged_attention_kernel(const AttentionParams p) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int dim = 16 * c + (kCodes ? 4 * q4 + 2 * i : 2 * q4 + 8 * i);
-              qf[c][n][i] = head < heads ? __ldg(reinterpret_cast<const uint32_t*>(q + head * p.q_head + dim)) : 0u;
+              qf[c][n][i] = head < heads ? load_arg(reinterpret_cast<const uint32_t*>(q + head * p.q_head + dim)) : 0u;
             }
           }
 #pragma unroll

@@ -80,7 +80,7 @@ __device__ __forceinline__ void join_and_store(const GemvParams& p, float* sums,
 
 // The row's expert; false: one that another GPU holds, whose row is stored as zeros.
 __device__ __forceinline__ bool find_expert(const GemvParams& p, int64_t out_row, int block, int32_t* expert) {
-  const int64_t local = static_cast<int64_t>(__ldg(p.expert_ids + out_row)) - p.expert_base;
+  const int64_t local = static_cast<int64_t>(load_arg(p.expert_ids + out_row)) - p.expert_base;
   *expert = static_cast<int32_t>(local);
   if (local >= 0 && local < p.num_experts) return true;
   if (blockIdx.x == 0 && threadIdx.x < 64) p.out[out_row * p.n + block * 64 + threadIdx.x] = __float2bfloat16(0.0f);
@@ -138,7 +138,7 @@ __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& a
       const bool there = token < at.rows && g < groups;
       const uint32_t* const from = reinterpret_cast<const uint32_t*>(x + (there ? 32 * g : 0));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xr[set][i] = there ? __ldg(from + 4 * i) : 0u;
+      for (int i = 0; i < 4; ++i) xr[set][i] = there ? load_arg(from + 4 * i) : 0u;
     }
 #pragma unroll
     for (int set = 0; set < kSets; ++set) {

@@ -81,7 +81,7 @@ __device__ __forceinline__ uint4 undeal(const uint4 v) {
 
 __device__ __forceinline__ uint2 undeal(const uint2 v) { return make_uint2(__byte_perm(v.x, v.y, 0x5140), __byte_perm(v.x, v.y, 0x7362)); }
 
-__device__ __forceinline__ uint2 load8_once_coherent(const void* p) {
+__device__ __forceinline__ uint2 load8_once_ordered(const void* p) {
   uint2 v;
   asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
   return v;
@@ -180,14 +180,14 @@ heads_kernel(const HeadsParams p) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const bool there = row + i * kSide < end && inside;
-        const uint2 a = there ? load8_once_coherent(from) : make_uint2(0, 0), b = there ? load8_once_coherent(from + away) : make_uint2(0, 0);
+        const uint2 a = there ? load8_once_ordered(from) : make_uint2(0, 0), b = there ? load8_once_ordered(from + away) : make_uint2(0, 0);
         raw[i] = make_uint4(a.x, a.y, b.x, b.y);
         from += kSide * stride;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        raw[i] = row + i * kSide < end && inside ? load_once_coherent(from) : make_uint4(0, 0, 0, 0);
+        raw[i] = row + i * kSide < end && inside ? load_once_ordered(from) : make_uint4(0, 0, 0, 0);
         from += kSide * stride;
       }
     }
@@ -199,13 +199,13 @@ heads_kernel(const HeadsParams p) {
   if constexpr (kRotate) {
     if (!is_v) {
       const __nv_bfloat16* const weight = is_q ? p.q_weight : p.k_weight;
-      const int32_t position = __ldg(p.positions + token);
+      const int32_t position = load_arg(p.positions + token);
       lost = position < 0 || position >= p.max_positions;
       if (lost && p.status != nullptr && lane == 0) atomicOr(p.status, kStatusIndex);
       uint2 w0 = make_uint2(0, 0), w1 = make_uint2(0, 0);
       if (inside) {
-        w0 = __ldg(reinterpret_cast<const uint2*>(weight + first));
-        w1 = __ldg(reinterpret_cast<const uint2*>(weight + second));
+        w0 = load_arg(reinterpret_cast<const uint2*>(weight + first));
+        w1 = load_arg(reinterpret_cast<const uint2*>(weight + second));
       }
       uint4 words = make_uint4(w0.x, w0.y, w1.x, w1.y);
       if (dealt) words = deal(words);
@@ -215,7 +215,7 @@ heads_kernel(const HeadsParams p) {
         own = Eight{};
       } else if (turned) {
         const float* const at = p.cos_sin + static_cast<int64_t>(position) * p.rotary + 4 * chunk;
-        const float4 c = __ldg(reinterpret_cast<const float4*>(at)), s = __ldg(reinterpret_cast<const float4*>(at + half));
+        const float4 c = load_arg(reinterpret_cast<const float4*>(at)), s = load_arg(reinterpret_cast<const float4*>(at + half));
         const float2 cs[2] = {{c.x, c.y}, {c.z, c.w}}, sn[2] = {{s.x, s.y}, {s.z, s.w}}, minus[2] = {{-s.x, -s.y}, {-s.z, -s.w}};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -231,7 +231,7 @@ heads_kernel(const HeadsParams p) {
   int64_t offset = 0, scale_offset = 0;  // of the token's first row here
   if constexpr (kWrite) {
     if (!is_q) {
-      const int32_t slot = __ldg(p.slots + token);
+      const int32_t slot = load_arg(p.slots + token);
       const uint32_t page = slot >= 0 ? p.cache.page_size.div(static_cast<uint32_t>(slot)) : 0;
       const uint32_t in_page = static_cast<uint32_t>(slot) - page * p.cache.page_size.d;
       kept = slot >= 0 && page < static_cast<uint32_t>(p.cache.num_pages);
@@ -372,18 +372,18 @@ cache_read_kernel(const ReadParams p) {
   while (count > 1) {
     const int32_t step = (count + 31) / 32;
     const int32_t at = lane * step;
-    const bool before = at < count && __ldg(p.offsets + low + at) <= token;
+    const bool before = at < count && load_arg(p.offsets + low + at) <= token;
     const uint32_t votes = __ballot_sync(0xffffffffu, before);
     const int32_t last = votes == 0 ? 0 : 31 - __clz(votes);
     low += last * step;
     count = min(step, count - last * step);
   }
-  const int32_t begin = __ldg(p.offsets + low);
+  const int32_t begin = load_arg(p.offsets + low);
   int64_t page_offset = -1, scale_offset = 0;
-  if (token >= begin && token < __ldg(p.offsets + low + 1)) {
+  if (token >= begin && token < load_arg(p.offsets + low + 1)) {
     const uint32_t at = static_cast<uint32_t>(token) - static_cast<uint32_t>(begin);
     const uint32_t index = p.cache.page_size.div(at), in_page = at - index * p.cache.page_size.d;
-    const int32_t page = begin >= 0 && index < static_cast<uint32_t>(p.max_pages) ? __ldg(p.tables + low * p.table_stride + index) : -1;
+    const int32_t page = begin >= 0 && index < static_cast<uint32_t>(p.max_pages) ? load_arg(p.tables + low * p.table_stride + index) : -1;
     if (page >= 0 && page < p.cache.num_pages) {
       page_offset = page * p.cache.page + in_page * p.cache.token;
       scale_offset = page * p.cache.scale_page + in_page * p.cache.scale_token;
@@ -417,8 +417,8 @@ cache_read_kernel(const ReadParams p) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const bool there = known && inside && first + i * kSide < end;
-        raw[i] = there ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
-        scale[i] = there ? __ldg(scale_at) : 0.0f;
+        raw[i] = there ? load_arg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+        scale[i] = there ? load_arg(scale_at) : 0.0f;
         at += kSide * p.cache.head;
         scale_at += kSide * p.cache.scale_head;
       }

@@ -65,3 +65,17 @@ int main() {
 def test_alignment_without_a_cluster(tmp_path):
     done = _run(tmp_path, ALIGNMENT)
     assert done.returncode == 0, done.stdout
+
+
+def test_early_launches_read_nothing_through_the_read_only_path():
+    """Kernels that are always launched while the one before them drains (kEarlyLaunch): what they read may be what
+    that one still writes, which the read-only path does not allow."""
+    found = []
+    for path in sorted(CSRC.glob("*.cu")):
+        if "kEarlyLaunch" not in path.read_text():
+            continue
+        for source in (path, CSRC / "warp_ops.cuh", CSRC / "kv_cache.cuh"):
+            code = "\n".join(line.split("//")[0] for line in source.read_text().splitlines())
+            found += [(source.name, word) for word in ("__ldg(", "ld.global.nc", "__restrict__") if word in code]
+    assert not found
+    assert "kEarlyLaunch" in (CSRC / "gemv.cu").read_text()
