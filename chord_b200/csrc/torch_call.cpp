@@ -109,6 +109,19 @@ PyObject* pair(at::Tensor&& a, at::Tensor&& b) {
   return both;
 }
 
+// Without the interpreter's lock: an allocation may wait for the device and a launch for room in its queue, behind
+// a host function that itself wants the lock.
+class Unlocked {
+ public:
+  Unlocked() : state_(PyEval_SaveThread()) {}
+  ~Unlocked() { PyEval_RestoreThread(state_); }
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+
+ private:
+  PyThreadState* state_;
+};
+
 using Call = PyObject* (*)(PyObject*, PyObject* const*, Py_ssize_t);
 
 // A C++ exception (out of memory) ends here; the wrapper then meets it itself.
@@ -151,11 +164,15 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t count) {
       return none();
     ids = t.const_data_ptr<int32_t>();
   }
-  at::Tensor out = empty({rows, n}, *x);
-  if (entries.gemv(x->const_data_ptr(), stride, static_cast<const int32_t*>(packed->const_data_ptr()), scale->const_data_ptr(), ids,
-                   out.mutable_data_ptr(), rows, n, k, experts, top_k, base, stream_of(device)))
-    return none();
-  return THPVariable_Wrap(std::move(out));
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = empty({rows, n}, *x);
+    rc = entries.gemv(x->const_data_ptr(), stride, static_cast<const int32_t*>(packed->const_data_ptr()), scale->const_data_ptr(), ids,
+                      out.mutable_data_ptr(), rows, n, k, experts, top_k, base, stream_of(device));
+  }
+  return rc ? none() : THPVariable_Wrap(std::move(out));
 }
 
 struct Rotation {
@@ -196,14 +213,19 @@ bool rotation(PyObject* const* a, int64_t kv_heads, Rotation* r) {
 PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
   Rotation r;
   if (count != 8 || !rotation(a, -1, &r)) return none();
-  at::Tensor q_out = empty(r.q->sizes(), *r.q), k_out = empty(r.k->sizes(), *r.k);
-  if (entries.qk_norm_rope(r.q->const_data_ptr(), r.q->stride(0), r.q->stride(1), r.k->const_data_ptr(), r.k->stride(0), r.k->stride(1),
-                           r.q_weight->const_data_ptr(), r.k_weight->const_data_ptr(), r.table->const_data_ptr<float>(),
-                           r.table->size(0), r.table->size(1), r.interleaved, r.positions, q_out.mutable_data_ptr(),
-                           k_out.mutable_data_ptr(), r.tokens, r.q->size(1), r.k->size(1), r.dim, devices[r.device].status, r.eps,
-                           stream_of(r.device)))
-    return none();
-  return pair(std::move(q_out), std::move(k_out));
+  int32_t* const status = devices[r.device].status;
+  at::Tensor q_out, k_out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    q_out = empty(r.q->sizes(), *r.q), k_out = empty(r.k->sizes(), *r.k);
+    rc = entries.qk_norm_rope(r.q->const_data_ptr(), r.q->stride(0), r.q->stride(1), r.k->const_data_ptr(), r.k->stride(0), r.k->stride(1),
+                              r.q_weight->const_data_ptr(), r.k_weight->const_data_ptr(), r.table->const_data_ptr<float>(),
+                              r.table->size(0), r.table->size(1), r.interleaved, r.positions, q_out.mutable_data_ptr(),
+                              k_out.mutable_data_ptr(), r.tokens, r.q->size(1), r.k->size(1), r.dim, status, r.eps,
+                              stream_of(r.device));
+  }
+  return rc ? none() : pair(std::move(q_out), std::move(k_out));
 }
 
 // qk_norm_rope_write(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, v, cache, device, slots)
@@ -217,14 +239,19 @@ PyObject* qk_norm_rope_write(PyObject*, PyObject* const* a, Py_ssize_t count) {
   const at::Tensor* v = tensor(a[8], at::kBFloat16, 3);
   const int32_t* slots = ints(a[11], device, r.tokens);
   if (!rows(v, device, r.tokens, cache->heads, r.dim) || slots == nullptr) return none();
-  at::Tensor q_out = empty(r.q->sizes(), *r.q);
-  if (entries.qk_norm_rope_write(r.q->const_data_ptr(), r.q->stride(0), r.q->stride(1), r.k->const_data_ptr(), r.k->stride(0),
-                                 r.k->stride(1), v->const_data_ptr(), v->stride(0), v->stride(1), r.q_weight->const_data_ptr(),
-                                 r.k_weight->const_data_ptr(), r.table->const_data_ptr<float>(), r.table->size(0), r.table->size(1),
-                                 r.interleaved, r.positions, q_out.mutable_data_ptr(), cache, slots, r.tokens, r.q->size(1),
-                                 devices[device].status, r.eps, stream_of(device)))
-    return none();
-  return THPVariable_Wrap(std::move(q_out));
+  int32_t* const status = devices[device].status;
+  at::Tensor q_out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    q_out = empty(r.q->sizes(), *r.q);
+    rc = entries.qk_norm_rope_write(r.q->const_data_ptr(), r.q->stride(0), r.q->stride(1), r.k->const_data_ptr(), r.k->stride(0),
+                                    r.k->stride(1), v->const_data_ptr(), v->stride(0), v->stride(1), r.q_weight->const_data_ptr(),
+                                    r.k_weight->const_data_ptr(), r.table->const_data_ptr<float>(), r.table->size(0), r.table->size(1),
+                                    r.interleaved, r.positions, q_out.mutable_data_ptr(), cache, slots, r.tokens, r.q->size(1),
+                                    status, r.eps, stream_of(device));
+  }
+  return rc ? none() : THPVariable_Wrap(std::move(q_out));
 }
 
 // cache_write(k, v, cache, device, slots) -> True
@@ -237,10 +264,15 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t count) {
       !rows(v, device, k->size(0), cache->heads, cache->head_dim))
     return none();
   const int32_t* slots = ints(a[4], device, k->size(0));
-  if (slots == nullptr ||
-      entries.cache_write(k->const_data_ptr(), k->stride(0), k->stride(1), v->const_data_ptr(), v->stride(0), v->stride(1), cache,
-                          slots, k->size(0), devices[device].status, stream_of(device)))
-    return none();
+  if (slots == nullptr) return none();
+  int32_t* const status = devices[device].status;
+  int rc;
+  {
+    const Unlocked unlocked;
+    rc = entries.cache_write(k->const_data_ptr(), k->stride(0), k->stride(1), v->const_data_ptr(), v->stride(0), v->stride(1), cache,
+                             slots, k->size(0), status, stream_of(device));
+  }
+  if (rc) return none();
   Py_RETURN_TRUE;
 }
 
@@ -268,11 +300,16 @@ PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t count) {
   if (offsets == nullptr || offsets->get_device() != device || offsets->size(0) < 2 || offsets->stride(0) != 1 ||
       !table_of(a[2], device, offsets->size(0) - 1, &table))
     return none();
-  at::Tensor k = empty({total, cache->heads, cache->head_dim}, *offsets), v = empty(k.sizes(), *offsets);
-  if (entries.cache_read(cache, table.at, table.stride, table.pages, offsets->const_data_ptr<int32_t>(), offsets->size(0) - 1,
-                         k.mutable_data_ptr(), v.mutable_data_ptr(), total, devices[device].status, stream_of(device)))
-    return none();
-  return pair(std::move(k), std::move(v));
+  int32_t* const status = devices[device].status;
+  at::Tensor k, v;
+  int rc;
+  {
+    const Unlocked unlocked;
+    k = empty({total, cache->heads, cache->head_dim}, *offsets), v = empty(k.sizes(), *offsets);
+    rc = entries.cache_read(cache, table.at, table.stride, table.pages, offsets->const_data_ptr<int32_t>(), offsets->size(0) - 1,
+                            k.mutable_data_ptr(), v.mutable_data_ptr(), total, status, stream_of(device));
+  }
+  return rc ? none() : pair(std::move(k), std::move(v));
 }
 
 // paged_attention(q, cache, device, block_tables, lengths, lse, window, scale)
@@ -304,12 +341,18 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   }
   const int64_t size = entries.workspace_bytes(cache->head_dim, heads / cache->heads);
   if (words == nullptr || size < 0) return none();
-  at::Tensor out = empty(q->sizes(), *q), workspace = empty({size}, *q, at::kByte);
-  if (entries.paged_attention(q->const_data_ptr(), q->stride(0), q->stride(1), cache, table.at, table.stride, table.pages, lengths,
-                              out.mutable_data_ptr(), lse, words, word_count, workspace.mutable_data_ptr(), size,
-                              devices[device].status, batch, heads, window, scale, stream))
-    return none();
-  return THPVariable_Wrap(std::move(out));
+  int32_t* const status = devices[device].status;
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = empty(q->sizes(), *q);
+    const at::Tensor workspace = empty({size}, *q, at::kByte);
+    rc = entries.paged_attention(q->const_data_ptr(), q->stride(0), q->stride(1), cache, table.at, table.stride, table.pages, lengths,
+                                 out.mutable_data_ptr(), lse, words, word_count, workspace.mutable_data_ptr(), size, status, batch,
+                                 heads, window, scale, stream);
+  }
+  return rc ? none() : THPVariable_Wrap(std::move(out));
 }
 
 // entries(addresses of the seven functions, in the struct's order)
