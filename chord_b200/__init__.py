@@ -45,6 +45,8 @@ def __getattr__(name: str) -> Any:
         value = getattr(import_module(_EXPORTS[name]), name)
         globals()[name] = value
         return value
+    if f"{__name__}.{name}" in _EXPORTS.values():  # a module that no name has brought in yet
+        return import_module(f"{__name__}.{name}")
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
