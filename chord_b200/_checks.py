@@ -132,6 +132,26 @@ def bf16_output(outputs, shape: tuple[int, int], device: torch.device, *, exact_
     return outputs
 
 
+def _span(t) -> tuple[int, int]:
+    """The addresses from a tensor's first element to behind its last."""
+    size = t.element_size()
+    return t.data_ptr(), t.data_ptr() + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def apart(name: str, out, other_name: str, other, *, in_place: bool = False) -> None:
+    """A caller's result may not lie where other rows of the same call are still read: ``out`` and ``other``
+    share no memory or, ``in_place``, are the same contiguous elements."""
+    if out.numel() == 0 or other.numel() == 0:
+        return
+    begin, end = _span(out)
+    other_begin, other_end = _span(other)
+    if begin >= other_end or other_begin >= end:
+        return
+    if in_place and begin == other_begin and out.shape == other.shape and other.is_contiguous():
+        return
+    raise ValueError(f"{name} must not overlap {other_name}" + (" unless it is the same contiguous tensor" if in_place else ""))
+
+
 def routing_tensors(sorted_ids, expert_ids, num_tokens_padded, device: torch.device) -> None:
     """The three routing tensors of ``indexed``: contiguous int32 on ``device``, two vectors and one
     element.  All conditions in one expression first, then one by one for the message."""

@@ -178,7 +178,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     columns), element ``i`` with ``i + rotary_dim / 2`` or, ``interleaved``, ``2 i`` with ``2 i + 1``.
     ``positions`` is int32 ``[tokens]``; a position outside the table gives zeros and is reported by
     :func:`chord_b200.check_status`.  Returns BF16 ``(q_out, k_out)``, contiguous; contiguous inputs may be
-    given as their own outputs."""
+    given as their own outputs, and outputs overlap nothing else of the call."""
     direct = _lib.direct()
     if direct is not None and q_out is None and k_out is None:
         result = direct.qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved)
@@ -186,8 +186,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
             return result
     device, tokens, heads, dim, q_rows, k_rows, rest = _rotation(q, k, q_weight, k_weight, cos_sin, positions, eps,
                                                                  interleaved, None)
+    given = q_out is not None or k_out is not None
     q_out = _bf16_like("q_out", q_out, q.shape, device)
     k_out = _bf16_like("k_out", k_out, k.shape, device)
+    if given:
+        _checks.apart("q_out", q_out, "q", q, in_place=True)
+        _checks.apart("k_out", k_out, "k", k, in_place=True)
+        for name, out, other_name, other in (("q_out", q_out, "k", k), ("k_out", k_out, "q", q), ("q_out", q_out, "k_out", k_out)):
+            _checks.apart(name, out, other_name, other)
     with _lib.on_device(device):
         _lib.check(_lib.native().chord_b200_qk_norm_rope(
             *q_rows, *k_rows, *rest, q_out.data_ptr(), k_out.data_ptr(), tokens, heads, k.shape[1], dim,
@@ -215,7 +221,12 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
         raise ValueError(f"q and k have head_dim={dim} on {device}, the cache {cache.head_dim} on {cache.device}")
     v_rows = _rows("v", v, device, tokens, cache.heads, dim)
     at = _ints("slots", slots, tokens, device)
+    given = q_out is not None
     q_out = _bf16_like("q_out", q_out, q.shape, device)
+    if given:
+        _checks.apart("q_out", q_out, "q", q, in_place=True)
+        for name, other in (("k", k), ("v", v)):
+            _checks.apart("q_out", q_out, name, other)
     with _lib.on_device(device):
         _lib.check(_lib.native().chord_b200_qk_norm_rope_write(
             *q_rows, *k_rows, *v_rows, *rest, q_out.data_ptr(), cache.address, at, tokens, heads,
@@ -267,7 +278,10 @@ def cache_read(cache: KVCache, block_tables: torch.Tensor, offsets: torch.Tensor
     at = _ints("offsets", offsets, batch + 1, device)
     table = _table(block_tables, device, batch)
     shape = (total, cache.heads, cache.head_dim)
+    given = k_out is not None and v_out is not None
     k_out, v_out = _bf16_like("k_out", k_out, shape, device), _bf16_like("v_out", v_out, shape, device)
+    if given:
+        _checks.apart("k_out", k_out, "v_out", v_out)
     with _lib.on_device(device):
         _lib.check(_lib.native().chord_b200_cache_read(
             cache.address, *table, at, batch, k_out.data_ptr(), v_out.data_ptr(), total,
@@ -297,7 +311,8 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     128, 192 or 256.  ``block_tables`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` say
     where each sequence's tokens are; the new token's own key and value are the last of them if they
     are written first.  ``window`` keeps the last so many tokens.  ``scale`` is ``head_dim ** -0.5``
-    where it is not given.  Returns BF16 ``[batch, heads, head_dim]``; ``lse``, if given, FP32 ``[batch,
+    where it is not given.  Returns BF16 ``[batch, heads, head_dim]`` (``outputs``, where given, must not overlap
+    ``q``); ``lse``, if given, FP32 ``[batch,
     heads]``, receives the logarithm of each softmax's sum, with which results over parts of a
     sequence can be joined.  A sequence of length zero gives zeros and minus infinity; a head whose query
     holds an infinity gives NaN over an 8-bit cache.
@@ -335,7 +350,10 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
         _checks.integer("window", window, minimum=1)
         if window >= 2**31:
             raise ValueError(f"window must be below 2^31, got {window}")
+    given = outputs is not None
     outputs = _bf16_like("outputs", outputs, q.shape, device)
+    if given:
+        _checks.apart("outputs", outputs, "q", q)
     if lse is not None and not (isinstance(lse, torch.Tensor) and lse.dtype is torch.float32
                                 and lse.shape == (batch, heads) and lse.device == device and lse.is_contiguous()):
         _checks.tensor("lse", lse, dtype=torch.float32, ndim=2, device=device)

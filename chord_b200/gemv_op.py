@@ -29,7 +29,7 @@ def gemv(x: torch.Tensor, weight: PreparedWeight, *, expert_ids: torch.Tensor | 
     tokens; from about a dozen on ``moe_align_block_size`` and ``indexed`` read shared experts once.
     For the down projection pass the routed activations and ``top_k=1``.
 
-    The rows of ``x`` may be a view with a row stride.  Weights are ``(code - 8) * scale`` without a
+    The rows of ``x`` may be a view with a row stride; ``outputs`` must not overlap it.  Weights are ``(code - 8) * scale`` without a
     rounding to BF16; sums are FP32, the result is rounded once.
     """
     direct = _lib.direct()
@@ -74,6 +74,7 @@ def gemv(x: torch.Tensor, weight: PreparedWeight, *, expert_ids: torch.Tensor | 
         outputs = torch.empty((rows, shape_n), dtype=torch.bfloat16, device=device)
     else:
         _checks.bf16_output(outputs, (rows, shape_n), device, exact_shape=True)
+        _checks.apart("outputs", outputs, "x", x)
     if rows == 0:
         return outputs
     status_word(device)  # (the short way above goes to devices that have one)

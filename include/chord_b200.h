@@ -378,7 +378,7 @@ int chord_b200_ep_combine_wait(void* state, int64_t world, int64_t epoch, void* 
  * and zeros where expert_ids[r] lies outside [expert_base, expert_base + num_experts), an
  * expert that another GPU holds.  dequant(W) = (code - 8) * scale, not rounded to BF16: sums
  * and scales are FP32, the result is rounded once.  x is bf16, its rows x_stride elements apart
- * (even); out is bf16 [rows, n].  No scratch, no locks; the same inputs give the same bits. */
+ * (even); out is bf16 [rows, n] and overlaps none of the others.  No scratch, no locks; the same inputs give the same bits. */
 int chord_b200_gemv(const void* x, int64_t x_stride, const int32_t* packed, const void* scale,
                     const int32_t* expert_ids, void* out, int64_t rows, int64_t n, int64_t k,
                     int64_t num_experts, int64_t top_k, int64_t expert_base, void* stream);
@@ -413,7 +413,8 @@ typedef struct chord_b200_kv_cache {
  *  weights    bf16 [head_dim];  cos_sin fp32 [max_positions, rotary_dim]: cosines, then sines
  *  positions  int32 [tokens]; a token at a position outside the table gets zeros and status bit 32
  *  q_out, k_out  bf16 [tokens, heads / kv_heads, head_dim], contiguous
- * All in FP32 with one rounding at the end. */
+ * All in FP32 with one rounding at the end.  q_out may be q and k_out k where those are contiguous; else results
+ * overlap no input and not one another. */
 int chord_b200_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* k,
                             int64_t k_token, int64_t k_head, const void* q_weight,
                             const void* k_weight, const float* cos_sin, int64_t max_positions,
@@ -462,7 +463,7 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
  *  cache    head_dim 64, 96, 128, 192 or 256; heads % cache->heads == 0
  *  tables, table_stride, max_pages  as above; lengths int32 [batch], at most
  *           max_pages * page_size (more: cut, status bit 32)
- *  out      bf16 [batch, heads, head_dim];  lse fp32 [batch, heads]
+ *  out      bf16 [batch, heads, head_dim], not overlapping q;  lse fp32 [batch, heads]
  *  locks    int32, chord_b200_paged_attention_lock_words() words, zero on entry and on exit
  *  workspace  chord_b200_paged_attention_workspace_bytes(head_dim, heads / cache->heads) bytes,
  *           16-byte aligned
