@@ -206,8 +206,8 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
                        slots: torch.Tensor, *, eps: float = 1e-6, interleaved: bool = False,
                        q_out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`qk_norm_rope` whose keys go, with the values as they are, straight into the cache: token
-    ``t`` at slot ``slots[t]`` (int32, page * page_size + place; negative: not kept).  Keys are
-    quantised from FP32.  Returns the queries."""
+    ``t`` at slot ``slots[t]`` (int32, page * page_size + place; negative: not kept).  The slots that are kept are
+    distinct, as for :func:`cache_write`.  Keys are quantised from FP32.  Returns the queries."""
     _cache(cache)
     direct = _lib.direct()
     if direct is not None and q_out is None:
@@ -236,8 +236,8 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
 
 def cache_write(k: torch.Tensor, v: torch.Tensor, cache: KVCache, slots: torch.Tensor) -> None:
     """Keys and values, BF16 ``[tokens, kv_heads, head_dim]``, into the cache: token ``t`` at slot
-    ``slots[t]`` (int32, page * page_size + place; negative: not kept).  A slot outside the cache is
-    not written and is reported by :func:`chord_b200.check_status`.  A row that holds an infinity or a
+    ``slots[t]`` (int32, page * page_size + place; negative: not kept).  The slots that are kept are distinct: a row
+    that two tokens of a call name holds parts of either.  A slot outside the cache is not written and is reported by :func:`chord_b200.check_status`.  A row that holds an infinity or a
     NaN reads back as NaN from an 8-bit cache."""
     _cache(cache)
     direct = _lib.direct()

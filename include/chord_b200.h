@@ -424,8 +424,8 @@ int chord_b200_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, cons
                             void* stream);
 
 /* The same with the keys, and the values as they are, written into the cache: token t at slot
- * slots[t], nowhere where that is negative.  Keys are quantised from FP32.  Two tokens with one
- * slot leave either's row. */
+ * slots[t], nowhere where that is negative.  Keys are quantised from FP32.  The slots of a call are
+ * distinct: a row that two of its tokens name holds parts of either (several warps write it, in no order). */
 int chord_b200_qk_norm_rope_write(const void* q, int64_t q_token, int64_t q_head, const void* k,
                                   int64_t k_token, int64_t k_head, const void* v, int64_t v_token,
                                   int64_t v_head, const void* q_weight, const void* k_weight,
@@ -435,7 +435,7 @@ int chord_b200_qk_norm_rope_write(const void* q, int64_t q_token, int64_t q_head
                                   int64_t tokens, int64_t heads, int32_t* status, double eps,
                                   void* stream);
 
-/* Keys and values bf16 [tokens, kv_heads, head_dim] into the cache, as above.  A row that holds an
+/* Keys and values bf16 [tokens, kv_heads, head_dim] into the cache, as above (distinct slots too).  A row that holds an
  * infinity or a NaN reads back as NaN from an 8-bit cache. */
 int chord_b200_cache_write(const void* k, int64_t k_token, int64_t k_head, const void* v,
                            int64_t v_token, int64_t v_head, const chord_b200_kv_cache* cache,

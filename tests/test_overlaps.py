@@ -1,5 +1,7 @@
 """Results that would lie where a call still reads are refused."""
 
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -56,3 +58,11 @@ def test_operators(device):
     with pytest.raises(ValueError, match="k_out must not overlap v_out"):
         chord_b200.cache_read(cache, table[:1], torch.tensor([0, 2], dtype=torch.int32, device=device), 2, k_out=out, v_out=out)
     chord_b200.check_status(device)
+
+
+def test_what_is_said_of_slots():
+    """Rows are written by several warps in no order, so nothing is promised of a slot that two tokens name."""
+    header = (Path(__file__).resolve().parents[1] / "include" / "chord_b200.h").read_text()
+    assert "leave either's row" not in header and "slots of a call are\n * distinct" in header
+    for operator in (chord_b200.cache_write, chord_b200.qk_norm_rope_write):
+        assert "distinct" in operator.__doc__
