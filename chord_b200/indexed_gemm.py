@@ -51,11 +51,23 @@ def status_word(device: torch.device) -> torch.Tensor:
     return word
 
 
+def _status_message(bits: int) -> str:
+    said = []
+    if bits & ~_INDEX_BIT:
+        names = [name for bit, name in _STATUS_BITS.items() if bits & bit]
+        said.append(f"a chord_b200 kernel gave up on a bounded wait ({', '.join(names)}; status {bits})")
+    if bits & _INDEX_BIT:
+        said.append("a chord_b200 kernel met an index outside a cache, a block table or a table of positions "
+                    f"(status {bits})")
+    return "; ".join(said)
+
+
 def check_status(device=None) -> None:
     """Synchronise ``device`` and raise ``RuntimeError`` if any kernel since the last
     check gave up on a bounded wait or met an index outside a cache, a block table or a table
-    of positions (its output is then not to be trusted).  Clears the word.  After a stream-K lock timeout the caller's ``locks`` tensor must be zeroed
-    again before it is reused."""
+    of positions (its output is then not to be trusted); the message names all that happened.  Clears the
+    word.  After a stream-K lock timeout the caller's ``locks`` tensor must be zeroed again before it is
+    reused."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     word = _STATUS.get(_device_index(device))
     if word is None:
@@ -64,12 +76,7 @@ def check_status(device=None) -> None:
     bits = int(word.item())
     if bits:
         word.zero_()
-        if bits == _INDEX_BIT:
-            raise RuntimeError("a chord_b200 kernel met an index outside a cache, a block table or a table of "
-                               f"positions (status {bits})")
-        names = [name for bit, name in _STATUS_BITS.items() if bits & bit]
-        raise RuntimeError(f"a chord_b200 kernel gave up on a bounded wait ({', '.join(names)}; "
-                           f"status {bits})")
+        raise RuntimeError(_status_message(bits))
 
 
 def default_locks(device: torch.device) -> torch.Tensor:
