@@ -77,7 +77,8 @@ def gemv(x: torch.Tensor, weight: PreparedWeight, *, expert_ids: torch.Tensor | 
         _checks.apart("outputs", outputs, "x", x)
     if rows == 0:
         return outputs
-    status_word(device)  # (the short way above goes to devices that have one)
+    if not torch.cuda.is_current_stream_capturing():
+        status_word(device)  # (the kernel has no use for it; the short way above goes to devices that have one)
     with _lib.on_device(device):
         _lib.check(_lib.native().chord_b200_gemv(
             x.data_ptr(), stride, packed.data_ptr(), scale.data_ptr(), ids, outputs.data_ptr(), rows, shape_n,
