@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import warnings
 from pathlib import Path
 from types import SimpleNamespace
 
@@ -26,6 +27,10 @@ try:  # the same, where torch's headers are
     from . import _torch_call
 except ImportError:
     _torch_call = None
+else:
+    if getattr(_torch_call, "built_for", None) != f"built for torch {torch.__version__}":
+        warnings.warn("chord_b200._torch_call was built for another torch and is not used; run python -m chord_b200.build")
+        _torch_call = None
 
 _LIB = None
 _NATIVE = None

@@ -11,6 +11,7 @@ from __future__ import annotations
 import concurrent.futures
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -99,6 +100,15 @@ def _torch_module_path() -> Path:
     return PACKAGE_DIR / ("_torch_call" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
+def _torch_version() -> str | None:
+    """``torch.__version__`` of the torch that would be imported, without importing it."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        return None
+    found = re.search(r"^__version__ = ['\"](.+)['\"]$", (Path(spec.origin).parent / "version.py").read_text(), re.M)
+    return found.group(1) if found else None
+
+
 def _torch_compiler() -> list[str] | None:
     """What compiles the `_torch_call` module, without its source and output, or None where that
     cannot be done here."""
@@ -113,7 +123,7 @@ def _torch_compiler() -> list[str] | None:
                                                             (3, "cuda_runtime_api.h"))):
         return None
     libraries = ["torch_python", "torch_cuda", "torch_cpu", "c10_cuda", "c10"]
-    return [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{h}" for h in headers), f"-L{torch / 'lib'}",
+    return [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", f'-DCHORD_TORCH_VERSION="{_torch_version()}"', *(f"-I{h}" for h in headers), f"-L{torch / 'lib'}",
             *(f"-l{name}" for name in libraries)]
 
 
@@ -122,7 +132,9 @@ def _torch_module_is_fresh() -> bool:
     path = _torch_module_path()
     if path.exists():
         sources = (CSRC / "torch_call.cpp", PACKAGE_DIR.parent / "include" / "chord_b200.h")
-        return path.stat().st_mtime >= max(f.stat().st_mtime for f in sources)
+        # (it holds code of torch's headers, whatever its symbols: only for the torch that it names)
+        built_for = f"built for torch {_torch_version()}\0".encode()
+        return path.stat().st_mtime >= max(f.stat().st_mtime for f in sources) and built_for in path.read_bytes()
     return _torch_compiler() is None
 
 

@@ -397,8 +397,18 @@ PyMethodDef methods[] = {METHOD("gemv", gemv), METHOD("qk_norm_rope", qk_norm_ro
                          METHOD("paged_attention", paged_attention), METHOD("entries", set_entries), METHOD("device", set_device),
                          METHOD("locks", set_locks), {nullptr, nullptr, 0, nullptr}};
 
+// The torch whose headers this is compiled with; the package does not use it with another.
+constexpr char kBuiltFor[] = "built for torch " CHORD_TORCH_VERSION;
+
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_call(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__torch_call(void) {
+  PyObject* const made = PyModule_Create(&module);
+  if (made != nullptr && PyModule_AddStringConstant(made, "built_for", kBuiltFor) != 0) {
+    Py_DECREF(made);
+    return nullptr;
+  }
+  return made;
+}
