@@ -132,20 +132,20 @@ def bf16_output(outputs, shape: tuple[int, int], device: torch.device, *, exact_
     return outputs
 
 
-def _span(t) -> tuple[int, int]:
-    """The addresses from a tensor's first element to behind its last."""
-    size = t.element_size()
-    return t.data_ptr(), t.data_ptr() + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-
-
 def apart(name: str, out, other_name: str, other, *, in_place: bool = False) -> None:
-    """A caller's result may not lie where other rows of the same call are still read: ``out`` and ``other``
-    share no memory or, ``in_place``, are the same contiguous elements."""
+    """A caller's result may not lie where other rows of the same call are still read: ``out``, which is
+    contiguous, and ``other`` share no memory or, ``in_place``, are the same elements."""
+    begin, other_begin = out.data_ptr(), other.data_ptr()
+    if begin < other_begin:  # (the end of the one that begins first decides)
+        if begin + out.nbytes <= other_begin:
+            return
+    elif begin > other_begin:
+        last = 0
+        for n, stride in zip(other.shape, other.stride()):
+            last += (n - 1) * stride
+        if other_begin + (last + 1) * other.element_size() <= begin:
+            return
     if out.numel() == 0 or other.numel() == 0:
-        return
-    begin, end = _span(out)
-    other_begin, other_end = _span(other)
-    if begin >= other_end or other_begin >= end:
         return
     if in_place and begin == other_begin and out.shape == other.shape and other.is_contiguous():
         return
