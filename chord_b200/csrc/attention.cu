@@ -327,10 +327,10 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 // 2^kSlack; until then P is up to 2^kSlack, which costs no precision, and no lane needs another's scores.
 //
 // Long rows are bounded by memory and by how unequally the SMs are served: 64 sequences of up to 8192 tokens in
-// BF16, 64 + 8 heads of 128, 1.36 GB, 248 us = 5.5 TB/s, 83 % of a plain copy's rate (of 64 x 4096, equal lots, 12
+// BF16, 64 + 8 heads of 128, 1.36 GB, 231 to 250 us from GPU to GPU = 5.4 to 5.9 TB/s, 83 to 90 % of a plain copy's rate (of 64 x 4096, equal lots, 12
 // SMs were done after 127 us, 96 after 152, 40 after 174; lots by ticket or two and three times as many were no
-// better).  Codes also by instructions, some 600 for 32 tokens: 131072 tokens of one sequence, 277 MB, 58 us =
-// 4.8 TB/s, of which about 8 are the launch, the rings' filling and two joins.  Three CTAs of an SM with steps of 16
+// better).  Codes also by instructions, some 630 for 32 tokens: 131072 tokens of one sequence, 277 MB, 59 us =
+// 4.7 TB/s, of which about 8 are the launch, the rings' filling and two joins.  Three CTAs of an SM with steps of 16
 // tokens instead of two with 32 gain 9 % on 64 x 4096 of codes, and lose 10 % on that one and 40 % on 37 x 1000.  Short
 // rows are bounded by latency: 333 tokens of 8 heads 8.4 us, some five dependent round trips to memory and one join.
 template <int kDim, bool kCodes, int kTiles>

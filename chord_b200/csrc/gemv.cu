@@ -97,7 +97,7 @@ struct GemvPlace {
 // Up to four rows: words go straight into the registers that the products read, those of kBatch scale
 // groups at a time, all in flight at once.  A warp's loads and products take turns, and instructions (14.6 for a
 // word) fill half of an SM's issue slots: eight experts of 4096 x 7168, 132 MB, 27.5 us = 4.8 TB/s, 74 % of a plain
-// copy's rate; one row of 14336 x 14336, whose 224 CTAs are two on some SMs and one on others, 26.5 us = 4.4 TB/s.  One
+// copy's rate (29.6 us on the slowest of six GPUs, 69 %); one row of 14336 x 14336, whose 224 CTAs are two on some SMs and one on others, 26.5 us = 4.4 TB/s.  One
 // row of 4096 x 7168, 16.5 MB, 5.6 us: a launch, one turn and the join of a cluster.
 template <int kTokens, int kSlots, int kBatch, int kWarps>
 __device__ __forceinline__ void gemv_few(const GemvParams& p, const GemvPlace& at, float (&acc)[4][2]) {
@@ -209,7 +209,7 @@ gemv_few_kernel(const GemvParams p) {
 // scales and the rows' inputs, which ldmatrix then reads as operands (with loads of four bytes straight
 // into registers they took most of the time: 16 rows of 14336 x 7168 39.7 us, 23.1 like this).  Instructions bound it,
 // 18 for a word with one product and 26 with two, 83 and 72 % of the busiest SM's issue slots: eight rows of 14336 x
-// 14336 27.6 us = 4.2 TB/s, 16 of 14336 x 7168 23.1 us = 2.5 TB/s.
+// 14336 28.0 us = 4.1 TB/s, 16 of 14336 x 7168 23.1 us = 2.5 TB/s.
 template <int kTokens>
 struct GemvLayout {
   static constexpr int kTiles = kTokens > 8 ? 2 : 1;  // products of eight columns

@@ -147,9 +147,9 @@ enum class Keep { kNothing, kNumbers, kCodes };
 // the codes.
 //
 // Memory bounds it once there are many tokens, and instructions just before: 8192 tokens of 64 + 8 heads of 128,
-// 302 MB, 53.4 us = 5.7 TB/s, 87 % of a plain copy's rate (184 instructions for a set of rows took 60.2, 115
+// 302 MB, 53 to 56 us from GPU to GPU = 5.4 to 5.7 TB/s, 82 to 87 % of a plain copy's rate (184 instructions for a set of rows took 60.2, 115
 // take this); 16384 tokens of 8 heads of 128 written as codes and read back, 203 MB, 36 to 37 us, 85 % (44.8
-// with 149 and 137 instructions for a set, now 103 and 69).  Three or two sets in flight are slower (8192 tokens
+// with 149 and 137 instructions for a set, now 105 and 69).  Three or two sets in flight are slower (8192 tokens
 // 63 and 59 us), as are fewer warps with more registers (64 us); one token takes a launch and two round trips
 // to memory, 1.9 us.
 template <int kLanes, int kRows, bool kRotate, Keep kKeep>

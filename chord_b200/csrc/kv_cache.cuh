@@ -12,7 +12,8 @@ namespace chord {
 // ORed into the status word when a kernel meets an index outside a cache or a table.
 constexpr int32_t kStatusIndex = 32;
 
-// n / d for n < 2^31, as a multiplication.
+// n / d for n < 2^31, as a multiplication (T. Granlund and P. Montgomery, "Division by invariant integers using
+// multiplication", 1994).
 struct Divisor {
   uint32_t d = 1, mul = 0, shift = 0;  // mul == 0: division by one
   Divisor() = default;
