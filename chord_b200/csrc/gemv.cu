@@ -25,18 +25,19 @@ struct GemvParams {
 };
 
 // The packed word is the A fragment of mma.m16n8k16 (16 weight rows x 16 K of a lane): 16 bytes of a lane
-// are the operands of four products.  Operands are the codes themselves, (code - 8) / 64, exact in BF16: one
-// mask and one multiply-add for every two.  A group's sum of 32 products is exact in FP32 up to its
+// are the operands of four products.  Operands are the codes themselves, (code - 8) / 512, exact in BF16: one
+// mask and one multiply-add for every two.  (By 512 so that 32 products of any finite inputs are finite.)  A group's sum of 32 products is exact in FP32 up to its
 // additions and is then multiplied by the group's scale, so that no weight is rounded.  (Masked codes as
 // they stand, with their offset taken off the sums by one more product, save those multiply-adds; one row
 // of 14336 x 14336 took 30.6 us like that and 31.2 like this, eight rows 34.4 and 30.5.)
 __device__ __forceinline__ void operand(uint32_t word, uint32_t (&a)[4]) {
-  constexpr uint32_t kOffset = 0xBE00BE00u;  // -8 / 64, twice
+  constexpr uint32_t kOffset = 0xBC80BC80u;                          // -8 / 512, twice
+  constexpr uint32_t kTwo124 = 0x7D807D80u, kTwo120 = 0x7B807B80u;  // 2^124 and 2^120, twice
   const uint32_t high = word >> 8;
-  a[0] = bf16x2_fma(word & 0x000F000Fu, kTwo127, kOffset);
-  a[1] = bf16x2_fma(high & 0x000F000Fu, kTwo127, kOffset);
-  a[2] = bf16x2_fma(word & 0x00F000F0u, kTwo123, kOffset);
-  a[3] = bf16x2_fma(high & 0x00F000F0u, kTwo123, kOffset);
+  a[0] = bf16x2_fma(word & 0x000F000Fu, kTwo124, kOffset);
+  a[1] = bf16x2_fma(high & 0x000F000Fu, kTwo124, kOffset);
+  a[2] = bf16x2_fma(word & 0x00F000F0u, kTwo120, kOffset);
+  a[3] = bf16x2_fma(high & 0x00F000F0u, kTwo120, kOffset);
 }
 
 // The product has eight columns, so fewer rows than eight leave columns idle: column n holds row n / kSlots,
@@ -61,7 +62,7 @@ __device__ __forceinline__ void join_and_store(const GemvParams& p, float* sums,
     if (cluster > 1) {
       part[i] = v;
     } else if (token < rows) {
-      p.out[(out_row + token) * p.n + block * 64 + i % 64] = __float2bfloat16(64.0f * v);
+      p.out[(out_row + token) * p.n + block * 64 + i % 64] = __float2bfloat16(512.0f * v);
     }
   }
   if (cluster > 1) {
@@ -71,7 +72,7 @@ __device__ __forceinline__ void join_and_store(const GemvParams& p, float* sums,
       const uint32_t addr = ptx::smem_u32(part + i);
       float v = 0.0f;
       for (int j = 0; j < cluster; ++j) v += ld_cluster_f32(ptx::map_to_cta(addr, j));
-      p.out[(out_row + i / 64) * p.n + block * 64 + i % 64] = __float2bfloat16(64.0f * v);
+      p.out[(out_row + i / 64) * p.n + block * 64 + i % 64] = __float2bfloat16(512.0f * v);
     }
     __syncwarp();
     ptx::cluster_sync();  // the others have read this CTA's sums

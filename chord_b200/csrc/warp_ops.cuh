@@ -26,7 +26,6 @@ __device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t 
 }
 
 constexpr uint32_t kTwo127 = 0x7F007F00u;    // 2^127, twice
-constexpr uint32_t kTwo123 = 0x7D007D00u;    // 2^123, twice
 
 __device__ __forceinline__ float bf16_lo(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
