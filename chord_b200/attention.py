@@ -169,7 +169,8 @@ def _rotation(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, kv
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
                  cos_sin: torch.Tensor, positions: torch.Tensor, *, eps: float = 1e-6, interleaved: bool = False,
                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
-    """Root-mean-square norms of each head's queries and keys and the position rotation, in one pass.
+    """Root-mean-square norms of each head's queries and keys and the position rotation, in one pass, in FP32
+    (squares too: finite elements of 2^60 or more may count as infinite).
 
     ``q`` is BF16 ``[tokens, heads, head_dim]`` and ``k`` ``[tokens, kv_heads, head_dim]``; both may be
     views of the fused projection's result.  ``q_weight`` and ``k_weight`` are BF16 ``[head_dim]``.

@@ -413,7 +413,8 @@ typedef struct chord_b200_kv_cache {
  *  weights    bf16 [head_dim];  cos_sin fp32 [max_positions, rotary_dim]: cosines, then sines
  *  positions  int32 [tokens]; a token at a position outside the table gets zeros and status bit 32
  *  q_out, k_out  bf16 [tokens, heads / kv_heads, head_dim], contiguous
- * All in FP32 with one rounding at the end.  q_out may be q and k_out k where those are contiguous; else results
+ * All in FP32 with one rounding at the end: squares too, so finite |x| of 2^60 or more may count as infinite and, with
+ * eps below 2^-120, |x| below 2^-60 as zeros.  q_out may be q and k_out k where those are contiguous; else results
  * overlap no input and not one another. */
 int chord_b200_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* k,
                             int64_t k_token, int64_t k_head, const void* q_weight,
@@ -459,6 +460,8 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
  * infinity; a head whose query holds an infinity gets NaN over an 8-bit cache.
  * Scores over an 8-bit cache are exact to (head_dim / 16 + 4) 2^-22 383 |scale| k_scale sum |q|, half a percent of
  * what the keys' rounding to codes may cost; over BF16 to (head_dim / 16 + 4) 2^-22 |scale| sum |q k|.
+ * Scores, and values times weights of up to 2^8, are added up in FP32: beyond 2^119 / (tokens seen) values may
+ * give infinities.
  *  q        bf16 [batch, heads, head_dim], strides in elements (multiples of 8)
  *  cache    head_dim 64, 96, 128, 192 or 256; heads % cache->heads == 0
  *  tables, table_stride, max_pages  as above; lengths int32 [batch], at most
