@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 constexpr int kMaxStreams = 16;
+constexpr int64_t kMaxRoutedRows = 65535;  // of gemv, rows with an expert each
 
 struct Entries {
   decltype(&chord_b200_gemv) gemv;
@@ -151,7 +152,7 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t count) {
   int64_t rows = x->size(0);
   const int64_t stride = rows > 1 ? x->stride(0) : k;
   if (rows == 0 || x->stride(1) != 1 || stride < k || stride % 2 != 0 || (reinterpret_cast<uintptr_t>(x->const_data_ptr()) & 3) != 0 ||
-      top_k < 1 || base < 0)
+      top_k < 1 || top_k > kMaxRoutedRows || base < 0)
     return none();
   const int32_t* ids = nullptr;
   if (a[6] == Py_None) {
@@ -160,7 +161,7 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (!THPVariable_Check(a[6])) return none();
     const at::Tensor& t = THPVariable_Unpack(a[6]);
     rows *= top_k;
-    if (t.scalar_type() != at::kInt || !t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.numel() != rows || rows > 65535)
+    if (t.scalar_type() != at::kInt || !t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.numel() != rows || rows > kMaxRoutedRows)
       return none();
     ids = t.const_data_ptr<int32_t>();
   }
