@@ -35,6 +35,8 @@ _EXPORTS = {
     "cache_read": "chord_b200.attention",
     "cache_write": "chord_b200.attention",
     "paged_attention": "chord_b200.attention",
+    "prompt_attention": "chord_b200.prompt",
+    "shared_prefix_attention": "chord_b200.prompt",
     "qk_norm_rope": "chord_b200.attention",
     "qk_norm_rope_write": "chord_b200.attention",
 }

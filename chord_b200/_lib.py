@@ -95,9 +95,24 @@ SIGNATURES = {
     "chord_b200_cache_read": (_int, [_ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr, _i64, _ptr, _ptr]),
     "chord_b200_paged_attention": (_int, [_ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64,
                                           _ptr, _i64, _ptr, _i64, _i64, _i64, _f64, _ptr]),
+    "chord_b200_paged_attention_shaped": (_int, [_ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64,
+                                                 _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr]),
     "chord_b200_paged_attention_lock_words": (_int, []),
     "chord_b200_paged_attention_workspace_bytes": (_i64, [_i64, _i64]),
+    "chord_b200_prompt_attention": (_int, [_ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                           _ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr]),
+    "chord_b200_prompt_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "chord_b200_shared_prefix_attention": (_int, [_ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr, _i64,
+                                                  _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr,
+                                                  _ptr]),
+    "chord_b200_shared_prefix_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
 }
+
+
+class ScoresDescriptor(ctypes.Structure):
+    """``chord_b200_scores`` of include/chord_b200.h."""
+
+    _fields_ = [("scale", _f64), ("cap", _f64), ("slopes", _ptr), ("window", _i64)]
 
 
 class KVCacheDescriptor(ctypes.Structure):

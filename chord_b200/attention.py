@@ -110,14 +110,14 @@ def _ints(name: str, x, count: int, device) -> int:
     raise ValueError(f"{name} must hold {count} values, got {x.numel()}")
 
 
-def _table(x, device, batch: int):
+def _table(x, device, batch: int, name: str = "block_tables"):
     """A block table int32 ``[batch, pages]``: (address, row stride, pages)."""
     if not isinstance(x, torch.Tensor) or x.dtype is not torch.int32:
-        raise TypeError("block_tables must be a torch.int32 tensor")
+        raise TypeError(f"{name} must be a torch.int32 tensor")
     if x.ndim != 2 or x.shape[0] != batch or x.shape[1] == 0 or x.device != device:
-        raise ValueError(f"block_tables must be [{batch}, pages] on {device}, got {tuple(x.shape)} on {x.device}")
+        raise ValueError(f"{name} must be [{batch}, pages] on {device}, got {tuple(x.shape)} on {x.device}")
     if x.stride(1) != 1 and x.shape[1] > 1:
-        raise ValueError("the rows of block_tables must be contiguous")
+        raise ValueError(f"the rows of {name} must be contiguous")
     return x.data_ptr(), x.stride(0), x.shape[1]
 
 
@@ -290,6 +290,65 @@ def cache_read(cache: KVCache, block_tables: torch.Tensor, offsets: torch.Tensor
     return k_out, v_out
 
 
+def _scores(cache: KVCache, heads: int, scale, window, cap, slopes) -> _lib.ScoresDescriptor:
+    """The checks of what shapes scores: their C form."""
+    if scale is None:
+        scale = cache.scale
+    elif isinstance(scale, bool) or not isinstance(scale, (int, float)) or not math.isfinite(scale):
+        raise ValueError(f"scale must be a finite number, got {scale!r}")
+    if window is None:
+        window = 0
+    else:
+        _checks.integer("window", window, minimum=1)
+        if window >= 2**31:
+            raise ValueError(f"window must be below 2^31, got {window}")
+    if cap is None:
+        cap = 0.0
+    elif isinstance(cap, bool) or not isinstance(cap, (int, float)) or not 1e-30 <= cap <= 1e30:
+        raise ValueError(f"cap must be a number from 1e-30 to 1e30, got {cap!r}")
+    address = None
+    if slopes is not None:
+        if not (isinstance(slopes, torch.Tensor) and slopes.dtype is torch.float32 and slopes.shape == (heads,)
+                and slopes.device == cache.device and slopes.is_contiguous()):
+            _checks.tensor("slopes", slopes, dtype=torch.float32, ndim=1, device=cache.device)
+            raise ValueError(f"slopes must hold {heads} values, got {slopes.numel()}")
+        address = slopes.data_ptr()
+    return _lib.ScoresDescriptor(scale, cap, address, window)
+
+
+def _sums(lse, tokens: int, heads: int, device) -> int | None:
+    """The address of FP32 ``[tokens, heads]``, if given."""
+    if lse is None:
+        return None
+    if not (isinstance(lse, torch.Tensor) and lse.dtype is torch.float32 and lse.shape == (tokens, heads)
+            and lse.device == device and lse.is_contiguous()):
+        _checks.tensor("lse", lse, dtype=torch.float32, ndim=2, device=device)
+        raise ValueError(f"lse must have shape {(tokens, heads)}, got {tuple(lse.shape)}")
+    return lse.data_ptr()
+
+
+def _queries(q, cache: KVCache):
+    """``q`` as BF16 ``[tokens, heads, head_dim]`` over ``cache``: (address, token stride, head stride)."""
+    if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype is not torch.bfloat16:
+        raise TypeError("q must be a 3D torch.bfloat16 tensor")
+    _checks.supported_gpu(cache.device)
+    rows = _rows("q", q, cache.device, q.shape[0], None, cache.head_dim)
+    if cache.head_dim not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {cache.head_dim}")
+    if q.shape[1] % cache.heads:
+        raise ValueError(f"the number of query heads must be a multiple of the cache's {cache.heads}, got {q.shape[1]}")
+    return rows
+
+
+def _locks(locks, words: int, device) -> torch.Tensor:
+    if locks is None:
+        return default_locks(device)
+    _checks.tensor("locks", locks, dtype=torch.int32, ndim=1, device=device)
+    if locks.numel() < words:
+        raise RuntimeError(f"locks has {locks.numel()} lock words, this launch needs at least {words}")
+    return locks
+
+
 @functools.lru_cache(maxsize=64)
 def _attention_scratch(device_index: int, head_dim: int, group: int):
     """(lock words, workspace bytes), asked of the library once per device and shape."""
@@ -303,7 +362,8 @@ def _attention_scratch(device_index: int, head_dim: int, group: int):
 
 
 def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor, lengths: torch.Tensor, *,
-                    scale: float | None = None, window: int | None = None, outputs: torch.Tensor | None = None,
+                    scale: float | None = None, window: int | None = None, cap: float | None = None,
+                    slopes: torch.Tensor | None = None, outputs: torch.Tensor | None = None,
                     lse: torch.Tensor | None = None, locks: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one new token per sequence over its tokens in the cache.
 
@@ -312,8 +372,9 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     128, 192 or 256.  ``block_tables`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` say
     where each sequence's tokens are; the new token's own key and value are the last of them if they
     are written first.  ``window`` keeps the last so many tokens.  ``scale`` is ``head_dim ** -0.5``
-    where it is not given.  Returns BF16 ``[batch, heads, head_dim]`` (``outputs``, where given, must not overlap
-    ``q``); ``lse``, if given, FP32 ``[batch,
+    where it is not given.  With ``cap`` scores become ``cap * tanh(score / cap)``; with ``slopes`` (FP32 ``[heads]``)
+    ``slopes[h]`` times a token's distance to the new one is then taken off.  Returns BF16 ``[batch, heads, head_dim]``
+    (``outputs``, where given, must not overlap ``q``); ``lse``, if given, FP32 ``[batch,
     heads]``, receives the logarithm of each softmax's sum, with which results over parts of a
     sequence can be joined.  A sequence of length zero gives zeros and minus infinity; a head whose query
     holds an infinity gives NaN over an 8-bit cache.
@@ -323,57 +384,38 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     int32, left zeroed, one buffer per launches that may overlap; with ``None`` a per-stream buffer of
     the library's.  The same inputs give the same bits."""
     _cache(cache)
+    shaped = cap is not None or slopes is not None
     direct = _lib.direct()
-    if direct is not None and outputs is None and locks is None and window != 0:
+    if direct is not None and not shaped and outputs is None and locks is None and window != 0:
         result = direct.paged_attention(q, cache.address, cache.index, block_tables, lengths, lse,
                                         0 if window is None else window, cache.scale if scale is None else scale)
         if result is not None:
             return result
-    if not isinstance(q, torch.Tensor) or q.ndim != 3 or q.dtype is not torch.bfloat16:
-        raise TypeError("q must be a 3D torch.bfloat16 tensor")
-    device, dim = cache.device, cache.head_dim
-    _checks.supported_gpu(device)
-    batch, heads = q.shape[0], q.shape[1]
-    q_rows = _rows("q", q, device, batch, None, dim)
-    if dim not in HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {dim}")
-    if heads % cache.heads:
-        raise ValueError(f"the number of query heads must be a multiple of the cache's {cache.heads}, got {heads}")
+    q_rows = _queries(q, cache)
+    device, dim, (batch, heads) = cache.device, cache.head_dim, q.shape[:2]
     table = _table(block_tables, device, batch)
     at = _ints("lengths", lengths, batch, device)
-    if scale is None:
-        scale = dim ** -0.5
-    elif isinstance(scale, bool) or not isinstance(scale, (int, float)) or not math.isfinite(scale):
-        raise ValueError(f"scale must be a finite number, got {scale!r}")
-    if window is None:
-        window = 0
-    else:
-        _checks.integer("window", window, minimum=1)
-        if window >= 2**31:
-            raise ValueError(f"window must be below 2^31, got {window}")
+    scores = _scores(cache, heads, scale, window, cap, slopes)
     given = outputs is not None
     outputs = _bf16_like("outputs", outputs, q.shape, device)
     if given:
         _checks.apart("outputs", outputs, "q", q)
-    if lse is not None and not (isinstance(lse, torch.Tensor) and lse.dtype is torch.float32
-                                and lse.shape == (batch, heads) and lse.device == device and lse.is_contiguous()):
-        _checks.tensor("lse", lse, dtype=torch.float32, ndim=2, device=device)
-        raise ValueError(f"lse must have shape {(batch, heads)}, got {tuple(lse.shape)}")
+    sums = _sums(lse, batch, heads, device)
     if batch == 0:
         return outputs
     with _lib.on_device(device):
         words, size = _attention_scratch(_device_index(device), dim, heads // cache.heads)
-        if locks is None:
-            locks = default_locks(device)
-        else:
-            _checks.tensor("locks", locks, dtype=torch.int32, ndim=1, device=device)
-            if locks.numel() < words:
-                raise RuntimeError(f"locks has {locks.numel()} lock words, this launch needs at least {words}")
+        locks = _locks(locks, words, device)
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        _lib.check(_lib.native().chord_b200_paged_attention(
-            *q_rows, cache.address, *table, at, outputs.data_ptr(), None if lse is None else lse.data_ptr(),
-            locks.data_ptr(), locks.numel(), workspace.data_ptr(), size, status_word(device).data_ptr(), batch, heads,
-            window, scale, _lib.stream_handle(device)))
+        rest = (outputs.data_ptr(), sums, locks.data_ptr(), locks.numel(), workspace.data_ptr(), size,
+                status_word(device).data_ptr(), batch, heads)
+        stream = _lib.stream_handle(device)
+        if shaped:
+            _lib.check(_lib.native().chord_b200_paged_attention_shaped(*q_rows, cache.address, *table, at, *rest,
+                                                                       ctypes.addressof(scores), stream))
+        else:
+            _lib.check(_lib.native().chord_b200_paged_attention(*q_rows, cache.address, *table, at, *rest, scores.window,
+                                                                scores.scale, stream))
     return outputs
 
 

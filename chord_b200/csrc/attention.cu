@@ -4,6 +4,7 @@
 #include <mutex>
 
 #include "../../include/chord_b200.h"
+#include "attention.h"
 #include "common.h"
 #include "join_plan.h"
 #include "kv_cache.cuh"
@@ -35,6 +36,10 @@ struct AttentionParams {
   int32_t batch, heads, group, head_blocks, capacity, window;
   float scale;  // of the scores, with log2(e)
   bool whole_groups;
+  // Of the kernels with kShaped alone.
+  const float* slopes;  // [heads] or null: taken off the scores for each token between
+  float* wide_out;      // [batch, heads, dim] in place of out, where not null
+  float cap, two_over_cap;  // tanh(x / cap) cap, with log2(e); zero: none
 };
 
 // What follows from the head's width and the cache's type.  A warp takes kStep tokens at a time, whose
@@ -132,6 +137,15 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
   return n / d;
 }
 
+constexpr float kLog2E = 1.44269504088896341f;
+
+// cap tanh(u log(2) / 2), from the one exponential: exact for large and small ones, off by 2^-22 of the cap.
+__device__ __forceinline__ float capped(float u, float cap) {
+  float rate;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rate) : "f"(exp2_approx(u) + 1.0f));
+  return fmaf(-2.0f * cap, rate, cap);
+}
+
 // What outputs are multiplied with: those of codes are 64ths.
 template <bool kCodes>
 __device__ __forceinline__ float rate_of(float sum) { return sum == 0.0f ? 0.0f : (kCodes ? 64.0f : 1.0f) / sum; }
@@ -156,7 +170,7 @@ struct Row {
   }
   // Four heads' values of one dim, the `place`-th of the products' order: with codes a 16-byte piece has
   // its even dims first.
-  template <int kDim, bool kCodes>
+  template <int kDim, bool kCodes, bool kShaped>
   __device__ __forceinline__ void finish(const AttentionParams& p, int head, int place, const float4& v, const float4& all,
                                          const float4& most) const {
     const int dim = kCodes ? place / 16 * 16 + place % 8 * 2 + place % 16 / 8 : place;
@@ -164,7 +178,12 @@ struct Row {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (head + i >= heads) break;
-      p.out[(head0 + head + i) * kDim + dim] = __float2bfloat16(value[i] * rate_of<kCodes>(sum[i]));
+      const int64_t at = (head0 + head + i) * kDim + dim;
+      if (kShaped && p.wide_out != nullptr) {
+        p.wide_out[at] = value[i] * rate_of<kCodes>(sum[i]);
+      } else {
+        p.out[at] = __float2bfloat16(value[i] * rate_of<kCodes>(sum[i]));
+      }
       if (place == 0 && p.lse != nullptr) p.lse[head0 + head + i] = lse_of(top[i], sum[i]);
     }
   }
@@ -207,7 +226,7 @@ struct Joined {
     return make_float4(factor(from.x, to.x), factor(from.y, to.y), factor(from.z, to.z), factor(from.w, to.w));
   }
   // To a part, or to the results (to == null).
-  template <bool kCodes>
+  template <bool kCodes, bool kShaped>
   __device__ __forceinline__ void give(const AttentionParams& p, const Row& of, float* to) const {
     const int32_t head = threadIdx.x % kQuads * 4;
 #pragma unroll
@@ -215,7 +234,7 @@ struct Joined {
       if (!mine(i)) break;
       const int32_t index = threadIdx.x + i * kThreads;
       if (to == nullptr) {
-        of.template finish<kDim, kCodes>(p, head, index / kQuads, value[i], sum, top);
+        of.template finish<kDim, kCodes, kShaped>(p, head, index / kQuads, value[i], sum, top);
       } else {
         __stcg(reinterpret_cast<float4*>(to + 4 * index), value[i]);
       }
@@ -230,7 +249,7 @@ struct Joined {
 // Joins `count` (at most kFan) parts that other CTAs have written, source(j) the j-th of them, into a part or
 // the results.  What they hold comes into shared memory by cp.async, all of it at once where there is room;
 // the weights are worked out while the values are on their way, by every warp for itself.
-template <int kDim, bool kCodes, int kHeads, int kSmem, typename Source>
+template <int kDim, bool kCodes, bool kShaped, int kHeads, int kSmem, typename Source>
 __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& of, uint8_t* smem, int32_t count, float* to, Source source) {
   using Join = Joined<kDim, kHeads>;
   constexpr int kStats = 2 * kHeads * 4, kValues = kDim * kHeads * 4;  // bytes of a part
@@ -300,7 +319,7 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
   }
   joined.top = *reinterpret_cast<const float4*>(result + threadIdx.x % Join::kQuads * 4);
   joined.sum = *reinterpret_cast<const float4*>(result + kHeads + threadIdx.x % Join::kQuads * 4);
-  joined.template give<kCodes>(p, of, to);
+  joined.template give<kCodes, kShaped>(p, of, to);
 }
 
 // One row of work is a sequence, one of its key-value heads and a block of up to 16 of the query heads
@@ -333,7 +352,10 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 // 4.7 TB/s, of which about 8 are the launch, the rings' filling and two joins.  Three CTAs of an SM with steps of 16
 // tokens instead of two with 32 gain 9 % on 64 x 4096 of codes, and lose 10 % on that one and 40 % on 37 x 1000.  Short
 // rows are bounded by latency: 333 tokens of 8 heads 8.4 us, some five dependent round trips to memory and one join.
-template <int kDim, bool kCodes, int kTiles>
+//
+// kShaped: scores may be capped and leaned on by distance, and the results may stay in FP32.  Kernels of their own: the plain
+// ones keep their registers, and the cap's three operations per score (two of them of the 4-lane unit) are only paid there.
+template <int kDim, bool kCodes, int kTiles, bool kShaped>
 __global__ void __launch_bounds__(kThreads, (Layout<kDim, kCodes, kTiles>::kCtas))
 paged_attention_kernel(const AttentionParams p) {
   using L = Layout<kDim, kCodes, kTiles>;
@@ -436,7 +458,12 @@ paged_attention_kernel(const AttentionParams p) {
     const int64_t row = static_cast<int64_t>(b) * p.heads;
 #pragma unroll 1
     for (int32_t i = threadIdx.x; i < p.heads * (kDim / 8); i += kThreads) {
-      *reinterpret_cast<uint4*>(p.out + row * kDim + 8 * static_cast<int64_t>(i)) = make_uint4(0, 0, 0, 0);
+      if (kShaped && p.wide_out != nullptr) {
+        float4* const to = reinterpret_cast<float4*>(p.wide_out + row * kDim + 8 * static_cast<int64_t>(i));
+        to[0] = to[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      } else {
+        *reinterpret_cast<uint4*>(p.out + row * kDim + 8 * static_cast<int64_t>(i)) = make_uint4(0, 0, 0, 0);
+      }
     }
     if (p.lse != nullptr) {
 #pragma unroll 1
@@ -605,6 +632,7 @@ paged_attention_kernel(const AttentionParams p) {
     float of_scores = p.scale, of_codes = 1.0f;  // factors of the scores
     // A lane's heads are 8 n + 2 q4 and the next; of the dims it has rows r8 and r8 + 8 of each chunk.
     float out[kChunks][kTiles][4], top[kTiles][2], sum[kTiles][2];
+    float slope[kShaped ? kTiles : 1][2] = {};
     bool began = at.token > at.begin;  // in an earlier share
     bool fresh = true;
     int32_t stage_index = 0;
@@ -632,6 +660,16 @@ paged_attention_kernel(const AttentionParams p) {
           for (int c = 0; c < kChunks; ++c) out[c][n][0] = out[c][n][1] = out[c][n][2] = out[c][n][3] = 0.0f;
           top[n][0] = top[n][1] = -INFINITY;
           sum[n][0] = sum[n][1] = 0.0f;
+          if constexpr (kShaped) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int of_head = 8 * n + 2 * q4 + i;
+              slope[n][i] = 0.0f;
+              if (p.slopes != nullptr && of_head < heads) {
+                slope[n][i] = load_arg(p.slopes + (of.head0 - static_cast<int64_t>(at.b) * p.heads) + of_head) * kLog2E;
+              }
+            }
+          }
         }
         if constexpr (kCodes) {
           // The largest magnitude among the row's heads, infinities and NaN left out (their heads are NaN).
@@ -741,6 +779,29 @@ paged_attention_kernel(const AttentionParams p) {
           }
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) s[j][n][2 * i] *= f, s[j][n][2 * i + 1] *= f;
+        }
+      }
+      if constexpr (kShaped) {
+        if (p.cap > 0.0f) {
+#pragma unroll
+          for (int j = 0; j < kGroups; ++j) {
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[j][n][i] = capped(s[j][n][i] * p.two_over_cap, p.cap);
+            }
+          }
+        }
+        if (p.slopes != nullptr) {
+          const float behind = static_cast<float>(at.end - 1 - at.token - r8);  // tokens between
+#pragma unroll
+          for (int j = 0; j < kGroups; ++j) {
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[j][n][i] = fmaf(-slope[n][i & 1], behind - (16 * j + i / 2 * 8), s[j][n][i]);
+            }
+          }
         }
       }
       if (at.token < at.begin || at.token + L::kStep > at.end) {
@@ -872,6 +933,21 @@ paged_attention_kernel(const AttentionParams p) {
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
           const float rate[2] = {rate_of<kCodes>(sum[n][0]), rate_of<kCodes>(sum[n][1])};
+          if constexpr (kShaped) {
+            if (p.wide_out != nullptr) {
+              // heads 2 q4 and 2 q4 + 1, dims r8 and r8 + 8 of the products' order
+#pragma unroll
+              for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int head = 8 * n + 2 * q4 + (i & 1), place = r8 + i / 2 * 8;
+                  const int dim = 16 * c + (kCodes ? place % 8 * 2 + place / 8 : place);
+                  if (head < heads) p.wide_out[(head0 + head) * kDim + dim] = out[c][n][i] * rate[i & 1];
+                }
+              }
+            }
+          }
+          if (!kShaped || p.wide_out == nullptr) {
           __nv_bfloat16* to = p.out + (head0 + 8 * n + r8) * kDim;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
@@ -886,6 +962,7 @@ paged_attention_kernel(const AttentionParams p) {
                 *reinterpret_cast<uint2*>(to + 16 * c + 4 * q4) = make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
               }
             }
+          }
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -954,7 +1031,7 @@ paged_attention_kernel(const AttentionParams p) {
     const bool began = parts[first].began, whole = ended && !began;
     if (!whole) pending[waiting++] = first;
     const Row of(p, parts[first].b, parts[first].row);
-    joined.template give<kCodes>(p, of, whole ? nullptr : slot_of(lot, began ? kSlotInside : kSlotFirst));
+    joined.template give<kCodes, kShaped>(p, of, whole ? nullptr : slot_of(lot, began ? kSlotInside : kSlotFirst));
   }
   if (waiting == 0) return;
 
@@ -980,7 +1057,7 @@ paged_attention_kernel(const AttentionParams p) {
       __syncthreads();
       if (!answer[level]) break;
       float* const to = level == 0 ? slot_of(part.first_lot + begin, kSlotGroup) : nullptr;
-      join_parts<kDim, kCodes, kHeads, L::kSmem>(p, of, smem, count, to, [&](int32_t j) {
+      join_parts<kDim, kCodes, kShaped, kHeads, L::kSmem>(p, of, smem, count, to, [&](int32_t j) {
         const PartPlace at_part = level == 0 ? join.part(begin, j) : join.joined(j);
         return slot_of(at_part.lot, at_part.slot);
       });
@@ -993,35 +1070,36 @@ struct Variant {
   int smem, step, ctas;
 };
 
-template <int kDim, bool kCodes, int kTiles>
+template <int kDim, bool kCodes, int kTiles, bool kShaped>
 Variant variant() {
   using L = Layout<kDim, kCodes, kTiles>;
-  return {paged_attention_kernel<kDim, kCodes, kTiles>, L::kSmem, L::kStep, L::kCtas};
+  return {paged_attention_kernel<kDim, kCodes, kTiles, kShaped>, L::kSmem, L::kStep, L::kCtas};
 }
 
-template <int kDim>
+template <int kDim, bool kShaped>
 Variant variant_of(bool codes, bool wide) {
-  if (codes) return wide ? variant<kDim, true, 2>() : variant<kDim, true, 1>();
-  return wide ? variant<kDim, false, 2>() : variant<kDim, false, 1>();
+  if (codes) return wide ? variant<kDim, true, 2, kShaped>() : variant<kDim, true, 1, kShaped>();
+  return wide ? variant<kDim, false, 2, kShaped>() : variant<kDim, false, 1, kShaped>();
 }
 
+template <bool kShaped>
 bool variant_for(int64_t dim, bool codes, bool wide, Variant* out) {
   switch (dim) {
-    case 64: *out = variant_of<64>(codes, wide); return true;
-    case 96: *out = variant_of<96>(codes, wide); return true;
-    case 128: *out = variant_of<128>(codes, wide); return true;
-    case 192: *out = variant_of<192>(codes, wide); return true;
-    case 256: *out = variant_of<256>(codes, wide); return true;
+    case 64: *out = variant_of<64, kShaped>(codes, wide); return true;
+    case 96: *out = variant_of<96, kShaped>(codes, wide); return true;
+    case 128: *out = variant_of<128, kShaped>(codes, wide); return true;
+    case 192: *out = variant_of<192, kShaped>(codes, wide); return true;
+    case 256: *out = variant_of<256, kShaped>(codes, wide); return true;
   }
   return false;
 }
 
 // Allows a kernel its shared memory, once per device.
-int allow_smem(const Variant& v, int64_t dim, bool codes, bool wide, int device) {
+int allow_smem(const Variant& v, int64_t dim, bool codes, bool wide, bool shaped, int device) {
   static std::mutex mutex;
-  static bool done[64][5][2][2];
+  static bool done[64][5][2][2][2];
   std::lock_guard<std::mutex> guard(mutex);
-  bool& known = done[device & 63][dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : dim == 192 ? 3 : 4][codes][wide];
+  bool& known = done[device & 63][dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : dim == 192 ? 3 : 4][codes][wide][shaped];
   if (known) return kOk;
   CHORD_CUDA(cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem));
   known = true;
@@ -1029,47 +1107,25 @@ int allow_smem(const Variant& v, int64_t dim, bool codes, bool wide, int device)
 }
 
 }  // namespace
-}  // namespace chord
 
-extern "C" {
-
-int chord_b200_paged_attention_lock_words(void) {
-  chord::DeviceInfo device;
-  if (chord::current_device_info(&device)) return -1;
-  const int ctas = device.sm_count * chord::kMaxCtasPerSm;
-  return ctas < chord::kMaxCtas ? ctas : chord::kMaxCtas;
-}
-
-int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t group) {
-  using namespace chord;
-  DeviceInfo device;
-  if (current_device_info(&device)) return -1;
-  Variant v, w;  // of either type of cache
-  if (!variant_for(head_dim, false, group > 8, &v) || !variant_for(head_dim, true, group > 8, &w)) {
-    return fail(kInvalidArgument, "head_dim must be 64, 96, 128, 192 or 256"), -1;
-  }
-  const int ctas = device.sm_count * (v.ctas > w.ctas ? v.ctas : w.ctas);
-  return 4 * workspace_floats(ctas < kMaxCtas ? ctas : kMaxCtas, static_cast<int>(head_dim), group > 8 ? 16 : 8);
-}
-
-int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, const chord_b200_kv_cache* cache,
-                               const int32_t* tables, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
-                               void* out, float* lse, int32_t* locks, int64_t num_locks, void* workspace,
-                               int64_t workspace_bytes, int32_t* status, int64_t batch, int64_t heads, int64_t window,
-                               double scale, void* stream) {
-  using namespace chord;
+int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const chord_b200_kv_cache* cache, const int32_t* tables,
+                    int64_t table_stride, int64_t max_pages, const int32_t* lengths, void* out, float* wide_out, float* lse,
+                    int32_t* locks, int64_t num_locks, void* workspace, int64_t workspace_bytes, int32_t* status, int64_t batch,
+                    int64_t heads, const chord_b200_scores& scores, bool shaped, void* stream) {
+  const int64_t window = scores.window;
+  const double scale = scores.scale;
   AttentionParams p = {};
   if (int rc = make_cache(cache, &p.cache)) return rc;
   CHORD_REQUIRE(batch >= 0 && batch < (1ll << 31), "batch out of range");
   if (batch == 0) return kOk;
-  CHORD_REQUIRE(q != nullptr && tables != nullptr && lengths != nullptr && out != nullptr && locks != nullptr &&
+  CHORD_REQUIRE(q != nullptr && tables != nullptr && lengths != nullptr && (out != nullptr || wide_out != nullptr) && locks != nullptr &&
                     workspace != nullptr,
                 "null pointer");
   CHORD_REQUIRE(heads > 0 && heads <= 65535 && heads % cache->heads == 0,
                 "the number of query heads (%lld) must be a multiple of the cache's (%lld)",
                 static_cast<long long>(heads), static_cast<long long>(cache->heads));
   CHORD_REQUIRE(q_batch >= 0 && q_head >= 0 && q_batch % 8 == 0 && q_head % 8 == 0 &&
-                    ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
+                    ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(wide_out) |
                       reinterpret_cast<uintptr_t>(workspace)) & 15u) == 0,
                 "q's rows, out and the workspace must lie on 16-byte boundaries");
   CHORD_REQUIRE(max_pages > 0 && table_stride >= 0 && max_pages < (1ll << 31), "a block table has a page or more");
@@ -1079,12 +1135,13 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, c
   const int64_t group = heads / cache->heads;
   const bool wide = group > 8;
   Variant v;
-  CHORD_REQUIRE(variant_for(cache->head_dim, codes, wide, &v), "head_dim must be 64, 96, 128, 192 or 256, got %lld",
+  CHORD_REQUIRE(scores.cap >= 0.0 && scores.cap - scores.cap == 0.0, "the cap must be finite and at least zero");
+  CHORD_REQUIRE(shaped ? variant_for<true>(cache->head_dim, codes, wide, &v) : variant_for<false>(cache->head_dim, codes, wide, &v), "head_dim must be 64, 96, 128, 192 or 256, got %lld",
                 static_cast<long long>(cache->head_dim));
   DeviceInfo device;
   if (int rc = current_device_info(&device)) return rc;
   if (int rc = require_blackwell(device)) return rc;
-  if (int rc = allow_smem(v, cache->head_dim, codes, wide, device.device)) return rc;
+  if (int rc = allow_smem(v, cache->head_dim, codes, wide, shaped, device.device)) return rc;
   const int64_t head_blocks = (group + 15) / 16;
   // No more CTAs than there can be shares.
   // (token numbers, those of the steps loaded ahead too, fit 32 bits)
@@ -1118,10 +1175,58 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, c
   p.head_blocks = static_cast<int32_t>(head_blocks);
   p.window = static_cast<int32_t>(window);
   p.scale = static_cast<float>(scale * 1.4426950408889634074);
+  p.slopes = scores.slopes;
+  p.wide_out = wide_out;
+  p.cap = static_cast<float>(scores.cap * 1.4426950408889634074);
+  p.two_over_cap = scores.cap > 0.0 ? static_cast<float>(2.0 / scores.cap) : 0.0f;
   p.whole_groups = cache->page_size % 16 == 0 && p.cache.token < (1ll << 31);
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), v.smem,
                            static_cast<cudaStream_t>(stream), kEarlyLaunch, p));
   return kOk;
+}
+
+}  // namespace chord
+
+extern "C" {
+
+int chord_b200_paged_attention_lock_words(void) {
+  chord::DeviceInfo device;
+  if (chord::current_device_info(&device)) return -1;
+  const int ctas = device.sm_count * chord::kMaxCtasPerSm;
+  return ctas < chord::kMaxCtas ? ctas : chord::kMaxCtas;
+}
+
+int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t group) {
+  using namespace chord;
+  DeviceInfo device;
+  if (current_device_info(&device)) return -1;
+  Variant v, w;  // of either type of cache
+  if (!variant_for<false>(head_dim, false, group > 8, &v) || !variant_for<false>(head_dim, true, group > 8, &w)) {
+    return fail(kInvalidArgument, "head_dim must be 64, 96, 128, 192 or 256"), -1;
+  }
+  const int ctas = device.sm_count * (v.ctas > w.ctas ? v.ctas : w.ctas);
+  return 4 * workspace_floats(ctas < kMaxCtas ? ctas : kMaxCtas, static_cast<int>(head_dim), group > 8 ? 16 : 8);
+}
+
+int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head, const chord_b200_kv_cache* cache,
+                               const int32_t* tables, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                               void* out, float* lse, int32_t* locks, int64_t num_locks, void* workspace,
+                               int64_t workspace_bytes, int32_t* status, int64_t batch, int64_t heads, int64_t window,
+                               double scale, void* stream) {
+  const chord_b200_scores scores = {scale, 0.0, nullptr, window};
+  return chord::paged_attention(q, q_batch, q_head, cache, tables, table_stride, max_pages, lengths, out, nullptr, lse, locks, num_locks,
+                                workspace, workspace_bytes, status, batch, heads, scores, false, stream);
+}
+
+int chord_b200_paged_attention_shaped(const void* q, int64_t q_batch, int64_t q_head, const chord_b200_kv_cache* cache,
+                                      const int32_t* tables, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                                      void* out, float* lse, int32_t* locks, int64_t num_locks, void* workspace,
+                                      int64_t workspace_bytes, int32_t* status, int64_t batch, int64_t heads,
+                                      const chord_b200_scores* scores, void* stream) {
+  using namespace chord;
+  CHORD_REQUIRE(scores != nullptr, "null pointer");
+  return paged_attention(q, q_batch, q_head, cache, tables, table_stride, max_pages, lengths, out, nullptr, lse, locks, num_locks,
+                         workspace, workspace_bytes, status, batch, heads, *scores, true, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,410 @@
+// How the work of prompt.cuh is dealt out, and the entry points.
+#include <mutex>
+
+#include "../../include/chord_b200.h"
+#include "attention.h"
+#include "common.h"
+#include "prompt_kernels.cuh"
+#include "register_split.h"
+
+namespace chord {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+// The sum of `value` over the threads before this one, and of all.
+__device__ __forceinline__ int64_t sum_before(int64_t value, int64_t* of_warps, int64_t& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t upto = value;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t below = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += below;
+  }
+  __syncthreads();  // (of_warps may still be read from the call before)
+  if (lane == 31) of_warps[warp] = upto;
+  __syncthreads();
+  int64_t before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) before += of_warps[w];
+    all += of_warps[w];
+  }
+  return before + upto - value;
+}
+
+// One CTA: the items of every sequence, the tokens that each of them sees, and where the main kernel's CTAs begin.
+__global__ void __launch_bounds__(kPlanThreads, 1) prompt_plan_kernel(const __grid_constant__ PromptParams p, int32_t item_rows, int32_t step_tokens) {
+  __shared__ int64_t of_warps[kPlanThreads / 32];
+  __shared__ int32_t longest_of[kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ptx::grid_dependency_wait();
+
+  // Items of the sequences before each.
+  int64_t items = 0;
+#pragma unroll 1
+  for (int32_t b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+    const int32_t b = b0 + threadIdx.x;
+    int64_t mine = 0;
+    if (b < p.batch) {
+      const PromptSequence of(p, b);
+      mine = (static_cast<int64_t>(of.count) * p.group.d + item_rows - 1) / item_rows;
+      const bool wrong = load_arg(p.lengths + b) > p.capacity || load_arg(p.offsets + b) < 0 || load_arg(p.offsets + b + 1) > p.tokens ||
+                         load_arg(p.offsets + b + 1) < load_arg(p.offsets + b);
+      if (wrong && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+    }
+    int64_t all;
+    const int64_t before = items + sum_before(mine, of_warps, all);
+    if (b < p.batch) p.tiles_before[b] = static_cast<int32_t>(min(before, static_cast<int64_t>(p.max_items)));
+    items += all;
+  }
+  // (more only where offsets fall)
+  const int32_t count = static_cast<int32_t>(min(items, static_cast<int64_t>(p.max_items)));
+  if (items > p.max_items && threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+  __syncthreads();
+
+  // Each item's tokens.  Where they follow from its first and last query token a thread does, else a warp.
+  const bool by_token = p.starts != nullptr || (p.own != nullptr && p.window > 0);
+  auto make = [&](int32_t item, int32_t begin_lane, int32_t lanes) {
+    int32_t low = 0, high = p.batch - 1;  // the last sequence with tiles_before <= item
+    while (low < high) {
+      const int32_t middle = (low + high + 1) / 2;
+      if (p.tiles_before[middle] <= item) low = middle; else high = middle - 1;
+    }
+    PromptItem it;
+    it.b = low;
+    const PromptSequence of(p, low);
+    const int64_t row0 = static_cast<int64_t>(item - p.tiles_before[low]) * item_rows;
+    const int64_t rows = min(static_cast<int64_t>(item_rows), static_cast<int64_t>(of.count) * p.group.d - row0);
+    it.row0 = static_cast<int32_t>(row0);
+    it.rows = static_cast<int32_t>(max(rows, static_cast<int64_t>(0)));
+    int32_t lo = INT32_MAX, hi = 0;
+    if (it.rows > 0) {
+      const int32_t t0 = p.group.div(it.row0), t1 = p.group.div(it.row0 + it.rows - 1);
+      if (by_token) {
+#pragma unroll 1
+        for (int32_t i = t0 + begin_lane; i <= t1; i += lanes) {
+          const PromptView v = of.view(p, i);
+          if (v.hi > v.lo) lo = min(lo, v.lo), hi = max(hi, v.hi);
+        }
+      } else {
+        const PromptView a = of.view(p, t0), z = of.view(p, t1);
+        if (z.hi > a.lo) lo = a.lo, hi = z.hi;
+      }
+    }
+    if (lanes > 1) {
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      hi = __reduce_max_sync(0xffffffffu, hi);
+    }
+    it.lo = hi > lo ? lo : 0;
+    it.hi = hi > lo ? hi : 0;
+    it.steps = max(1, (it.hi + step_tokens - 1) / step_tokens - it.lo / step_tokens);
+    it.first = 0;
+    return it;
+  };
+  if (by_token) {
+#pragma unroll 1
+    for (int32_t item = warp; item < count; item += kPlanThreads / 32) {
+      const PromptItem it = make(item, lane, 32);
+      if (lane == 0) p.items[item] = it;
+    }
+  } else {
+#pragma unroll 1
+    for (int32_t item = threadIdx.x; item < count; item += kPlanThreads) p.items[item] = make(item, 0, 1);
+  }
+  __syncthreads();
+
+  // Number the steps.
+  int64_t steps = 0;
+  int32_t longest = 0;
+#pragma unroll 1
+  for (int32_t i0 = 0; i0 < count; i0 += kPlanThreads) {
+    const int32_t item = i0 + threadIdx.x;
+    const int32_t mine = item < count ? p.items[item].steps : 0;
+    int64_t all;
+    const int64_t before = steps + sum_before(mine, of_warps, all);
+    if (item < count) p.items[item].first = before;
+    longest = max(longest, mine);
+    steps += all;
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 0) longest_of[warp] = longest;
+  __syncthreads();
+  longest = __reduce_max_sync(0xffffffffu, longest_of[lane]);
+
+  // An item to a CTA where there are no more of them and the longest one takes hardly longer than equal runs and a join.
+  constexpr int32_t kAlone = 4;
+  const int64_t total = steps * p.kv_heads, runs = static_cast<int64_t>(count) * p.kv_heads;
+  const int64_t share = (total + p.ctas - 1) / p.ctas;
+  const bool cut = runs > p.ctas || longest > share + kAlone;
+  if (threadIdx.x == 0) {
+    p.plan->items = count;
+    p.plan->cut = cut;
+    p.plan->head_steps = steps;
+  }
+#pragma unroll 1
+  for (int32_t cta = threadIdx.x; cta < p.ctas; cta += kPlanThreads) {
+    PromptStart s = {0, 0, 0, 0, 0, 0};
+    if (!cut) {
+      if (cta < runs) {
+        s.head = cta / count;
+        s.item = cta % count;
+        s.count = p.items[s.item].steps;
+        s.begin = s.head * steps + p.items[s.item].first;
+      }
+    } else if (cta * share < total) {
+      s.begin = cta * share;
+      s.count = min(share, total - s.begin);
+      s.head = static_cast<int32_t>(s.begin / steps);
+      const int64_t wanted = s.begin - s.head * steps;
+      int32_t low = 0, high = count - 1;  // the last item that begins there or before
+      while (low < high) {
+        const int32_t middle = (low + high + 1) / 2;
+        if (p.items[middle].first <= wanted) low = middle; else high = middle - 1;
+      }
+      s.item = low;
+      s.step = static_cast<int32_t>(wanted - p.items[low].first);
+    }
+    p.cta_starts[cta] = s;
+  }
+}
+
+bool prompt_variant_of(int64_t dim, bool codes, bool bent, PromptVariant* out) {
+  if (codes) return bent ? prompt_codes_bent(dim, out) : prompt_codes(dim, out);
+  return bent ? prompt_bf16_bent(dim, out) : prompt_bf16(dim, out);
+}
+
+// Allows a kernel its shared memory and checks that its warps can divide its registers, once per device.
+int allow_prompt(const PromptVariant& v, int64_t dim, bool codes, bool bent, int device) {
+  static std::mutex mutex;
+  static bool done[64][5][2][2];
+  std::lock_guard<std::mutex> guard(mutex);
+  bool& known = done[device & 63][dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : dim == 192 ? 3 : 4][codes][bent];
+  if (known) return kOk;
+  cudaFuncAttributes attributes;
+  CHORD_CUDA(cudaFuncGetAttributes(&attributes, v.kernel));
+  if (!register_split_fits(attributes.numRegs, 8, v.other_regs, 8, v.row_regs)) {
+    return fail(kUnsupportedDevice, "the attention kernel was compiled to %d registers, its warps divide 128", attributes.numRegs);
+  }
+  CHORD_CUDA(cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem));
+  known = true;
+  return kOk;
+}
+
+constexpr int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int64_t most_items(int64_t batch, int64_t tokens, int64_t group, int64_t tiles) {
+  return tokens * group / (tiles * kPromptTile) + batch;
+}
+
+// Where things lie in the workspace.
+struct PromptScratch {
+  int64_t starts, items, before, parts, end;
+  PromptScratch(int64_t max_items, int64_t batch, int64_t ctas, int64_t part_floats) {
+    starts = aligned(sizeof(PromptPlan));
+    items = starts + aligned(ctas * sizeof(PromptStart));
+    before = items + aligned(max_items * sizeof(PromptItem));
+    parts = before + aligned(batch * 4);
+    end = parts + ctas * 2 * part_floats * 4;
+  }
+};
+
+struct PromptCall {
+  const void* q;
+  int64_t q_token, q_head;
+  const chord_b200_kv_cache* cache;
+  const int32_t* tables;
+  int64_t table_stride, max_pages;
+  const int32_t *lengths, *offsets, *starts, *prefixes, *own;
+  int64_t own_capacity;
+  const float *extra, *extra_lse;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  int64_t batch, tokens, heads;
+  const chord_b200_scores* scores;
+  void* stream;
+};
+
+int64_t token_capacity(int64_t max_pages, const chord_b200_kv_cache* cache) {
+  // (token numbers, those of a step behind the last too, fit 32 bits)
+  const int64_t capacity = max_pages * cache->page_size;
+  return capacity > (1ll << 31) - 65536 ? (1ll << 31) - 65536 : capacity;
+}
+
+// The checks that the entry points share.
+int check_prompt(const PromptCall& c) {
+  CHORD_REQUIRE(c.q != nullptr && c.tables != nullptr && c.lengths != nullptr && c.offsets != nullptr && c.out != nullptr &&
+                    c.workspace != nullptr && c.scores != nullptr,
+                "null pointer");
+  CHORD_REQUIRE(c.heads > 0 && c.heads <= 65535 && c.heads % c.cache->heads == 0,
+                "the number of query heads (%lld) must be a multiple of the cache's (%lld)", static_cast<long long>(c.heads),
+                static_cast<long long>(c.cache->heads));
+  CHORD_REQUIRE(c.q_token >= 0 && c.q_head >= 0 && c.q_token % 8 == 0 && c.q_head % 8 == 0 &&
+                    ((reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.out) | reinterpret_cast<uintptr_t>(c.workspace)) & 15u) == 0,
+                "q's rows, out and the workspace must lie on 16-byte boundaries");
+  CHORD_REQUIRE(c.max_pages > 0 && c.table_stride >= 0 && c.max_pages < (1ll << 31), "a block table has a page or more");
+  CHORD_REQUIRE(c.scores->window >= 0 && c.scores->window < (1ll << 31), "window out of range");
+  CHORD_REQUIRE(c.scores->scale - c.scores->scale == 0.0, "scale must be finite");
+  CHORD_REQUIRE(c.scores->cap >= 0.0 && c.scores->cap - c.scores->cap == 0.0, "the cap must be finite and at least zero");
+  // (rows of a sequence are numbered in 32 bits)
+  CHORD_REQUIRE(c.tokens * (c.heads / c.cache->heads) < (1ll << 31) - 65536, "too many query tokens and heads: %lld x %lld",
+                static_cast<long long>(c.tokens), static_cast<long long>(c.heads));
+  return kOk;
+}
+
+int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& device) {
+  PromptParams p = {};
+  p.cache = cache;
+  const int64_t group = c.heads / c.cache->heads;
+  const bool codes = c.cache->k_scale != nullptr;
+  // (the plain kernels find the largest score before they scale it)
+  const bool bent = c.scores->cap > 0.0 || c.scores->slopes != nullptr || c.scores->scale <= 0.0;
+  PromptVariant v;
+  CHORD_REQUIRE(prompt_variant_of(c.cache->head_dim, codes, bent, &v), "head_dim must be 64, 96, 128, 192 or 256, got %lld",
+                static_cast<long long>(c.cache->head_dim));
+  if (int rc = allow_prompt(v, c.cache->head_dim, codes, bent, device.device)) return rc;
+  const int64_t max_items = most_items(c.batch, c.tokens, group, v.tiles);
+  const int64_t ctas = device.sm_count;
+  const PromptScratch at(max_items, c.batch, ctas, v.part_floats);
+  CHORD_REQUIRE(c.workspace_bytes >= at.end, "the workspace has %lld bytes, this launch needs %lld",
+                static_cast<long long>(c.workspace_bytes), static_cast<long long>(at.end));
+  uint8_t* const w = static_cast<uint8_t*>(c.workspace);
+  p.plan = reinterpret_cast<PromptPlan*>(w);
+  p.cta_starts = reinterpret_cast<PromptStart*>(w + at.starts);
+  p.items = reinterpret_cast<PromptItem*>(w + at.items);
+  p.tiles_before = reinterpret_cast<int32_t*>(w + at.before);
+  p.parts = reinterpret_cast<float*>(w + at.parts);
+  p.q = static_cast<const __nv_bfloat16*>(c.q);
+  p.q_token = c.q_token;
+  p.q_head = c.q_head;
+  p.tables = c.tables;
+  p.table_stride = c.table_stride;
+  p.lengths = c.lengths;
+  p.offsets = c.offsets;
+  p.starts = c.starts;
+  p.prefixes = c.prefixes;
+  p.own = c.own;
+  p.slopes = c.scores->slopes;
+  p.extra = c.extra;
+  p.extra_lse = c.extra_lse;
+  p.out = static_cast<__nv_bfloat16*>(c.out);
+  p.lse = c.lse;
+  p.status = c.status;
+  constexpr double kLog2E = 1.4426950408889634074;
+  p.scale = static_cast<float>(c.scores->scale * kLog2E);
+  p.cap = static_cast<float>(c.scores->cap * kLog2E);
+  p.cap_scale = c.scores->cap > 0.0 ? static_cast<float>(2.0 * kLog2E * c.scores->scale / c.scores->cap) : 0.0f;
+  p.batch = static_cast<int32_t>(c.batch);
+  p.tokens = static_cast<int32_t>(c.tokens);
+  p.heads = static_cast<int32_t>(c.heads);
+  p.kv_heads = static_cast<int32_t>(c.cache->heads);
+  p.capacity = static_cast<int32_t>(token_capacity(c.max_pages, c.cache));
+  p.own_capacity = static_cast<int32_t>(c.own_capacity);
+  p.window = static_cast<int32_t>(c.scores->window);
+  p.max_items = static_cast<int32_t>(max_items);
+  p.ctas = static_cast<int32_t>(ctas);
+  p.group = Divisor(static_cast<uint32_t>(group));
+  const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+  CHORD_CUDA(launch_kernel(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, kEarlyLaunch, p, v.tiles * kPromptTile, v.step_tokens));
+  CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kPromptThreads), v.smem, stream, kEarlyLaunch, p));
+  if (ctas > 1) {
+    CHORD_CUDA(launch_kernel(v.join, dim3(static_cast<unsigned>(ctas - 1), static_cast<unsigned>(v.tiles * c.cache->head_dim / 8)),
+                             dim3(kPromptTile), 0, stream, kEarlyLaunch, p));
+  }
+  return kOk;
+}
+
+int64_t prompt_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, const DeviceInfo& device) {
+  PromptVariant v, w;
+  if (kv_heads <= 0 || heads <= 0 || batch < 0 || tokens < 0 || !prompt_bf16(head_dim, &v) || !prompt_codes(head_dim, &w)) {
+    return fail(kInvalidArgument, "head_dim must be 64, 96, 128, 192 or 256, and no size negative"), -1;
+  }
+  const int64_t floats = v.part_floats > w.part_floats ? v.part_floats : w.part_floats;
+  return PromptScratch(most_items(batch, tokens, heads / kv_heads, v.tiles), batch, device.sm_count, floats).end;
+}
+
+}  // namespace
+}  // namespace chord
+
+extern "C" {
+
+int64_t chord_b200_prompt_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  using namespace chord;
+  DeviceInfo device;
+  if (current_device_info(&device)) return -1;
+  return prompt_bytes(batch, tokens, heads, kv_heads, head_dim, device);
+}
+
+int chord_b200_prompt_attention(const void* q, int64_t q_token, int64_t q_head, const chord_b200_kv_cache* cache,
+                                const int32_t* tables, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                                const int32_t* offsets, const int32_t* starts, const int32_t* prefixes, void* out, float* lse,
+                                void* workspace, int64_t workspace_bytes, int32_t* status, int64_t batch, int64_t tokens,
+                                int64_t heads, const chord_b200_scores* scores, void* stream) {
+  using namespace chord;
+  Cache pages;
+  if (int rc = make_cache(cache, &pages)) return rc;
+  CHORD_REQUIRE(batch >= 0 && batch < (1ll << 31) && tokens >= 0 && tokens < (1ll << 31), "sizes out of range");
+  if (batch == 0 || tokens == 0) return kOk;
+  const PromptCall c = {q, q_token, q_head, cache, tables, table_stride, max_pages, lengths, offsets, starts, prefixes, nullptr,
+                        0, nullptr, nullptr, out, lse, workspace, workspace_bytes, status, batch, tokens, heads, scores, stream};
+  if (int rc = check_prompt(c)) return rc;
+  DeviceInfo device;
+  if (int rc = current_device_info(&device)) return rc;
+  if (int rc = require_blackwell(device)) return rc;
+  return launch_prompt(c, pages, device);
+}
+
+int64_t chord_b200_shared_prefix_attention_workspace_bytes(int64_t groups, int64_t batch, int64_t heads, int64_t kv_heads,
+                                                           int64_t head_dim) {
+  using namespace chord;
+  DeviceInfo device;
+  if (current_device_info(&device)) return -1;
+  const int64_t prompt = prompt_bytes(groups, batch, heads, kv_heads, head_dim, device);
+  if (prompt < 0) return -1;
+  const int64_t token = chord_b200_paged_attention_workspace_bytes(head_dim, heads / kv_heads);
+  if (token < 0) return -1;
+  // the tokens' own parts, their sums, and room for either kernel
+  return aligned(batch * heads * head_dim * 4) + aligned(batch * heads * 4) + (prompt > token ? prompt : token);
+}
+
+int chord_b200_shared_prefix_attention(const void* q, int64_t q_batch, int64_t q_head, const chord_b200_kv_cache* cache,
+                                       const int32_t* prefix_tables, int64_t prefix_stride, int64_t prefix_pages,
+                                       const int32_t* prefix_lengths, const int32_t* group_offsets, int64_t groups,
+                                       const int32_t* tables, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                                       void* out, float* lse, int32_t* locks, int64_t num_locks, void* workspace,
+                                       int64_t workspace_bytes, int32_t* status, int64_t batch, int64_t heads,
+                                       const chord_b200_scores* scores, void* stream) {
+  using namespace chord;
+  Cache pages;
+  if (int rc = make_cache(cache, &pages)) return rc;
+  CHORD_REQUIRE(batch >= 0 && batch < (1ll << 31) && groups >= 0 && groups < (1ll << 31), "sizes out of range");
+  if (batch == 0 || groups == 0) return kOk;
+  const int64_t own_bytes = aligned(batch * heads * cache->head_dim * 4), sum_bytes = aligned(batch * heads * 4);
+  uint8_t* const w = static_cast<uint8_t*>(workspace);
+  CHORD_REQUIRE(workspace != nullptr && workspace_bytes >= own_bytes + sum_bytes, "the workspace has %lld bytes, this launch needs more",
+                static_cast<long long>(workspace_bytes));
+  float* const own = reinterpret_cast<float*>(w);
+  float* const own_lse = reinterpret_cast<float*>(w + own_bytes);
+  void* const rest = w + own_bytes + sum_bytes;
+  const int64_t rest_bytes = workspace_bytes - own_bytes - sum_bytes;
+  const PromptCall c = {q, q_batch, q_head, cache, prefix_tables, prefix_stride, prefix_pages, prefix_lengths, group_offsets, nullptr,
+                        nullptr, lengths, max_pages > 0 ? token_capacity(max_pages, cache) : 0, own, own_lse, out, lse, rest, rest_bytes,
+                        status, groups, batch, heads, scores, stream};
+  CHORD_REQUIRE(lengths != nullptr, "null pointer");
+  if (int rc = check_prompt(c)) return rc;
+  DeviceInfo device;
+  if (int rc = current_device_info(&device)) return rc;
+  if (int rc = require_blackwell(device)) return rc;
+  // Each token's own part first, left in FP32; the kernel over the prefixes adds it.
+  if (int rc = paged_attention(q, q_batch, q_head, cache, tables, table_stride, max_pages, lengths, nullptr, own, own_lse, locks, num_locks,
+                               rest, rest_bytes, status, batch, heads, *scores, true, stream)) {
+    return rc;
+  }
+  return launch_prompt(c, pages, device);
+}
+
+}  // extern "C"

@@ -1,0 +1,8 @@
+// Instantiations of prompt.cuh.
+#include "prompt_kernels.cuh"
+
+namespace chord {
+
+bool prompt_codes(int64_t dim, PromptVariant* out) { return prompt_variant_for<true, false>(dim, out); }
+
+}  // namespace chord

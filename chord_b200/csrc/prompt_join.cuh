@@ -1,0 +1,51 @@
+// How parts of prompt.cuh's items are joined.
+#pragma once
+
+#include "prompt.cuh"
+
+namespace chord {
+
+// Joins the parts of the items that CTAs' runs have cut: block (x, y) does what CTA x + 1 finds cut at its begin, 128
+// rows and 8 values of each, where x was the first of them.  Parts in their order, so the same inputs give the same bits.
+template <int kDim, bool kCodes>
+__global__ void __launch_bounds__(kPromptTile) prompt_join_kernel(const __grid_constant__ PromptParams p) {
+  constexpr int64_t kPart = prompt_part_floats<kDim, kCodes>();
+  ptx::grid_dependency_wait();
+  const PromptPlan plan = *p.plan;
+  if (!plan.cut) return;
+  const PromptStart at = p.cta_starts[blockIdx.x + 1], before = p.cta_starts[blockIdx.x];
+  if (at.count == 0 || at.step == 0) return;
+  if (before.head == at.head && before.item == at.item && before.step > 0) return;  // its begin lies further back
+  const PromptItem it = p.items[at.item];
+  const int tile = blockIdx.y / (kDim / 8), dim = blockIdx.y % (kDim / 8) * 8;
+  const int32_t row = threadIdx.x, r = tile * kPromptTile + row;
+  if (r >= it.rows) return;
+  const int64_t end = at.head * plan.head_steps + it.first + it.steps;
+
+  float o[8] = {}, top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+  for (int32_t cta = blockIdx.x; cta < p.ctas; ++cta) {
+    if (cta > static_cast<int32_t>(blockIdx.x)) {
+      const PromptStart s = p.cta_starts[cta];
+      if (s.count == 0 || s.begin >= end) break;
+    }
+    const float* const part = p.parts + (2 * static_cast<int64_t>(cta) + (cta == static_cast<int32_t>(blockIdx.x) ? 1 : 0)) * kPart +
+                              static_cast<int64_t>(tile) * kPromptTile * (kDim + 2);
+    const float m = __ldcg(part + kDim * kPromptTile + row), l = __ldcg(part + (kDim + 1) * kPromptTile + row);
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(part) + dim / 4 * kPromptTile + row);
+    const float4 b = __ldcg(reinterpret_cast<const float4*>(part) + (dim / 4 + 1) * kPromptTile + row);
+    const float next = fmaxf(top, m), to = next == -INFINITY ? 0.0f : next;
+    const float old = exp2_fast(top - to), weight = exp2_fast(m - to);
+    top = next;
+    sum = fmaf(sum, old, l * weight);
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], old, v[i] * weight);
+  }
+  const PromptSequence of(p, it.b);
+  const int32_t token = p.group.div(it.row0 + r);
+  const int64_t head = static_cast<int64_t>(at.head) * p.group.d + (it.row0 + r - token * static_cast<int32_t>(p.group.d));
+  prompt_finish<8>(p, (of.begin + static_cast<int64_t>(token)) * p.heads + head, dim, kDim, o, top, sum, kCodes ? 64.0f : 1.0f, dim == 0);
+}
+
+}  // namespace chord

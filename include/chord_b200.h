@@ -452,6 +452,15 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
                           int64_t batch, void* k_out, void* v_out, int64_t total, int32_t* status,
                           void* stream);
 
+/* How a query's scores come about: x = scale q . k; with cap > 0 x = cap tanh(x / cap); with slopes (fp32 [heads], on the
+ * device) x -= slopes[h] |p - j| for a query at position p and the token at j; with window > 0 only tokens j > p - window
+ * are seen.  scale and cap are finite, cap and window at least zero. */
+typedef struct chord_b200_scores {
+  double scale, cap;
+  const float* slopes;
+  int64_t window;
+} chord_b200_scores;
+
 /* ---- attention of one new token over the paged cache ----------------------------------
  *   out[b, h] = sum_t p_t v_t,  p = softmax_t(scale * q[b, h] . k_t)
  * over the last min(window, lengths[b]) tokens of sequence b (window 0: all), with the keys and
@@ -480,8 +489,62 @@ int chord_b200_paged_attention(const void* q, int64_t q_batch, int64_t q_head,
                                void* workspace, int64_t workspace_bytes, int32_t* status,
                                int64_t batch, int64_t heads, int64_t window, double scale,
                                void* stream);
+/* The same with scores capped or leaned on by distance; a query's position is lengths[b] - 1.  A capped score is off by at
+ * most 2^-21 of the cap more. */
+int chord_b200_paged_attention_shaped(const void* q, int64_t q_batch, int64_t q_head,
+                                      const chord_b200_kv_cache* cache, const int32_t* tables,
+                                      int64_t table_stride, int64_t max_pages,
+                                      const int32_t* lengths, void* out, float* lse,
+                                      int32_t* locks, int64_t num_locks, void* workspace,
+                                      int64_t workspace_bytes, int32_t* status, int64_t batch,
+                                      int64_t heads, const chord_b200_scores* scores,
+                                      void* stream);
 int chord_b200_paged_attention_lock_words(void);
 int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t group);
+
+/* ---- attention of many new tokens ----------------------------------------------------
+ * Query tokens offsets[b] to offsets[b + 1] (int32 [batch + 1], never falling, within `tokens`) are the last ones of
+ * sequence b, in order: the i-th of n stands at position p = lengths[b] - n + i and sees the tokens j of the cache with
+ *   max(0, p + 1 - window (where > 0), starts[token] (where given)) <= j < max(p + 1, min(prefixes[b], lengths[b]) (where given))
+ *  q        bf16 [tokens, heads, head_dim], strides in elements (multiples of 8), rows on 16-byte boundaries
+ *  tables, table_stride, max_pages, lengths, cache   as above
+ *  starts   int32 [tokens] or null: the first token of a query token's document
+ *  prefixes int32 [batch] or null: so many first tokens are seen by all of the sequence's
+ *  out      bf16 [tokens, heads, head_dim], not overlapping q;  lse fp32 [tokens, heads] or null
+ *  workspace  chord_b200_prompt_attention_workspace_bytes(...) bytes, 16-byte aligned
+ * A token that sees nothing, or whose scores are all minus infinity, gets zeros and an lse of minus infinity.  Rows of
+ * tokens of no sequence are not written.  What a token does not see, infinities and NaN too, does not change its
+ * result.  Weights are rounded to BF16 before they multiply values; sums are FP32 and, where a sequence is cut over the
+ * device, joined in their order: the same inputs give the same bits.  Three launches; no kernel waits for another CTA. */
+int chord_b200_prompt_attention(const void* q, int64_t q_token, int64_t q_head,
+                                const chord_b200_kv_cache* cache, const int32_t* tables,
+                                int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                                const int32_t* offsets, const int32_t* starts,
+                                const int32_t* prefixes, void* out, float* lse, void* workspace,
+                                int64_t workspace_bytes, int32_t* status, int64_t batch,
+                                int64_t tokens, int64_t heads, const chord_b200_scores* scores,
+                                void* stream);
+int64_t chord_b200_prompt_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads,
+                                                    int64_t kv_heads, int64_t head_dim);
+
+/* One new token for each of `batch` sequences, of which those from group_offsets[g] to group_offsets[g + 1] (int32 [groups
+ * + 1], never falling, within batch) share a prefix: sequence b's tokens are the prefix_lengths[g] ones of row g of
+ * prefix_tables, then its own lengths[b] ones of row b of tables.  Its query stands at the last of them.  The prefix is read
+ * once for a group.  Results of sequences of no group are not written.  locks and their words as for
+ * chord_b200_paged_attention; workspace chord_b200_shared_prefix_attention_workspace_bytes(...) bytes, 16-byte aligned. */
+int chord_b200_shared_prefix_attention(const void* q, int64_t q_batch, int64_t q_head,
+                                       const chord_b200_kv_cache* cache,
+                                       const int32_t* prefix_tables, int64_t prefix_stride,
+                                       int64_t prefix_pages, const int32_t* prefix_lengths,
+                                       const int32_t* group_offsets, int64_t groups,
+                                       const int32_t* tables, int64_t table_stride,
+                                       int64_t max_pages, const int32_t* lengths, void* out,
+                                       float* lse, int32_t* locks, int64_t num_locks,
+                                       void* workspace, int64_t workspace_bytes, int32_t* status,
+                                       int64_t batch, int64_t heads,
+                                       const chord_b200_scores* scores, void* stream);
+int64_t chord_b200_shared_prefix_attention_workspace_bytes(int64_t groups, int64_t batch, int64_t heads,
+                                                           int64_t kv_heads, int64_t head_dim);
 
 #ifdef __cplusplus
 }
