@@ -37,6 +37,8 @@ _EXPORTS = {
     "paged_attention": "chord_b200.attention",
     "prompt_attention": "chord_b200.prompt",
     "shared_prefix_attention": "chord_b200.prompt",
+    "attention_weights": "chord_b200.eviction",
+    "cache_evict": "chord_b200.eviction",
     "qk_norm_rope": "chord_b200.attention",
     "qk_norm_rope_write": "chord_b200.attention",
 }

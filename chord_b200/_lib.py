@@ -106,6 +106,11 @@ SIGNATURES = {
                                                   _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr,
                                                   _ptr]),
     "chord_b200_shared_prefix_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "chord_b200_attention_weights": (_int, [_ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64,
+                                            _int, _ptr, _i64, _i64, _ptr, _ptr]),
+    "chord_b200_cache_evict": (_int, [_ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _ptr, _ptr,
+                                      _i64, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr]),
+    "chord_b200_cache_evict_workspace_bytes": (_i64, [_i64, _i64, _i64]),
 }
 
 

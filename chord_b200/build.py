@@ -23,7 +23,7 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 CSRC = PACKAGE_DIR / "csrc"
 LIB_PATH = PACKAGE_DIR / "libchord_b200.so"
 SOURCES = ("core.cu", "gemm.cu", "pack.cu", "fused.cu", "ep.cu", "gemv.cu", "heads.cu", "attention.cu",
-           "prompt.cu", "prompt_bf16.cu", "prompt_bf16_bent.cu", "prompt_codes.cu", "prompt_codes_bent.cu")
+           "prompt.cu", "prompt_bf16.cu", "prompt_bf16_bent.cu", "prompt_codes.cu", "prompt_codes_bent.cu", "evict.cu")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 
 

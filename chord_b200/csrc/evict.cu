@@ -1,0 +1,600 @@
+// What each token of the cache got of a new token's attention, and eviction by what has been gathered of it.
+#include "../../include/chord_b200.h"
+#include "common.h"
+#include "kv_cache.cuh"
+#include "warp_ops.cuh"
+
+namespace chord {
+namespace {
+
+constexpr float kLog2E = 1.44269504088896341f;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float reciprocal_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ------------------------------------------------------------------- weights --
+
+struct WeighParams {
+  Cache cache;
+  const __nv_bfloat16* q;  // [batch, heads, dim]
+  int64_t q_batch, q_head;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const float* lse;      // [batch, heads]
+  const float* slopes;   // [heads] or null
+  float* weights;        // [batch, kv_heads, width]
+  int64_t weight_batch, weight_head;
+  int32_t* status;
+  float scale, cap, two_over_cap;  // as of paged_attention
+  int32_t heads, group, capacity, width, window, add;
+};
+
+constexpr int kWeighWarps = 4;
+constexpr int kWeighRun = 64;  // tokens of a warp
+constexpr int kWeighTokens = kWeighWarps * kWeighRun;
+
+// A warp takes 64 tokens of one key-value head, 16 at a time as the rows of mma.m16n8k16, 8 of the heads that share it as
+// columns.  A lane's fragments come straight from memory: a product's sum does not depend on the order of its terms, so
+// the dims of a lane's 16 bytes (8 of codes) of a key and of the same piece of a query stand for the columns that
+// the instruction wants there.  The weights of a token's heads are summed in one order, so the same inputs give the
+// same bits.
+template <int kDim, bool kCodes>
+__global__ void __launch_bounds__(kWeighWarps * 32) attention_weights_kernel(const WeighParams p) {
+  constexpr int kChunks = kDim / 32;  // of 8 dims for each of four lanes
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q4 = lane & 3, r8 = lane >> 2;
+  ptx::grid_dependency_wait();
+  const int32_t b = blockIdx.z, kv_head = blockIdx.y;
+  const int32_t given = load_arg(p.lengths + b), length = max(0, min(given, min(p.capacity, p.width)));
+  if (given > min(p.capacity, p.width) && threadIdx.x == 0 && blockIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+  const int32_t low = p.window > 0 ? max(0, length - p.window) : 0;
+  const int32_t token0 = blockIdx.x * kWeighTokens + warp * kWeighRun;
+  float* const row = p.weights + b * p.weight_batch + kv_head * p.weight_head;
+  if (token0 >= length || token0 + kWeighRun <= low) {
+    if (!p.add) {
+      for (int32_t t = token0 + lane; t < min(token0 + kWeighRun, p.width); t += 32) row[t] = 0.0f;
+    }
+    return;
+  }
+  // Where the run's tokens lie: two to a lane, as offsets in bytes, negative for none.
+  int64_t offset[2];
+  float key_scale[2] = {1.0f, 1.0f};
+  const int32_t* const table = p.tables + b * p.table_stride;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int32_t token = token0 + 32 * i + lane;
+    offset[i] = -1;
+    if (token >= low && token < length) {
+      const uint32_t index = p.cache.page_size.div(token), place = token - index * p.cache.page_size.d;
+      const int32_t page = load_arg(table + index);
+      if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.num_pages)) {
+        offset[i] = page * p.cache.page + place * p.cache.token + kv_head * p.cache.head;
+        if constexpr (kCodes) {
+          key_scale[i] = 64.0f * load_arg(p.cache.k_scale + page * p.cache.scale_page + place * p.cache.scale_token + kv_head * p.cache.scale_head);
+        }
+      } else if (p.status != nullptr) {
+        atomicOr(p.status, kStatusIndex);
+      }
+    }
+  }
+  float sum[kWeighRun / 16][2] = {};
+#pragma unroll 1
+  for (int32_t h0 = 0; h0 < p.group; h0 += 8) {
+    const int64_t head0 = static_cast<int64_t>(kv_head) * p.group + h0;
+    // Queries: head r8's, the lane's 8 dims of each 32.
+    uint4 qf[kChunks];
+    {
+      const bool there = h0 + r8 < p.group;
+      const __nv_bfloat16* const q = p.q + b * p.q_batch + (head0 + (there ? r8 : 0)) * p.q_head + 8 * q4;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) qf[c] = there ? load_once(q + 32 * c) : make_uint4(0, 0, 0, 0);
+    }
+    // Of the columns' heads, 2 q4 and the next: what the exponent starts from, and the slope.
+    float base[2], slope[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool there = h0 + 2 * q4 + i < p.group;
+      const float lse = there ? load_arg(p.lse + static_cast<int64_t>(b) * p.heads + head0 + 2 * q4 + i) : -INFINITY;
+      base[i] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;  // (nothing was seen: no weight)
+      slope[i] = there && p.slopes != nullptr ? load_arg(p.slopes + head0 + 2 * q4 + i) * kLog2E : 0.0f;
+    }
+#pragma unroll
+    for (int step = 0; step < kWeighRun / 16; ++step) {
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint4 kf[2][kChunks];
+      float factor[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // tokens r8 and r8 + 8
+        const int from = (16 * step + 8 * i) % 32 + r8;
+        const int64_t o = __shfl_sync(0xffffffffu, offset[step / 2], from);
+        factor[i] = p.scale * (kCodes ? __shfl_sync(0xffffffffu, key_scale[step / 2], from) : 1.0f);
+        const uint8_t* const at = p.cache.k + (o < 0 ? 0 : o) + q4 * (kCodes ? 8 : 16);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          if constexpr (kCodes) {
+            const uint2 v = o < 0 ? make_uint2(0x80808080u, 0x80808080u) : load_arg(reinterpret_cast<const uint2*>(at + 32 * c));
+            kf[i][c].x = v.x;
+            kf[i][c].y = v.y;
+          } else {
+            kf[i][c] = o < 0 ? make_uint4(0, 0, 0, 0) : load_once(at + 64 * c);
+          }
+        }
+      }
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            constexpr uint32_t kOffset = 0xC000C000u;  // -128 / 64, twice
+            const uint32_t x = kf[i][c].x, y = kf[i][c].y;
+            kf[i][c] = make_uint4(bf16x2_fma(__byte_perm(x, 0, 0x4140), kTwo127, kOffset), bf16x2_fma(__byte_perm(x, 0, 0x4342), kTwo127, kOffset),
+                                  bf16x2_fma(__byte_perm(y, 0, 0x4140), kTwo127, kOffset), bf16x2_fma(__byte_perm(y, 0, 0x4342), kTwo127, kOffset));
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const uint32_t a0[4] = {kf[0][c].x, kf[1][c].x, kf[0][c].y, kf[1][c].y};
+        const uint32_t a1[4] = {kf[0][c].z, kf[1][c].z, kf[0][c].w, kf[1][c].w};
+        ptx::mma_m16n8k16(s, a0, qf[c].x, qf[c].y);
+        ptx::mma_m16n8k16(s, a1, qf[c].z, qf[c].w);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float behind = static_cast<float>(length - 1 - (token0 + 16 * step + 8 * i + r8));
+        float two = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float x = s[2 * i + k] * factor[i];
+          if (p.cap > 0.0f) x = fmaf(-2.0f * p.cap, reciprocal_approx(exp2_approx(x * p.two_over_cap) + 1.0f), p.cap);
+          x = fmaf(-slope[k], behind, x);
+          const float weight = exp2_approx(x + base[k]);
+          two += base[k] == -INFINITY ? 0.0f : weight;
+        }
+        two += __shfl_xor_sync(0xffffffffu, two, 1);
+        two += __shfl_xor_sync(0xffffffffu, two, 2);
+        sum[step][i] += two;
+      }
+    }
+  }
+#pragma unroll
+  for (int step = 0; step < kWeighRun / 16; ++step) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int32_t token = token0 + 16 * step + 8 * i + r8;
+      if (q4 != 0 || token >= p.width) continue;
+      const bool seen = token >= low && token < length;
+      if (!p.add) {
+        row[token] = seen ? sum[step][i] : 0.0f;
+      } else if (seen) {
+        row[token] += sum[step][i];
+      }
+    }
+  }
+}
+
+using WeighKernel = void (*)(WeighParams);
+
+template <bool kCodes>
+WeighKernel weigh_kernel(int64_t dim) {
+  switch (dim) {
+    case 64: return attention_weights_kernel<64, kCodes>;
+    case 96: return attention_weights_kernel<96, kCodes>;
+    case 128: return attention_weights_kernel<128, kCodes>;
+    case 192: return attention_weights_kernel<192, kCodes>;
+    case 256: return attention_weights_kernel<256, kCodes>;
+  }
+  return nullptr;
+}
+
+// ------------------------------------------------------------------ eviction --
+
+struct EvictParams {
+  Cache cache;
+  const int32_t* tables;
+  const int32_t* new_tables;
+  int64_t table_stride, new_stride;
+  const int32_t* lengths;
+  const float* weights;  // [batch, kv_heads, width]
+  int64_t weight_batch, weight_head;
+  int32_t* new_lengths;  // [batch]
+  float* new_weights;    // [batch, kv_heads, new_width], contiguous
+  int32_t* kept;         // [batch, kv_heads, keep]
+  int32_t* status;
+  int32_t capacity, new_capacity, width, new_width, keep, first, recent, row_bytes;
+};
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectItems = 4;  // of a thread, one after another
+constexpr int kBins = 2048;
+constexpr int32_t kSelectHeld = 40960;  // weights that are kept in shared memory between the passes
+
+// Order of weights as that of whole numbers: zeros alike, NaN above all.
+__device__ __forceinline__ uint32_t rank_of(float w) {
+  if (w != w) return 0xFFFFFFFFu;
+  const uint32_t bits = __float_as_uint(w + 0.0f);
+  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+// One CTA for a sequence's key-value head: the smallest weight that is kept, found by its digits (11, 11 and 10 bits),
+// then the kept tokens in order.  Counts do not depend on the order in which they are counted.
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
+  extern __shared__ uint32_t held[];  // the weights' ranks, where there is room
+  __shared__ uint32_t bins[kBins];
+  __shared__ uint32_t of_warps[2][kSelectThreads / 32];
+  __shared__ uint32_t found[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ptx::grid_dependency_wait();
+  const int32_t b = blockIdx.y, head = blockIdx.x;
+  const int32_t given = load_arg(p.lengths + b), limit = min(p.capacity, p.width), length = max(0, min(given, limit));
+  const int32_t count = min(length, p.keep);
+  if (threadIdx.x == 0 && head == 0) {
+    p.new_lengths[b] = count;
+    if (given > limit && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+  }
+  const float* const weights = p.weights + b * p.weight_batch + head * p.weight_head;
+  const int64_t row = static_cast<int64_t>(b) * gridDim.x + head;
+  float* const out = p.new_weights + row * p.new_width;
+  int32_t* const kept = p.kept + row * p.keep;
+  for (int32_t i = count + threadIdx.x; i < p.new_width; i += kSelectThreads) out[i] = 0.0f;
+  if (length <= p.keep) {
+    for (int32_t i = threadIdx.x; i < count; i += kSelectThreads) {
+      kept[i] = i;
+      out[i] = load_arg(weights + i);
+    }
+    return;
+  }
+  const int32_t begin = p.first, end = length - p.recent;
+  uint32_t wanted = p.keep - p.first - p.recent;  // of the tokens between
+  uint32_t prefix = 0, least = 0xFFFFFFFFu;
+  const bool hold = end - begin <= kSelectHeld;
+  auto rank_at = [&](int32_t i) { return hold ? held[i - begin] : rank_of(load_arg(weights + i)); };
+  if (hold && wanted > 0) {
+    for (int32_t i = begin + threadIdx.x; i < end; i += kSelectThreads) held[i - begin] = rank_of(load_arg(weights + i));
+  }
+  if (wanted > 0) {
+    int shift = 21;
+#pragma unroll 1
+    for (int digit = 0; digit < 3; ++digit) {
+      for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
+      __syncthreads();
+      const uint32_t mask = digit == 2 ? 0x3FFu : 0x7FFu;
+#pragma unroll 4
+      for (int32_t i0 = begin; i0 < end; i0 += kSelectThreads) {
+        const int32_t i = i0 + threadIdx.x;
+        const uint32_t rank = i < end ? rank_at(i) : 0;
+        const bool counts = i < end && (digit == 0 || rank >> (shift + (digit == 2 ? 10 : 11)) == prefix);
+        const uint32_t bin = rank >> shift & mask;
+        // (many equal ones, zeros as a rule, would wait for one another: the first lane's kind in one go)
+        const uint32_t some = __ballot_sync(0xffffffffu, counts);
+        if (some == 0) continue;
+        const int leader = __ffs(some) - 1;
+        const uint32_t its_bin = __shfl_sync(0xffffffffu, bin, leader);
+        const uint32_t same = __ballot_sync(0xffffffffu, counts && bin == its_bin);
+        if (lane == leader) {
+          atomicAdd(&bins[bin], static_cast<uint32_t>(__popc(same)));
+        } else if (counts && !(same >> lane & 1)) {
+          atomicAdd(&bins[bin], 1u);
+        }
+      }
+      __syncthreads();
+      // The bin in which the wanted-th largest lies: two bins to a thread, from the top.
+      const int top = kBins - 1 - 2 * static_cast<int>(threadIdx.x);
+      const uint32_t high = bins[top], lower = bins[top - 1];
+      uint32_t upto = high + lower;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t below = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += below;
+      }
+      if (lane == 31) of_warps[0][warp] = upto;
+      __syncthreads();
+      uint32_t before = upto - high - lower;
+      for (int w = 0; w < warp; ++w) before += of_warps[0][w];
+      if (before < wanted && wanted <= before + high) {
+        found[0] = top;
+        found[1] = before;
+      } else if (before + high < wanted && wanted <= before + high + lower) {
+        found[0] = top - 1;
+        found[1] = before + high;
+      }
+      __syncthreads();
+      prefix = digit == 0 ? found[0] : prefix << (digit == 2 ? 10 : 11) | found[0];
+      wanted -= found[1];
+      shift = digit == 0 ? 10 : 0;
+      __syncthreads();
+    }
+    least = prefix;
+  }
+  // In order: `wanted` of those equal to the least, all above it.
+  uint32_t above = 0, level = 0;  // so far
+#pragma unroll 1
+  for (int32_t i0 = 0; i0 < length; i0 += kSelectThreads * kSelectItems) {
+    const int32_t mine = i0 + threadIdx.x * kSelectItems;
+    bool is_above[kSelectItems], is_level[kSelectItems];
+    uint32_t above_here = 0, level_here = 0;
+#pragma unroll
+    for (int k = 0; k < kSelectItems; ++k) {
+      const int32_t i = mine + k;
+      const bool between = i >= begin && i < end && i < length;
+      const uint32_t rank = between && p.keep > p.first + p.recent ? rank_at(i) : 0;
+      is_above[k] = i < length && (!between || (p.keep > p.first + p.recent && rank > least));
+      is_level[k] = between && p.keep > p.first + p.recent && rank == least;
+      above_here += is_above[k];
+      level_here += is_level[k];
+    }
+    uint32_t a = above_here, l = level_here;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, l, d);
+      if (lane >= d) a += x, l += y;
+    }
+    __syncthreads();
+    if (lane == 31) of_warps[0][warp] = a, of_warps[1][warp] = l;
+    __syncthreads();
+    const uint32_t from_a = of_warps[0][lane], from_l = of_warps[1][lane];
+    uint32_t a_before = above + a - above_here + __reduce_add_sync(0xffffffffu, lane < warp ? from_a : 0);
+    uint32_t l_before = level + l - level_here + __reduce_add_sync(0xffffffffu, lane < warp ? from_l : 0);
+    above += __reduce_add_sync(0xffffffffu, from_a);
+    level += __reduce_add_sync(0xffffffffu, from_l);
+#pragma unroll
+    for (int k = 0; k < kSelectItems; ++k) {
+      if (is_above[k] || (is_level[k] && l_before < wanted)) {
+        const uint32_t at = a_before + min(l_before, wanted);
+        kept[at] = mine + k;
+        out[at] = load_arg(weights + mine + k);
+      }
+      a_before += is_above[k];
+      l_before += is_level[k];
+    }
+  }
+}
+
+struct RowPlace {
+  int64_t page, place;  // page < 0: none
+};
+
+__device__ __forceinline__ RowPlace row_place(const EvictParams& p, const int32_t* table, int32_t capacity, int32_t token) {
+  if (token >= capacity) return {-1, 0};
+  const uint32_t index = p.cache.page_size.div(token);
+  const int32_t page = load_arg(table + index);
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.cache.num_pages)) return {-1, 0};
+  return {page, token - index * p.cache.page_size.d};
+}
+
+constexpr int kCopyThreads = 256;
+
+// Rows into other pages: every 16 bytes of keys and of values on their own.
+__global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictParams p) {
+  ptx::grid_dependency_wait();
+  const int32_t b = blockIdx.z, head = blockIdx.y, pieces = p.row_bytes / 16;
+  const int32_t count = p.new_lengths[b];
+  const int32_t* const kept = p.kept + (static_cast<int64_t>(b) * gridDim.y + head) * p.keep;
+  const int32_t* const from_table = p.tables + b * p.table_stride;
+  const int32_t* const to_table = p.new_tables + b * p.new_stride;
+  const int32_t rows = kCopyThreads / pieces;  // of a round
+  const int32_t row = threadIdx.x / pieces, piece = threadIdx.x % pieces;
+  if (row >= rows) return;
+  for (int32_t i = blockIdx.x * rows + row; i < count; i += gridDim.x * rows) {
+    const RowPlace from = row_place(p, from_table, p.capacity, kept[i]), to = row_place(p, to_table, p.new_capacity, i);
+    if ((from.page < 0 || to.page < 0) && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+    if (to.page < 0) continue;
+    const int64_t read = from.page * p.cache.page + from.place * p.cache.token + head * p.cache.head + piece * 16;
+    const int64_t write = to.page * p.cache.page + to.place * p.cache.token + head * p.cache.head + piece * 16;
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
+    if (from.page >= 0) k = load_once(p.cache.k + read), v = load_once(p.cache.v + read);
+    *reinterpret_cast<uint4*>(p.cache.k + write) = k;
+    *reinterpret_cast<uint4*>(p.cache.v + write) = v;
+    if (p.cache.k_scale != nullptr && piece == 0) {
+      const int64_t read_scale = from.page * p.cache.scale_page + from.place * p.cache.scale_token + head * p.cache.scale_head;
+      const int64_t write_scale = to.page * p.cache.scale_page + to.place * p.cache.scale_token + head * p.cache.scale_head;
+      p.cache.k_scale[write_scale] = from.page >= 0 ? load_arg(p.cache.k_scale + read_scale) : 0.0f;
+      p.cache.v_scale[write_scale] = from.page >= 0 ? load_arg(p.cache.v_scale + read_scale) : 0.0f;
+    }
+  }
+}
+
+constexpr int kShiftThreads = 1024;
+
+// Keeps its place among the barriers and stores.
+__device__ __forceinline__ float load_ordered(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// Rows forward within their pages.  A kept token never moves back, so rows are moved in order, a round of them at a time,
+// read whole before any of it is written; a CTA has some columns of a head's rows of its own (64 bytes or, of rows that
+// do not divide so, 32), so that no two have to wait for each other.  One more takes the scales.
+__global__ void __launch_bounds__(kShiftThreads) evict_shift_kernel(const EvictParams p, int32_t slice_bytes) {
+  __shared__ int32_t first_moved;
+  ptx::grid_dependency_wait();
+  const int32_t b = blockIdx.z, head = blockIdx.y, slices = p.row_bytes / slice_bytes;
+  const int32_t count = p.new_lengths[b];
+  const int32_t* const kept = p.kept + (static_cast<int64_t>(b) * gridDim.y + head) * p.keep;
+  const int32_t* const table = p.tables + b * p.table_stride;
+  if (threadIdx.x == 0) {  // (kept[i] - i never falls)
+    int32_t low = 0, high = count;
+    while (low < high) {
+      const int32_t middle = (low + high) / 2;
+      if (kept[middle] == middle) low = middle + 1; else high = middle;
+    }
+    first_moved = low;
+  }
+  __syncthreads();
+  const int32_t begin = first_moved;
+  const bool of_scales = blockIdx.x == 2 * slices;
+  const int32_t lanes = of_scales ? 2 : slice_bytes / 16, rows = kShiftThreads / lanes;
+  const int32_t row = threadIdx.x / lanes, piece = threadIdx.x % lanes;
+  uint8_t* const values = blockIdx.x < slices ? p.cache.k : p.cache.v;
+  const int64_t column = static_cast<int64_t>(blockIdx.x % slices) * slice_bytes + piece * 16;
+  float* const scales = piece == 0 ? p.cache.k_scale : p.cache.v_scale;
+  auto place_of = [&](const RowPlace& at) { return at.page * p.cache.page + at.place * p.cache.token + head * p.cache.head + column; };
+  auto scale_of = [&](const RowPlace& at) { return at.page * p.cache.scale_page + at.place * p.cache.scale_token + head * p.cache.scale_head; };
+  uint4 ahead = make_uint4(0, 0, 0, 0);
+  RowPlace ahead_to = {-1, 0};
+  auto read = [&](int32_t i) {
+    ahead_to.page = -1;
+    if (i >= count) return;
+    const RowPlace from = row_place(p, table, p.capacity, kept[i]);
+    ahead_to = row_place(p, table, p.capacity, i);
+    if ((from.page < 0 || ahead_to.page < 0) && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+    ahead = make_uint4(0, 0, 0, 0);
+    if (from.page < 0) return;
+    if (of_scales) ahead.x = __float_as_uint(load_ordered(scales + scale_of(from))); else ahead = load_once_ordered(values + place_of(from));
+  };
+  read(begin + row);
+#pragma unroll 1
+  for (int32_t i0 = begin; i0 < count; i0 += rows) {
+    const uint4 now = ahead;
+    const RowPlace to = ahead_to;
+    read(i0 + rows + row);
+    __syncthreads();  // the round has been read (and the next: its rows lie behind what is written now)
+    if (to.page < 0) continue;
+    if (of_scales) scales[scale_of(to)] = __uint_as_float(now.x); else *reinterpret_cast<uint4*>(values + place_of(to)) = now;
+  }
+}
+
+}  // namespace
+}  // namespace chord
+
+extern "C" {
+
+int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head, const chord_b200_kv_cache* cache,
+                                 const int32_t* tables, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                                 const float* lse, float* weights, int64_t weight_batch, int64_t weight_head, int64_t width,
+                                 int add, int32_t* status, int64_t batch, int64_t heads, const chord_b200_scores* scores,
+                                 void* stream) {
+  using namespace chord;
+  WeighParams p = {};
+  if (int rc = make_cache(cache, &p.cache)) return rc;
+  CHORD_REQUIRE(batch >= 0 && batch <= 65535, "the batch must be in [0, 65535], got %lld", static_cast<long long>(batch));
+  if (batch == 0 || width == 0) return kOk;
+  CHORD_REQUIRE(q != nullptr && tables != nullptr && lengths != nullptr && lse != nullptr && weights != nullptr && scores != nullptr,
+                "null pointer");
+  CHORD_REQUIRE(heads > 0 && heads <= 65535 && heads % cache->heads == 0,
+                "the number of query heads (%lld) must be a multiple of the cache's (%lld)", static_cast<long long>(heads),
+                static_cast<long long>(cache->heads));
+  CHORD_REQUIRE(q_batch >= 0 && q_head >= 0 && q_batch % 8 == 0 && q_head % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15u) == 0,
+                "q's rows must lie on 16-byte boundaries");
+  CHORD_REQUIRE(max_pages > 0 && table_stride >= 0 && max_pages < (1ll << 31), "a block table has a page or more");
+  CHORD_REQUIRE(width > 0 && width < (1ll << 31) - 65536 && weight_batch >= 0 && weight_head >= 0, "sizes of the weights out of range");
+  CHORD_REQUIRE(scores->window >= 0 && scores->window < (1ll << 31), "window out of range");
+  CHORD_REQUIRE(scores->scale - scores->scale == 0.0 && scores->cap >= 0.0 && scores->cap - scores->cap == 0.0, "scale and cap must be finite");
+  const WeighKernel kernel = cache->k_scale != nullptr ? weigh_kernel<true>(cache->head_dim) : weigh_kernel<false>(cache->head_dim);
+  CHORD_REQUIRE(kernel != nullptr, "head_dim must be 64, 96, 128, 192 or 256, got %lld", static_cast<long long>(cache->head_dim));
+  DeviceInfo device;
+  if (int rc = current_device_info(&device)) return rc;
+  if (int rc = require_blackwell(device)) return rc;
+  const int64_t capacity = max_pages * cache->page_size;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_batch = q_batch;
+  p.q_head = q_head;
+  p.tables = tables;
+  p.table_stride = table_stride;
+  p.lengths = lengths;
+  p.lse = lse;
+  p.slopes = scores->slopes;
+  p.weights = weights;
+  p.weight_batch = weight_batch;
+  p.weight_head = weight_head;
+  p.status = status;
+  p.scale = static_cast<float>(scores->scale * 1.4426950408889634074);
+  p.cap = static_cast<float>(scores->cap * 1.4426950408889634074);
+  p.two_over_cap = scores->cap > 0.0 ? static_cast<float>(2.0 / scores->cap) : 0.0f;
+  p.heads = static_cast<int32_t>(heads);
+  p.group = static_cast<int32_t>(heads / cache->heads);
+  p.capacity = static_cast<int32_t>(capacity < (1ll << 31) - 65536 ? capacity : (1ll << 31) - 65536);
+  p.width = static_cast<int32_t>(width);
+  p.window = static_cast<int32_t>(scores->window);
+  p.add = add;
+  const dim3 grid(static_cast<unsigned>((width + kWeighTokens - 1) / kWeighTokens), static_cast<unsigned>(cache->heads), static_cast<unsigned>(batch));
+  CHORD_CUDA(launch_kernel(kernel, grid, dim3(kWeighWarps * 32), 0, static_cast<cudaStream_t>(stream), kEarlyLaunch, p));
+  return kOk;
+}
+
+int64_t chord_b200_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t keep) {
+  using namespace chord;
+  if (batch < 0 || kv_heads < 0 || keep < 0) return fail(kInvalidArgument, "no size may be negative"), -1;
+  return batch * kv_heads * keep * 4;
+}
+
+int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tables, int64_t table_stride, int64_t max_pages,
+                           const int32_t* new_tables, int64_t new_stride, int64_t new_pages, const int32_t* lengths,
+                           const float* weights, int64_t weight_batch, int64_t weight_head, int64_t width, int32_t* new_lengths,
+                           float* new_weights, int64_t new_width, void* workspace, int64_t workspace_bytes, int32_t* status,
+                           int64_t batch, int64_t keep, int64_t first, int64_t recent, void* stream) {
+  using namespace chord;
+  EvictParams p = {};
+  if (int rc = make_cache(cache, &p.cache)) return rc;
+  CHORD_REQUIRE(batch >= 0 && batch <= 65535, "the batch must be in [0, 65535], got %lld", static_cast<long long>(batch));
+  if (batch == 0) return kOk;
+  CHORD_REQUIRE(tables != nullptr && lengths != nullptr && weights != nullptr && new_lengths != nullptr && new_weights != nullptr &&
+                    workspace != nullptr,
+                "null pointer");
+  CHORD_REQUIRE(max_pages > 0 && table_stride >= 0 && max_pages < (1ll << 31), "a block table has a page or more");
+  CHORD_REQUIRE(new_tables == nullptr || (new_pages > 0 && new_stride >= 0 && new_pages < (1ll << 31)), "a block table has a page or more");
+  CHORD_REQUIRE(keep > 0 && keep < (1ll << 31) - 65536 && first >= 0 && recent >= 0 && first + recent <= keep,
+                "first and recent are at least zero and no more than keep, %lld, together, got %lld and %lld",
+                static_cast<long long>(keep), static_cast<long long>(first), static_cast<long long>(recent));
+  CHORD_REQUIRE(width > 0 && width < (1ll << 31) - 65536 && new_width > 0 && new_width < (1ll << 31) - 65536 && keep <= new_width &&
+                    weight_batch >= 0 && weight_head >= 0,
+                "sizes of the weights out of range");
+  CHORD_REQUIRE(workspace_bytes >= chord_b200_cache_evict_workspace_bytes(batch, cache->heads, keep) && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0,
+                "the workspace has %lld bytes, this launch needs %lld", static_cast<long long>(workspace_bytes),
+                static_cast<long long>(chord_b200_cache_evict_workspace_bytes(batch, cache->heads, keep)));
+  DeviceInfo device;
+  if (int rc = current_device_info(&device)) return rc;
+  if (int rc = require_blackwell(device)) return rc;
+  const auto capacity = [&](int64_t pages) {
+    const int64_t tokens = pages * cache->page_size;
+    return static_cast<int32_t>(tokens < (1ll << 31) - 65536 ? tokens : (1ll << 31) - 65536);
+  };
+  p.tables = tables;
+  p.table_stride = table_stride;
+  p.new_tables = new_tables;
+  p.new_stride = new_stride;
+  p.lengths = lengths;
+  p.weights = weights;
+  p.weight_batch = weight_batch;
+  p.weight_head = weight_head;
+  p.new_lengths = new_lengths;
+  p.new_weights = new_weights;
+  p.kept = static_cast<int32_t*>(workspace);
+  p.status = status;
+  p.capacity = capacity(max_pages);
+  p.new_capacity = new_tables != nullptr ? capacity(new_pages) : p.capacity;
+  p.width = static_cast<int32_t>(width);
+  p.new_width = static_cast<int32_t>(new_width);
+  p.keep = static_cast<int32_t>(keep);
+  p.first = static_cast<int32_t>(first);
+  p.recent = static_cast<int32_t>(recent);
+  p.row_bytes = static_cast<int32_t>(cache->head_dim * (cache->k_scale != nullptr ? 1 : 2));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned heads = static_cast<unsigned>(cache->heads), sequences = static_cast<unsigned>(batch);
+  const int64_t most = width < p.capacity ? width : p.capacity;
+  const size_t held = 4 * static_cast<size_t>(most < kSelectHeld ? most : kSelectHeld);
+  if (held > 32768) CHORD_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kSelectHeld));
+  CHORD_CUDA(launch_kernel(evict_select_kernel, dim3(heads, sequences), dim3(kSelectThreads), held, s, kEarlyLaunch, p));
+  if (new_tables != nullptr) {
+    const int rows = kCopyThreads / (p.row_bytes / 16);
+    const int64_t rounds = (keep + rows - 1) / rows;
+    CHORD_CUDA(launch_kernel(evict_copy_kernel, dim3(static_cast<unsigned>((rounds + 3) / 4), heads, sequences), dim3(kCopyThreads), 0, s, kEarlyLaunch, p));
+  } else {
+    const int32_t slice = p.row_bytes % 64 == 0 ? 64 : p.row_bytes % 32 == 0 ? 32 : 16;
+    const unsigned slices = static_cast<unsigned>(2 * (p.row_bytes / slice) + (cache->k_scale != nullptr ? 1 : 0));
+    CHORD_CUDA(launch_kernel(evict_shift_kernel, dim3(slices, heads, sequences), dim3(kShiftThreads), 0, s, kEarlyLaunch, p, slice));
+  }
+  return kOk;
+}
+
+}  // extern "C"

@@ -546,6 +546,41 @@ int chord_b200_shared_prefix_attention(const void* q, int64_t q_batch, int64_t q
 int64_t chord_b200_shared_prefix_attention_workspace_bytes(int64_t groups, int64_t batch, int64_t heads,
                                                            int64_t kv_heads, int64_t head_dim);
 
+/* ---- eviction by attention weight --------------------------------------------------
+ * What each token of sequence b got of its new token's attention:
+ *   w[b, g, j] = sum of exp(x_h,j - lse[b, h]) over the heads h that share key-value head g
+ * for the tokens j that it sees, with x as of `scores` and lse fp32 [batch, heads] as paged attention gives it (a head whose
+ * lse is minus infinity gives nothing).  weights is fp32 [batch, kv_heads, width], rows contiguous, strides in elements;
+ * add == 0: written whole, zeros for tokens that are not seen; else added to what is there.  lengths beyond the table or
+ * width: cut, status bit 32; a page outside the cache counts as keys of zero.  batch <= 65535. */
+int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
+                                 const chord_b200_kv_cache* cache, const int32_t* tables,
+                                 int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                                 const float* lse, float* weights, int64_t weight_batch,
+                                 int64_t weight_head, int64_t width, int add, int32_t* status,
+                                 int64_t batch, int64_t heads, const chord_b200_scores* scores,
+                                 void* stream);
+
+/* Cuts sequences down to `keep` tokens, each key-value head on its own: it keeps its first `first`, its last `recent` and, of
+ * those between, the ones of the largest weights (equal ones from the first on; NaN counts as the largest), in order.
+ * A sequence of no more than keep tokens keeps them all.  The rows of kept token i go to place i of the sequence's pages in
+ * new_tables (int32 [batch, new_pages]), pages that no table of the call holds otherwise, or forward in its own pages where
+ * new_tables is null; what lies behind stays as it is.  Two sequences of a call share no page that is written.
+ *  weights      fp32 [batch, kv_heads, width], rows contiguous; lengths beyond width or the table: cut, status bit 32
+ *  new_lengths  int32 [batch]: min(lengths, keep)
+ *  new_weights  fp32 [batch, kv_heads, new_width >= keep], contiguous: the kept tokens' weights, then zeros
+ *  workspace    chord_b200_cache_evict_workspace_bytes(batch, kv_heads, keep) bytes, 4-byte aligned
+ * first + recent <= keep.  A row whose page lies outside the cache moves as zeros, or is not written. */
+int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tables,
+                           int64_t table_stride, int64_t max_pages, const int32_t* new_tables,
+                           int64_t new_stride, int64_t new_pages, const int32_t* lengths,
+                           const float* weights, int64_t weight_batch, int64_t weight_head,
+                           int64_t width, int32_t* new_lengths, float* new_weights,
+                           int64_t new_width, void* workspace, int64_t workspace_bytes,
+                           int32_t* status, int64_t batch, int64_t keep, int64_t first,
+                           int64_t recent, void* stream);
+int64_t chord_b200_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t keep);
+
 #ifdef __cplusplus
 }
 #endif
