@@ -6,30 +6,12 @@
 
 #include "../../include/chord_b200.h"
 #include "common.h"
+#include "tensor_map.h"
 #include "w4a16_decode.cuh"
 #include "w4a16_gemm.cuh"
 
 namespace chord {
 namespace {
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result) !=
-            cudaSuccess ||
-        result != cudaDriverEntryPointSuccess) {
-      ptr = nullptr;
-    }
-    return reinterpret_cast<EncodeTiledFn>(ptr);
-  }();
-  return fn;
-}
 
 struct MapKey {
   const void* base;

@@ -6,6 +6,7 @@
 #include "common.h"
 #include "prompt_kernels.cuh"
 #include "register_split.h"
+#include "tensor_map.h"
 
 namespace chord {
 namespace {
@@ -256,6 +257,24 @@ int check_prompt(const PromptCall& c) {
   return kOk;
 }
 
+// A descriptor of BF16 rows of `dim` elements in up to three further dimensions (sizes, strides in bytes), boxes of 64
+// elements, swizzled as the products read them.  False where there is none (strides of zero, for one).
+bool make_rows_map(CUtensorMap* out, const void* base, int64_t dim, int rank, const int64_t* sizes, const int64_t* strides, const uint32_t* box) {
+  const EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr) return false;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim)}, steps[3];
+  cuuint32_t boxes[4] = {64}, ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank - 1; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(sizes[i]);
+    steps[i] = static_cast<cuuint64_t>(sizes[i] == 1 ? 16 : strides[i]);  // (of one only, no stride counts)
+    boxes[i + 1] = box[i];
+    if (steps[i] == 0 || steps[i] % 16 != 0 || steps[i] >= (1ull << 40)) return false;
+  }
+  return encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, steps, boxes, ones,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& device) {
   PromptParams p = {};
   p.cache = cache;
@@ -308,6 +327,22 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
   p.max_items = static_cast<int32_t>(max_items);
   p.ctas = static_cast<int32_t>(ctas);
   p.group = Divisor(static_cast<uint32_t>(group));
+  if (!codes) {
+    const int64_t page = c.cache->page_size;
+    int32_t box = 1;
+    while (box < v.step_tokens && page % (2 * box) == 0) box *= 2;
+    const int64_t sizes[3] = {page, c.cache->heads, c.cache->num_pages}, strides[3] = {cache.token, cache.head, cache.page};
+    const uint32_t boxes[3] = {static_cast<uint32_t>(box), 1, 1};
+    if (box >= 8 && make_rows_map(&p.k_map, c.cache->k, c.cache->head_dim, 4, sizes, strides, boxes) &&
+        make_rows_map(&p.v_map, c.cache->v, c.cache->head_dim, 4, sizes, strides, boxes)) {
+      p.box = box;
+    }
+  }
+  if (kPromptTile % group == 0) {
+    const int64_t sizes[2] = {c.heads, c.tokens}, strides[2] = {2 * c.q_head, 2 * c.q_token};
+    const uint32_t boxes[2] = {static_cast<uint32_t>(group), static_cast<uint32_t>(kPromptTile / group)};
+    p.q_boxes = make_rows_map(&p.q_map, c.q, c.cache->head_dim, 3, sizes, strides, boxes);
+  }
   const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
   CHORD_CUDA(launch_kernel(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, kEarlyLaunch, p, v.tiles * kPromptTile, v.step_tokens));
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kPromptThreads), v.smem, stream, kEarlyLaunch, p));

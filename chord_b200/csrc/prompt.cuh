@@ -17,6 +17,7 @@
 // that in FP32.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "../../include/chord_b200.h"
@@ -47,6 +48,8 @@ struct PromptPlan {
 };
 
 struct PromptParams {
+  CUtensorMap k_map, v_map;  // [pages][heads][page_size][dim], boxes of 64 elements of `box` tokens
+  CUtensorMap q_map;         // [tokens][heads][dim], boxes of 64 elements of a group's heads of 128 / group tokens
   Cache cache;
   const __nv_bfloat16* q;  // [tokens, heads, dim]
   int64_t q_token, q_head;
@@ -71,6 +74,8 @@ struct PromptParams {
   float scale, cap;         // the scale times log2(e); the cap times log2(e), or zero
   float cap_scale;          // 2 log2(e) scale / cap
   int32_t batch, tokens, heads, kv_heads, capacity, own_capacity, window, max_items, ctas;
+  int32_t box;    // tokens of a TMA box of keys and values, which divides pages and steps; zero: loaded by cp.async
+  bool q_boxes;   // queries by TMA
   Divisor group;
 };
 
@@ -289,11 +294,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     ptx::tmem_relinquish();
   }
   if (threadIdx.x == 0) {
-    ptx::mbar_init(bar(c.q_full), 4);
+    ptx::mbar_init(bar(c.q_full), p.q_boxes ? 1 : p.box != 0 ? 3 : 4);
     ptx::mbar_init(bar(c.q_empty), 1);
     ptx::mbar_init(bar(c.drained), 1);
     for (int i = 0; i < 8; ++i) {
-      ptx::mbar_init(bar(c.kv_full[i]), 4);
+      ptx::mbar_init(bar(c.kv_full[i]), p.box != 0 ? 1 : 4);
       ptx::mbar_init(bar(c.kv_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -317,7 +322,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
 
   if (warp >= 8 && warp < 12) {
     // ---- loads: queries once per item, keys and values step by step, each into a slot of the ring ----
+    // By TMA where boxes of 8 tokens or more fit pages and steps: the first warp's lanes have a box each.  A step of
+    // 128 tokens of 128 elements by cp.async takes its warps some 4700 cycles, the products 2000.  Boxes bring tokens
+    // behind the last one with them; one outside the tokens that are seen, or whose page is not there, is asked for
+    // behind the cache's last page, which gives zeros.
     const int w = warp - 8;
+    const bool boxes = !kCodes && p.box != 0;
     constexpr int kOwn = kN / 4;  // tokens of a warp
     constexpr int kPieces = kDim * (kCodes ? 1 : 2) / 16;
     uint32_t slot = 0, slot_phase = 0, q_phase = 0;
@@ -359,12 +369,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       const int32_t* const table = p.tables + it.b * p.table_stride;
       const int32_t token0 = (it.lo / kN + walk.step) * kN;
       const int64_t head_offset = static_cast<int64_t>(walk.head) * p.cache.head;
-      const int32_t mine = w * kOwn + lane % kOwn;  // the token that the lane looks up
+      const int32_t mine = boxes ? lane * p.box : w * kOwn + lane % kOwn;  // the token that the lane looks up
+      const int32_t others = boxes ? p.box - 1 : 0;                        // and those with it
       int32_t page = 0, place = -1;
       auto look_up = [&](int32_t j) {
         const int32_t token = token0 + j * kN + mine;
         place = -1;
-        if (j < n && token >= it.lo && token < it.hi) {
+        if (j < n && token + others >= it.lo && token < it.hi && mine < kN) {
           const uint32_t index = p.cache.page_size.div(token);
           place = token - index * p.cache.page_size.d;
           page = load_arg(table + index);
@@ -418,14 +429,41 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           }
         }
       };
-      auto load_queries = [&]() {
+      auto load_boxes = [&](const CUtensorMap& map, uint32_t at, bool there) {
+        if (lane == 0) ptx::mbar_arrive_expect_tx(at, L::kSlotBytes);
+        __syncwarp();
+        if (mine < kN) {
+          const uint32_t to = ptx::smem_u32(slots) + slot * L::kSlotBytes + mine * 128;
+#pragma unroll
+          for (int b = 0; b < L::kBlocks; ++b) {
+            ptx::tma_load_4d(to + b * (kN * 128), &map, at, 64 * b, there ? place : 0, walk.head, there ? page : p.cache.num_pages);
+          }
+        }
+        __syncwarp();
+      };
+      auto load_query_boxes = [&]() {
+        const PromptSequence of(p, it.b);
+        const int tiles = L::kTwo && it.rows > kPromptTile ? 2 : 1;
+        if (lane == 0) {
+          ptx::mbar_arrive_expect_tx(bar(c.q_full), tiles * (L::kBlocks * kPromptTile * 128));
+          const int32_t token = of.begin + static_cast<int32_t>(p.group.div(it.row0)), per_tile = p.group.div(kPromptTile);
+          for (int t = 0; t < tiles; ++t) {
+#pragma unroll
+            for (int b = 0; b < L::kBlocks; ++b) {
+              ptx::tma_load_3d(ptx::smem_u32(q_tile) + (t * L::kBlocks + b) * (kPromptTile * 128), &p.q_map, bar(c.q_full), 64 * b,
+                               walk.head * static_cast<int32_t>(p.group.d), token + t * per_tile);
+            }
+          }
+        }
+        __syncwarp();
+      };
+      auto load_queries = [&](int32_t of_warps, int32_t number) {  // as the number-th of so many warps
         const PromptSequence of(p, it.b);
         const uint32_t to = ptx::smem_u32(q_tile);
         constexpr int kQPieces = kDim / 8;
-        constexpr int kRows = L::kTiles * kPromptTile / 4;  // of a warp
 #pragma unroll 1
-        for (int r0 = 0; r0 < kRows; r0 += 32) {
-          const int32_t r = it.row0 + w * kRows + r0 + lane;
+        for (int r0 = 32 * number; r0 < L::kTiles * kPromptTile; r0 += 32 * of_warps) {
+          const int32_t r = it.row0 + r0 + lane;
           int64_t offset = -1;
           if (r < it.row0 + it.rows) {
             const int32_t i = p.group.div(r), h = r - i * p.group.d;
@@ -433,7 +471,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           }
 #pragma unroll 4
           for (int i = 0; i < kQPieces; ++i) {
-            const int at = i * 32 + lane, row = at / kQPieces, piece = at % kQPieces, tile_row = w * kRows + r0 + row;
+            const int at = i * 32 + lane, row = at / kQPieces, piece = at % kQPieces, tile_row = r0 + row;
             const int64_t o = __shfl_sync(0xffffffffu, offset, row);
             const uint32_t dst = to + (tile_row / kPromptTile) * (L::kBlocks * kPromptTile * 128) + (piece >> 3) * (kPromptTile * 128) +
                                  (tile_row % kPromptTile) * 128 + ((piece ^ tile_row) & 7) * 16;
@@ -442,6 +480,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         }
       };
 
+      if (boxes) {
+        if (w != 0) {
+          if (!p.q_boxes) {
+            wait_for(bar(c.q_empty), q_phase ^ 1);
+            if (bad != 0) break;
+            load_queries(3, w - 1);
+            filled(bar(c.q_full));
+            flush();
+            q_phase ^= 1;
+          }
+          walk.next(n);
+          continue;
+        }
+        look_up(0);
+#pragma unroll 1
+        for (int32_t j = 0; j < n; ++j) {
+          const bool there = place >= 0 && static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.num_pages);
+          if (place >= 0 && !there && p.status != nullptr) atomicOr(p.status, kStatusIndex);
+          wait_for(bar(c.kv_empty[slot]), slot_phase ^ 1);
+          if (bad != 0) break;
+          load_boxes(p.k_map, bar(c.kv_full[slot]), there);
+          advance();
+          if (j == 0 && p.q_boxes) {
+            wait_for(bar(c.q_empty), q_phase ^ 1);
+            if (bad != 0) break;
+            load_query_boxes();
+            q_phase ^= 1;
+          }
+          wait_for(bar(c.kv_empty[slot]), slot_phase ^ 1);
+          if (bad != 0) break;
+          load_boxes(p.v_map, bar(c.kv_full[slot]), there);
+          advance();
+          look_up(j + 1);
+        }
+        walk.next(n);
+        continue;
+      }
       look_up(0);
 #pragma unroll 1
       for (int32_t j = 0; j < n && bad == 0; ++j) {
@@ -470,9 +545,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         if (j == 0) {
           wait_for(bar(c.q_empty), q_phase ^ 1);
           if (bad != 0) break;
-          load_queries();
-          filled(bar(c.q_full));
-          if constexpr (kCodes) flush();
+          if (p.q_boxes) {
+            if (w == 0) load_query_boxes();
+          } else {
+            load_queries(4, w);
+            filled(bar(c.q_full));
+            if constexpr (kCodes) flush();
+          }
           q_phase ^= 1;
         }
         wait_for(bar(c.kv_empty[slot]), slot_phase ^ 1);
@@ -711,25 +790,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           }
           const float base = top == -INFINITY ? 0.0f : -top;
           if constexpr (!kCodes) {
-            // Values that some rows do not see: zero times an infinity or a NaN would be a NaN for those rows too.
+            // Values that some rows do not see: zero times an infinity or a NaN would be a NaN for those rows too.  What
+            // no row of the item sees (rows of a box outside its tokens) is set to zero.
             bool found = false;
-            if (highest_lo > max(first, it.lo) || lowest_hi < min(first + kN, it.hi)) {
+            if (highest_lo > first || lowest_hi < first + kN) {
               wait(bar(c.kv_full[v_slot]), v_phase);
               uint32_t most = 0;
-              const uint8_t* const v = slots + v_slot * L::kSlotBytes + (warp & 3) * (kN / 4 * 128) + lane * 16;
+              uint8_t* const v = slots + v_slot * L::kSlotBytes + (warp & 3) * (kN / 4 * 128) + lane * 16;
+              const int32_t token = first + (warp & 3) * (kN / 4) + lane / 8;
 #pragma unroll
               for (int b = 0; b < L::kBlocks; ++b) {
 #pragma unroll
                 for (int i = 0; i < kN / 16; ++i) {
                   const int logical = (lane ^ (i * 4 + lane / 8)) & 7;  // the token's parity with its place
-                  if (kDim - 64 * b >= 64 || 64 * b + 8 * logical < kDim) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(v + b * (kN * 128) + i * 512);
+                  uint4* const at = reinterpret_cast<uint4*>(v + b * (kN * 128) + i * 512);
+                  if (token + 4 * i < it.lo || token + 4 * i >= it.hi) {
+                    *at = make_uint4(0, 0, 0, 0);
+                  } else if (kDim - 64 * b >= 64 || 64 * b + 8 * logical < kDim) {
+                    const uint4 w = *at;
                     most = __vmaxu2(__vmaxu2(most, __vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu)),
                                     __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
                   }
                 }
               }
               const bool any = __any_sync(0xffffffffu, (most & 0xFFFFu) >= 0x7F80u || (most >> 16) >= 0x7F80u);
+              ptx::fence_proxy_async();
               ++looks;
               if (any && lane == 0) *const_cast<volatile uint32_t*>(&c.odd[tile]) = looks;
               __syncwarp();
