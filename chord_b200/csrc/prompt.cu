@@ -43,13 +43,21 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prompt_plan_kernel(const __gr
   ptx::grid_dependency_wait();
 
   // Items of the sequences before each.
+  auto sequence = [&](int32_t b, PromptItem& it) {
+    it.b = b;
+    it.begin = max(0, min(load_arg(p.offsets + b), p.tokens));
+    it.count = max(0, min(load_arg(p.offsets + b + 1), p.tokens) - it.begin);
+    it.length = max(0, min(load_arg(p.lengths + b), p.capacity));
+    it.both_ways = p.prefixes == nullptr ? 0 : min(load_arg(p.prefixes + b), it.length);
+  };
   int64_t items = 0;
 #pragma unroll 1
   for (int32_t b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
     const int32_t b = b0 + threadIdx.x;
     int64_t mine = 0;
     if (b < p.batch) {
-      const PromptSequence of(p, b);
+      PromptItem of;
+      sequence(b, of);
       mine = (static_cast<int64_t>(of.count) * p.group.d + item_rows - 1) / item_rows;
       const bool wrong = load_arg(p.lengths + b) > p.capacity || load_arg(p.offsets + b) < 0 || load_arg(p.offsets + b + 1) > p.tokens ||
                          load_arg(p.offsets + b + 1) < load_arg(p.offsets + b);
@@ -74,25 +82,39 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prompt_plan_kernel(const __gr
       if (p.tiles_before[middle] <= item) low = middle; else high = middle - 1;
     }
     PromptItem it;
-    it.b = low;
-    const PromptSequence of(p, low);
+    sequence(low, it);
     const int64_t row0 = static_cast<int64_t>(item - p.tiles_before[low]) * item_rows;
-    const int64_t rows = min(static_cast<int64_t>(item_rows), static_cast<int64_t>(of.count) * p.group.d - row0);
+    const int64_t rows = min(static_cast<int64_t>(item_rows), static_cast<int64_t>(it.count) * p.group.d - row0);
     it.row0 = static_cast<int32_t>(row0);
     it.rows = static_cast<int32_t>(max(rows, static_cast<int64_t>(0)));
     int32_t lo = INT32_MAX, hi = 0;
-    if (it.rows > 0) {
-      const int32_t t0 = p.group.div(it.row0), t1 = p.group.div(it.row0 + it.rows - 1);
-      if (by_token) {
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      int32_t highest_lo = 0, lowest_hi = INT32_MAX;
+      const int32_t r0 = it.row0 + tile * kPromptTile, r1 = min(it.row0 + it.rows, r0 + kPromptTile) - 1;
+      if (r0 <= r1) {
+        const int32_t t0 = p.group.div(r0), t1 = p.group.div(r1);
+        if (by_token) {
 #pragma unroll 1
-        for (int32_t i = t0 + begin_lane; i <= t1; i += lanes) {
-          const PromptView v = of.view(p, i);
-          if (v.hi > v.lo) lo = min(lo, v.lo), hi = max(hi, v.hi);
+          for (int32_t i = t0 + begin_lane; i <= t1; i += lanes) {
+            const PromptView v(p, it, i);
+            highest_lo = max(highest_lo, v.lo);
+            lowest_hi = min(lowest_hi, v.hi);
+            if (v.hi > v.lo) lo = min(lo, v.lo), hi = max(hi, v.hi);
+          }
+        } else {
+          const PromptView a(p, it, t0), z(p, it, t1);  // (neither bound falls from token to token)
+          highest_lo = z.lo;
+          lowest_hi = a.hi;
+          if (z.hi > a.lo) lo = min(lo, a.lo), hi = max(hi, z.hi);
         }
-      } else {
-        const PromptView a = of.view(p, t0), z = of.view(p, t1);
-        if (z.hi > a.lo) lo = a.lo, hi = z.hi;
       }
+      if (lanes > 1) {
+        highest_lo = __reduce_max_sync(0xffffffffu, highest_lo);
+        lowest_hi = __reduce_min_sync(0xffffffffu, lowest_hi);
+      }
+      it.highest_lo[tile] = highest_lo;
+      it.lowest_hi[tile] = lowest_hi;
     }
     if (lanes > 1) {
       lo = __reduce_min_sync(0xffffffffu, lo);
@@ -185,8 +207,8 @@ int allow_prompt(const PromptVariant& v, int64_t dim, bool codes, bool bent, int
   if (known) return kOk;
   cudaFuncAttributes attributes;
   CHORD_CUDA(cudaFuncGetAttributes(&attributes, v.kernel));
-  if (!register_split_fits(attributes.numRegs, 8, v.other_regs, 8, v.row_regs)) {
-    return fail(kUnsupportedDevice, "the attention kernel was compiled to %d registers, its warps divide 128", attributes.numRegs);
+  if (!register_split_fits(attributes.numRegs, v.threads / 32 - kLoadWarp, v.other_regs, kLoadWarp, v.row_regs)) {
+    return fail(kUnsupportedDevice, "the attention kernel was compiled to %d registers, too few for its warps", attributes.numRegs);
   }
   CHORD_CUDA(cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem));
   known = true;
@@ -257,21 +279,23 @@ int check_prompt(const PromptCall& c) {
   return kOk;
 }
 
-// A descriptor of BF16 rows of `dim` elements in up to three further dimensions (sizes, strides in bytes), boxes of 64
-// elements, swizzled as the products read them.  False where there is none (strides of zero, for one).
-bool make_rows_map(CUtensorMap* out, const void* base, int64_t dim, int rank, const int64_t* sizes, const int64_t* strides, const uint32_t* box) {
+// A descriptor of rows of `dim` elements in up to three further dimensions (sizes, strides in bytes): BF16 in boxes of 64
+// elements, swizzled as the products read them, or codes in whole rows.  False where there is none (strides of zero, for one).
+bool make_rows_map(CUtensorMap* out, const void* base, bool codes, int64_t dim, int rank, const int64_t* sizes, const int64_t* strides,
+                   const uint32_t* box) {
   const EncodeTiledFn encode = encode_tiled_fn();
   if (encode == nullptr) return false;
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim)}, steps[3];
-  cuuint32_t boxes[4] = {64}, ones[4] = {1, 1, 1, 1};
+  cuuint32_t boxes[4] = {codes ? static_cast<cuuint32_t>(dim) : 64}, ones[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank - 1; ++i) {
     dims[i + 1] = static_cast<cuuint64_t>(sizes[i]);
     steps[i] = static_cast<cuuint64_t>(sizes[i] == 1 ? 16 : strides[i]);  // (of one only, no stride counts)
     boxes[i + 1] = box[i];
     if (steps[i] == 0 || steps[i] % 16 != 0 || steps[i] >= (1ull << 40)) return false;
   }
-  return encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, steps, boxes, ones,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return encode(out, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
+                const_cast<void*>(base), dims, steps, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -327,25 +351,33 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
   p.max_items = static_cast<int32_t>(max_items);
   p.ctas = static_cast<int32_t>(ctas);
   p.group = Divisor(static_cast<uint32_t>(group));
-  if (!codes) {
+  {
     const int64_t page = c.cache->page_size;
     int32_t box = 1;
     while (box < v.step_tokens && page % (2 * box) == 0) box *= 2;
-    const int64_t sizes[3] = {page, c.cache->heads, c.cache->num_pages}, strides[3] = {cache.token, cache.head, cache.page};
+    // (heads or pages that are all one: views with a stride of zero)
+    p.head_step = cache.head != 0;
+    p.page_step = cache.page != 0;
+    const int64_t sizes[3] = {page, p.head_step ? c.cache->heads : 1, p.page_step ? c.cache->num_pages : 1};
+    const int64_t strides[3] = {cache.token, cache.head, cache.page};
     const uint32_t boxes[3] = {static_cast<uint32_t>(box), 1, 1};
-    if (box >= 8 && make_rows_map(&p.k_map, c.cache->k, c.cache->head_dim, 4, sizes, strides, boxes) &&
-        make_rows_map(&p.v_map, c.cache->v, c.cache->head_dim, 4, sizes, strides, boxes)) {
-      p.box = box;
+    // a box starts on 128 bytes of shared memory
+    if (!codes || box * c.cache->head_dim % 128 == 0) {
+      if (make_rows_map(&p.k_map, c.cache->k, codes, c.cache->head_dim, 4, sizes, strides, boxes) &&
+          make_rows_map(&p.v_map, c.cache->v, codes, c.cache->head_dim, 4, sizes, strides, boxes)) {
+        p.box = box;
+      }
     }
+    CHORD_REQUIRE(codes || p.box != 0, "the cache's strides must be from 16 to 2^40 - 16 bytes (those of heads and pages may be zero)");
   }
   if (kPromptTile % group == 0) {
     const int64_t sizes[2] = {c.heads, c.tokens}, strides[2] = {2 * c.q_head, 2 * c.q_token};
     const uint32_t boxes[2] = {static_cast<uint32_t>(group), static_cast<uint32_t>(kPromptTile / group)};
-    p.q_boxes = make_rows_map(&p.q_map, c.q, c.cache->head_dim, 3, sizes, strides, boxes);
+    p.q_boxes = make_rows_map(&p.q_map, c.q, false, c.cache->head_dim, 3, sizes, strides, boxes);
   }
   const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
   CHORD_CUDA(launch_kernel(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, kEarlyLaunch, p, v.tiles * kPromptTile, v.step_tokens));
-  CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kPromptThreads), v.smem, stream, kEarlyLaunch, p));
+  CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(v.threads)), v.smem, stream, kEarlyLaunch, p));
   if (ctas > 1) {
     CHORD_CUDA(launch_kernel(v.join, dim3(static_cast<unsigned>(ctas - 1), static_cast<unsigned>(v.tiles * c.cache->head_dim / 8)),
                              dim3(kPromptTile), 0, stream, kEarlyLaunch, p));

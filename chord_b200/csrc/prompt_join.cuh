@@ -42,10 +42,10 @@ __global__ void __launch_bounds__(kPromptTile) prompt_join_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], old, v[i] * weight);
   }
-  const PromptSequence of(p, it.b);
   const int32_t token = p.group.div(it.row0 + r);
   const int64_t head = static_cast<int64_t>(at.head) * p.group.d + (it.row0 + r - token * static_cast<int32_t>(p.group.d));
-  prompt_finish<8>(p, (of.begin + static_cast<int64_t>(token)) * p.heads + head, dim, kDim, o, top, sum, kCodes ? 64.0f : 1.0f, dim == 0);
+  const int64_t result = (it.begin + static_cast<int64_t>(token)) * p.heads + head;
+  PromptRates(p, result, top, sum, kCodes ? 64.0f : 1.0f, dim == 0).write(p, result * kDim + dim, o);
 }
 
 }  // namespace chord

@@ -8,15 +8,15 @@ namespace chord {
 struct PromptVariant {
   void (*kernel)(PromptParams);
   void (*join)(PromptParams);
-  int smem, tiles, step_tokens, row_regs, other_regs;
+  int smem, threads, tiles, step_tokens, row_regs, other_regs;
   int64_t part_floats;
 };
 
 template <int kDim, bool kCodes, bool kBent>
 PromptVariant prompt_variant() {
   using L = PromptLayout<kDim, kCodes>;
-  return {prompt_attention_kernel<kDim, kCodes, kBent>, prompt_join_kernel<kDim, kCodes>, L::kSmem, L::kTiles, L::kN,
-          L::kRowRegs, L::kOtherRegs, prompt_part_floats<kDim, kCodes>()};
+  return {prompt_attention_kernel<kDim, kCodes, kBent>, prompt_join_kernel<kDim, kCodes>, L::kSmem, L::kThreads, L::kTiles,
+          L::kN, L::kRowRegs, L::kOtherRegs, prompt_part_floats<kDim, kCodes>()};
 }
 
 template <bool kCodes, bool kBent>
