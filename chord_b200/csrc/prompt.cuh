@@ -206,7 +206,8 @@ struct __align__(16) PromptControl {
   uint64_t kv_full[8], kv_empty[8];  // by slot
   uint64_t looked[8];                // by the values' turn: there are no more than four of them in the ring
   uint64_t raw_full[4], raw_empty[4];
-  uint64_t s_full[2], p_full[2][2], o_done[2];  // p_full: [half of the tokens][buffer]
+  uint64_t s_full[2], p_full[2][2];  // p_full: [half of the tokens][buffer]
+  uint64_t o_done[2];                // by tile; of one tile's products, two in turn
   uint32_t odd[8];   // as looked, the values in turn: number of the values in which infinities or NaN were found, and one
   uint32_t skip[2];  // by buffer: the product of its P and V is made by the rows' warps
   uint32_t tmem, abort;
@@ -250,6 +251,80 @@ struct PromptRates {
     *reinterpret_cast<uint4*>(p.out + at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
   }
 };
+
+__device__ __forceinline__ void store_32_bytes(void* to, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// Four lanes with a word for each of four places each: lane q receives the four lanes' words for place q.
+__device__ __forceinline__ void exchange4(uint32_t (&w)[4], int q) {
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    // pairs of places that differ in bit d: the one that is not the lane's goes
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((i & d) != 0) continue;
+      const bool upper = (q & d) != 0;
+      const uint32_t gone = upper ? w[i] : w[i | d];
+      const uint32_t come = __shfl_xor_sync(0xffffffffu, gone, d);
+      if (upper) w[i] = come; else w[i | d] = come;
+    }
+  }
+}
+
+// Writes 64 or 32 values, from `dim` on, of a warp's 32 rows as BF16.  Rows are spread over four lanes each (with a row to a
+// lane, every store touches 32 lines of memory: 6500 cycles for two tiles of 128 values, as long as two steps), which
+// then write 128 or 64 bytes of it in one go.  `row`, `mine` and `other` are those of the lane's own row; row < 0: none.
+template <int kCount>
+__device__ __forceinline__ void write_rows(const PromptParams& p, uint32_t from, int dims, int dim, int64_t row, float mine, float other, int lane) {
+  constexpr int kGroups = kCount / 8;
+  const int q = lane & 3;
+#pragma unroll
+  for (int lower = 0; lower < 32; lower += 16) {
+    uint32_t o[4 * kGroups];
+    __syncwarp();
+    if constexpr (kGroups == 8) ptx::tmem_ld_16x256b_x8(from + (static_cast<uint32_t>(lower) << 16), o);
+    if constexpr (kGroups == 4) ptx::tmem_ld_16x256b_x4(from + (static_cast<uint32_t>(lower) << 16), o);
+    ptx::tmem_wait_ld();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int of = lower + 8 * r + lane / 4;
+      const int64_t to = __shfl_sync(0xffffffffu, row, of);
+      const float scale = __shfl_sync(0xffffffffu, mine, of);
+      float v[2 * kGroups];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        v[2 * g] = __uint_as_float(o[4 * g + 2 * r]) * scale;
+        v[2 * g + 1] = __uint_as_float(o[4 * g + 2 * r + 1]) * scale;
+      }
+      if (p.extra != nullptr) {
+        const float beside = __shfl_sync(0xffffffffu, other, of);
+        if (to >= 0) {
+          const float* const x = p.extra + to * dims + dim + 2 * q;
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            v[2 * g] = fmaf(load_arg(x + 8 * g), beside, v[2 * g]);
+            v[2 * g + 1] = fmaf(load_arg(x + 8 * g + 1), beside, v[2 * g + 1]);
+          }
+        }
+        __syncwarp();
+      }
+      // Lane q gets groups 2 q and 2 q + 1 (of four groups, group q).
+      uint32_t w[kGroups / 4][4];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) w[g % (kGroups / 4)][g / (kGroups / 4)] = pack_bf16(v[2 * g], v[2 * g + 1]);
+#pragma unroll
+      for (int i = 0; i < kGroups / 4; ++i) exchange4(w[i], q);
+      __nv_bfloat16* const at = p.out + to * dims + dim + q * (2 * kGroups);
+      if (to >= 0) {
+        if constexpr (kGroups == 8) store_32_bytes(at, &w[0][0]);
+        if constexpr (kGroups == 4) *reinterpret_cast<uint4*>(at) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+      }
+    }
+  }
+}
 
 // The product of a tile's weights and values on the CUDA cores, for values among which are infinities or NaN that not all
 // of its rows see: tokens of no weight are left out.  The scores lie in tensor memory at `s_at`; returns their weights' sum.
@@ -488,7 +563,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     const uint32_t o_desc = ptx::idesc_bf16_f32(kPromptTile, kDim) | ptx::kIdescBMnMajor;
     const bool leader = ptx::elect_one();
     uint32_t taken = 0;  // slots before this item
-    uint32_t p_phase = 0, q_phase = 0, o_phase = 0;
+    uint32_t p_phase = 0, q_phase = 0, products[2] = {0, 0};  // the latter: issued, by tile
     auto wait_to_issue = [&](uint32_t at, uint32_t parity) {
       wait(at, parity);
       ptx::tc_fence_after();
@@ -499,9 +574,9 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     };
     // Scores go where weights were that the product before has read.  Products with other accumulators or of another
     // shape are not bound to run in order, so that one has to have ended.
-    auto ended = [&](int tile) {
-      wait_to_issue(bar(c.o_done[tile]), o_phase >> tile & 1);
-      o_phase ^= 1u << tile;
+    auto ended = [&](int tile) {  // the last one
+      const uint32_t last = products[tile] - 1;
+      wait_to_issue(bar(c.o_done[L::kTwo ? tile : last & 1]), (L::kTwo ? last : last >> 1) & 1);
     };
     auto scores = [&](int tile, int buffer, uint32_t number) {
       if (leader) {
@@ -537,7 +612,8 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
           }
         }
       }
-      if (leader) ptx::mma_commit(bar(c.o_done[tile]));
+      if (leader) ptx::mma_commit(bar(c.o_done[L::kTwo ? tile : products[tile] & 1]));
+      ++products[tile];
     };
 
     PromptWalk walk(p);
@@ -645,9 +721,15 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
           }
           uint8_t* const v = slots + slot * L::kSlotBytes;
           uint32_t most = 0;
-#pragma unroll 4
+          // (tokens from `low` to `high` are seen by all rows)
+          const bool two = L::kTwo && it.rows > kPromptTile;
+          const int32_t low = (two ? max(it.highest_lo[0], it.highest_lo[1]) : it.highest_lo[0]) - first;
+          const int32_t high = (two ? min(it.lowest_hi[0], it.lowest_hi[1]) : it.lowest_hi[0]) - first;
+#pragma unroll 2
           for (int i = w; i < L::kSlotBytes / 512; i += kLookWarps) {
-            const int at = i * 512 + lane * 16, token = at % (kN * 128) / 128, logical = (lane ^ token) & 7;
+            const int token0 = i * 4 % kN;
+            if (token0 >= low && token0 + 4 <= high) continue;
+            const int at = i * 512 + lane * 16, token = token0 + lane / 8, logical = (lane ^ token) & 7;
             uint4* const of = reinterpret_cast<uint4*>(v + at);
             if (first + token < it.lo || first + token >= it.hi) {
               *of = make_uint4(0, 0, 0, 0);
@@ -774,6 +856,13 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     const uint32_t pair = 1 + tile * 4 + (warp & 3);
     uint32_t s_phase = 0, outputs = 0, taken = 0;
     uint32_t skipping = 0;  // by buffer, what c.skip holds
+    // For the product of the last step.  A parity tells one product from the one before, no further: of one tile's, the last
+    // but one may not have ended either, so these take turns at two barriers.
+    auto product_ended = [&]() {
+      const uint32_t last = outputs - 1;
+      wait(bar(c.o_done[L::kTwo ? tile : last & 1]), (L::kTwo ? last : last >> 1) & 1);
+      ptx::tc_fence_after();
+    };
 
     PromptWalk walk(p);
     while (walk.left > 0) {
@@ -880,7 +969,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
             sum *= factor;
             if (j != 0 && half == 0) {  // (the products wait for this half)
               // (with two tiles the scores were made after the product before)
-              if constexpr (!L::kTwo) wait(bar(c.o_done[tile]), (outputs - 1) & 1);
+              if constexpr (!L::kTwo) product_ended();
               ptx::tc_fence_after();
 #pragma unroll 1
               for (int i = 0; i < kDim; i += 16) {
@@ -905,8 +994,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
               ptx::tc_fence_after();
               if (half == 0) {
                 if constexpr (!L::kTwo) {
-                  if (j != 0) wait(bar(c.o_done[tile]), (outputs - 1) & 1);
-                  ptx::tc_fence_after();
+                  if (j != 0) product_ended();
                 }
                 const uint32_t scores_at = tmem + lanes + buffer * kN;
                 sum += product_by_row<kDim, kN>(scores_at, out_at, slots + v_slot * L::kSlotBytes, 0, of_scores, base, j == 0);
@@ -962,28 +1050,22 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
         shared[half * kPromptTile] = sum;
         ptx::named_bar_sync(pair, 64);
         sum += *const_cast<volatile float*>(shared + (1 - half) * kPromptTile);
-        if constexpr (!L::kTwo) {
-          // (the last scores were made before the last product but one had ended, and a parity tells of one product only)
-          if (n > 1) wait(bar(c.o_done[tile]), (outputs - 2) & 1);
-        }
-        wait(bar(c.o_done[tile]), (outputs - 1) & 1);
-        ptx::tc_fence_after();
+        product_ended();
         const bool whole = walk.step == 0 && n == it.steps;
         float* const part = p.parts + (2 * static_cast<int64_t>(blockIdx.x) + (walk.step == 0 ? 1 : 0)) * prompt_part_floats<kDim, kCodes>() +
                             static_cast<int64_t>(tile) * kPromptTile * (kDim + 2);
         if (whole) {
           const bool there = result >= 0;
           const PromptRates rates(p, there ? result : 0, top, sum, kUnit, there && half == 0);
-#pragma unroll
-          for (int i = 0; i < kDim / 2; i += 16) {
-            uint32_t o[16];
-            __syncwarp();
-            ptx::tmem_ld_32x32b_x16(out_at + half * (kDim / 2) + i, o);
-            ptx::tmem_wait_ld();
-            if (there) {
-              const int64_t at = result * kDim + half * (kDim / 2) + i;
-              rates.write(p, at, reinterpret_cast<const float*>(o));
-              rates.write(p, at + 8, reinterpret_cast<const float*>(o + 8));
+          // in 64s while there are, the first half one more of them
+          constexpr int kFirst = (kDim / 2 + 63) / 64 * 64 <= kDim ? (kDim / 2 + 31) / 32 * 32 : kDim / 2;
+          const int begin = half == 0 ? 0 : kFirst, end = half == 0 ? kFirst : kDim;
+#pragma unroll 1
+          for (int i = begin; i < end; i += 64) {
+            if (end - i >= 64) {
+              write_rows<64>(p, out_at + i, kDim, i, result, rates.mine, rates.other, lane);
+            } else {
+              write_rows<32>(p, out_at + i, kDim, i, result, rates.mine, rates.other, lane);
             }
           }
         } else {
