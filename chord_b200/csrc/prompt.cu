@@ -13,183 +13,17 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 
-// The sum of `value` over the threads before this one, and of all.
-__device__ __forceinline__ int64_t sum_before(int64_t value, int64_t* of_warps, int64_t& all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t upto = value;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t below = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += below;
-  }
-  __syncthreads();  // (of_warps may still be read from the call before)
-  if (lane == 31) of_warps[warp] = upto;
-  __syncthreads();
-  int64_t before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    if (w < warp) before += of_warps[w];
-    all += of_warps[w];
-  }
-  return before + upto - value;
-}
-
-// One CTA: the items of every sequence, the tokens that each of them sees, and where the main kernel's CTAs begin.
+// The plan by one CTA, for more items or sequences than the main kernel's CTAs go through on their own.
 __global__ void __launch_bounds__(kPlanThreads, 1) prompt_plan_kernel(const __grid_constant__ PromptParams p, int32_t item_rows, int32_t step_tokens) {
-  __shared__ int64_t of_warps[kPlanThreads / 32];
-  __shared__ int32_t longest_of[kPlanThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ PromptPlanScratch scratch;
   ptx::grid_dependency_wait();
-
-  // Items of the sequences before each.
-  auto sequence = [&](int32_t b, PromptItem& it) {
-    it.b = b;
-    it.begin = max(0, min(load_arg(p.offsets + b), p.tokens));
-    it.count = max(0, min(load_arg(p.offsets + b + 1), p.tokens) - it.begin);
-    it.length = max(0, min(load_arg(p.lengths + b), p.capacity));
-    it.both_ways = p.prefixes == nullptr ? 0 : min(load_arg(p.prefixes + b), it.length);
-  };
-  int64_t items = 0;
-#pragma unroll 1
-  for (int32_t b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
-    const int32_t b = b0 + threadIdx.x;
-    int64_t mine = 0;
-    if (b < p.batch) {
-      PromptItem of;
-      sequence(b, of);
-      mine = (static_cast<int64_t>(of.count) * p.group.d + item_rows - 1) / item_rows;
-      const bool wrong = load_arg(p.lengths + b) > p.capacity || load_arg(p.offsets + b) < 0 || load_arg(p.offsets + b + 1) > p.tokens ||
-                         load_arg(p.offsets + b + 1) < load_arg(p.offsets + b);
-      if (wrong && p.status != nullptr) atomicOr(p.status, kStatusIndex);
-    }
-    int64_t all;
-    const int64_t before = items + sum_before(mine, of_warps, all);
-    if (b < p.batch) p.tiles_before[b] = static_cast<int32_t>(min(before, static_cast<int64_t>(p.max_items)));
-    items += all;
-  }
-  // (more only where offsets fall)
-  const int32_t count = static_cast<int32_t>(min(items, static_cast<int64_t>(p.max_items)));
-  if (items > p.max_items && threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusIndex);
-  __syncthreads();
-
-  // Each item's tokens.  Where they follow from its first and last query token a thread does, else a warp.
-  const bool by_token = p.starts != nullptr || (p.own != nullptr && p.window > 0);
-  auto make = [&](int32_t item, int32_t begin_lane, int32_t lanes) {
-    int32_t low = 0, high = p.batch - 1;  // the last sequence with tiles_before <= item
-    while (low < high) {
-      const int32_t middle = (low + high + 1) / 2;
-      if (p.tiles_before[middle] <= item) low = middle; else high = middle - 1;
-    }
-    PromptItem it;
-    sequence(low, it);
-    const int64_t row0 = static_cast<int64_t>(item - p.tiles_before[low]) * item_rows;
-    const int64_t rows = min(static_cast<int64_t>(item_rows), static_cast<int64_t>(it.count) * p.group.d - row0);
-    it.row0 = static_cast<int32_t>(row0);
-    it.rows = static_cast<int32_t>(max(rows, static_cast<int64_t>(0)));
-    int32_t lo = INT32_MAX, hi = 0;
-#pragma unroll
-    for (int tile = 0; tile < 2; ++tile) {
-      int32_t highest_lo = 0, lowest_hi = INT32_MAX;
-      const int32_t r0 = it.row0 + tile * kPromptTile, r1 = min(it.row0 + it.rows, r0 + kPromptTile) - 1;
-      if (r0 <= r1) {
-        const int32_t t0 = p.group.div(r0), t1 = p.group.div(r1);
-        if (by_token) {
-#pragma unroll 1
-          for (int32_t i = t0 + begin_lane; i <= t1; i += lanes) {
-            const PromptView v(p, it, i);
-            highest_lo = max(highest_lo, v.lo);
-            lowest_hi = min(lowest_hi, v.hi);
-            if (v.hi > v.lo) lo = min(lo, v.lo), hi = max(hi, v.hi);
-          }
-        } else {
-          const PromptView a(p, it, t0), z(p, it, t1);  // (neither bound falls from token to token)
-          highest_lo = z.lo;
-          lowest_hi = a.hi;
-          if (z.hi > a.lo) lo = min(lo, a.lo), hi = max(hi, z.hi);
-        }
-      }
-      if (lanes > 1) {
-        highest_lo = __reduce_max_sync(0xffffffffu, highest_lo);
-        lowest_hi = __reduce_min_sync(0xffffffffu, lowest_hi);
-      }
-      it.highest_lo[tile] = highest_lo;
-      it.lowest_hi[tile] = lowest_hi;
-    }
-    if (lanes > 1) {
-      lo = __reduce_min_sync(0xffffffffu, lo);
-      hi = __reduce_max_sync(0xffffffffu, hi);
-    }
-    it.lo = hi > lo ? lo : 0;
-    it.hi = hi > lo ? hi : 0;
-    it.steps = max(1, (it.hi + step_tokens - 1) / step_tokens - it.lo / step_tokens);
-    it.first = 0;
-    return it;
-  };
-  if (by_token) {
-#pragma unroll 1
-    for (int32_t item = warp; item < count; item += kPlanThreads / 32) {
-      const PromptItem it = make(item, lane, 32);
-      if (lane == 0) p.items[item] = it;
-    }
-  } else {
-#pragma unroll 1
-    for (int32_t item = threadIdx.x; item < count; item += kPlanThreads) p.items[item] = make(item, 0, 1);
-  }
-  __syncthreads();
-
-  // Number the steps.
-  int64_t steps = 0;
-  int32_t longest = 0;
-#pragma unroll 1
-  for (int32_t i0 = 0; i0 < count; i0 += kPlanThreads) {
-    const int32_t item = i0 + threadIdx.x;
-    const int32_t mine = item < count ? p.items[item].steps : 0;
-    int64_t all;
-    const int64_t before = steps + sum_before(mine, of_warps, all);
-    if (item < count) p.items[item].first = before;
-    longest = max(longest, mine);
-    steps += all;
-  }
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  if (lane == 0) longest_of[warp] = longest;
-  __syncthreads();
-  longest = __reduce_max_sync(0xffffffffu, longest_of[lane]);
-
-  // An item to a CTA where there are no more of them and the longest one takes hardly longer than equal runs and a join.
-  constexpr int32_t kAlone = 4;
-  const int64_t total = steps * p.kv_heads, runs = static_cast<int64_t>(count) * p.kv_heads;
-  const int64_t share = (total + p.ctas - 1) / p.ctas;
-  const bool cut = runs > p.ctas || longest > share + kAlone;
-  if (threadIdx.x == 0) {
-    p.plan->items = count;
-    p.plan->cut = cut;
-    p.plan->head_steps = steps;
-  }
+  PromptPlanner<kPlanThreads> planner(p, scratch, item_rows, step_tokens);
+  planner.items([&](int32_t item, const PromptItem& it) { p.items[item] = it; });
+  const PromptPlan plan = planner.plan();
+  if (threadIdx.x == 0) *p.plan = plan;
 #pragma unroll 1
   for (int32_t cta = threadIdx.x; cta < p.ctas; cta += kPlanThreads) {
-    PromptStart s = {0, 0, 0, 0, 0, 0};
-    if (!cut) {
-      if (cta < runs) {
-        s.head = cta / count;
-        s.item = cta % count;
-        s.count = p.items[s.item].steps;
-        s.begin = s.head * steps + p.items[s.item].first;
-      }
-    } else if (cta * share < total) {
-      s.begin = cta * share;
-      s.count = min(share, total - s.begin);
-      s.head = static_cast<int32_t>(s.begin / steps);
-      const int64_t wanted = s.begin - s.head * steps;
-      int32_t low = 0, high = count - 1;  // the last item that begins there or before
-      while (low < high) {
-        const int32_t middle = (low + high + 1) / 2;
-        if (p.items[middle].first <= wanted) low = middle; else high = middle - 1;
-      }
-      s.item = low;
-      s.step = static_cast<int32_t>(wanted - p.items[low].first);
-    }
-    p.cta_starts[cta] = s;
+    p.cta_starts[cta] = planner.start(plan, cta, [&](int32_t item) { return p.items[item].first; }, [&](int32_t item) { return p.items[item].steps; });
   }
 }
 
@@ -376,9 +210,14 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
     p.q_boxes = make_rows_map(&p.q_map, c.q, false, c.cache->head_dim, 3, sizes, strides, boxes);
   }
   const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
-  CHORD_CUDA(launch_kernel(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, kEarlyLaunch, p, v.tiles * kPromptTile, v.step_tokens));
+  p.self = max_items <= kPlanHeld && c.batch <= kPlanHeld;
+  if (!p.self) {
+    CHORD_CUDA(launch_kernel(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, kEarlyLaunch, p, v.tiles * kPromptTile, v.step_tokens));
+  }
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(v.threads)), v.smem, stream, kEarlyLaunch, p));
-  if (ctas > 1) {
+  // Nothing is cut, whatever the lengths, where there are CTAs for all items and no table holds more than a few steps.
+  const bool whole = max_items * c.cache->heads <= ctas && (token_capacity(c.max_pages, c.cache) + v.step_tokens - 1) / v.step_tokens <= kPromptAlone;
+  if (ctas > 1 && !whole) {
     CHORD_CUDA(launch_kernel(v.join, dim3(static_cast<unsigned>(ctas - 1), static_cast<unsigned>(v.tiles * c.cache->head_dim / 8)),
                              dim3(kPromptTile), 0, stream, kEarlyLaunch, p));
   }

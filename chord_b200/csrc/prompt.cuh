@@ -17,73 +17,10 @@
 // that in FP32.
 #pragma once
 
-#include <cuda.h>
-#include <cuda_bf16.h>
-
-#include "../../include/chord_b200.h"
-#include "common.h"
-#include "kv_cache.cuh"
-#include "warp_ops.cuh"
+#include "prompt_plan.cuh"
 
 namespace chord {
 
-// The rows of two tiles (or one) of one sequence, for each of its key-value heads, and the tokens that any of them sees.
-struct __align__(16) PromptItem {
-  int32_t b, row0, rows, steps;          // at least one step
-  int32_t lo, hi, begin, count;          // tokens; the sequence's first query token and how many it has
-  int32_t length, both_ways;             // tokens in the cache, and those seen by all
-  int32_t highest_lo[2], lowest_hi[2];   // of each tile's rows: between them every row sees every token
-  int64_t first;                         // number of its first step among those of a key-value head
-};
-static_assert(sizeof(PromptItem) == 64, "read as four vectors");
-
-// Where a CTA begins, and how many steps it takes.
-struct PromptStart {
-  int32_t head, item, step, pad;
-  int64_t count;
-  int64_t begin;  // the step's number among all
-};
-
-struct PromptPlan {
-  int32_t items, cut;  // cut: the CTAs take equal runs of steps; else an item each
-  int64_t head_steps;  // of one key-value head
-};
-
-struct PromptParams {
-  CUtensorMap k_map, v_map;  // [pages][heads][page_size][dim], boxes of `box` tokens, 64 elements or a row of codes
-  CUtensorMap q_map;         // [tokens][heads][dim], boxes of 64 elements of a group's heads of 128 / group tokens
-  Cache cache;
-  const __nv_bfloat16* q;  // [tokens, heads, dim]
-  int64_t q_token, q_head;
-  const int32_t* tables;
-  int64_t table_stride;
-  const int32_t* lengths;   // [batch] tokens in the cache
-  const int32_t* offsets;   // [batch + 1] first query token of each
-  const int32_t* starts;    // [tokens] or null
-  const int32_t* prefixes;  // [batch] or null
-  const int32_t* own;       // [tokens] or null: each query token stands behind so many more tokens of its own
-  const float* slopes;      // [heads] or null
-  const float* extra;       // [tokens, heads, dim] or null: what the tokens' own parts gave, with
-  const float* extra_lse;   // [tokens, heads]
-  __nv_bfloat16* out;       // [tokens, heads, dim]
-  float* lse;               // [tokens, heads] or null
-  int32_t* status;
-  PromptPlan* plan;
-  PromptStart* cta_starts;  // [ctas]
-  PromptItem* items;        // [max_items]
-  int32_t* tiles_before;    // [batch]
-  float* parts;             // [ctas][2][tiles][dim / 4][128][4] sums, then [128] maxima and [128] sums of weights
-  float scale, cap;         // the scale times log2(e); the cap times log2(e), or zero
-  float cap_scale;          // 2 log2(e) scale / cap
-  int32_t batch, tokens, heads, kv_heads, capacity, own_capacity, window, max_items, ctas;
-  int32_t box;         // tokens of a TMA box of keys and values, which divides pages and steps; zero (codes): loaded as they are turned
-  int32_t head_step;   // from head to head in k_map and v_map: zero where all heads are one
-  int32_t page_step;   // the same of pages
-  bool q_boxes;        // queries by TMA
-  Divisor group;
-};
-
-constexpr int kPromptTile = 128;  // rows
 // Warps: 16 for the rows, one that loads by TMA, one that issues products, two that look at values and load queries that
 // TMA does not, and, over codes, four that turn these into BF16.
 constexpr int kLoadWarp = 16, kIssueWarp = 17, kLookWarp = 18, kLookWarps = 2, kTurnWarp = 20, kTurnWarps = 4;
@@ -149,36 +86,12 @@ __device__ __forceinline__ void add_pair(float (&sum)[2], float x, float y) {
       : "f"(x), "f"(y));
 }
 
-// The tokens of a sequence that its i-th query token sees, and where it stands.
-struct PromptView {
-  int32_t lo, hi, position;
-  __device__ __forceinline__ PromptView() : lo(0), hi(INT32_MAX), position(0) {}
-  __device__ __forceinline__ PromptView(const PromptParams& p, const PromptItem& of, int32_t i) {
-    if (p.own != nullptr) {
-      position = of.length + max(0, min(load_arg(p.own + of.begin + i), p.own_capacity)) - 1;
-      hi = of.length;
-    } else {
-      position = of.length - of.count + i;
-      hi = max(max(position + 1, 0), of.both_ways);
-    }
-    lo = p.window > 0 ? max(0, position + 1 - p.window) : 0;
-    if (p.starts != nullptr) lo = max(lo, load_arg(p.starts + of.begin + i));
-  }
-};
-
 // A warp's walk over its CTA's steps.
 struct PromptWalk {
   int64_t left;
   int32_t head, item, step, items, number;  // number: of the item among the CTA's
-  __device__ __forceinline__ explicit PromptWalk(const PromptParams& p) {
-    const PromptStart* const s = p.cta_starts + blockIdx.x;
-    items = p.plan->items;
-    left = s->count;
-    head = s->head;
-    item = s->item;
-    step = s->step;
-    number = 0;
-  }
+  __device__ __forceinline__ PromptWalk(const PromptStart& s, int32_t of)
+      : left(s.count), head(s.head), item(s.item), step(s.step), items(of), number(0) {}
   __device__ __forceinline__ int32_t here(const PromptItem& it) const {
     return static_cast<int32_t>(min(left, static_cast<int64_t>(it.steps - step)));
   }
@@ -201,6 +114,8 @@ __device__ __forceinline__ PromptItem load_item(const PromptParams& p, int32_t i
 enum PromptStatus : int32_t { kPromptLoadTimeout = 1, kPromptIssueTimeout = 2, kPromptRowTimeout = 8 };
 
 struct __align__(16) PromptControl {
+  PromptStart start;
+  int32_t plan_items;
   PromptItem items[2];  // of the CTA, in turn
   uint64_t item_full[2], item_empty[2], q_full, q_empty, drained;
   uint64_t kv_full[8], kv_empty[8];  // by slot
@@ -441,6 +356,53 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
   ptx::tc_fence_after();
   const uint32_t tmem = c.tmem;
   ptx::grid_dependency_wait();
+  if (p.self) {
+    // The plan, in the tiles' place: every CTA goes through all items and keeps those of its run.  (Several keep the same
+    // ones, alike; a kernel of its own took 8 us and its launch.)
+    static_assert(sizeof(PromptPlanScratch) + kPlanHeld * 12 <= L::kQBytes + kRing * L::kSlotBytes, "room");
+    PromptPlanScratch& scratch = *reinterpret_cast<PromptPlanScratch*>(smem);
+    int64_t* const firsts = reinterpret_cast<int64_t*>(smem + sizeof(PromptPlanScratch));
+    int32_t* const steps = reinterpret_cast<int32_t*>(firsts + kPlanHeld);
+    PromptPlanner<L::kThreads> planner(p, scratch, L::kTiles * kPromptTile, kN);
+    planner.items([&](int32_t item, const PromptItem& it) {
+      firsts[item] = it.first;
+      steps[item] = it.steps;
+    });
+    const PromptPlan plan = planner.plan();
+    if (threadIdx.x == 0) {
+      const PromptStart start = planner.start(plan, blockIdx.x, [&](int32_t item) { return firsts[item]; }, [&](int32_t item) { return steps[item]; });
+      c.start = start;
+      c.plan_items = plan.items;
+      p.cta_starts[blockIdx.x] = start;  // (for the join)
+      if (blockIdx.x == 0) *p.plan = plan;
+    }
+    __syncthreads();
+    // Those of the run, of one key-value head or more.
+    const int64_t begin = c.start.begin, end = begin + c.start.count;
+    const int32_t at_once = planner.by_token ? L::kThreads / planner.kSome : L::kThreads, some = planner.by_token ? planner.kSome : 1;
+#pragma unroll 1
+    for (int32_t i0 = 0; i0 < plan.items; i0 += at_once) {
+      const int32_t item = min(i0 + static_cast<int32_t>(threadIdx.x) / some, plan.items - 1);
+      bool wanted = false;
+      for (int64_t head = c.start.head; !wanted && head * plan.head_steps < end; ++head) {
+        const int64_t first = head * plan.head_steps + firsts[item];
+        wanted = first < end && first + steps[item] > begin;
+      }
+      if (!__any_sync(0xffffffffu, wanted)) continue;
+      PromptItem it = planner.make(item, threadIdx.x % some);
+      it.first = firsts[item];
+      if (wanted && threadIdx.x % some == 0) p.items[item] = it;
+    }
+    __syncthreads();
+    ptx::fence_proxy_async();  // (the tiles' copies come next)
+    __syncthreads();
+  } else {
+    if (threadIdx.x == 0) {
+      c.start = p.cta_starts[blockIdx.x];
+      c.plan_items = p.plan->items;
+    }
+    __syncthreads();
+  }
 
   // An item's description is read from global memory by the loading warp alone, which goes ahead of the others.
   auto item_of = [&](const PromptWalk& walk) {
@@ -473,7 +435,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     // page, which gives zeros.  Codes come as they are into a ring of their own.
     constexpr int kSlots = kCodes ? L::kRaw : kRing;
     uint32_t slot = 0, slot_phase = 0, q_phase = 0;
-    PromptWalk walk(p);
+    PromptWalk walk(c.start, c.plan_items);
     while (walk.left > 0 && bad == 0) {
       const PromptItem it = load_item(p, walk.item);
       const int32_t n = walk.here(it);
@@ -616,7 +578,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
       ++products[tile];
     };
 
-    PromptWalk walk(p);
+    PromptWalk walk(c.start, c.plan_items);
     while (walk.left > 0 && bad == 0) {
       const PromptItem it = item_of(walk);
       if (bad != 0) break;
@@ -677,7 +639,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     // finite.)
     const int w = warp - kLookWarp;
     uint32_t taken = 0, q_phase = 0;
-    PromptWalk walk(p);
+    PromptWalk walk(c.start, c.plan_items);
     while (walk.left > 0 && bad == 0) {
       const PromptItem it = item_of(walk);
       if (bad != 0) break;
@@ -754,7 +716,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
       constexpr int kOwn = kN / kTurnWarps;
       constexpr int kPieces = kDim / 16;
       uint32_t slot = 0, slot_phase = 0, raw_slot = 0, raw_phase = 0;
-      PromptWalk walk(p);
+      PromptWalk walk(c.start, c.plan_items);
       while (walk.left > 0 && bad == 0) {
         const PromptItem it = item_of(walk);
         if (bad != 0) break;
@@ -864,7 +826,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
       ptx::tc_fence_after();
     };
 
-    PromptWalk walk(p);
+    PromptWalk walk(c.start, c.plan_items);
     while (walk.left > 0) {
       PromptItem it = item_of(walk);
       if (bad != 0) it = load_item(p, walk.item);

@@ -22,25 +22,28 @@ __global__ void __launch_bounds__(kPromptTile) prompt_join_kernel(const __grid_c
   if (r >= it.rows) return;
   const int64_t end = at.head * plan.head_steps + it.first + it.steps;
 
+  // Parts: the last one of this CTA, then the first ones of those up to the item's end.  The highest maximum first, then all
+  // values as they come: no load waits for another's.
+  const int32_t parts = static_cast<int32_t>((end - 1) / plan.share) - blockIdx.x + 1;
+  auto part_of = [&](int32_t i) {
+    return p.parts + (2 * static_cast<int64_t>(blockIdx.x + i) + (i == 0 ? 1 : 0)) * kPart + static_cast<int64_t>(tile) * kPromptTile * (kDim + 2) + row * 4;
+  };
+  const int stats = kDim * kPromptTile - row * 3;
   float o[8] = {}, top = -INFINITY, sum = 0.0f;
-#pragma unroll 1
-  for (int32_t cta = blockIdx.x; cta < p.ctas; ++cta) {
-    if (cta > static_cast<int32_t>(blockIdx.x)) {
-      const PromptStart s = p.cta_starts[cta];
-      if (s.count == 0 || s.begin >= end) break;
-    }
-    const float* const part = p.parts + (2 * static_cast<int64_t>(cta) + (cta == static_cast<int32_t>(blockIdx.x) ? 1 : 0)) * kPart +
-                              static_cast<int64_t>(tile) * kPromptTile * (kDim + 2);
-    const float m = __ldcg(part + kDim * kPromptTile + row), l = __ldcg(part + (kDim + 1) * kPromptTile + row);
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(part) + dim / 4 * kPromptTile + row);
-    const float4 b = __ldcg(reinterpret_cast<const float4*>(part) + (dim / 4 + 1) * kPromptTile + row);
-    const float next = fmaxf(top, m), to = next == -INFINITY ? 0.0f : next;
-    const float old = exp2_fast(top - to), weight = exp2_fast(m - to);
-    top = next;
-    sum = fmaf(sum, old, l * weight);
+#pragma unroll 4
+  for (int32_t i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(part_of(i) + stats));
+  const float to = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+  for (int32_t i = 0; i < parts; ++i) {
+    const float* const part = part_of(i);
+    const float weight = exp2_fast(__ldcg(part + stats) - to);
+    const float l = __ldcg(part + stats + kPromptTile);
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(part + dim * kPromptTile));
+    const float4 b = __ldcg(reinterpret_cast<const float4*>(part + (dim + 4) * kPromptTile));
+    sum = fmaf(l, weight, sum);
     const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], old, v[i] * weight);
+    for (int k = 0; k < 8; ++k) o[k] = fmaf(v[k], weight, o[k]);
   }
   const int32_t token = p.group.div(it.row0 + r);
   const int64_t head = static_cast<int64_t>(at.head) * p.group.d + (it.row0 + r - token * static_cast<int32_t>(p.group.d));

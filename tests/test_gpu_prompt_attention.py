@@ -177,3 +177,21 @@ def test_in_a_graph_and_on_another_stream(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, chord_b200.prompt_attention(case.q, case.cache, case.table, case.lengths, case.offsets))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_many_sequences_and_items(device, bits):
+    """More sequences, and more items of one, than the kernel's CTAs plan on their own; with and without documents."""
+    case = Prompt(device, [((7 * b) % 50, (b % 4) * (b % 3)) for b in range(1100)], 2, 1, 64, 16, bits, seed=2)
+    case.check()
+    starts = torch.zeros(case.q.shape[0], dtype=torch.int32, device=device)
+    starts[::3] = 4
+    case.check(starts=starts, window=20)
+    case = Prompt(device, [(0, 900), (3, 5)], 384, 3, 64, 16, bits, seed=2)  # 128 heads share one: two tokens an item
+    out, lse = case.run()
+    again, _ = case.run(starts=torch.zeros(905, dtype=torch.int32, device=device))
+    assert torch.equal(out, again)
+    some = torch.tensor([0, 1, 2, 450, 898, 899, 900, 904])
+    want = case.want()
+    from tests.prompt_cases import close
+    close((out[some.to(device)], lse[some.to(device)]), tuple(x[some.to(device)] for x in want))
