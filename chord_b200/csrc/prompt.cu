@@ -14,10 +14,10 @@ namespace {
 constexpr int kPlanThreads = 1024;
 
 // The plan by one CTA, for more items or sequences than the main kernel's CTAs go through on their own.
-__global__ void __launch_bounds__(kPlanThreads, 1) prompt_plan_kernel(const __grid_constant__ PromptParams p, int32_t item_rows, int32_t step_tokens) {
+__global__ void __launch_bounds__(kPlanThreads, 1) prompt_plan_kernel(const __grid_constant__ PromptParams p, int32_t log_rows, int32_t log_tokens) {
   __shared__ PromptPlanScratch scratch;
   ptx::grid_dependency_wait();
-  PromptPlanner<kPlanThreads> planner(p, scratch, item_rows, step_tokens);
+  PromptPlanner<kPlanThreads> planner(p, scratch, log_rows, log_tokens);
   planner.items([&](int32_t item, const PromptItem& it) { p.items[item] = it; });
   const PromptPlan plan = planner.plan();
   if (threadIdx.x == 0) *p.plan = plan;
@@ -212,7 +212,8 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
   const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
   p.self = max_items <= kPlanHeld && c.batch <= kPlanHeld;
   if (!p.self) {
-    CHORD_CUDA(launch_kernel(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, kEarlyLaunch, p, v.tiles * kPromptTile, v.step_tokens));
+    CHORD_CUDA(launch_kernel(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, kEarlyLaunch, p, v.tiles == 2 ? 8 : 7,
+                             v.step_tokens == 128 ? 7 : 6));
   }
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(static_cast<unsigned>(v.threads)), v.smem, stream, kEarlyLaunch, p));
   // Nothing is cut, whatever the lengths, where there are CTAs for all items and no table holds more than a few steps.

@@ -45,6 +45,7 @@ struct PromptLayout {
   static constexpr int kRing = kFit > 8 ? 8 : kFit;
   static constexpr int kSmem = kQBytes + kRing * (kSlotBytes + kScaleBytes) + kRaw * kRawBytes + kMaxBytes + kControl;
   static constexpr uint32_t kOutColumn = kTwo ? 256 : 128;  // of tensor memory; the scores' buffers come first
+  static_assert(kTiles * kPromptTile == (kTwo ? 256 : 128) && kN == (kTwo ? 128 : 64), "the plan's logarithms");
   static_assert(kRing >= 3, "keys of one step and values of the one before, and one on its way");
 };
 
@@ -325,6 +326,11 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     ptx::tmem_alloc(ptx::smem_u32(&c.tmem), 512);
     ptx::tmem_relinquish();
   }
+  if (threadIdx.x == 32 * kLoadWarp) {
+    ptx::prefetch_tensormap(&p.k_map);
+    ptx::prefetch_tensormap(&p.v_map);
+    if (p.q_boxes) ptx::prefetch_tensormap(&p.q_map);
+  }
   if (threadIdx.x == 0) {
     ptx::mbar_init(bar(c.q_full), p.q_boxes ? 1 : kLookWarps);
     ptx::mbar_init(bar(c.q_empty), 1);
@@ -359,18 +365,15 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
   if (p.self) {
     // The plan, in the tiles' place: every CTA goes through all items and keeps those of its run.  (Several keep the same
     // ones, alike; a kernel of its own took 8 us and its launch.)
-    static_assert(sizeof(PromptPlanScratch) + kPlanHeld * 12 <= L::kQBytes + kRing * L::kSlotBytes, "room");
+    static_assert(sizeof(PromptPlanScratch) % 16 == 0 && sizeof(PromptPlanScratch) + kPlanHeld * sizeof(PromptItem) <= L::kQBytes + kRing * L::kSlotBytes, "room");
     PromptPlanScratch& scratch = *reinterpret_cast<PromptPlanScratch*>(smem);
-    int64_t* const firsts = reinterpret_cast<int64_t*>(smem + sizeof(PromptPlanScratch));
-    int32_t* const steps = reinterpret_cast<int32_t*>(firsts + kPlanHeld);
-    PromptPlanner<L::kThreads> planner(p, scratch, L::kTiles * kPromptTile, kN);
-    planner.items([&](int32_t item, const PromptItem& it) {
-      firsts[item] = it.first;
-      steps[item] = it.steps;
-    });
+    PromptItem* const items = reinterpret_cast<PromptItem*>(smem + sizeof(PromptPlanScratch));
+    PromptPlanner<L::kThreads> planner(p, scratch, L::kTwo ? 8 : 7, L::kTwo ? 7 : 6);
+    planner.items([&](int32_t item, const PromptItem& it) { items[item] = it; });
     const PromptPlan plan = planner.plan();
     if (threadIdx.x == 0) {
-      const PromptStart start = planner.start(plan, blockIdx.x, [&](int32_t item) { return firsts[item]; }, [&](int32_t item) { return steps[item]; });
+      const PromptStart start =
+          planner.start(plan, blockIdx.x, [&](int32_t item) { return items[item].first; }, [&](int32_t item) { return items[item].steps; });
       c.start = start;
       c.plan_items = plan.items;
       p.cta_starts[blockIdx.x] = start;  // (for the join)
@@ -379,19 +382,14 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     __syncthreads();
     // Those of the run, of one key-value head or more.
     const int64_t begin = c.start.begin, end = begin + c.start.count;
-    const int32_t at_once = planner.by_token ? L::kThreads / planner.kSome : L::kThreads, some = planner.by_token ? planner.kSome : 1;
 #pragma unroll 1
-    for (int32_t i0 = 0; i0 < plan.items; i0 += at_once) {
-      const int32_t item = min(i0 + static_cast<int32_t>(threadIdx.x) / some, plan.items - 1);
+    for (int32_t item = threadIdx.x; item < plan.items; item += L::kThreads) {
+      const int64_t first = items[item].first, steps = items[item].steps;
       bool wanted = false;
       for (int64_t head = c.start.head; !wanted && head * plan.head_steps < end; ++head) {
-        const int64_t first = head * plan.head_steps + firsts[item];
-        wanted = first < end && first + steps[item] > begin;
+        wanted = head * plan.head_steps + first < end && head * plan.head_steps + first + steps > begin;
       }
-      if (!__any_sync(0xffffffffu, wanted)) continue;
-      PromptItem it = planner.make(item, threadIdx.x % some);
-      it.first = firsts[item];
-      if (wanted && threadIdx.x % some == 0) p.items[item] = it;
+      if (wanted) p.items[item] = items[item];
     }
     __syncthreads();
     ptx::fence_proxy_async();  // (the tiles' copies come next)
@@ -477,11 +475,13 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
       };
       int32_t page = 0, place = -1;
       if (p.box != 0) look_up(0, lane, page, place);
+      // (the queries of all but the first item wait for the one before; its first keys need not)
+      const int first_which = walk.number == 0 ? 0 : 1;
 #pragma unroll 1
       for (int32_t j = 0; j < n; ++j) {
 #pragma unroll 1
         for (int which = 0; which < 2; ++which) {
-          if (j == 0 && which == 1) begin_item();
+          if (j == 0 && which == first_which) begin_item();
           if (bad != 0) break;
           if (p.box == 0) continue;
           const uint32_t at = kCodes ? bar(c.raw_full[slot]) : bar(c.kv_full[slot]);

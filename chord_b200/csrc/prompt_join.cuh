@@ -24,7 +24,7 @@ __global__ void __launch_bounds__(kPromptTile) prompt_join_kernel(const __grid_c
 
   // Parts: the last one of this CTA, then the first ones of those up to the item's end.  The highest maximum first, then all
   // values as they come: no load waits for another's.
-  const int32_t parts = static_cast<int32_t>((end - 1) / plan.share) - blockIdx.x + 1;
+  const int32_t parts = static_cast<int32_t>(plan_quotient(end - 1, plan.share)) - blockIdx.x + 1;
   auto part_of = [&](int32_t i) {
     return p.parts + (2 * static_cast<int64_t>(blockIdx.x + i) + (i == 0 ? 1 : 0)) * kPart + static_cast<int64_t>(tile) * kPromptTile * (kDim + 2) + row * 4;
   };

@@ -17,6 +17,12 @@ struct PromptPlanScratch {
   int64_t steps;
 };
 
+// n / d for n, d >= 0, in 32 bits where they do.
+__device__ __forceinline__ int64_t plan_quotient(int64_t n, int64_t d) {
+  if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+
 // A CTA of kThreads: the items of every sequence, the tokens that each of them sees, and where the main kernel's CTAs begin.
 // Bounded by the latency of its loads, so sequences are kept in shared memory (with all of it in global memory the
 // items of one sequence after another were some seven loads apart).
@@ -25,7 +31,7 @@ struct PromptPlanner {
   static constexpr int kWarps = kThreads / 32;
   const PromptParams& p;
   PromptPlanScratch& s;
-  const int32_t item_rows, step_tokens;
+  const int32_t log_rows, log_tokens;  // of an item and of a step, both powers of two
   const int lane, warp;
   const bool by_token;  // an item's tokens do not follow from its first and last query token
 
@@ -40,15 +46,15 @@ struct PromptPlanner {
     __syncthreads();  // (of_warps may still be read from the call before)
     if (lane == 31) s.of_warps[warp] = upto;
     __syncthreads();
-    int64_t before = 0;
-    all = 0;
+    int64_t warps = lane < kWarps ? s.of_warps[lane] : 0;  // up to each one, inclusive
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const int64_t of = s.of_warps[w];
-      if (w < warp) before += of;
-      all += of;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t below = __shfl_up_sync(0xffffffffu, warps, d);
+      if (lane >= d) warps += below;
     }
-    return before + upto - value;
+    all = __shfl_sync(0xffffffffu, warps, 31);
+    const int64_t before = __shfl_sync(0xffffffffu, warps, max(warp - 1, 0));
+    return (warp == 0 ? 0 : before) + upto - value;
   }
 
   __device__ __forceinline__ int4 load_sequence(int32_t b) const {
@@ -65,7 +71,7 @@ struct PromptPlanner {
   }
 
   __device__ __forceinline__ PromptPlanner(const PromptParams& params, PromptPlanScratch& scratch, int32_t rows, int32_t tokens)
-      : p(params), s(scratch), item_rows(rows), step_tokens(tokens), lane(threadIdx.x & 31), warp(threadIdx.x >> 5),
+      : p(params), s(scratch), log_rows(rows), log_tokens(tokens), lane(threadIdx.x & 31), warp(threadIdx.x >> 5),
         by_token(params.starts != nullptr || (params.own != nullptr && params.window > 0)) {
     int64_t items = 0;
 #pragma unroll 1
@@ -75,7 +81,7 @@ struct PromptPlanner {
       if (b < p.batch) {
         const int4 of = load_sequence(b);
         if (b < kPlanHeld) s.sequences[b] = of;
-        mine = (static_cast<int64_t>(of.y) * p.group.d + item_rows - 1) / item_rows;
+        mine = (static_cast<int64_t>(of.y) * p.group.d + (1 << log_rows) - 1) >> log_rows;
       }
       int64_t all;
       const int64_t before = items + sum_before(mine, all);
@@ -107,8 +113,8 @@ struct PromptPlanner {
     PromptItem it;
     it.b = low;
     it.begin = of.x, it.count = of.y, it.length = of.z, it.both_ways = of.w;
-    const int64_t row0 = static_cast<int64_t>(item - before(low)) * item_rows;
-    const int64_t rows = min(static_cast<int64_t>(item_rows), static_cast<int64_t>(it.count) * p.group.d - row0);
+    const int64_t row0 = static_cast<int64_t>(item - before(low)) << log_rows;
+    const int64_t rows = min(static_cast<int64_t>(1 << log_rows), static_cast<int64_t>(it.count) * p.group.d - row0);
     it.row0 = static_cast<int32_t>(row0);
     it.rows = static_cast<int32_t>(max(rows, static_cast<int64_t>(0)));
     int32_t lo = INT32_MAX, hi = 0;
@@ -150,7 +156,7 @@ struct PromptPlanner {
     }
     it.lo = hi > lo ? lo : 0;
     it.hi = hi > lo ? hi : 0;
-    it.steps = max(1, (it.hi + step_tokens - 1) / step_tokens - it.lo / step_tokens);
+    it.steps = max(1, ((it.hi + (1 << log_tokens) - 1) >> log_tokens) - (it.lo >> log_tokens));
     it.first = 0;
     return it;
   }
@@ -192,7 +198,7 @@ struct PromptPlanner {
     PromptPlan plan;
     plan.items = s.count;
     plan.head_steps = s.steps;
-    plan.share = (total + p.ctas - 1) / p.ctas;
+    plan.share = plan_quotient(total + p.ctas - 1, p.ctas);
     plan.cut = runs > p.ctas || s.longest > plan.share + kPromptAlone;
     return plan;
   }
@@ -211,7 +217,7 @@ struct PromptPlanner {
     } else if (cta * plan.share < total) {
       at.begin = cta * plan.share;
       at.count = min(plan.share, total - at.begin);
-      at.head = static_cast<int32_t>(at.begin / plan.head_steps);
+      at.head = static_cast<int32_t>(plan_quotient(at.begin, plan.head_steps));
       const int64_t wanted = at.begin - at.head * plan.head_steps;
       int32_t low = 0, high = plan.items - 1;  // the last item that begins there or before
       while (low < high) {
