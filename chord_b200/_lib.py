@@ -184,7 +184,10 @@ def direct():
     names = ("gemv", "qk_norm_rope", "qk_norm_rope_write", "cache_write", "cache_read", "paged_attention",
              "paged_attention_workspace_bytes")
     lib = load()
-    known = _torch_call.entries(*(ctypes.cast(getattr(lib, "chord_b200_" + name), ctypes.c_void_p).value for name in names))
+    more = ("paged_attention_shaped", "prompt_attention", "prompt_attention_workspace_bytes", "shared_prefix_attention",
+            "shared_prefix_attention_workspace_bytes", "attention_weights", "cache_evict")
+    known = all(put(*(ctypes.cast(getattr(lib, "chord_b200_" + name), ctypes.c_void_p).value for name in of))
+                for put, of in ((_torch_call.entries, names), (_torch_call.more_entries, more)))
     return _torch_call if known else None
 
 

@@ -386,9 +386,13 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     _cache(cache)
     shaped = cap is not None or slopes is not None
     direct = _lib.direct()
-    if direct is not None and not shaped and outputs is None and locks is None and window != 0:
-        result = direct.paged_attention(q, cache.address, cache.index, block_tables, lengths, lse,
-                                        0 if window is None else window, cache.scale if scale is None else scale)
+    if direct is not None and outputs is None and locks is None and window != 0:
+        if shaped:
+            result = direct.paged_attention_shaped(q, cache.address, cache.index, block_tables, lengths, lse,
+                                                   cache.scale if scale is None else scale, window, cap, slopes)
+        else:
+            result = direct.paged_attention(q, cache.address, cache.index, block_tables, lengths, lse,
+                                            0 if window is None else window, cache.scale if scale is None else scale)
         if result is not None:
             return result
     q_rows = _queries(q, cache)

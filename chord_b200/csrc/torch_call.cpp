@@ -1,4 +1,4 @@
-// The plain calls of gemv, qk_norm_rope, the cache's operators and paged_attention without the Python
+// The plain calls of gemv, qk_norm_rope, the cache's operators and attention over it without the Python
 // wrappers' cost: arguments are looked at and results allocated here.  A call that is not as it should be, or
 // has an option that is not known here, gets None and goes through the wrapper, which says what is wrong.  (A
 // tensor's checks cost some 1 us in Python and an allocation 2 us; one launch is 2.3 us.)  Built where torch's
@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -29,6 +30,16 @@ struct Entries {
   decltype(&chord_b200_paged_attention) paged_attention;
   decltype(&chord_b200_paged_attention_workspace_bytes) workspace_bytes;
 } entries;
+
+struct MoreEntries {
+  decltype(&chord_b200_paged_attention_shaped) paged_attention_shaped = nullptr;
+  decltype(&chord_b200_prompt_attention) prompt_attention = nullptr;
+  decltype(&chord_b200_prompt_attention_workspace_bytes) prompt_workspace_bytes = nullptr;
+  decltype(&chord_b200_shared_prefix_attention) shared_prefix_attention = nullptr;
+  decltype(&chord_b200_shared_prefix_attention_workspace_bytes) shared_workspace_bytes = nullptr;
+  decltype(&chord_b200_attention_weights) attention_weights = nullptr;
+  decltype(&chord_b200_cache_evict) cache_evict = nullptr;
+} more;
 
 // What the wrappers keep for a device: its status word and the lock buffers of its streams.  (Under the
 // interpreter's lock.)
@@ -356,6 +367,243 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   return rc ? none() : THPVariable_Wrap(std::move(out));
 }
 
+// Lock words of a stream, as the wrappers gave them; null for a stream that they have not met.
+int32_t* locks_of(int device, void* stream, int64_t* count) {
+  for (const auto& l : devices[device].locks) {
+    if (l.words != nullptr && l.stream == stream) return *count = l.count, l.words;
+  }
+  return nullptr;
+}
+
+// scale, window (None or 1 and more), cap (None or from 1e-30 to 1e30), slopes (None or [heads])
+bool scores_of(PyObject* const* a, int device, int64_t heads, chord_b200_scores* scores) {
+  *scores = {0.0, 0.0, nullptr, 0};
+  if (!number(a[0], &scores->scale)) return false;
+  if (a[1] != Py_None && (!integer(a[1], &scores->window) || scores->window < 1 || scores->window >= (1ll << 31))) return false;
+  if (a[2] != Py_None && (!number(a[2], &scores->cap) || scores->cap < 1e-30 || scores->cap > 1e30)) return false;
+  if (a[3] != Py_None) {
+    const at::Tensor* t = tensor(a[3], at::kFloat, 1);
+    if (t == nullptr || t->get_device() != device || t->size(0) != heads || (heads > 1 && t->stride(0) != 1)) return false;
+    scores->slopes = t->const_data_ptr<float>();
+  }
+  return true;
+}
+
+// None, or [tokens, heads] in a row.
+bool sums_of(PyObject* o, int device, int64_t tokens, int64_t heads, float** lse) {
+  *lse = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = tensor(o, at::kFloat, 2);
+  if (t == nullptr || t->get_device() != device || t->size(0) != tokens || t->size(1) != heads || !t->is_contiguous()) return false;
+  *lse = t->mutable_data_ptr<float>();
+  return true;
+}
+
+// None, or `count` values.
+bool optional_ints(PyObject* o, int device, int64_t count, const int32_t** at) {
+  *at = nullptr;
+  return o == Py_None || (*at = ints(o, device, count)) != nullptr;
+}
+
+const at::Tensor* queries_of(PyObject* o, int device, const chord_b200_kv_cache* cache) {
+  const at::Tensor* q = tensor(o, at::kBFloat16, 3);
+  return q != nullptr && q->size(0) > 0 && rows(q, device, q->size(0), -1, cache->head_dim) && q->size(1) % cache->heads == 0 ? q : nullptr;
+}
+
+// paged_attention_shaped(q, cache, device, block_tables, lengths, lse, scale, window, cap, slopes)
+PyObject* paged_attention_shaped(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  const chord_b200_kv_cache* cache;
+  int device;
+  if (count != 10 || more.paged_attention_shaped == nullptr || !cache_of(a[1], a[2], &cache, &device)) return none();
+  const at::Tensor* const q = queries_of(a[0], device, cache);
+  if (q == nullptr) return none();
+  const int64_t batch = q->size(0), heads = q->size(1);
+  Table table;
+  float* lse;
+  chord_b200_scores scores;
+  const int32_t* const lengths = ints(a[4], device, batch);
+  if (lengths == nullptr || !table_of(a[3], device, batch, &table) || !sums_of(a[5], device, batch, heads, &lse) ||
+      !scores_of(a + 6, device, heads, &scores))
+    return none();
+  void* const stream = stream_of(device);
+  int64_t word_count = 0;
+  int32_t* const words = locks_of(device, stream, &word_count);
+  const int64_t size = entries.workspace_bytes(cache->head_dim, heads / cache->heads);
+  if (words == nullptr || size < 0) return none();
+  int32_t* const status = devices[device].status;
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = empty(q->sizes(), *q);
+    const at::Tensor workspace = empty({size}, *q, at::kByte);
+    rc = more.paged_attention_shaped(q->const_data_ptr(), q->stride(0), q->stride(1), cache, table.at, table.stride, table.pages, lengths,
+                                     out.mutable_data_ptr(), lse, words, word_count, workspace.mutable_data_ptr(), size, status, batch,
+                                     heads, &scores, stream);
+  }
+  return rc ? none() : THPVariable_Wrap(std::move(out));
+}
+
+// prompt_attention(q, cache, device, block_tables, lengths, offsets, starts, prefixes, lse, scale, window, cap, slopes)
+PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  const chord_b200_kv_cache* cache;
+  int device;
+  if (count != 13 || more.prompt_attention == nullptr || !cache_of(a[1], a[2], &cache, &device)) return none();
+  const at::Tensor* const q = queries_of(a[0], device, cache);
+  const at::Tensor* const offsets = tensor(a[5], at::kInt, 1);
+  if (q == nullptr || offsets == nullptr || offsets->get_device() != device || offsets->size(0) < 2 || offsets->stride(0) != 1) return none();
+  const int64_t tokens = q->size(0), heads = q->size(1), batch = offsets->size(0) - 1;
+  Table table;
+  float* lse;
+  chord_b200_scores scores;
+  const int32_t *starts, *prefixes, *const lengths = ints(a[4], device, batch);
+  if (lengths == nullptr || !table_of(a[3], device, batch, &table) || !optional_ints(a[6], device, tokens, &starts) ||
+      !optional_ints(a[7], device, batch, &prefixes) || !sums_of(a[8], device, tokens, heads, &lse) || !scores_of(a + 9, device, heads, &scores))
+    return none();
+  const int64_t size = more.prompt_workspace_bytes(batch, tokens, heads, cache->heads, cache->head_dim);
+  if (size < 0) return none();
+  int32_t* const status = devices[device].status;
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = empty(q->sizes(), *q);
+    const at::Tensor workspace = empty({size}, *q, at::kByte);
+    rc = more.prompt_attention(q->const_data_ptr(), q->stride(0), q->stride(1), cache, table.at, table.stride, table.pages, lengths,
+                               offsets->const_data_ptr<int32_t>(), starts, prefixes, out.mutable_data_ptr(), lse,
+                               workspace.mutable_data_ptr(), size, status, batch, tokens, heads, &scores, stream_of(device));
+  }
+  return rc ? none() : THPVariable_Wrap(std::move(out));
+}
+
+// shared_prefix_attention(q, cache, device, prefix_tables, prefix_lengths, group_offsets, block_tables, lengths, lse, scale, window,
+// cap, slopes)
+PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  const chord_b200_kv_cache* cache;
+  int device;
+  if (count != 13 || more.shared_prefix_attention == nullptr || !cache_of(a[1], a[2], &cache, &device)) return none();
+  const at::Tensor* const q = queries_of(a[0], device, cache);
+  const at::Tensor* const offsets = tensor(a[5], at::kInt, 1);
+  if (q == nullptr || offsets == nullptr || offsets->get_device() != device || offsets->size(0) < 2 || offsets->stride(0) != 1) return none();
+  const int64_t batch = q->size(0), heads = q->size(1), groups = offsets->size(0) - 1;
+  Table table, prefix_table;
+  float* lse;
+  chord_b200_scores scores;
+  const int32_t *const prefix_lengths = ints(a[4], device, groups), *const lengths = ints(a[7], device, batch);
+  if (prefix_lengths == nullptr || lengths == nullptr || !table_of(a[3], device, groups, &prefix_table) || !table_of(a[6], device, batch, &table) ||
+      !sums_of(a[8], device, batch, heads, &lse) || !scores_of(a + 9, device, heads, &scores))
+    return none();
+  void* const stream = stream_of(device);
+  int64_t word_count = 0;
+  int32_t* const words = locks_of(device, stream, &word_count);
+  const int64_t size = more.shared_workspace_bytes(groups, batch, heads, cache->heads, cache->head_dim);
+  if (words == nullptr || size < 0) return none();
+  int32_t* const status = devices[device].status;
+  at::Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = empty(q->sizes(), *q);
+    const at::Tensor workspace = empty({size}, *q, at::kByte);
+    rc = more.shared_prefix_attention(q->const_data_ptr(), q->stride(0), q->stride(1), cache, prefix_table.at, prefix_table.stride,
+                                      prefix_table.pages, prefix_lengths, offsets->const_data_ptr<int32_t>(), groups, table.at,
+                                      table.stride, table.pages, lengths, out.mutable_data_ptr(), lse, words, word_count,
+                                      workspace.mutable_data_ptr(), size, status, batch, heads, &scores, stream);
+  }
+  return rc ? none() : THPVariable_Wrap(std::move(out));
+}
+
+// attention_weights(q, cache, device, block_tables, lengths, lse, weights, scale, window, cap, slopes)
+PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  const chord_b200_kv_cache* cache;
+  int device;
+  if (count != 11 || more.attention_weights == nullptr || !cache_of(a[1], a[2], &cache, &device)) return none();
+  const at::Tensor* const q = queries_of(a[0], device, cache);
+  if (q == nullptr || q->size(0) > 65535) return none();
+  const int64_t batch = q->size(0), heads = q->size(1);
+  Table table;
+  float* lse;
+  chord_b200_scores scores;
+  const int32_t* const lengths = ints(a[4], device, batch);
+  if (lengths == nullptr || a[5] == Py_None || !table_of(a[3], device, batch, &table) || !sums_of(a[5], device, batch, heads, &lse) ||
+      !scores_of(a + 7, device, heads, &scores))
+    return none();
+  const bool add = a[6] != Py_None;
+  const at::Tensor* given = nullptr;
+  if (add) {
+    given = tensor(a[6], at::kFloat, 3);
+    if (given == nullptr || given->get_device() != device || given->size(0) != batch || given->size(1) != cache->heads || given->size(2) == 0 ||
+        !given->is_contiguous())
+      return none();
+  }
+  const int64_t width = add ? given->size(2) : table.pages * cache->page_size;
+  int32_t* const status = devices[device].status;
+  at::Tensor made;
+  int rc;
+  {
+    const Unlocked unlocked;
+    if (!add) made = empty({batch, cache->heads, width}, *q, at::kFloat);
+    const at::Tensor& to = add ? *given : made;
+    rc = more.attention_weights(q->const_data_ptr(), q->stride(0), q->stride(1), cache, table.at, table.stride, table.pages, lengths, lse,
+                                to.mutable_data_ptr<float>(), cache->heads * width, width, width, add, status, batch, heads, &scores,
+                                stream_of(device));
+  }
+  if (rc) return none();
+  if (!add) return THPVariable_Wrap(std::move(made));
+  Py_INCREF(a[6]);
+  return a[6];
+}
+
+// cache_evict(cache, device, block_tables, lengths, weights, keep, first, recent, new_tables)
+PyObject* cache_evict(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  const chord_b200_kv_cache* cache;
+  int device;
+  int64_t keep, first, recent;
+  if (count != 9 || more.cache_evict == nullptr || !cache_of(a[0], a[1], &cache, &device) || !integer(a[5], &keep) || !integer(a[6], &first) ||
+      !integer(a[7], &recent) || keep < 1 || first < 0 || recent < 0 || first > keep || recent > keep - first)
+    return none();
+  const at::Tensor *const lengths = tensor(a[3], at::kInt, 1), *const weights = tensor(a[4], at::kFloat, 3);
+  if (lengths == nullptr || lengths->get_device() != device || lengths->size(0) == 0 || lengths->size(0) > 65535 || !lengths->is_contiguous())
+    return none();
+  const int64_t batch = lengths->size(0);
+  Table table, new_table = {nullptr, 0, 0};
+  if (weights == nullptr || weights->get_device() != device || weights->size(0) != batch || weights->size(1) != cache->heads ||
+      weights->size(2) == 0 || !weights->is_contiguous() || !table_of(a[2], device, batch, &table) ||
+      (a[8] != Py_None && !table_of(a[8], device, batch, &new_table)))
+    return none();
+  const int64_t width = weights->size(2), new_width = width > keep ? width : keep;
+  const int64_t most = std::min(std::min(keep, width), table.pages * cache->page_size);
+  if (keep >= (1ll << 31) - 65536 || (a[8] != Py_None && new_table.pages * cache->page_size < most)) return none();
+  int32_t* const status = devices[device].status;
+  at::Tensor new_lengths, new_weights;
+  int rc;
+  {
+    const Unlocked unlocked;
+    new_lengths = empty({batch}, *lengths, at::kInt), new_weights = empty({batch, cache->heads, new_width}, *lengths, at::kFloat);
+    const int64_t size = batch * cache->heads * keep * 4;
+    const at::Tensor workspace = empty({size}, *lengths, at::kByte);
+    rc = more.cache_evict(cache, table.at, table.stride, table.pages, new_table.at, new_table.stride, new_table.pages,
+                          lengths->const_data_ptr<int32_t>(), weights->const_data_ptr<float>(), cache->heads * width, width, width,
+                          new_lengths.mutable_data_ptr<int32_t>(), new_weights.mutable_data_ptr<float>(), new_width,
+                          workspace.mutable_data_ptr(), size, status, batch, keep, first, recent, stream_of(device));
+  }
+  return rc ? none() : pair(std::move(new_lengths), std::move(new_weights));
+}
+
+// more_entries(addresses of the seven functions, in the struct's order)
+PyObject* set_more_entries(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  int64_t at[7];
+  if (count != 7) return none();
+  for (int i = 0; i < 7; ++i) {
+    if (!integer(a[i], at + i)) return none();
+  }
+  more = {reinterpret_cast<decltype(more.paged_attention_shaped)>(at[0]), reinterpret_cast<decltype(more.prompt_attention)>(at[1]),
+          reinterpret_cast<decltype(more.prompt_workspace_bytes)>(at[2]), reinterpret_cast<decltype(more.shared_prefix_attention)>(at[3]),
+          reinterpret_cast<decltype(more.shared_workspace_bytes)>(at[4]), reinterpret_cast<decltype(more.attention_weights)>(at[5]),
+          reinterpret_cast<decltype(more.cache_evict)>(at[6])};
+  Py_RETURN_TRUE;
+}
+
 // entries(addresses of the seven functions, in the struct's order)
 PyObject* set_entries(PyObject*, PyObject* const* a, Py_ssize_t count) {
   int64_t at[7];
@@ -395,7 +643,10 @@ PyObject* set_locks(PyObject*, PyObject* const* a, Py_ssize_t count) {
 #define METHOD(name, function) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&guarded<function>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD("gemv", gemv), METHOD("qk_norm_rope", qk_norm_rope), METHOD("qk_norm_rope_write", qk_norm_rope_write),
                          METHOD("cache_write", cache_write), METHOD("cache_read", cache_read),
-                         METHOD("paged_attention", paged_attention), METHOD("entries", set_entries), METHOD("device", set_device),
+                         METHOD("paged_attention", paged_attention), METHOD("paged_attention_shaped", paged_attention_shaped),
+                         METHOD("prompt_attention", prompt_attention), METHOD("shared_prefix_attention", shared_prefix_attention),
+                         METHOD("attention_weights", attention_weights), METHOD("cache_evict", cache_evict),
+                         METHOD("more_entries", set_more_entries), METHOD("entries", set_entries), METHOD("device", set_device),
                          METHOD("locks", set_locks), {nullptr, nullptr, 0, nullptr}};
 
 // The torch whose headers this is compiled with; the package does not use it with another.

@@ -34,6 +34,12 @@ def attention_weights(q: torch.Tensor, cache: KVCache, block_tables: torch.Tenso
     wider, rows contiguous) they are added to it, token by token, and it is returned.  The same inputs give the same bits.
     What :func:`paged_attention` reports is reported, and lengths beyond ``weights``."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None:
+        result = direct.attention_weights(q, cache.address, cache.index, block_tables, lengths, lse, weights,
+                                          cache.scale if scale is None else scale, window, cap, slopes)
+        if result is not None:
+            return result
     q_rows = _queries(q, cache)
     device, (batch, heads) = cache.device, q.shape[:2]
     table = _table(block_tables, device, batch)
@@ -74,6 +80,11 @@ def cache_evict(cache: KVCache, block_tables: torch.Tensor, lengths: torch.Tenso
     wide, if that is more), zeros behind them.  Lengths beyond the table or the weights and pages outside the cache are
     reported by :func:`chord_b200.check_status`."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None:
+        result = direct.cache_evict(cache.address, cache.index, block_tables, lengths, weights, keep, first, recent, new_tables)
+        if result is not None:
+            return result
     device = cache.device
     _checks.supported_gpu(device)
     if not isinstance(lengths, torch.Tensor) or lengths.ndim != 1:

@@ -44,6 +44,12 @@ def prompt_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor
     Offsets that fall or lie outside ``q``, lengths beyond the table and pages outside the cache are reported by
     :func:`chord_b200.check_status`; nothing outside is read or written.  The same inputs give the same bits."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None and outputs is None:
+        result = direct.prompt_attention(q, cache.address, cache.index, block_tables, lengths, offsets, starts, prefixes, lse,
+                                         cache.scale if scale is None else scale, window, cap, slopes)
+        if result is not None:
+            return result
     q_rows = _queries(q, cache)
     device, (tokens, heads) = cache.device, q.shape[:2]
     at_offsets, batch = _offsets("offsets", offsets, device)
@@ -84,6 +90,13 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCache, prefix_tables: torc
     are read once for its whole group.  The other arguments, the results and what is reported are as for
     :func:`paged_attention`, over the sequence as a whole: its window, distances and ``lse``."""
     _cache(cache)
+    direct = _lib.direct()
+    if direct is not None and outputs is None and locks is None:
+        result = direct.shared_prefix_attention(q, cache.address, cache.index, prefix_tables, prefix_lengths, group_offsets,
+                                                block_tables, lengths, lse, cache.scale if scale is None else scale, window,
+                                                cap, slopes)
+        if result is not None:
+            return result
     q_rows = _queries(q, cache)
     device, (batch, heads) = cache.device, q.shape[:2]
     at_groups, groups = _offsets("group_offsets", group_offsets, device)
