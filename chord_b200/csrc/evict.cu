@@ -1,4 +1,8 @@
 // What each token of the cache got of a new token's attention, and eviction by what has been gathered of it.
+#include <mutex>
+#include <set>
+#include <utility>
+
 #include "../../include/chord_b200.h"
 #include "common.h"
 #include "kv_cache.cuh"
@@ -37,163 +41,251 @@ struct WeighParams {
   int32_t* status;
   float scale, cap, two_over_cap;  // as of paged_attention
   int32_t heads, group, capacity, width, window, add;
+  int32_t runs;  // of 64 tokens for a warp
 };
 
 constexpr int kWeighWarps = 4;
-constexpr int kWeighRun = 64;  // tokens of a warp
-constexpr int kWeighTokens = kWeighWarps * kWeighRun;
+constexpr int kWeighRun = 64;  // tokens that a warp looks up at once
 
-// A warp takes 64 tokens of one key-value head, 16 at a time as the rows of mma.m16n8k16, 8 of the heads that share it as
-// columns.  A lane's fragments come straight from memory: a product's sum does not depend on the order of its terms, so
-// the dims of a lane's 16 bytes (8 of codes) of a key and of the same piece of a query stand for the columns that
-// the instruction wants there.  The weights of a token's heads are summed in one order, so the same inputs give the
-// same bits.
+// What a lane has of a row: words (two elements) in the order of its loads.  A product's sum does not depend on the order of
+// its terms, so a lane's words of a key and of a query, wherever they lie, stand for the columns that the instruction wants
+// there, as long as they are the same dims.  Loads are of 16 bytes, the last one of 8 where codes of 96 dims leave no more.
+// A warp has a ring of stages of 16 tokens, some 12 KB on their way or in use.
+template <int kDim, bool kCodes>
+struct WeighRow {
+  static constexpr int kLoadDims = kCodes ? 64 : 32;  // of the four lanes of a row together
+  static constexpr int kLoads = kDim / kLoadDims, kRest = kDim % kLoadDims / 32;
+  static constexpr int kWords = kDim / 8;
+  static constexpr int kBytes = kDim * (kCodes ? 1 : 2), kPieces = kBytes / 16;
+  static constexpr int kStage = 16 * kBytes + (kCodes ? 64 : 0);  // with the rows' scales
+  static constexpr int kStages = 12 * 1024 / kStage < 2 ? 2 : 12 * 1024 / kStage > 6 ? 6 : 12 * 1024 / kStage;
+  static constexpr int kSmem = kWeighWarps * kStages * kStage;
+  // Rows of a multiple of 128 bytes: the lanes of an odd one read the other half of the banks.
+  static __device__ __forceinline__ int place(int row, int piece) { return row * kBytes + (kBytes % 128 == 0 ? piece ^ (row & 1) << 2 : piece) * 16; }
+};
+
+// A warp takes p.runs times 64 tokens of one key-value head, 16 at a time as the rows of mma.m16n8k16, 8 of the heads that
+// share it as columns.  The weights of a token's heads are summed in one order, so the same inputs give the same bits.
+// Bounded by memory and by what is on its way (with fragments straight from memory into registers, three warps of a
+// scheduler had 2 to 4 KB each on their way: 131072 tokens in 8 bits 46 us).
 template <int kDim, bool kCodes>
 __global__ void __launch_bounds__(kWeighWarps * 32) attention_weights_kernel(const WeighParams p) {
-  constexpr int kChunks = kDim / 32;  // of 8 dims for each of four lanes
+  using R = WeighRow<kDim, kCodes>;
+  extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q4 = lane & 3, r8 = lane >> 2;
   ptx::grid_dependency_wait();
   const int32_t b = blockIdx.z, kv_head = blockIdx.y;
   const int32_t given = load_arg(p.lengths + b), length = max(0, min(given, min(p.capacity, p.width)));
   if (given > min(p.capacity, p.width) && threadIdx.x == 0 && blockIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusIndex);
   const int32_t low = p.window > 0 ? max(0, length - p.window) : 0;
-  const int32_t token0 = blockIdx.x * kWeighTokens + warp * kWeighRun;
+  const int32_t first = (blockIdx.x * kWeighWarps + warp) * (kWeighRun * p.runs);
+  const int32_t last = min(first + kWeighRun * p.runs, p.width);
   float* const row = p.weights + b * p.weight_batch + kv_head * p.weight_head;
-  if (token0 >= length || token0 + kWeighRun <= low) {
+  if (first >= length || last <= low) {
     if (!p.add) {
-      for (int32_t t = token0 + lane; t < min(token0 + kWeighRun, p.width); t += 32) row[t] = 0.0f;
+      for (int32_t t = first + lane; t < last; t += 32) row[t] = 0.0f;
     }
     return;
   }
-  // Where the run's tokens lie: two to a lane, as offsets in bytes, negative for none.
-  int64_t offset[2];
-  float key_scale[2] = {1.0f, 1.0f};
+  uint8_t* const ring = smem + warp * (R::kStages * R::kStage);
+  const uint32_t ring_at = ptx::smem_u32(ring);
   const int32_t* const table = p.tables + b * p.table_stride;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int32_t token = token0 + 32 * i + lane;
-    offset[i] = -1;
-    if (token >= low && token < length) {
-      const uint32_t index = p.cache.page_size.div(token), place = token - index * p.cache.page_size.d;
-      const int32_t page = load_arg(table + index);
-      if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.num_pages)) {
-        offset[i] = page * p.cache.page + place * p.cache.token + kv_head * p.cache.head;
-        if constexpr (kCodes) {
-          key_scale[i] = 64.0f * load_arg(p.cache.k_scale + page * p.cache.scale_page + place * p.cache.scale_token + kv_head * p.cache.scale_head);
-        }
-      } else if (p.status != nullptr) {
-        atomicOr(p.status, kStatusIndex);
-      }
-    }
-  }
-  float sum[kWeighRun / 16][2] = {};
-#pragma unroll 1
-  for (int32_t h0 = 0; h0 < p.group; h0 += 8) {
-    const int64_t head0 = static_cast<int64_t>(kv_head) * p.group + h0;
-    // Queries: head r8's, the lane's 8 dims of each 32.
-    uint4 qf[kChunks];
-    {
-      const bool there = h0 + r8 < p.group;
-      const __nv_bfloat16* const q = p.q + b * p.q_batch + (head0 + (there ? r8 : 0)) * p.q_head + 8 * q4;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) qf[c] = there ? load_once(q + 32 * c) : make_uint4(0, 0, 0, 0);
-    }
-    // Of the columns' heads, 2 q4 and the next: what the exponent starts from, and the slope.
-    float base[2], slope[2];
+
+  // The loads, ahead of the products.  Pages are looked up for 64 tokens, two to a lane, one run before they are needed.
+  int32_t page[2], place[2], ahead = first;
+  int64_t offset[2] = {-1, -1}, scale_offset[2] = {0, 0};
+  int load_stage = 0;
+  auto look_up = [&](int32_t token0) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool there = h0 + 2 * q4 + i < p.group;
-      const float lse = there ? load_arg(p.lse + static_cast<int64_t>(b) * p.heads + head0 + 2 * q4 + i) : -INFINITY;
-      base[i] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;  // (nothing was seen: no weight)
-      slope[i] = there && p.slopes != nullptr ? load_arg(p.slopes + head0 + 2 * q4 + i) * kLog2E : 0.0f;
-    }
-#pragma unroll
-    for (int step = 0; step < kWeighRun / 16; ++step) {
-      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      uint4 kf[2][kChunks];
-      float factor[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {  // tokens r8 and r8 + 8
-        const int from = (16 * step + 8 * i) % 32 + r8;
-        const int64_t o = __shfl_sync(0xffffffffu, offset[step / 2], from);
-        factor[i] = p.scale * (kCodes ? __shfl_sync(0xffffffffu, key_scale[step / 2], from) : 1.0f);
-        const uint8_t* const at = p.cache.k + (o < 0 ? 0 : o) + q4 * (kCodes ? 8 : 16);
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          if constexpr (kCodes) {
-            const uint2 v = o < 0 ? make_uint2(0x80808080u, 0x80808080u) : load_arg(reinterpret_cast<const uint2*>(at + 32 * c));
-            kf[i][c].x = v.x;
-            kf[i][c].y = v.y;
-          } else {
-            kf[i][c] = o < 0 ? make_uint4(0, 0, 0, 0) : load_once(at + 64 * c);
-          }
-        }
+      const int32_t token = token0 + 32 * i + lane;
+      place[i] = -1;
+      if (token >= low && token < length && token < last) {
+        const uint32_t index = p.cache.page_size.div(token);
+        place[i] = token - index * p.cache.page_size.d;
+        page[i] = load_arg(table + index);
       }
-      if constexpr (kCodes) {
+    }
+  };
+  auto load = [&]() {  // 16 tokens from `ahead`
+    if (ahead < last) {
+      const int step = (ahead - first) % kWeighRun / 16;
+      if (step == 0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            constexpr uint32_t kOffset = 0xC000C000u;  // -128 / 64, twice
-            const uint32_t x = kf[i][c].x, y = kf[i][c].y;
-            kf[i][c] = make_uint4(bf16x2_fma(__byte_perm(x, 0, 0x4140), kTwo127, kOffset), bf16x2_fma(__byte_perm(x, 0, 0x4342), kTwo127, kOffset),
-                                  bf16x2_fma(__byte_perm(y, 0, 0x4140), kTwo127, kOffset), bf16x2_fma(__byte_perm(y, 0, 0x4342), kTwo127, kOffset));
+          offset[i] = -1;
+          if (place[i] >= 0) {
+            if (static_cast<uint32_t>(page[i]) < static_cast<uint32_t>(p.cache.num_pages)) {
+              offset[i] = page[i] * p.cache.page + place[i] * p.cache.token + kv_head * p.cache.head;
+              if constexpr (kCodes) scale_offset[i] = page[i] * p.cache.scale_page + place[i] * p.cache.scale_token + kv_head * p.cache.scale_head;
+            } else if (p.status != nullptr) {
+              atomicOr(p.status, kStatusIndex);
+            }
           }
         }
+        look_up(ahead + kWeighRun);
       }
+      const int64_t from = step < 2 ? offset[0] : offset[1];
+      const uint32_t to = ring_at + load_stage * R::kStage;
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const uint32_t a0[4] = {kf[0][c].x, kf[1][c].x, kf[0][c].y, kf[1][c].y};
-        const uint32_t a1[4] = {kf[0][c].z, kf[1][c].z, kf[0][c].w, kf[1][c].w};
-        ptx::mma_m16n8k16(s, a0, qf[c].x, qf[c].y);
-        ptx::mma_m16n8k16(s, a1, qf[c].z, qf[c].w);
+      for (int i = 0; i < R::kPieces / 2; ++i) {
+        const int at = i * 32 + lane, of = at / R::kPieces, piece = at % R::kPieces;
+        const int64_t o = __shfl_sync(0xffffffffu, from, step % 2 * 16 + of);
+        ptx::cp_async_16(to + R::place(of, piece), p.cache.k + (o < 0 ? 0 : o + piece * 16), o >= 0);
+      }
+      if constexpr (kCodes) {
+        if (lane / 16 == step % 2) {
+          const int64_t o = step < 2 ? scale_offset[0] : scale_offset[1];
+          cp_async_4(to + 16 * R::kBytes + lane % 16 * 4, p.cache.k_scale + (from < 0 ? 0 : o), from >= 0);
+        }
+        __syncwarp();
+      }
+      load_stage = load_stage + 1 == R::kStages ? 0 : load_stage + 1;
+      ahead += 16;
+    }
+    ptx::cp_async_commit();
+  };
+  look_up(first);
+#pragma unroll
+  for (int i = 0; i < R::kStages - 1; ++i) load();
+
+  // Queries of the first eight heads (often all): head r8's.  Of the columns' heads, 2 q4 and the next: what the exponent
+  // starts from, and the slope.
+  const int64_t head0 = static_cast<int64_t>(kv_head) * p.group;
+  uint32_t qw[R::kWords];
+  float base[2], slope[2];
+  auto load_heads = [&](int32_t h0) {
+    const bool there = h0 + r8 < p.group;
+    const __nv_bfloat16* const q = p.q + b * p.q_batch + (head0 + h0 + (there ? r8 : 0)) * p.q_head;
+    constexpr int kStep = kCodes ? 8 : 4;  // words of a load
+#pragma unroll
+    for (int w = 0; w < R::kWords; w += 4) {
+      const int of = w / kStep;
+      const int dim = of < R::kLoads ? of * R::kLoadDims + q4 * (2 * kStep) + 2 * (w % kStep) : R::kLoads * R::kLoadDims + q4 * 8;
+      const uint4 v = there ? load_once(q + dim) : make_uint4(0, 0, 0, 0);
+      qw[w] = v.x, qw[w + 1] = v.y, qw[w + 2] = v.z, qw[w + 3] = v.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool here = h0 + 2 * q4 + i < p.group;
+      const float lse = here ? load_arg(p.lse + static_cast<int64_t>(b) * p.heads + head0 + h0 + 2 * q4 + i) : -INFINITY;
+      base[i] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;  // (nothing was seen: no weight)
+      slope[i] = here && p.slopes != nullptr ? load_arg(p.slopes + head0 + h0 + 2 * q4 + i) * kLog2E : 0.0f;
+    }
+  };
+  load_heads(0);
+
+  int stage = 0;
+#pragma unroll 1
+  for (int32_t token0 = first; token0 < last; token0 += 16) {
+    ptx::cp_async_wait_group<R::kStages - 2>();
+    __syncwarp();
+    load();
+    const uint8_t* const keys = ring + stage * R::kStage;
+    stage = stage + 1 == R::kStages ? 0 : stage + 1;
+    float factor[2] = {p.scale, p.scale};
+    if constexpr (kCodes) {
+      const float* const of_rows = reinterpret_cast<const float*>(keys + 16 * R::kBytes);
+      factor[0] *= 64.0f * of_rows[r8];
+      factor[1] *= 64.0f * of_rows[r8 + 8];
+    }
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+    for (int32_t h0 = 0; h0 < p.group; h0 += 8) {
+      if (p.group > 8) load_heads(h0);
+      // (four sums, so that a product does not wait for the one before it: one chain of sixteen took half of a step's time)
+      float s4[4][4] = {};
+      auto multiply = [&](uint32_t a, uint32_t b2, uint32_t c, uint32_t d, int word) {  // words of the two rows
+        const uint32_t fragment[4] = {a, b2, c, d};
+        ptx::mma_m16n8k16(s4[word / 2 % 4], fragment, qw[word], qw[word + 1]);
+      };
+      auto two = [](uint32_t four, uint32_t select) {  // codes as (code - 128) / 64
+        constexpr uint32_t kOffset = 0xC000C000u;
+        return bf16x2_fma(__byte_perm(four, 0, select), kTwo127, kOffset);
+      };
+#pragma unroll
+      for (int c = 0; c < R::kLoads + R::kRest; ++c) {
+        uint32_t a[4], b2[4];
+        if (c < R::kLoads) {
+          const uint4 x = *reinterpret_cast<const uint4*>(keys + R::place(r8, 4 * c + q4));
+          const uint4 y = *reinterpret_cast<const uint4*>(keys + R::place(r8 + 8, 4 * c + q4));
+          a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
+          b2[0] = y.x, b2[1] = y.y, b2[2] = y.z, b2[3] = y.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(keys + R::place(r8, 4 * c) + 8 * q4);
+          const uint2 y = *reinterpret_cast<const uint2*>(keys + R::place(r8 + 8, 4 * c) + 8 * q4);
+          a[0] = x.x, a[1] = x.y, b2[0] = y.x, b2[1] = y.y;
+        }
+        if constexpr (kCodes) {
+#pragma unroll
+          for (int i = 0; i < (c < R::kLoads ? 4 : 2); ++i) {
+            multiply(two(a[i], 0x4140), two(b2[i], 0x4140), two(a[i], 0x4342), two(b2[i], 0x4342), 8 * c + 2 * i);
+          }
+        } else {
+          multiply(a[0], b2[0], a[1], b2[1], 4 * c);
+          multiply(a[2], b2[2], a[3], b2[3], 4 * c + 2);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float behind = static_cast<float>(length - 1 - (token0 + 16 * step + 8 * i + r8));
-        float two = 0.0f;
+        const float behind = static_cast<float>(length - 1 - (token0 + 8 * i + r8));
+        float both = 0.0f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          float x = s[2 * i + k] * factor[i];
+          float x = ((s4[0][2 * i + k] + s4[1][2 * i + k]) + (s4[2][2 * i + k] + s4[3][2 * i + k])) * factor[i];
           if (p.cap > 0.0f) x = fmaf(-2.0f * p.cap, reciprocal_approx(exp2_approx(x * p.two_over_cap) + 1.0f), p.cap);
           x = fmaf(-slope[k], behind, x);
           const float weight = exp2_approx(x + base[k]);
-          two += base[k] == -INFINITY ? 0.0f : weight;
+          both += base[k] == -INFINITY ? 0.0f : weight;
         }
-        two += __shfl_xor_sync(0xffffffffu, two, 1);
-        two += __shfl_xor_sync(0xffffffffu, two, 2);
-        sum[step][i] += two;
+        both += __shfl_xor_sync(0xffffffffu, both, 1);
+        both += __shfl_xor_sync(0xffffffffu, both, 2);
+        sum[i] += both;
       }
     }
-  }
-#pragma unroll
-  for (int step = 0; step < kWeighRun / 16; ++step) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int32_t token = token0 + 16 * step + 8 * i + r8;
-      if (q4 != 0 || token >= p.width) continue;
+    // Lanes 4 r and 4 r + 1 write tokens r and r + 8.
+    const int32_t token = token0 + 8 * q4 + r8;
+    const float mine = q4 == 0 ? sum[0] : sum[1];
+    if (q4 < 2 && token < last) {
       const bool seen = token >= low && token < length;
       if (!p.add) {
-        row[token] = seen ? sum[step][i] : 0.0f;
+        row[token] = seen ? mine : 0.0f;
       } else if (seen) {
-        row[token] += sum[step][i];
+        row[token] += mine;
       }
     }
   }
 }
 
-using WeighKernel = void (*)(WeighParams);
+struct WeighKernel {
+  void (*kernel)(WeighParams);
+  int smem;
+};
+
+template <int kDim, bool kCodes>
+WeighKernel weigh_variant() { return {attention_weights_kernel<kDim, kCodes>, WeighRow<kDim, kCodes>::kSmem}; }
 
 template <bool kCodes>
 WeighKernel weigh_kernel(int64_t dim) {
   switch (dim) {
-    case 64: return attention_weights_kernel<64, kCodes>;
-    case 96: return attention_weights_kernel<96, kCodes>;
-    case 128: return attention_weights_kernel<128, kCodes>;
-    case 192: return attention_weights_kernel<192, kCodes>;
-    case 256: return attention_weights_kernel<256, kCodes>;
+    case 64: return weigh_variant<64, kCodes>();
+    case 96: return weigh_variant<96, kCodes>();
+    case 128: return weigh_variant<128, kCodes>();
+    case 192: return weigh_variant<192, kCodes>();
+    case 256: return weigh_variant<256, kCodes>();
   }
-  return nullptr;
+  return {nullptr, 0};
+}
+
+// Allows a kernel its shared memory, once per device.
+int allow_smem(const void* kernel, int smem, int device) {
+  static std::mutex mutex;
+  static std::set<std::pair<int, const void*>> done;
+  std::lock_guard<std::mutex> guard(mutex);
+  if (done.count({device, kernel}) != 0) return kOk;
+  CHORD_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  done.insert({device, kernel});
+  return kOk;
 }
 
 // ------------------------------------------------------------------ eviction --
@@ -491,10 +583,11 @@ int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
   CHORD_REQUIRE(scores->window >= 0 && scores->window < (1ll << 31), "window out of range");
   CHORD_REQUIRE(scores->scale - scores->scale == 0.0 && scores->cap >= 0.0 && scores->cap - scores->cap == 0.0, "scale and cap must be finite");
   const WeighKernel kernel = cache->k_scale != nullptr ? weigh_kernel<true>(cache->head_dim) : weigh_kernel<false>(cache->head_dim);
-  CHORD_REQUIRE(kernel != nullptr, "head_dim must be 64, 96, 128, 192 or 256, got %lld", static_cast<long long>(cache->head_dim));
+  CHORD_REQUIRE(kernel.kernel != nullptr, "head_dim must be 64, 96, 128, 192 or 256, got %lld", static_cast<long long>(cache->head_dim));
   DeviceInfo device;
   if (int rc = current_device_info(&device)) return rc;
   if (int rc = require_blackwell(device)) return rc;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel.kernel), kernel.smem, device.device)) return rc;
   const int64_t capacity = max_pages * cache->page_size;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_batch = q_batch;
@@ -517,8 +610,13 @@ int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
   p.width = static_cast<int32_t>(width);
   p.window = static_cast<int32_t>(scores->window);
   p.add = add;
-  const dim3 grid(static_cast<unsigned>((width + kWeighTokens - 1) / kWeighTokens), static_cast<unsigned>(cache->heads), static_cast<unsigned>(batch));
-  CHORD_CUDA(launch_kernel(kernel, grid, dim3(kWeighWarps * 32), 0, static_cast<cudaStream_t>(stream), kEarlyLaunch, p));
+  // Several runs for a warp where that leaves a few warps for each of those that are resident: what a warp begins with is paid once.
+  p.runs = 1;
+  const int64_t warps = (width + kWeighRun - 1) / kWeighRun * cache->heads * batch;
+  while (p.runs < 8 && warps / (2 * p.runs) >= device.sm_count * 16) p.runs *= 2;
+  const int64_t tokens = kWeighWarps * kWeighRun * p.runs;
+  const dim3 grid(static_cast<unsigned>((width + tokens - 1) / tokens), static_cast<unsigned>(cache->heads), static_cast<unsigned>(batch));
+  CHORD_CUDA(launch_kernel(kernel.kernel, grid, dim3(kWeighWarps * 32), static_cast<size_t>(kernel.smem), static_cast<cudaStream_t>(stream), kEarlyLaunch, p));
   return kOk;
 }
 
@@ -583,7 +681,7 @@ int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tabl
   const unsigned heads = static_cast<unsigned>(cache->heads), sequences = static_cast<unsigned>(batch);
   const int64_t most = width < p.capacity ? width : p.capacity;
   const size_t held = 4 * static_cast<size_t>(most < kSelectHeld ? most : kSelectHeld);
-  if (held > 32768) CHORD_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kSelectHeld));
+  if (int rc = allow_smem(reinterpret_cast<const void*>(evict_select_kernel), 4 * kSelectHeld, device.device)) return rc;
   CHORD_CUDA(launch_kernel(evict_select_kernel, dim3(heads, sequences), dim3(kSelectThreads), held, s, kEarlyLaunch, p));
   if (new_tables != nullptr) {
     const int rows = kCopyThreads / (p.row_bytes / 16);
