@@ -41,7 +41,8 @@ struct WeighParams {
   int32_t* status;
   float scale, cap, two_over_cap;  // as of paged_attention
   int32_t heads, group, capacity, width, window, add;
-  int32_t runs;  // of 64 tokens for a warp
+  int32_t runs;    // of 64 tokens for a warp
+  bool in_a_row;   // 16 tokens from a multiple of 16 lie one after another
 };
 
 constexpr int kWeighWarps = 4;
@@ -50,14 +51,15 @@ constexpr int kWeighRun = 64;  // tokens that a warp looks up at once
 // What a lane has of a row: words (two elements) in the order of its loads.  A product's sum does not depend on the order of
 // its terms, so a lane's words of a key and of a query, wherever they lie, stand for the columns that the instruction wants
 // there, as long as they are the same dims.  Loads are of 16 bytes, the last one of 8 where codes of 96 dims leave no more.
-// A warp has a ring of stages of 16 tokens, some 12 KB on their way or in use.
+// A warp has a ring of stages of 32 tokens, of wide rows 16, some 12 KB on their way or in use.
 template <int kDim, bool kCodes>
 struct WeighRow {
   static constexpr int kLoadDims = kCodes ? 64 : 32;  // of the four lanes of a row together
   static constexpr int kLoads = kDim / kLoadDims, kRest = kDim % kLoadDims / 32;
   static constexpr int kWords = kDim / 8;
   static constexpr int kBytes = kDim * (kCodes ? 1 : 2), kPieces = kBytes / 16;
-  static constexpr int kStage = 16 * kBytes + (kCodes ? 64 : 0);  // with the rows' scales
+  static constexpr int kGroups = kBytes <= 256 ? 2 : 1, kTokens = 16 * kGroups;
+  static constexpr int kStage = kTokens * kBytes + (kCodes ? kTokens * 4 : 0);  // with the rows' scales
   static constexpr int kStages = 12 * 1024 / kStage < 2 ? 2 : 12 * 1024 / kStage > 6 ? 6 : 12 * 1024 / kStage;
   static constexpr int kSmem = kWeighWarps * kStages * kStage;
   // Rows of a multiple of 128 bytes: the lanes of an odd one read the other half of the banks.
@@ -107,10 +109,10 @@ __global__ void __launch_bounds__(kWeighWarps * 32) attention_weights_kernel(con
       }
     }
   };
-  auto load = [&]() {  // 16 tokens from `ahead`
+  auto load = [&]() {  // a stage's tokens from `ahead`
     if (ahead < last) {
-      const int step = (ahead - first) % kWeighRun / 16;
-      if (step == 0) {
+      const int32_t inside = (ahead - first) % kWeighRun;
+      if (inside == 0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           offset[i] = -1;
@@ -125,23 +127,40 @@ __global__ void __launch_bounds__(kWeighWarps * 32) attention_weights_kernel(con
         }
         look_up(ahead + kWeighRun);
       }
-      const int64_t from = step < 2 ? offset[0] : offset[1];
+      // (a lane's token of the 32 that hold the stage's, and where these begin)
+      const int64_t from = inside < 32 ? offset[0] : offset[1];
+      const int32_t lane0 = R::kGroups == 2 ? 0 : inside % 32;
       const uint32_t to = ring_at + load_stage * R::kStage;
+      const uint32_t there = __ballot_sync(0xffffffffu, from >= 0);
 #pragma unroll
-      for (int i = 0; i < R::kPieces / 2; ++i) {
-        const int at = i * 32 + lane, of = at / R::kPieces, piece = at % R::kPieces;
-        const int64_t o = __shfl_sync(0xffffffffu, from, step % 2 * 16 + of);
-        ptx::cp_async_16(to + R::place(of, piece), p.cache.k + (o < 0 ? 0 : o + piece * 16), o >= 0);
+      for (int g = 0; g < R::kGroups; ++g) {
+        const int32_t lane_of = lane0 + 16 * g;
+        if (p.in_a_row && (there >> lane_of & 0xFFFFu) == 0xFFFFu) {
+          // all there, one after another: a third of the instructions
+          const uint8_t* const at0 = p.cache.k + __shfl_sync(0xffffffffu, from, lane_of) + lane * 16;
+#pragma unroll
+          for (int i = 0; i < R::kPieces / 2; ++i) {
+            const int at = i * 32 + lane;
+            ptx::cp_async_16(to + R::place(16 * g + at / R::kPieces, at % R::kPieces), at0 + i * 512, true);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < R::kPieces / 2; ++i) {
+            const int at = i * 32 + lane, of = at / R::kPieces, piece = at % R::kPieces;
+            const int64_t o = __shfl_sync(0xffffffffu, from, lane_of + of);
+            ptx::cp_async_16(to + R::place(16 * g + of, piece), p.cache.k + (o < 0 ? 0 : o + piece * 16), o >= 0);
+          }
+        }
       }
       if constexpr (kCodes) {
-        if (lane / 16 == step % 2) {
-          const int64_t o = step < 2 ? scale_offset[0] : scale_offset[1];
-          cp_async_4(to + 16 * R::kBytes + lane % 16 * 4, p.cache.k_scale + (from < 0 ? 0 : o), from >= 0);
+        if (lane >= lane0 && lane < lane0 + R::kTokens) {
+          const int64_t o = inside < 32 ? scale_offset[0] : scale_offset[1];
+          cp_async_4(to + R::kTokens * R::kBytes + (lane - lane0) * 4, p.cache.k_scale + (from < 0 ? 0 : o), from >= 0);
         }
         __syncwarp();
       }
       load_stage = load_stage + 1 == R::kStages ? 0 : load_stage + 1;
-      ahead += 16;
+      ahead += R::kTokens;
     }
     ptx::cp_async_commit();
   };
@@ -177,76 +196,103 @@ __global__ void __launch_bounds__(kWeighWarps * 32) attention_weights_kernel(con
 
   int stage = 0;
 #pragma unroll 1
-  for (int32_t token0 = first; token0 < last; token0 += 16) {
+  for (int32_t token0 = first; token0 < last; token0 += R::kTokens) {
     ptx::cp_async_wait_group<R::kStages - 2>();
     __syncwarp();
     load();
     const uint8_t* const keys = ring + stage * R::kStage;
     stage = stage + 1 == R::kStages ? 0 : stage + 1;
-    float factor[2] = {p.scale, p.scale};
-    if constexpr (kCodes) {
-      const float* const of_rows = reinterpret_cast<const float*>(keys + 16 * R::kBytes);
-      factor[0] *= 64.0f * of_rows[r8];
-      factor[1] *= 64.0f * of_rows[r8 + 8];
+    float factor[R::kGroups][2];  // a lane's tokens are r8 and r8 + 8 of each 16
+#pragma unroll
+    for (int g = 0; g < R::kGroups; ++g) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        factor[g][i] = p.scale;
+        if constexpr (kCodes) factor[g][i] *= 64.0f * reinterpret_cast<const float*>(keys + R::kTokens * R::kBytes)[16 * g + 8 * i + r8];
+      }
     }
-    float sum[2] = {0.0f, 0.0f};
+    float sum[R::kGroups][2] = {};
 #pragma unroll 1
     for (int32_t h0 = 0; h0 < p.group; h0 += 8) {
       if (p.group > 8) load_heads(h0);
-      // (four sums, so that a product does not wait for the one before it: one chain of sixteen took half of a step's time)
-      float s4[4][4] = {};
-      auto multiply = [&](uint32_t a, uint32_t b2, uint32_t c, uint32_t d, int word) {  // words of the two rows
-        const uint32_t fragment[4] = {a, b2, c, d};
-        ptx::mma_m16n8k16(s4[word / 2 % 4], fragment, qw[word], qw[word + 1]);
-      };
-      auto two = [](uint32_t four, uint32_t select) {  // codes as (code - 128) / 64
-        constexpr uint32_t kOffset = 0xC000C000u;
-        return bf16x2_fma(__byte_perm(four, 0, select), kTwo127, kOffset);
-      };
 #pragma unroll
-      for (int c = 0; c < R::kLoads + R::kRest; ++c) {
-        uint32_t a[4], b2[4];
-        if (c < R::kLoads) {
-          const uint4 x = *reinterpret_cast<const uint4*>(keys + R::place(r8, 4 * c + q4));
-          const uint4 y = *reinterpret_cast<const uint4*>(keys + R::place(r8 + 8, 4 * c + q4));
-          a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
-          b2[0] = y.x, b2[1] = y.y, b2[2] = y.z, b2[3] = y.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(keys + R::place(r8, 4 * c) + 8 * q4);
-          const uint2 y = *reinterpret_cast<const uint2*>(keys + R::place(r8 + 8, 4 * c) + 8 * q4);
-          a[0] = x.x, a[1] = x.y, b2[0] = y.x, b2[1] = y.y;
-        }
-        if constexpr (kCodes) {
+      for (int g = 0; g < R::kGroups; ++g) {
+        float s2[2][4] = {};  // (two sums, so that a product does not wait for the one before it)
+        auto multiply = [&](uint32_t a, uint32_t b2, uint32_t c, uint32_t d, int word) {  // words of the two rows
+          const uint32_t fragment[4] = {a, b2, c, d};
+          ptx::mma_m16n8k16(s2[word / 2 % 2], fragment, qw[word], qw[word + 1]);
+        };
+        auto two = [](uint32_t four, uint32_t select) {  // codes as (code - 128) / 64
+          constexpr uint32_t kOffset = 0xC000C000u;
+          return bf16x2_fma(__byte_perm(four, 0, select), kTwo127, kOffset);
+        };
 #pragma unroll
-          for (int i = 0; i < (c < R::kLoads ? 4 : 2); ++i) {
-            multiply(two(a[i], 0x4140), two(b2[i], 0x4140), two(a[i], 0x4342), two(b2[i], 0x4342), 8 * c + 2 * i);
+        for (int c = 0; c < R::kLoads + R::kRest; ++c) {
+          uint32_t a[4], b2[4];
+          if (c < R::kLoads) {
+            const uint4 x = *reinterpret_cast<const uint4*>(keys + R::place(16 * g + r8, 4 * c + q4));
+            const uint4 y = *reinterpret_cast<const uint4*>(keys + R::place(16 * g + r8 + 8, 4 * c + q4));
+            a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
+            b2[0] = y.x, b2[1] = y.y, b2[2] = y.z, b2[3] = y.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(keys + R::place(16 * g + r8, 4 * c) + 8 * q4);
+            const uint2 y = *reinterpret_cast<const uint2*>(keys + R::place(16 * g + r8 + 8, 4 * c) + 8 * q4);
+            a[0] = x.x, a[1] = x.y, b2[0] = y.x, b2[1] = y.y;
           }
-        } else {
-          multiply(a[0], b2[0], a[1], b2[1], 4 * c);
-          multiply(a[2], b2[2], a[3], b2[3], 4 * c + 2);
-        }
-      }
+          if constexpr (kCodes) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float behind = static_cast<float>(length - 1 - (token0 + 8 * i + r8));
-        float both = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float x = ((s4[0][2 * i + k] + s4[1][2 * i + k]) + (s4[2][2 * i + k] + s4[3][2 * i + k])) * factor[i];
-          if (p.cap > 0.0f) x = fmaf(-2.0f * p.cap, reciprocal_approx(exp2_approx(x * p.two_over_cap) + 1.0f), p.cap);
-          x = fmaf(-slope[k], behind, x);
-          const float weight = exp2_approx(x + base[k]);
-          both += base[k] == -INFINITY ? 0.0f : weight;
+            for (int i = 0; i < (c < R::kLoads ? 4 : 2); ++i) {
+              multiply(two(a[i], 0x4140), two(b2[i], 0x4140), two(a[i], 0x4342), two(b2[i], 0x4342), 8 * c + 2 * i);
+            }
+          } else {
+            multiply(a[0], b2[0], a[1], b2[1], 4 * c);
+            multiply(a[2], b2[2], a[3], b2[3], 4 * c + 2);
+          }
         }
-        both += __shfl_xor_sync(0xffffffffu, both, 1);
-        both += __shfl_xor_sync(0xffffffffu, both, 2);
-        sum[i] += both;
+        float x[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) x[i][k] = (s2[0][2 * i + k] + s2[1][2 * i + k]) * factor[g][i];
+        }
+        if (p.cap > 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i / 2][i % 2] = fmaf(-2.0f * p.cap, reciprocal_approx(exp2_approx(x[i / 2][i % 2] * p.two_over_cap) + 1.0f), p.cap);
+        }
+        if (p.slopes != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float behind = static_cast<float>(length - 1 - (token0 + 16 * g + 8 * i + r8));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) x[i][k] = fmaf(-slope[k], behind, x[i][k]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // (no weight where the head's sum is nothing, whatever the score)
+          const float first_of = exp2_approx(x[i][0] + base[0]), second = exp2_approx(x[i][1] + base[1]);
+          sum[g][i] += (base[0] == -INFINITY ? 0.0f : first_of) + (base[1] == -INFINITY ? 0.0f : second);
+        }
       }
     }
-    // Lanes 4 r and 4 r + 1 write tokens r and r + 8.
-    const int32_t token = token0 + 8 * q4 + r8;
-    const float mine = q4 == 0 ? sum[0] : sum[1];
-    if (q4 < 2 && token < last) {
+    // Over the four lanes of a row's heads: each ends with the sum of one of the row's tokens (of one group, two do).
+    float mine;
+    int32_t place_of;
+    if constexpr (R::kGroups == 2) {
+      const bool odd = q4 & 1, upper = q4 & 2;
+      const float a = odd ? sum[0][1] : sum[0][0], b2 = odd ? sum[1][1] : sum[1][0];
+      const float a2 = a + __shfl_xor_sync(0xffffffffu, odd ? sum[0][0] : sum[0][1], 1);
+      const float b3 = b2 + __shfl_xor_sync(0xffffffffu, odd ? sum[1][0] : sum[1][1], 1);
+      mine = (upper ? b3 : a2) + __shfl_xor_sync(0xffffffffu, upper ? a2 : b3, 2);
+      place_of = 16 * (q4 >> 1) + 8 * (q4 & 1) + r8;
+    } else {
+      const bool odd = q4 & 1;
+      mine = (odd ? sum[0][1] : sum[0][0]) + __shfl_xor_sync(0xffffffffu, odd ? sum[0][0] : sum[0][1], 1);
+      mine += __shfl_xor_sync(0xffffffffu, mine, 2);
+      place_of = 8 * (q4 & 1) + r8;
+    }
+    const int32_t token = token0 + place_of;
+    if (token < last && (R::kGroups == 2 || q4 < 2)) {
       const bool seen = token >= low && token < length;
       if (!p.add) {
         row[token] = seen ? mine : 0.0f;
@@ -611,6 +657,7 @@ int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
   p.window = static_cast<int32_t>(scores->window);
   p.add = add;
   // Several runs for a warp where that leaves a few warps for each of those that are resident: what a warp begins with is paid once.
+  p.in_a_row = cache->page_size % 16 == 0 && p.cache.token == cache->head_dim * (cache->k_scale != nullptr ? 1 : 2);
   p.runs = 1;
   const int64_t warps = (width + kWeighRun - 1) / kWeighRun * cache->heads * batch;
   while (p.runs < 8 && warps / (2 * p.runs) >= device.sm_count * 16) p.runs *= 2;
