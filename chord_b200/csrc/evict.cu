@@ -351,10 +351,9 @@ struct EvictParams {
   int32_t capacity, new_capacity, width, new_width, keep, first, recent, row_bytes;
 };
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectItems = 4;  // of a thread, one after another
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
-constexpr int32_t kSelectHeld = 40960;  // weights that are kept in shared memory between the passes
+constexpr int32_t kSelectHeld = 32768;  // weights that are kept in shared memory between the passes
 
 // Order of weights as that of whole numbers: zeros alike, NaN above all.
 __device__ __forceinline__ uint32_t rank_of(float w) {
@@ -364,13 +363,16 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 // One CTA for a sequence's key-value head: the smallest weight that is kept, found by its digits (11, 11 and 10 bits),
-// then the kept tokens in order.  Counts do not depend on the order in which they are counted.
+// then the kept tokens in order, a run of them for each warp: it counts, and writes when it knows what the warps before it
+// have.  Counts do not depend on the order in which they are counted.  Bounded by the latency of its steps: 128 CTAs of
+// 16384 weights RESULT_S.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
-  extern __shared__ uint32_t held[];  // the weights' ranks, where there is room
-  __shared__ uint32_t bins[kBins];
-  __shared__ uint32_t of_warps[2][kSelectThreads / 32];
-  __shared__ uint32_t found[2];
+  extern __shared__ float held[];  // the weights, where there is room
+  __shared__ uint32_t bins[3][kBins];
+  __shared__ uint32_t of_warps[2][kSelectWarps];
+  __shared__ uint32_t found[3][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < 3 * kBins; i += kSelectThreads) bins[0][i] = 0;
   ptx::grid_dependency_wait();
   const int32_t b = blockIdx.y, head = blockIdx.x;
   const int32_t given = load_arg(p.lengths + b), limit = min(p.capacity, p.width), length = max(0, min(given, limit));
@@ -383,117 +385,110 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   const int64_t row = static_cast<int64_t>(b) * gridDim.x + head;
   float* const out = p.new_weights + row * p.new_width;
   int32_t* const kept = p.kept + row * p.keep;
-  for (int32_t i = count + threadIdx.x; i < p.new_width; i += kSelectThreads) out[i] = 0.0f;
   if (length <= p.keep) {
-    for (int32_t i = threadIdx.x; i < count; i += kSelectThreads) {
-      kept[i] = i;
-      out[i] = load_arg(weights + i);
+    for (int32_t i = threadIdx.x; i < p.new_width; i += kSelectThreads) {
+      if (i < count) kept[i] = i;
+      out[i] = i < count ? load_arg(weights + i) : 0.0f;
     }
     return;
   }
+  const bool hold = length <= kSelectHeld;
+  auto weight_at = [&](int32_t i) { return hold ? held[i] : load_arg(weights + i); };
+  if (hold) {
+    constexpr int kAhead = 16;  // loads of a thread on their way (one after another: 11 of 26 us for 16384 weights)
+#pragma unroll 1
+    for (int32_t i0 = threadIdx.x; i0 < length; i0 += kAhead * kSelectThreads) {
+      float w[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) w[k] = i0 + k * kSelectThreads < length ? load_arg(weights + i0 + k * kSelectThreads) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (i0 + k * kSelectThreads < length) held[i0 + k * kSelectThreads] = w[k];
+      }
+    }
+  }
+  for (int32_t i = count + threadIdx.x; i < p.new_width; i += kSelectThreads) out[i] = 0.0f;
+  __syncthreads();
   const int32_t begin = p.first, end = length - p.recent;
   uint32_t wanted = p.keep - p.first - p.recent;  // of the tokens between
-  uint32_t prefix = 0, least = 0xFFFFFFFFu;
-  const bool hold = end - begin <= kSelectHeld;
-  auto rank_at = [&](int32_t i) { return hold ? held[i - begin] : rank_of(load_arg(weights + i)); };
-  if (hold && wanted > 0) {
-    for (int32_t i = begin + threadIdx.x; i < end; i += kSelectThreads) held[i - begin] = rank_of(load_arg(weights + i));
-  }
-  if (wanted > 0) {
-    int shift = 21;
-#pragma unroll 1
+  uint32_t least = 0xFFFFFFFFu;
+  const bool any = wanted > 0;  // else none of those between stays
+  if (any) {
+    uint32_t prefix = 0;
+#pragma unroll
     for (int digit = 0; digit < 3; ++digit) {
-      for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
-      __syncthreads();
+      constexpr int kShift[3] = {21, 10, 0};
+      const int shift = kShift[digit];
       const uint32_t mask = digit == 2 ? 0x3FFu : 0x7FFu;
-#pragma unroll 4
-      for (int32_t i0 = begin; i0 < end; i0 += kSelectThreads) {
-        const int32_t i = i0 + threadIdx.x;
-        const uint32_t rank = i < end ? rank_at(i) : 0;
-        const bool counts = i < end && (digit == 0 || rank >> (shift + (digit == 2 ? 10 : 11)) == prefix);
-        const uint32_t bin = rank >> shift & mask;
-        // (many equal ones, zeros as a rule, would wait for one another: the first lane's kind in one go)
-        const uint32_t some = __ballot_sync(0xffffffffu, counts);
-        if (some == 0) continue;
-        const int leader = __ffs(some) - 1;
-        const uint32_t its_bin = __shfl_sync(0xffffffffu, bin, leader);
-        const uint32_t same = __ballot_sync(0xffffffffu, counts && bin == its_bin);
-        if (lane == leader) {
-          atomicAdd(&bins[bin], static_cast<uint32_t>(__popc(same)));
-        } else if (counts && !(same >> lane & 1)) {
-          atomicAdd(&bins[bin], 1u);
-        }
+#pragma unroll 8
+      for (int32_t i = begin + threadIdx.x; i < end; i += kSelectThreads) {
+        const uint32_t rank = rank_of(weight_at(i));
+        if (digit == 0 || rank >> kShift[digit == 0 ? 0 : digit - 1] == prefix) atomicAdd(&bins[digit][rank >> shift & mask], 1u);
       }
       __syncthreads();
       // The bin in which the wanted-th largest lies: two bins to a thread, from the top.
       const int top = kBins - 1 - 2 * static_cast<int>(threadIdx.x);
-      const uint32_t high = bins[top], lower = bins[top - 1];
+      const uint32_t high = bins[digit][top], lower = bins[digit][top - 1];
       uint32_t upto = high + lower;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const uint32_t below = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += below;
       }
-      if (lane == 31) of_warps[0][warp] = upto;
+      if (lane == 31) of_warps[digit & 1][warp] = upto;
       __syncthreads();
-      uint32_t before = upto - high - lower;
-      for (int w = 0; w < warp; ++w) before += of_warps[0][w];
+      const uint32_t before = upto - high - lower + __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[digit & 1][lane] : 0);
       if (before < wanted && wanted <= before + high) {
-        found[0] = top;
-        found[1] = before;
+        found[digit][0] = top;
+        found[digit][1] = before;
       } else if (before + high < wanted && wanted <= before + high + lower) {
-        found[0] = top - 1;
-        found[1] = before + high;
+        found[digit][0] = top - 1;
+        found[digit][1] = before + high;
       }
       __syncthreads();
-      prefix = digit == 0 ? found[0] : prefix << (digit == 2 ? 10 : 11) | found[0];
-      wanted -= found[1];
-      shift = digit == 0 ? 10 : 0;
-      __syncthreads();
+      prefix = prefix << (digit == 2 ? 10 : 11) | found[digit][0];
+      wanted -= found[digit][1];
     }
     least = prefix;
   }
   // In order: `wanted` of those equal to the least, all above it.
-  uint32_t above = 0, level = 0;  // so far
-#pragma unroll 1
-  for (int32_t i0 = 0; i0 < length; i0 += kSelectThreads * kSelectItems) {
-    const int32_t mine = i0 + threadIdx.x * kSelectItems;
-    bool is_above[kSelectItems], is_level[kSelectItems];
-    uint32_t above_here = 0, level_here = 0;
-#pragma unroll
-    for (int k = 0; k < kSelectItems; ++k) {
-      const int32_t i = mine + k;
-      const bool between = i >= begin && i < end && i < length;
-      const uint32_t rank = between && p.keep > p.first + p.recent ? rank_at(i) : 0;
-      is_above[k] = i < length && (!between || (p.keep > p.first + p.recent && rank > least));
-      is_level[k] = between && p.keep > p.first + p.recent && rank == least;
-      above_here += is_above[k];
-      level_here += is_level[k];
+  const int32_t rows = (length + 32 * kSelectWarps - 1) / (32 * kSelectWarps);  // of 32 tokens, of a warp
+  const int32_t from = warp * rows * 32, to = min(length, from + rows * 32);
+  auto look = [&](int32_t i, uint32_t& above, uint32_t& level) {
+    const bool between = i >= begin && i < end;
+    const uint32_t rank = between && any && i < to ? rank_of(weight_at(i)) : 0;
+    above = __ballot_sync(0xffffffffu, i < to && (between ? any && rank > least : true));
+    level = __ballot_sync(0xffffffffu, i < to && between && any && rank == least);
+  };
+  // What the warp's first 32 rows are is kept, a row to a lane, for the second time through them.
+  uint32_t all_above = 0, all_level = 0, row_above = 0, row_level = 0;
+#pragma unroll 4
+  for (int32_t r = 0; r < rows; ++r) {
+    uint32_t above, level;
+    look(from + 32 * r + lane, above, level);
+    all_above += __popc(above);
+    all_level += __popc(level);
+    if (lane == r) row_above = above, row_level = level;
+  }
+  __syncthreads();  // (of_warps have been read)
+  if (lane == 0) of_warps[0][warp] = all_above, of_warps[1][warp] = all_level;
+  __syncthreads();
+  uint32_t above_before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[0][lane] : 0);
+  uint32_t level_before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[1][lane] : 0);
+  const uint32_t below_lane = (1u << lane) - 1;
+#pragma unroll 4
+  for (int32_t r = 0; r < rows; ++r) {
+    uint32_t above = __shfl_sync(0xffffffffu, row_above, r & 31), level = __shfl_sync(0xffffffffu, row_level, r & 31);
+    const int32_t i = from + 32 * r + lane;
+    if (r >= 32) look(i, above, level);
+    const uint32_t l = level_before + __popc(level & below_lane);
+    if ((above >> lane & 1) != 0 || ((level >> lane & 1) != 0 && l < wanted)) {
+      const uint32_t at = above_before + __popc(above & below_lane) + min(l, wanted);
+      kept[at] = i;
+      out[at] = weight_at(i);
     }
-    uint32_t a = above_here, l = level_here;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, l, d);
-      if (lane >= d) a += x, l += y;
-    }
-    __syncthreads();
-    if (lane == 31) of_warps[0][warp] = a, of_warps[1][warp] = l;
-    __syncthreads();
-    const uint32_t from_a = of_warps[0][lane], from_l = of_warps[1][lane];
-    uint32_t a_before = above + a - above_here + __reduce_add_sync(0xffffffffu, lane < warp ? from_a : 0);
-    uint32_t l_before = level + l - level_here + __reduce_add_sync(0xffffffffu, lane < warp ? from_l : 0);
-    above += __reduce_add_sync(0xffffffffu, from_a);
-    level += __reduce_add_sync(0xffffffffu, from_l);
-#pragma unroll
-    for (int k = 0; k < kSelectItems; ++k) {
-      if (is_above[k] || (is_level[k] && l_before < wanted)) {
-        const uint32_t at = a_before + min(l_before, wanted);
-        kept[at] = mine + k;
-        out[at] = load_arg(weights + mine + k);
-      }
-      a_before += is_above[k];
-      l_before += is_level[k];
-    }
+    above_before += __popc(above);
+    level_before += __popc(level);
   }
 }
 
