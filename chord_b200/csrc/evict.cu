@@ -353,8 +353,6 @@ struct EvictParams {
 
 constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
-constexpr int32_t kSelectHeld = 32768;  // weights that are kept in shared memory between the passes
-
 // Order of weights as that of whole numbers: zeros alike, NaN above all.
 __device__ __forceinline__ uint32_t rank_of(float w) {
   if (w != w) return 0xFFFFFFFFu;
@@ -362,14 +360,43 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// The wanted-th largest of the counted ranks by their next digit: two bins to a thread, from the top.  Takes off `wanted`
+// what lies in higher bins.
+__device__ __forceinline__ uint32_t find_bin(const uint32_t* bins, uint32_t* of_warps, uint32_t* found, uint32_t& wanted) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int top = kBins - 1 - 2 * static_cast<int>(threadIdx.x);
+  const uint32_t high = bins[top], lower = bins[top - 1];
+  uint32_t upto = high + lower;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t below = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += below;
+  }
+  if (lane == 31) of_warps[warp] = upto;
+  __syncthreads();
+  const uint32_t before = upto - high - lower + __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[lane] : 0);
+  if (before < wanted && wanted <= before + high) {
+    found[0] = top;
+    found[1] = before;
+  } else if (before + high < wanted && wanted <= before + high + lower) {
+    found[0] = top - 1;
+    found[1] = before + high;
+  }
+  __syncthreads();
+  wanted -= found[1];
+  return found[0];
+}
+
 // One CTA for a sequence's key-value head: the smallest weight that is kept, found by its digits (11, 11 and 10 bits),
-// then the kept tokens in order, a run of them for each warp: it counts, and writes when it knows what the warps before it
-// have.  Counts do not depend on the order in which they are counted.  Bounded by the latency of its steps: 128 CTAs of
-// 16384 weights RESULT_S.
+// then the kept tokens in order.  Counts do not depend on the order in which they are counted.  A thread has up to kItems
+// neighbours' weights in registers, which come coalesced, by way of shared memory; with kItems zero, for longer sequences,
+// they are read from memory each time and a warp has a run of them.  Bounded by the latency of its steps: 128 CTAs of 16384
+// weights RESULT_S (with the runs' ballots from shared memory 20).
+template <int kItems>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
-  extern __shared__ float held[];  // the weights, where there is room
+  extern __shared__ float held[];
   __shared__ uint32_t bins[3][kBins];
-  __shared__ uint32_t of_warps[2][kSelectWarps];
+  __shared__ uint32_t of_warps[3][kSelectWarps];
   __shared__ uint32_t found[3][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < 3 * kBins; i += kSelectThreads) bins[0][i] = 0;
@@ -392,10 +419,19 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     }
     return;
   }
-  const bool hold = length <= kSelectHeld;
-  auto weight_at = [&](int32_t i) { return hold ? held[i] : load_arg(weights + i); };
-  if (hold) {
-    constexpr int kAhead = 16;  // loads of a thread on their way (one after another: 11 of 26 us for 16384 weights)
+  const int32_t begin = p.first, end = length - p.recent;
+  const uint32_t between = end - begin;           // of these the largest
+  uint32_t wanted = p.keep - p.first - p.recent;  // are kept, so many
+  const bool any = wanted > 0;
+  constexpr int kShift[3] = {21, 10, 0};
+  auto digit_of = [&](uint32_t rank, int digit) { return rank >> kShift[digit] & (digit == 2 ? 0x3FFu : 0x7FFu); };
+  uint32_t prefix = 0;
+
+  if constexpr (kItems != 0) {
+    static_assert(kItems * kSelectThreads <= 65536, "places in 16 bits");
+    uint16_t* const places = reinterpret_cast<uint16_t*>(held + kItems * (kSelectThreads / 32 * 33));  // the kept ones'
+    auto padded = [](int32_t i) { return i + (i >> 5); };  // (threads with 8, 16 or 32 neighbours each share no bank)
+    constexpr int kAhead = kItems < 16 ? kItems : 16;      // loads of a thread on their way
 #pragma unroll 1
     for (int32_t i0 = threadIdx.x; i0 < length; i0 += kAhead * kSelectThreads) {
       float w[kAhead];
@@ -403,92 +439,125 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
       for (int k = 0; k < kAhead; ++k) w[k] = i0 + k * kSelectThreads < length ? load_arg(weights + i0 + k * kSelectThreads) : 0.0f;
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (i0 + k * kSelectThreads < length) held[i0 + k * kSelectThreads] = w[k];
+        if (i0 + k * kSelectThreads < length) held[padded(i0 + k * kSelectThreads)] = w[k];
       }
     }
-  }
-  for (int32_t i = count + threadIdx.x; i < p.new_width; i += kSelectThreads) out[i] = 0.0f;
-  __syncthreads();
-  const int32_t begin = p.first, end = length - p.recent;
-  uint32_t wanted = p.keep - p.first - p.recent;  // of the tokens between
-  uint32_t least = 0xFFFFFFFFu;
-  const bool any = wanted > 0;  // else none of those between stays
-  if (any) {
-    uint32_t prefix = 0;
+    for (int32_t i = count + threadIdx.x; i < p.new_width; i += kSelectThreads) out[i] = 0.0f;
+    __syncthreads();
+    const int32_t items = (length + kSelectThreads - 1) / kSelectThreads, mine = threadIdx.x * items;
+    uint32_t rank[kItems];
 #pragma unroll
-    for (int digit = 0; digit < 3; ++digit) {
-      constexpr int kShift[3] = {21, 10, 0};
-      const int shift = kShift[digit];
-      const uint32_t mask = digit == 2 ? 0x3FFu : 0x7FFu;
+    for (int k = 0; k < kItems; ++k) {
+      rank[k] = 0;
+      if (k < items && mine + k < length) rank[k] = rank_of(held[padded(mine + k)]);
+    }
+    // The thread's items as bits: those there are, and those of which the largest are kept.
+    auto bits_below = [&](int32_t i) {
+      const int32_t n = max(0, min(i - mine, items));
+      return n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1;
+    };
+    const uint32_t there = bits_below(length), inside = bits_below(end) & ~bits_below(begin);
+    if (any) {
+#pragma unroll
+      for (int digit = 0; digit < 3; ++digit) {
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+          if ((inside >> k & 1) != 0 && (digit == 0 || rank[k] >> kShift[digit == 0 ? 0 : digit - 1] == prefix)) {
+            atomicAdd(&bins[digit][digit_of(rank[k], digit)], 1u);
+          }
+        }
+        __syncthreads();
+        prefix = prefix << (digit == 2 ? 10 : 11) | find_bin(bins[digit], of_warps[digit], found[digit], wanted);
+      }
+    }
+    // In order: `wanted` of those equal to the least, all above it, the first and the recent ones.
+    uint32_t above = 0, level = 0;
+    if (any) {
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) {
+        above |= static_cast<uint32_t>(rank[k] > prefix) << k;
+        level |= static_cast<uint32_t>(rank[k] == prefix) << k;
+      }
+    }
+    above = (above & inside) | (there & ~inside);
+    level &= inside;
+    const uint32_t my_above = __popc(above), my_level = __popc(level);
+    uint32_t a = my_above, l = my_level;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, l, d);
+      if (lane >= d) a += x, l += y;
+    }
+    if (lane == 31) of_warps[0][warp] = a, of_warps[1][warp] = l;  // (last read before the barriers of the last digit)
+    __syncthreads();
+    a += __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[0][lane] : 0) - my_above;
+    l += __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[1][lane] : 0) - my_level;
+    // Of its equal ones the thread keeps the first, as many as those before it have left.
+    uint32_t more = l < wanted ? min(wanted - l, my_level) : 0, chosen = above;
+    for (; more != 0; --more) {
+      chosen |= level & -level;
+      level &= level - 1;
+    }
+    for (uint32_t at = a + min(l, wanted); chosen != 0; chosen &= chosen - 1) places[at++] = static_cast<uint16_t>(mine + __ffs(chosen) - 1);
+    // (by way of shared memory: threads' own stores, each to lines of its own, took a third of the time)
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < count; i += kSelectThreads) {
+      const int32_t place = places[i];
+      kept[i] = place;
+      out[i] = held[padded(place)];
+    }
+  } else {
+    for (int32_t i = count + threadIdx.x; i < p.new_width; i += kSelectThreads) out[i] = 0.0f;
+    __syncthreads();
+    if (any) {
+#pragma unroll
+      for (int digit = 0; digit < 3; ++digit) {
 #pragma unroll 8
-      for (int32_t i = begin + threadIdx.x; i < end; i += kSelectThreads) {
-        const uint32_t rank = rank_of(weight_at(i));
-        if (digit == 0 || rank >> kShift[digit == 0 ? 0 : digit - 1] == prefix) atomicAdd(&bins[digit][rank >> shift & mask], 1u);
+        for (int32_t i = begin + threadIdx.x; i < end; i += kSelectThreads) {
+          const uint32_t rank = rank_of(load_arg(weights + i));
+          if (digit == 0 || rank >> kShift[digit == 0 ? 0 : digit - 1] == prefix) atomicAdd(&bins[digit][digit_of(rank, digit)], 1u);
+        }
+        __syncthreads();
+        prefix = prefix << (digit == 2 ? 10 : 11) | find_bin(bins[digit], of_warps[digit], found[digit], wanted);
       }
-      __syncthreads();
-      // The bin in which the wanted-th largest lies: two bins to a thread, from the top.
-      const int top = kBins - 1 - 2 * static_cast<int>(threadIdx.x);
-      const uint32_t high = bins[digit][top], lower = bins[digit][top - 1];
-      uint32_t upto = high + lower;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t below = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += below;
-      }
-      if (lane == 31) of_warps[digit & 1][warp] = upto;
-      __syncthreads();
-      const uint32_t before = upto - high - lower + __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[digit & 1][lane] : 0);
-      if (before < wanted && wanted <= before + high) {
-        found[digit][0] = top;
-        found[digit][1] = before;
-      } else if (before + high < wanted && wanted <= before + high + lower) {
-        found[digit][0] = top - 1;
-        found[digit][1] = before + high;
-      }
-      __syncthreads();
-      prefix = prefix << (digit == 2 ? 10 : 11) | found[digit][0];
-      wanted -= found[digit][1];
     }
-    least = prefix;
-  }
-  // In order: `wanted` of those equal to the least, all above it.
-  const int32_t rows = (length + 32 * kSelectWarps - 1) / (32 * kSelectWarps);  // of 32 tokens, of a warp
-  const int32_t from = warp * rows * 32, to = min(length, from + rows * 32);
-  auto look = [&](int32_t i, uint32_t& above, uint32_t& level) {
-    const bool between = i >= begin && i < end;
-    const uint32_t rank = between && any && i < to ? rank_of(weight_at(i)) : 0;
-    above = __ballot_sync(0xffffffffu, i < to && (between ? any && rank > least : true));
-    level = __ballot_sync(0xffffffffu, i < to && between && any && rank == least);
-  };
-  // What the warp's first 32 rows are is kept, a row to a lane, for the second time through them.
-  uint32_t all_above = 0, all_level = 0, row_above = 0, row_level = 0;
+    const int32_t rows = (length + 32 * kSelectWarps - 1) / (32 * kSelectWarps);  // of 32 tokens, of a warp
+    const int32_t from = warp * rows * 32, to = min(length, from + rows * 32);
+    auto look = [&](int32_t i, float w, uint32_t& above, uint32_t& level) {
+      const bool inside = static_cast<uint32_t>(i - begin) < between;
+      const uint32_t rank = rank_of(w);
+      above = __ballot_sync(0xffffffffu, i < to && (!inside || (any && rank > prefix)));
+      level = __ballot_sync(0xffffffffu, i < to && inside && any && rank == prefix);
+    };
+    uint32_t all_above = 0, all_level = 0;
 #pragma unroll 4
-  for (int32_t r = 0; r < rows; ++r) {
-    uint32_t above, level;
-    look(from + 32 * r + lane, above, level);
-    all_above += __popc(above);
-    all_level += __popc(level);
-    if (lane == r) row_above = above, row_level = level;
-  }
-  __syncthreads();  // (of_warps have been read)
-  if (lane == 0) of_warps[0][warp] = all_above, of_warps[1][warp] = all_level;
-  __syncthreads();
-  uint32_t above_before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[0][lane] : 0);
-  uint32_t level_before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[1][lane] : 0);
-  const uint32_t below_lane = (1u << lane) - 1;
-#pragma unroll 4
-  for (int32_t r = 0; r < rows; ++r) {
-    uint32_t above = __shfl_sync(0xffffffffu, row_above, r & 31), level = __shfl_sync(0xffffffffu, row_level, r & 31);
-    const int32_t i = from + 32 * r + lane;
-    if (r >= 32) look(i, above, level);
-    const uint32_t l = level_before + __popc(level & below_lane);
-    if ((above >> lane & 1) != 0 || ((level >> lane & 1) != 0 && l < wanted)) {
-      const uint32_t at = above_before + __popc(above & below_lane) + min(l, wanted);
-      kept[at] = i;
-      out[at] = weight_at(i);
+    for (int32_t r = 0; r < rows; ++r) {
+      const int32_t i = from + 32 * r + lane;
+      uint32_t above, level;
+      look(i, i < to ? load_arg(weights + i) : 0.0f, above, level);
+      all_above += __popc(above);
+      all_level += __popc(level);
     }
-    above_before += __popc(above);
-    level_before += __popc(level);
+    if (lane == 0) of_warps[0][warp] = all_above, of_warps[1][warp] = all_level;
+    __syncthreads();
+    uint32_t above_before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[0][lane] : 0);
+    uint32_t level_before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[1][lane] : 0);
+    const uint32_t below_lane = (1u << lane) - 1;
+#pragma unroll 4
+    for (int32_t r = 0; r < rows; ++r) {
+      const int32_t i = from + 32 * r + lane;
+      const float w = i < to ? load_arg(weights + i) : 0.0f;
+      uint32_t above, level;
+      look(i, w, above, level);
+      const uint32_t l = level_before + __popc(level & below_lane);
+      if ((above >> lane & 1) != 0 || ((level >> lane & 1) != 0 && l < wanted)) {
+        const uint32_t at = above_before + __popc(above & below_lane) + min(l, wanted);
+        kept[at] = i;
+        out[at] = w;
+      }
+      above_before += __popc(above);
+      level_before += __popc(level);
+    }
   }
 }
 
@@ -722,9 +791,15 @@ int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tabl
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned heads = static_cast<unsigned>(cache->heads), sequences = static_cast<unsigned>(batch);
   const int64_t most = width < p.capacity ? width : p.capacity;
-  const size_t held = 4 * static_cast<size_t>(most < kSelectHeld ? most : kSelectHeld);
-  if (int rc = allow_smem(reinterpret_cast<const void*>(evict_select_kernel), 4 * kSelectHeld, device.device)) return rc;
-  CHORD_CUDA(launch_kernel(evict_select_kernel, dim3(heads, sequences), dim3(kSelectThreads), held, s, kEarlyLaunch, p));
+  const auto select = [&](void (*kernel)(EvictParams), int items) {
+    const int held = items * (kSelectThreads / 32 * 33 * 4 + kSelectThreads * 2);
+    if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), held, device.device)) return rc;
+    CHORD_CUDA(launch_kernel(kernel, dim3(heads, sequences), dim3(kSelectThreads), static_cast<size_t>(held), s, kEarlyLaunch, p));
+    return static_cast<int>(kOk);
+  };
+  const int rc = most <= 2 * kSelectThreads ? select(evict_select_kernel<2>, 2) : most <= 8 * kSelectThreads ? select(evict_select_kernel<8>, 8) :
+                 most <= 16 * kSelectThreads ? select(evict_select_kernel<16>, 16) : most <= 32 * kSelectThreads ? select(evict_select_kernel<32>, 32) : select(evict_select_kernel<0>, 0);
+  if (rc) return rc;
   if (new_tables != nullptr) {
     const int rows = kCopyThreads / (p.row_bytes / 16);
     const int64_t rounds = (keep + rows - 1) / rows;
