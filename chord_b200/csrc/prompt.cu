@@ -174,7 +174,7 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
   constexpr double kLog2E = 1.4426950408889634074;
   p.scale = static_cast<float>(c.scores->scale * kLog2E);
   p.cap = static_cast<float>(c.scores->cap * kLog2E);
-  p.cap_scale = c.scores->cap > 0.0 ? static_cast<float>(2.0 * kLog2E * c.scores->scale / c.scores->cap) : 0.0f;
+  p.cap_scale = c.scores->cap > 0.0 ? static_cast<float>(c.scores->scale / c.scores->cap) : 0.0f;
   p.batch = static_cast<int32_t>(c.batch);
   p.tokens = static_cast<int32_t>(c.tokens);
   p.heads = static_cast<int32_t>(c.heads);

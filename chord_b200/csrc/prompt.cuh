@@ -38,12 +38,13 @@ struct PromptLayout {
   static constexpr int kSlotBytes = kBlocks * kN * 128;  // keys or values of a step
   static constexpr int kRaw = kCodes ? 3 : 0;            // codes on their way
   static constexpr int kRawBytes = kN * kDim;
-  static constexpr int kScaleBytes = kCodes ? 2 * kN * 4 : 0;
+  static constexpr int kScales = kCodes ? 4 : 0;         // steps whose codes' scales are held
+  static constexpr int kScaleBytes = 2 * kN * 4;
   static constexpr int kMaxBytes = 2 * 2 * kPromptTile * 4;
   static constexpr int kControl = 1024;
-  static constexpr int kFit = (232448 - kControl - kMaxBytes - kQBytes - kRaw * kRawBytes) / (kSlotBytes + kScaleBytes);
+  static constexpr int kFit = (232448 - kControl - kMaxBytes - kQBytes - kRaw * kRawBytes - kScales * kScaleBytes) / kSlotBytes;
   static constexpr int kRing = kFit > 8 ? 8 : kFit;
-  static constexpr int kSmem = kQBytes + kRing * (kSlotBytes + kScaleBytes) + kRaw * kRawBytes + kMaxBytes + kControl;
+  static constexpr int kSmem = kQBytes + kRing * kSlotBytes + kRaw * kRawBytes + kScales * kScaleBytes + kMaxBytes + kControl;
   static constexpr uint32_t kOutColumn = kTwo ? 256 : 128;  // of tensor memory; the scores' buffers come first
   static_assert(kTiles * kPromptTile == (kTwo ? 256 : 128) && kN == (kTwo ? 128 : 64), "the plan's logarithms");
   static_assert(kRing >= 3, "keys of one step and values of the one before, and one on its way");
@@ -87,6 +88,20 @@ __device__ __forceinline__ void add_pair(float (&sum)[2], float x, float y) {
       : "f"(x), "f"(y));
 }
 
+// cap tanh(x) and cap tanh(y) for |x|, |y| up to kTanhBound, by an odd polynomial with coefficients fitted to the least
+// largest error there: off by 9e-8 of the cap, FP32's roundings in it.  (By 1 - 2 / (e^2x + 1), good everywhere, two of the three
+// operations per score of the 4-lane unit are the cap's.)
+constexpr float kTanhBound = 0.75f;
+__device__ __forceinline__ void capped_pair(float& x, float& y, float cap) {
+  asm("{\n .reg .b64 t, w, p, c;\n mov.b64 t, {%0, %1};\n mul.rn.f32x2 w, t, t;\n"
+      " mov.b64 p, {%8, %8};\n mov.b64 c, {%7, %7};\n fma.rn.f32x2 p, p, w, c;\n mov.b64 c, {%6, %6};\n fma.rn.f32x2 p, p, w, c;\n"
+      " mov.b64 c, {%5, %5};\n fma.rn.f32x2 p, p, w, c;\n mov.b64 c, {%4, %4};\n fma.rn.f32x2 p, p, w, c;\n"
+      " mov.b64 c, {%3, %3};\n fma.rn.f32x2 p, p, w, c;\n mul.rn.f32x2 p, p, t;\n mov.b64 c, {%2, %2};\n mul.rn.f32x2 p, p, c;\n"
+      " mov.b64 {%0, %1}, p;\n}"
+      : "+f"(x), "+f"(y)
+      : "f"(cap), "f"(0.99999983f), "f"(-0.33332471f), "f"(0.13320579f), "f"(-0.05314925f), "f"(0.01923722f), "f"(-0.00449344f));
+}
+
 // A warp's walk over its CTA's steps.
 struct PromptWalk {
   int64_t left;
@@ -122,6 +137,7 @@ struct __align__(16) PromptControl {
   uint64_t kv_full[8], kv_empty[8];  // by slot
   uint64_t looked[8];                // by the values' turn: there are no more than four of them in the ring
   uint64_t raw_full[4], raw_empty[4];
+  uint64_t scales_empty[4];          // (they are there when the step has been looked at)
   uint64_t s_full[2], p_full[2][2];  // p_full: [half of the tokens][buffer]
   uint64_t o_done[2];                // by tile; of one tile's products, two in turn
   uint32_t odd[8];   // as looked, the values in turn: number of the values in which infinities or NaN were found, and one
@@ -309,7 +325,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
   uint8_t* const q_tile = smem;
   uint8_t* const slots = smem + L::kQBytes;
   uint8_t* const raw = slots + kRing * L::kSlotBytes;  // [kRaw][token][dim] codes
-  float* const scales = reinterpret_cast<float*>(raw + L::kRaw * L::kRawBytes);  // [slot of values][of keys, of values][kN]
+  float* const scales = reinterpret_cast<float*>(raw + L::kRaw * L::kRawBytes);  // [step][of keys, of values][kN]
   float* const maxima = reinterpret_cast<float*>(smem + L::kSmem - L::kControl - L::kMaxBytes);  // [tile or parity][half][row]
   PromptControl& c = *reinterpret_cast<PromptControl*>(smem + L::kSmem - L::kControl);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -344,6 +360,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     for (int i = 0; i < 4; ++i) {
       ptx::mbar_init(bar(c.raw_full[i]), 1);
       ptx::mbar_init(bar(c.raw_empty[i]), kTurnWarps);
+      ptx::mbar_init(bar(c.scales_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(bar(c.item_full[i]), 1);
@@ -618,6 +635,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
         }
         if (bad != 0) break;
         free_slot(v);
+        if (kCodes && leader) ptx::mma_commit(bar(c.scales_empty[v / 2 % 4]));
         if (more) free_slot(k);
         if (j + 2 == n && leader) ptx::mma_commit(bar(c.q_empty));
       }
@@ -633,10 +651,10 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     ptx::mbar_drain(bar(c.drained), 0);
     if (bad != 0 && lane == 0 && p.status != nullptr) atomicOr(p.status, kPromptIssueTimeout);
   } else if (warp >= kLookWarp && warp < kLookWarp + kLookWarps) {
-    // ---- queries that TMA does not load, and values that some rows do not see ----
+    // ---- queries that TMA does not load, and values that some rows do not see or, of codes, the scales ----
     // Zero times an infinity or a NaN would be a NaN for those rows too.  What no row of the item sees (rows of a box
     // outside its tokens) is set to zero; where something is left, the rows make the product themselves.  (Codes are
-    // finite.)
+    // finite.  Their scales come here and not with the codes, so that a step's weights need not wait for its values.)
     const int w = warp - kLookWarp;
     uint32_t taken = 0, q_phase = 0;
     PromptWalk walk(c.start, c.plan_items);
@@ -704,6 +722,53 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
           if (any && lane == 0) *const_cast<volatile uint32_t*>(&c.odd[turn]) = number + 1;
           publish(bar(c.looked[turn]));
         }
+      } else {
+        const int32_t* const table = p.tables + it.b * p.table_stride;
+        constexpr int kEach = kN / kLookWarps / 32;
+        int32_t page[kEach], place[kEach];
+        auto look_up = [&](int32_t j) {
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            const int32_t token = token0 + j * kN + (w * kEach + e) * 32 + lane;
+            place[e] = -1;
+            if (j < n && token >= it.lo && token < it.hi) {
+              const uint32_t index = p.cache.page_size.div(token);
+              place[e] = token - index * p.cache.page_size.d;
+              page[e] = load_arg(table + index);
+            }
+          }
+        };
+        look_up(0);
+#pragma unroll 1
+        for (int32_t j = 0; j < n; ++j) {
+          float of_key[kEach], of_value[kEach];
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            of_key[e] = of_value[e] = 0.0f;
+            if (place[e] < 0) continue;
+            if (static_cast<uint32_t>(page[e]) < static_cast<uint32_t>(p.cache.num_pages)) {
+              const int64_t at = page[e] * p.cache.scale_page + place[e] * p.cache.scale_token + walk.head * p.cache.scale_head;
+              of_key[e] = load_arg(p.cache.k_scale + at);
+              of_value[e] = load_arg(p.cache.v_scale + at);
+            } else if (p.status != nullptr) {
+              atomicOr(p.status, kStatusIndex);
+            }
+          }
+          look_up(j + 1);
+          const uint32_t step = taken / 2 + j;
+          float* const to = scales + step % 4 * (2 * kN) + w * (32 * kEach) + lane;
+          wait(bar(c.scales_empty[step % 4]), (step / 4 & 1) ^ 1);
+          if (bad != 0) break;
+          // scores times 64 (the keys' unit), the row's scale and what makes them logarithms to base 2 or fractions of the cap
+          const float to_score = 64.0f * (kBent && p.cap > 0.0f ? p.cap_scale : p.scale);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            to[32 * e] = of_key[e] * to_score;
+            to[kN + 32 * e] = of_value[e];
+          }
+          __syncwarp();
+          ptx::mbar_arrive_lane0(bar(c.looked[step % 8]), lane);
+        }
       }
       taken += 2 * n;
       walk.next(n);
@@ -722,75 +787,60 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
         if (bad != 0) break;
         const int32_t n = walk.here(it);
         const int32_t* const table = p.tables + it.b * p.table_stride;
-        const int32_t token0 = (it.lo / kN + walk.step) * kN, mine = w * kOwn + lane % kOwn;  // the token that the lane looks up
-        int32_t page = 0, place = -1;
-        auto look_up = [&](int32_t j) {
-          const int32_t token = token0 + j * kN + mine;
-          place = -1;
-          if (j < n && token >= it.lo && token < it.hi) {
-            const uint32_t index = p.cache.page_size.div(token);
-            place = token - index * p.cache.page_size.d;
-            page = load_arg(table + index);
-          }
-        };
+        const int32_t token0 = (it.lo / kN + walk.step) * kN;
         // Turns the warp's tokens' codes into a slot: from the ring of codes or, where boxes do not fit, from memory.
         auto turn = [&](const uint8_t* from, int64_t offset) {
           uint8_t* const to = slots + slot * L::kSlotBytes;
-          const uint8_t* const here = raw + raw_slot * L::kRawBytes + w * kOwn * kDim;
-          constexpr int kRounds = kOwn * kPieces / 32, kAtOnce = kRounds % 4 == 0 ? 4 : kRounds % 3 == 0 ? 3 : 2;
-          static_assert(kRounds % kAtOnce == 0, "whole batches");
+          constexpr int kRounds = kOwn * kPieces / 32;
+          auto put = [&](int at, const uint4& held) {
+            const int token = w * kOwn + at / kPieces, piece = at % kPieces;
+            uint4 low, high;
+            decode16(held, low, high);
+            // (lanes that write to the same 16 bytes of two blocks of 64 elements would share banks: odd blocks' second half first)
+            const int swap = piece >> 2 & 1;
+            *reinterpret_cast<uint4*>(to + place_of(token, 2 * piece + swap)) = swap ? high : low;
+            *reinterpret_cast<uint4*>(to + place_of(token, 2 * piece + 1 - swap)) = swap ? low : high;
+          };
+          if (from == nullptr) {
+            const uint8_t* const here = raw + raw_slot * L::kRawBytes + w * kOwn * kDim + lane * 16;
+            constexpr int kAtOnce = kRounds % 4 == 0 ? 4 : kRounds % 3 == 0 ? 3 : 2;  // (all at once, they were spilled: 2.6 ms for 2.1)
+            static_assert(kRounds % kAtOnce == 0, "whole batches");
 #pragma unroll 1
-          for (int i0 = 0; i0 < kRounds; i0 += kAtOnce) {
-            uint4 held[kAtOnce];
+            for (int i0 = 0; i0 < kRounds; i0 += kAtOnce) {
+              uint4 held[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-              const int at = (i0 + i) * 32 + lane, token = at / kPieces, piece = at % kPieces;
-              if (from == nullptr) {
-                held[i] = *reinterpret_cast<const uint4*>(here + at * 16);
-              } else {
-                const int64_t o = __shfl_sync(0xffffffffu, offset, token);
-                held[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (o >= 0) held[i] = load_once(from + o + piece * 16);
-              }
-            }
+              for (int i = 0; i < kAtOnce; ++i) held[i] = *reinterpret_cast<const uint4*>(here + (i0 + i) * 512);
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-              const int at = (i0 + i) * 32 + lane, token = w * kOwn + at / kPieces, piece = at % kPieces;
-              uint4 low, high;
-              decode16(held[i], low, high);
-              // (lanes that write to the same 16 bytes of two blocks of 64 elements would share banks: odd blocks' second half first)
-              const int swap = piece >> 2 & 1;
-              *reinterpret_cast<uint4*>(to + place_of(token, 2 * piece + swap)) = swap ? high : low;
-              *reinterpret_cast<uint4*>(to + place_of(token, 2 * piece + 1 - swap)) = swap ? low : high;
+              for (int i = 0; i < kAtOnce; ++i) put((i0 + i) * 32 + lane, held[i]);
             }
+            return;
+          }
+#pragma unroll 2
+          for (int i = 0; i < kRounds; ++i) {
+            const int at = i * 32 + lane;
+            const int64_t o = __shfl_sync(0xffffffffu, offset, at / kPieces);
+            put(at, o >= 0 ? load_once(from + o + at % kPieces * 16) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u));
           }
         };
-        look_up(0);
 #pragma unroll 1
         for (int32_t j = 0; j < n && bad == 0; ++j) {
-          const bool there = place >= 0 && static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.num_pages);
-          if (place >= 0 && !there && p.status != nullptr) atomicOr(p.status, kStatusIndex);
-          int64_t offset = -1;
-          float key_scale = 0.0f, value_scale = 0.0f;
-          if (there) {
-            offset = page * p.cache.page + place * p.cache.token + walk.head * p.cache.head;
-            const int64_t at = page * p.cache.scale_page + place * p.cache.scale_token + walk.head * p.cache.scale_head;
-            key_scale = load_arg(p.cache.k_scale + at);
-            value_scale = load_arg(p.cache.v_scale + at);
+          int64_t offset = -1;  // of the token that the lane looks up (the scales' warps report pages that are not there)
+          if (p.box == 0) {
+            const int32_t token = token0 + j * kN + w * kOwn + lane % kOwn;
+            if (token >= it.lo && token < it.hi) {
+              const uint32_t index = p.cache.page_size.div(token);
+              const int32_t page = load_arg(table + index);
+              if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.cache.num_pages)) {
+                offset = page * p.cache.page + (token - index * p.cache.page_size.d) * p.cache.token + walk.head * p.cache.head;
+              }
+            }
           }
-          look_up(j + 1);
 #pragma unroll 1
           for (int which = 0; which < 2; ++which) {
             if (p.box != 0) wait(bar(c.raw_full[raw_slot]), raw_phase);
             wait(bar(c.kv_empty[slot]), slot_phase ^ 1);
             if (bad != 0) break;
             turn(p.box != 0 ? nullptr : which == 0 ? p.cache.k : p.cache.v, offset);
-            if (which == 1 && lane < kOwn) {
-              // scores times 64 (the keys' unit), the row's scale and what makes them logarithms to base 2 or the
-              // argument of the cap's exponential
-              scales[slot * 2 * kN + mine] = key_scale * (64.0f * (kBent && p.cap > 0.0f ? p.cap_scale : p.scale));
-              scales[slot * 2 * kN + kN + mine] = value_scale;
-            }
             publish(bar(c.kv_full[slot]));
             if (p.box != 0) {
               ptx::mbar_arrive_lane0(bar(c.raw_empty[raw_slot]), lane);
@@ -857,10 +907,8 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
           const uint32_t v_number = taken + 2 * j + 1, v_slot = v_number % kRing;
           const bool partial = any_masked(it, first);
           bool odd = false;
-          if constexpr (kCodes) {
-            wait(bar(c.kv_full[v_slot]), v_number / kRing & 1);  // the scales lie there
-          } else if (partial) {
-            wait(bar(c.looked[v_number / 2 % 8]), v_number / 16 & 1);
+          if (kCodes || partial) wait(bar(c.looked[v_number / 2 % 8]), v_number / 16 & 1);
+          if (!kCodes && partial) {
             odd = *const_cast<volatile uint32_t*>(&c.odd[v_number / 2 % 8]) == v_number + 1;
           }
           wait(bar(c.s_full[buffer]), s_phase >> buffer & 1);
@@ -877,7 +925,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
             ptx::tmem_ld_32x32b_x32(s_at + 32 * chunk, bits);
             ptx::tmem_wait_ld();
             if constexpr (kCodes) {
-              const float4* const factor = reinterpret_cast<const float4*>(scales + v_slot * 2 * kN + half * kHalf + 32 * chunk);
+              const float4* const factor = reinterpret_cast<const float4*>(scales + v_number / 2 % 4 * (2 * kN) + half * kHalf + 32 * chunk);
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const float4 f = factor[i / 4];
@@ -886,9 +934,20 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
             }
             if constexpr (kBent) {
               if (p.cap > 0.0f) {
-                const float factor = kCodes ? 1.0f : p.cap_scale, twice = -2.0f * p.cap;
+                float most = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = fmaf(twice, reciprocal_fast(exp2_fast(x[i] * factor) + 1.0f), p.cap);
+                for (int i = 0; i < 32; i += 2) {
+                  if constexpr (!kCodes) x[i] *= p.cap_scale, x[i + 1] *= p.cap_scale;
+                  most = max3(most, fabsf(x[i]), fabsf(x[i + 1]));
+                }
+                if (__any_sync(0xffffffffu, most > kTanhBound)) {
+                  const float twice = -2.0f * p.cap;
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) x[i] = fmaf(twice, reciprocal_fast(exp2_fast(x[i] * 2.8853900817779268f) + 1.0f), p.cap);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 32; i += 2) capped_pair(x[i], x[i + 1], p.cap);
+                }
               } else if constexpr (!kCodes) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] *= p.scale;
@@ -976,7 +1035,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
               ptx::tmem_ld_32x32b_x32(s_at + 32 * chunk, bits);
               ptx::tmem_wait_ld();
             }
-            const float4* const value_factor = reinterpret_cast<const float4*>(scales + v_slot * 2 * kN + kN + half * kHalf + 32 * chunk);
+            const float4* const value_factor = reinterpret_cast<const float4*>(scales + v_number / 2 % 4 * (2 * kN) + kN + half * kHalf + 32 * chunk);
             uint32_t w[16];
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {

@@ -59,7 +59,7 @@ struct PromptParams {
   int32_t* tiles_before;    // [batch]
   float* parts;             // [ctas][2][tiles][dim / 4][128][4] sums, then [128] maxima and [128] sums of weights
   float scale, cap;         // the scale times log2(e); the cap times log2(e), or zero
-  float cap_scale;          // 2 log2(e) scale / cap
+  float cap_scale;          // the scale / the cap
   int32_t batch, tokens, heads, kv_heads, capacity, own_capacity, window, max_items, ctas;
   int32_t box;         // tokens of a TMA box of keys and values, which divides pages and steps; zero (codes): loaded as they are turned
   int32_t head_step;   // from head to head in k_map and v_map: zero where all heads are one
