@@ -22,16 +22,18 @@
 namespace chord {
 
 // Warps: 16 for the rows, one that loads by TMA, one that issues products, two that look at values and load queries that
-// TMA does not, and, over codes, four that turn these into BF16.
-constexpr int kLoadWarp = 16, kIssueWarp = 17, kLookWarp = 18, kLookWarps = 2, kTurnWarp = 20, kTurnWarps = 4;
+// TMA does not, and, over codes, those that turn these into BF16: four more, or the eight that one tile's rows leave (with
+// four more there too, 4 x 1,024 queries of 16 heads of 256 after 30,000 tokens: 2.04 ms for 1.91).
+constexpr int kLoadWarp = 16, kIssueWarp = 17, kLookWarp = 18, kLookWarps = 2;
 
 template <int kDim, bool kCodes>
 struct PromptLayout {
-  static constexpr int kThreads = 32 * (kCodes ? kTurnWarp + kTurnWarps : kTurnWarp);
-  // Of a CTA launched with 96 registers a thread, 80 over codes: what the rows' warps have, and the others.
-  static constexpr int kRowRegs = kCodes ? 88 : 104, kOtherRegs = 64;
   static constexpr bool kTwo = kDim <= 128;  // row tiles of an item
   static constexpr int kTiles = kTwo ? 2 : 1;
+  static constexpr int kTurnWarp = kTwo ? 20 : 8, kTurnWarps = kTwo ? 4 : 8;
+  static constexpr int kThreads = 32 * (kCodes && kTwo ? 24 : 20);
+  // Of a CTA launched with 96 registers a thread, 80 with 24 warps: what the first 16 warps have, and the others.
+  static constexpr int kRowRegs = kCodes && kTwo ? 88 : 104, kOtherRegs = 64;
   static constexpr int kN = kTwo ? 128 : 64;             // tokens of a step
   static constexpr int kBlocks = (kDim + 63) / 64;       // of 64 elements, 128 bytes
   static constexpr int kQBytes = kTiles * kBlocks * kPromptTile * 128;
@@ -352,19 +354,19 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     ptx::mbar_init(bar(c.q_empty), 1);
     ptx::mbar_init(bar(c.drained), 1);
     for (int i = 0; i < 8; ++i) {
-      ptx::mbar_init(bar(c.kv_full[i]), kCodes ? kTurnWarps : 1);
+      ptx::mbar_init(bar(c.kv_full[i]), kCodes ? L::kTurnWarps : 1);
       ptx::mbar_init(bar(c.kv_empty[i]), 1);
       ptx::mbar_init(bar(c.looked[i]), kLookWarps);
       c.odd[i] = 0;
     }
     for (int i = 0; i < 4; ++i) {
       ptx::mbar_init(bar(c.raw_full[i]), 1);
-      ptx::mbar_init(bar(c.raw_empty[i]), kTurnWarps);
+      ptx::mbar_init(bar(c.raw_empty[i]), L::kTurnWarps);
       ptx::mbar_init(bar(c.scales_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(bar(c.item_full[i]), 1);
-      ptx::mbar_init(bar(c.item_empty[i]), 8 * L::kTiles + 1 + kLookWarps + (kCodes ? kTurnWarps : 0));
+      ptx::mbar_init(bar(c.item_empty[i]), 8 * L::kTiles + 1 + kLookWarps + (kCodes ? L::kTurnWarps : 0));
       ptx::mbar_init(bar(c.s_full[i]), 1);
       ptx::mbar_init(bar(c.p_full[0][i]), 4);
       ptx::mbar_init(bar(c.p_full[1][i]), 4);
@@ -774,11 +776,12 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
       walk.next(n);
     }
     if (bad != 0 && lane == 0 && p.status != nullptr) atomicOr(p.status, kPromptLoadTimeout);
-  } else if (warp >= kTurnWarp) {
+  } else if (kCodes && warp >= L::kTurnWarp) {
     if constexpr (kCodes) {
-      // ---- codes into BF16, a quarter of a step's tokens for each warp ----
-      const int w = warp - kTurnWarp;
-      constexpr int kOwn = kN / kTurnWarps;
+      // ---- codes into BF16, a quarter or an eighth of a step's tokens for each warp ----
+      if constexpr (!L::kTwo) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kRowRegs));
+      const int w = warp - L::kTurnWarp;
+      constexpr int kOwn = kN / L::kTurnWarps;
       constexpr int kPieces = kDim / 16;
       uint32_t slot = 0, slot_phase = 0, raw_slot = 0, raw_phase = 0;
       PromptWalk walk(c.start, c.plan_items);
