@@ -39,7 +39,7 @@ struct AttentionParams {
   // Of the kernels with kShaped alone.
   const float* slopes;  // [heads] or null: taken off the scores for each token between
   float* wide_out;      // [batch, heads, dim] in place of out, where not null
-  float cap, two_over_cap;  // tanh(x / cap) cap, with log2(e); zero: none
+  float cap, over_cap;  // tanh(x over_cap) cap, x with log2(e); zero: none
 };
 
 // What follows from the head's width and the cache's type.  A warp takes kStep tokens at a time, whose
@@ -138,13 +138,6 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
 }
 
 constexpr float kLog2E = 1.44269504088896341f;
-
-// cap tanh(u log(2) / 2), from the one exponential: exact for large and small ones, off by 2^-22 of the cap.
-__device__ __forceinline__ float capped(float u, float cap) {
-  float rate;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rate) : "f"(exp2_approx(u) + 1.0f));
-  return fmaf(-2.0f * cap, rate, cap);
-}
 
 // What outputs are multiplied with: those of codes are 64ths.
 template <bool kCodes>
@@ -787,8 +780,8 @@ paged_attention_kernel(const AttentionParams p) {
           for (int j = 0; j < kGroups; ++j) {
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) s[j][n][i] = capped(s[j][n][i] * p.two_over_cap, p.cap);
+              cap_pair(s[j][n][0], s[j][n][1], p.over_cap, p.cap);
+              cap_pair(s[j][n][2], s[j][n][3], p.over_cap, p.cap);
             }
           }
         }
@@ -1135,7 +1128,7 @@ int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const chord_
   const int64_t group = heads / cache->heads;
   const bool wide = group > 8;
   Variant v;
-  CHORD_REQUIRE(scores.cap >= 0.0 && scores.cap - scores.cap == 0.0, "the cap must be finite and at least zero");
+  CHORD_REQUIRE(cap_fits(scores), "the cap must be zero or from 1e-30 to 1e30, and the scale no more than 1e36 of it");
   CHORD_REQUIRE(shaped ? variant_for<true>(cache->head_dim, codes, wide, &v) : variant_for<false>(cache->head_dim, codes, wide, &v), "head_dim must be 64, 96, 128, 192 or 256, got %lld",
                 static_cast<long long>(cache->head_dim));
   DeviceInfo device;
@@ -1178,7 +1171,7 @@ int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const chord_
   p.slopes = scores.slopes;
   p.wide_out = wide_out;
   p.cap = static_cast<float>(scores.cap * 1.4426950408889634074);
-  p.two_over_cap = scores.cap > 0.0 ? static_cast<float>(2.0 / scores.cap) : 0.0f;
+  p.over_cap = scores.cap > 0.0 ? static_cast<float>(1.0 / (scores.cap * 1.4426950408889634074)) : 0.0f;
   p.whole_groups = cache->page_size % 16 == 0 && p.cache.token < (1ll << 31);
   CHORD_CUDA(launch_kernel(v.kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), v.smem,
                            static_cast<cudaStream_t>(stream), kEarlyLaunch, p));

@@ -4,6 +4,7 @@
 #include <utility>
 
 #include "../../include/chord_b200.h"
+#include "attention.h"
 #include "common.h"
 #include "kv_cache.cuh"
 #include "warp_ops.cuh"
@@ -16,12 +17,6 @@ constexpr float kLog2E = 1.44269504088896341f;
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float reciprocal_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -39,7 +34,7 @@ struct WeighParams {
   float* weights;        // [batch, kv_heads, width]
   int64_t weight_batch, weight_head;
   int32_t* status;
-  float scale, cap, two_over_cap;  // as of paged_attention
+  float scale, cap, over_cap;  // as of paged_attention
   int32_t heads, group, capacity, width, window, add;
   int32_t runs;    // of 64 tokens for a warp
   bool in_a_row;   // 16 tokens from a multiple of 16 lie one after another
@@ -257,7 +252,7 @@ __global__ void __launch_bounds__(kWeighWarps * 32) attention_weights_kernel(con
         }
         if (p.cap > 0.0f) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i / 2][i % 2] = fmaf(-2.0f * p.cap, reciprocal_approx(exp2_approx(x[i / 2][i % 2] * p.two_over_cap) + 1.0f), p.cap);
+          for (int i = 0; i < 2; ++i) cap_pair(x[i][0], x[i][1], p.over_cap, p.cap);
         }
         if (p.slopes != nullptr) {
 #pragma unroll
@@ -391,7 +386,7 @@ __device__ __forceinline__ uint32_t find_bin(const uint32_t* bins, uint32_t* of_
 // then the kept tokens in order.  Counts do not depend on the order in which they are counted.  A thread has up to kItems
 // neighbours' weights in registers, which come coalesced, by way of shared memory; with kItems zero, for longer sequences,
 // they are read from memory each time and a warp has a run of them.  Bounded by the latency of its steps: 128 CTAs of 16384
-// weights RESULT_S (with the runs' ballots from shared memory 20).
+// weights 12 us (with the runs' ballots from shared memory 20).
 template <int kItems>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
   extern __shared__ float held[];
@@ -691,7 +686,8 @@ int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
   CHORD_REQUIRE(max_pages > 0 && table_stride >= 0 && max_pages < (1ll << 31), "a block table has a page or more");
   CHORD_REQUIRE(width > 0 && width < (1ll << 31) - 65536 && weight_batch >= 0 && weight_head >= 0, "sizes of the weights out of range");
   CHORD_REQUIRE(scores->window >= 0 && scores->window < (1ll << 31), "window out of range");
-  CHORD_REQUIRE(scores->scale - scores->scale == 0.0 && scores->cap >= 0.0 && scores->cap - scores->cap == 0.0, "scale and cap must be finite");
+  CHORD_REQUIRE(scores->scale - scores->scale == 0.0, "scale must be finite");
+  CHORD_REQUIRE(cap_fits(*scores), "the cap must be zero or from 1e-30 to 1e30, and the scale no more than 1e36 of it");
   const WeighKernel kernel = cache->k_scale != nullptr ? weigh_kernel<true>(cache->head_dim) : weigh_kernel<false>(cache->head_dim);
   CHORD_REQUIRE(kernel.kernel != nullptr, "head_dim must be 64, 96, 128, 192 or 256, got %lld", static_cast<long long>(cache->head_dim));
   DeviceInfo device;
@@ -713,7 +709,7 @@ int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
   p.status = status;
   p.scale = static_cast<float>(scores->scale * 1.4426950408889634074);
   p.cap = static_cast<float>(scores->cap * 1.4426950408889634074);
-  p.two_over_cap = scores->cap > 0.0 ? static_cast<float>(2.0 / scores->cap) : 0.0f;
+  p.over_cap = scores->cap > 0.0 ? static_cast<float>(1.0 / (scores->cap * 1.4426950408889634074)) : 0.0f;
   p.heads = static_cast<int32_t>(heads);
   p.group = static_cast<int32_t>(heads / cache->heads);
   p.capacity = static_cast<int32_t>(capacity < (1ll << 31) - 65536 ? capacity : (1ll << 31) - 65536);
@@ -734,6 +730,7 @@ int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
 int64_t chord_b200_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t keep) {
   using namespace chord;
   if (batch < 0 || kv_heads < 0 || keep < 0) return fail(kInvalidArgument, "no size may be negative"), -1;
+  if (batch > 65535 || kv_heads > 65535 || keep >= (1ll << 28)) return fail(kInvalidArgument, "no sizes of an eviction"), -1;
   return batch * kv_heads * keep * 4;
 }
 
@@ -752,8 +749,8 @@ int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tabl
                 "null pointer");
   CHORD_REQUIRE(max_pages > 0 && table_stride >= 0 && max_pages < (1ll << 31), "a block table has a page or more");
   CHORD_REQUIRE(new_tables == nullptr || (new_pages > 0 && new_stride >= 0 && new_pages < (1ll << 31)), "a block table has a page or more");
-  CHORD_REQUIRE(keep > 0 && keep < (1ll << 31) - 65536 && first >= 0 && recent >= 0 && first + recent <= keep,
-                "first and recent are at least zero and no more than keep, %lld, together, got %lld and %lld",
+  CHORD_REQUIRE(keep > 0 && keep < (1ll << 28) && first >= 0 && recent >= 0 && first <= keep && recent <= keep - first,
+                "keep is below 2^28, first and recent are at least zero and no more than keep, %lld, together, got %lld and %lld",
                 static_cast<long long>(keep), static_cast<long long>(first), static_cast<long long>(recent));
   CHORD_REQUIRE(width > 0 && width < (1ll << 31) - 65536 && new_width > 0 && new_width < (1ll << 31) - 65536 && keep <= new_width &&
                     weight_batch >= 0 && weight_head >= 0,

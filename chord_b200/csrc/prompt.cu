@@ -106,7 +106,9 @@ int check_prompt(const PromptCall& c) {
   CHORD_REQUIRE(c.max_pages > 0 && c.table_stride >= 0 && c.max_pages < (1ll << 31), "a block table has a page or more");
   CHORD_REQUIRE(c.scores->window >= 0 && c.scores->window < (1ll << 31), "window out of range");
   CHORD_REQUIRE(c.scores->scale - c.scores->scale == 0.0, "scale must be finite");
-  CHORD_REQUIRE(c.scores->cap >= 0.0 && c.scores->cap - c.scores->cap == 0.0, "the cap must be finite and at least zero");
+  CHORD_REQUIRE(cap_fits(*c.scores), "the cap must be zero or from 1e-30 to 1e30, and the scale no more than 1e36 of it");
+  PromptVariant v;
+  CHORD_REQUIRE(prompt_bf16(c.cache->head_dim, &v), "head_dim must be 64, 96, 128, 192 or 256, got %lld", static_cast<long long>(c.cache->head_dim));
   // (rows of a sequence are numbered in 32 bits)
   CHORD_REQUIRE(c.tokens * (c.heads / c.cache->heads) < (1ll << 31) - 65536, "too many query tokens and heads: %lld x %lld",
                 static_cast<long long>(c.tokens), static_cast<long long>(c.heads));
@@ -301,7 +303,8 @@ int chord_b200_shared_prefix_attention(const void* q, int64_t q_batch, int64_t q
   const PromptCall c = {q, q_batch, q_head, cache, prefix_tables, prefix_stride, prefix_pages, prefix_lengths, group_offsets, nullptr,
                         nullptr, lengths, max_pages > 0 ? token_capacity(max_pages, cache) : 0, own, own_lse, out, lse, rest, rest_bytes,
                         status, groups, batch, heads, scores, stream};
-  CHORD_REQUIRE(lengths != nullptr, "null pointer");
+  CHORD_REQUIRE(lengths != nullptr && tables != nullptr && locks != nullptr, "null pointer");
+  CHORD_REQUIRE(max_pages > 0 && table_stride >= 0 && max_pages < (1ll << 31), "a block table has a page or more");
   if (int rc = check_prompt(c)) return rc;
   DeviceInfo device;
   if (int rc = current_device_info(&device)) return rc;

@@ -64,12 +64,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-__device__ __forceinline__ float reciprocal_fast(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -88,20 +82,6 @@ __device__ __forceinline__ void add_pair(float (&sum)[2], float x, float y) {
   asm("{\n .reg .b64 v, s;\n mov.b64 s, {%0, %1};\n mov.b64 v, {%2, %3};\n add.rn.f32x2 s, s, v;\n mov.b64 {%0, %1}, s;\n}"
       : "+f"(sum[0]), "+f"(sum[1])
       : "f"(x), "f"(y));
-}
-
-// cap tanh(x) and cap tanh(y) for |x|, |y| up to kTanhBound, by an odd polynomial with coefficients fitted to the least
-// largest error there: off by 9e-8 of the cap, FP32's roundings in it.  (By 1 - 2 / (e^2x + 1), good everywhere, two of the three
-// operations per score of the 4-lane unit are the cap's.)
-constexpr float kTanhBound = 0.75f;
-__device__ __forceinline__ void capped_pair(float& x, float& y, float cap) {
-  asm("{\n .reg .b64 t, w, p, c;\n mov.b64 t, {%0, %1};\n mul.rn.f32x2 w, t, t;\n"
-      " mov.b64 p, {%8, %8};\n mov.b64 c, {%7, %7};\n fma.rn.f32x2 p, p, w, c;\n mov.b64 c, {%6, %6};\n fma.rn.f32x2 p, p, w, c;\n"
-      " mov.b64 c, {%5, %5};\n fma.rn.f32x2 p, p, w, c;\n mov.b64 c, {%4, %4};\n fma.rn.f32x2 p, p, w, c;\n"
-      " mov.b64 c, {%3, %3};\n fma.rn.f32x2 p, p, w, c;\n mul.rn.f32x2 p, p, t;\n mov.b64 c, {%2, %2};\n mul.rn.f32x2 p, p, c;\n"
-      " mov.b64 {%0, %1}, p;\n}"
-      : "+f"(x), "+f"(y)
-      : "f"(cap), "f"(0.99999983f), "f"(-0.33332471f), "f"(0.13320579f), "f"(-0.05314925f), "f"(0.01923722f), "f"(-0.00449344f));
 }
 
 // A warp's walk over its CTA's steps.
@@ -935,22 +915,28 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
                 x[i] *= f.x, x[i + 1] *= f.y, x[i + 2] *= f.z, x[i + 3] *= f.w;
               }
             }
+            const uint32_t begin = view.lo - first - half * kHalf - 32 * chunk, span = max(view.hi - view.lo, 0);
             if constexpr (kBent) {
               if (p.cap > 0.0f) {
+                // (by what the row itself sees, so that nothing else changes its bits)
+                if (partial) {
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) x[i] = i - begin < span ? x[i] : 0.0f;
+                }
                 float most = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                   if constexpr (!kCodes) x[i] *= p.cap_scale, x[i + 1] *= p.cap_scale;
                   most = max3(most, fabsf(x[i]), fabsf(x[i + 1]));
                 }
-                if (__any_sync(0xffffffffu, most > kTanhBound)) {
-                  const float twice = -2.0f * p.cap;
+                if (most > kTanhBound) {
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) x[i] = fmaf(twice, reciprocal_fast(exp2_fast(x[i] * 2.8853900817779268f) + 1.0f), p.cap);
+                  for (int i = 0; i < 32; ++i) x[i] = capped(x[i], p.cap);
                 } else {
 #pragma unroll
                   for (int i = 0; i < 32; i += 2) capped_pair(x[i], x[i + 1], p.cap);
                 }
+                __syncwarp();
               } else if constexpr (!kCodes) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] *= p.scale;
@@ -962,7 +948,6 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
               }
             }
             if (partial) {
-              const uint32_t begin = view.lo - first - half * kHalf - 32 * chunk, span = max(view.hi - view.lo, 0);
 #pragma unroll
               for (int i = 0; i < 32; ++i) x[i] = i - begin < span ? x[i] : -INFINITY;
             }
@@ -987,7 +972,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
           ptx::named_bar_sync(pair, 64);
           highest = fmaxf(highest, *const_cast<volatile float*>(shared + (1 - half) * kPromptTile)) * of_scores;
           if (__any_sync(0xffffffffu, highest > top + kSlack)) {
-            const float next = fmaxf(top, highest);
+            const float next = highest > top + kSlack ? highest : top;  // (rows that need no other base keep theirs, and their bits)
             const float factor = next == -INFINITY ? 1.0f : exp2_fast(top - next);
             top = next;
             sum *= factor;

@@ -66,6 +66,17 @@ int device_of(const at::Tensor& t) {
   return index >= 0 && index < kMaxDevices && devices[index].status != nullptr && index == c10::cuda::current_device() ? index : -1;
 }
 
+// Whether a contiguous tensor shares memory with so many bytes, or with what lies between another's first and last element.
+bool overlap(const at::Tensor& t, const void* other, int64_t bytes) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(t.const_data_ptr()), at = reinterpret_cast<uintptr_t>(other);
+  return begin < at + bytes && at < begin + t.nbytes();
+}
+bool overlap(const at::Tensor& t, const at::Tensor& other) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < other.dim(); ++i) last += (other.size(i) - 1) * other.stride(i);
+  return other.numel() > 0 && overlap(t, other.const_data_ptr(), (last + 1) * static_cast<int64_t>(other.element_size()));
+}
+
 bool aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
 
 // [tokens, heads, dim] with rows on 16-byte boundaries; heads < 0: any but none.
@@ -460,6 +471,7 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   if (lengths == nullptr || !table_of(a[3], device, batch, &table) || !optional_ints(a[6], device, tokens, &starts) ||
       !optional_ints(a[7], device, batch, &prefixes) || !sums_of(a[8], device, tokens, heads, &lse) || !scores_of(a + 9, device, heads, &scores))
     return none();
+  if (lse != nullptr && overlap(THPVariable_Unpack(a[8]), *q)) return none();
   const int64_t size = more.prompt_workspace_bytes(batch, tokens, heads, cache->heads, cache->head_dim);
   if (size < 0) return none();
   int32_t* const status = devices[device].status;
@@ -493,6 +505,7 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t coun
   if (prefix_lengths == nullptr || lengths == nullptr || !table_of(a[3], device, groups, &prefix_table) || !table_of(a[6], device, batch, &table) ||
       !sums_of(a[8], device, batch, heads, &lse) || !scores_of(a + 9, device, heads, &scores))
     return none();
+  if (lse != nullptr && overlap(THPVariable_Unpack(a[8]), *q)) return none();
   void* const stream = stream_of(device);
   int64_t word_count = 0;
   int32_t* const words = locks_of(device, stream, &word_count);
@@ -533,7 +546,7 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t count) {
   if (add) {
     given = tensor(a[6], at::kFloat, 3);
     if (given == nullptr || given->get_device() != device || given->size(0) != batch || given->size(1) != cache->heads || given->size(2) == 0 ||
-        !given->is_contiguous())
+        !given->is_contiguous() || overlap(*given, lse, batch * heads * 4) || overlap(*given, *q))
       return none();
   }
   const int64_t width = add ? given->size(2) : table.pages * cache->page_size;
@@ -573,7 +586,7 @@ PyObject* cache_evict(PyObject*, PyObject* const* a, Py_ssize_t count) {
     return none();
   const int64_t width = weights->size(2), new_width = width > keep ? width : keep;
   const int64_t most = std::min(std::min(keep, width), table.pages * cache->page_size);
-  if (keep >= (1ll << 31) - 65536 || (a[8] != Py_None && new_table.pages * cache->page_size < most)) return none();
+  if (keep >= (1ll << 28) || (a[8] != Py_None && new_table.pages * cache->page_size < most)) return none();
   int32_t* const status = devices[device].status;
   at::Tensor new_lengths, new_weights;
   int rc;

@@ -113,4 +113,36 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
                : "memory");
 }
 
+// cap tanh(x) from one exponential: off by 2^-22 of the cap, infinities in it.
+__device__ __forceinline__ float capped(float x, float cap) {
+  float e, rate;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.8853900817779268f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rate) : "f"(e + 1.0f));
+  return fmaf(-2.0f * cap, rate, cap);
+}
+
+// cap tanh(x) and cap tanh(y) for |x|, |y| up to kTanhBound, by an odd polynomial with coefficients fitted to the least
+// largest error there: off by 2^-23 of themselves and FP32's roundings, where the form above is off by 2^-22 of the cap; and
+// without its two operations of the 4-lane unit, of a score's three.
+constexpr float kTanhBound = 0.75f;
+__device__ __forceinline__ void capped_pair(float& x, float& y, float cap) {
+  asm("{\n .reg .b64 t, w, p, c;\n mov.b64 t, {%0, %1};\n mul.rn.f32x2 w, t, t;\n"
+      " mov.b64 p, {%8, %8};\n mov.b64 c, {%7, %7};\n fma.rn.f32x2 p, p, w, c;\n mov.b64 c, {%6, %6};\n fma.rn.f32x2 p, p, w, c;\n"
+      " mov.b64 c, {%5, %5};\n fma.rn.f32x2 p, p, w, c;\n mov.b64 c, {%4, %4};\n fma.rn.f32x2 p, p, w, c;\n"
+      " mov.b64 c, {%3, %3};\n fma.rn.f32x2 p, p, w, c;\n mul.rn.f32x2 p, p, t;\n mov.b64 c, {%2, %2};\n mul.rn.f32x2 p, p, c;\n"
+      " mov.b64 {%0, %1}, p;\n}"
+      : "+f"(x), "+f"(y)
+      : "f"(cap), "f"(0.99999983f), "f"(-0.33332471f), "f"(0.13320579f), "f"(-0.05314925f), "f"(0.01923722f), "f"(-0.00449344f));
+}
+
+// Two scores of one token times over_cap, capped by the form that fits them (so that no other token changes their bits).
+__device__ __forceinline__ void cap_pair(float& x, float& y, float over_cap, float cap) {
+  x *= over_cap, y *= over_cap;
+  if (fmaxf(fabsf(x), fabsf(y)) <= kTanhBound) {
+    capped_pair(x, y, cap);
+  } else {
+    x = capped(x, cap), y = capped(y, cap);
+  }
+}
+
 }  // namespace chord

@@ -31,7 +31,7 @@ def attention_weights(q: torch.Tensor, cache: KVCache, block_tables: torch.Tenso
 
     The arguments are those of the :func:`paged_attention` call that gave ``lse``.  Without ``weights`` the result is new,
     as wide as the table, with zeros for tokens that are not seen; with it (FP32, as wide as the longest sequence or
-    wider, rows contiguous) they are added to it, token by token, and it is returned.  The same inputs give the same bits.
+    wider, rows contiguous and apart from each other, ``q`` and ``lse``) they are added to it, token by token, and it is returned.  The same inputs give the same bits.
     What :func:`paged_attention` reports is reported, and lengths beyond ``weights``."""
     _cache(cache)
     direct = _lib.direct()
@@ -54,8 +54,13 @@ def attention_weights(q: torch.Tensor, cache: KVCache, block_tables: torch.Tenso
     if not add:
         weights = torch.empty((batch, cache.heads, table[2] * cache.page_size), dtype=torch.float32, device=device)
     *to, width = _weights("weights", weights, batch, cache.heads, device) if batch else (0, 0, 0, 0)
-    if add and batch and any(n > 1 and s < width for n, s in zip(weights.shape[:2], weights.stride()[:2])):
-        raise ValueError(f"rows of weights must not overlap, got strides {weights.stride()}")
+    if add and batch:
+        (inner, rows), (outer, others) = sorted(zip(weights.stride()[:2], weights.shape[:2]))
+        if (rows > 1 and inner < width) or (others > 1 and outer < (rows - 1) * inner + width):
+            raise ValueError(f"rows of weights must not overlap, got strides {weights.stride()}")
+        extent = weights.as_strided((sum((n - 1) * s for n, s in zip(weights.shape, weights.stride())) + 1,), (1,))
+        _checks.apart("weights", extent, "lse", lse)
+        _checks.apart("weights", extent, "q", q)
     if batch == 0:
         return weights
     with _lib.on_device(device):
@@ -95,6 +100,8 @@ def cache_evict(cache: KVCache, block_tables: torch.Tensor, lengths: torch.Tenso
     new_table = (None, 0, 0) if new_tables is None else _table(new_tables, device, batch, "new_tables")
     *held, width = _weights("weights", weights, batch, cache.heads, device)
     _checks.integer("keep", keep, minimum=1)
+    if keep >= 2**28:
+        raise ValueError(f"keep must be below 2^28, got {keep}")
     _checks.integer("first", first, minimum=0)
     _checks.integer("recent", recent, minimum=0)
     if first + recent > keep:

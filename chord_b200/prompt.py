@@ -39,8 +39,9 @@ def prompt_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor
       (the window and the document still bound it below).
 
     ``slopes`` take the distance either way.  Returns BF16 ``[tokens, heads, head_dim]``; ``lse`` as for
-    :func:`paged_attention`.  A token that sees nothing gives zeros and minus infinity.  Rows of tokens of no sequence
-    are left as they are.  Whatever a token does not see, infinities and NaN too, does not change its result.
+    :func:`paged_attention` (and apart from ``q``).  A token that sees nothing gives zeros and minus infinity.  Rows of tokens of no sequence
+    are left as they are.  What a token does not see does not change its bits; infinities and NaN there change no more than how
+    its weights are rounded (where neighbours see such a value, weights of that step are not rounded to BF16).
     Offsets that fall or lie outside ``q``, lengths beyond the table and pages outside the cache are reported by
     :func:`chord_b200.check_status`; nothing outside is read or written.  The same inputs give the same bits."""
     _cache(cache)
@@ -63,6 +64,10 @@ def prompt_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor
     if given:
         _checks.apart("outputs", outputs, "q", q)
     sums = _sums(lse, tokens, heads, device)
+    if lse is not None:
+        _checks.apart("lse", lse, "q", q)
+        if given:
+            _checks.apart("lse", lse, "outputs", outputs)
     if tokens == 0:
         return outputs
     with _lib.on_device(device):
@@ -110,6 +115,10 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCache, prefix_tables: torc
     if given:
         _checks.apart("outputs", outputs, "q", q)
     sums = _sums(lse, batch, heads, device)
+    if lse is not None:
+        _checks.apart("lse", lse, "q", q)
+        if given:
+            _checks.apart("lse", lse, "outputs", outputs)
     if batch == 0:
         return outputs
     with _lib.on_device(device):

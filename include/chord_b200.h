@@ -454,7 +454,7 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
 
 /* How a query's scores come about: x = scale q . k; with cap > 0 x = cap tanh(x / cap); with slopes (fp32 [heads], on the
  * device) x -= slopes[h] |p - j| for a query at position p and the token at j; with window > 0 only tokens j > p - window
- * are seen.  scale and cap are finite, cap and window at least zero. */
+ * are seen.  scale is finite, cap zero or from 1e-30 to 1e30 with |scale| <= 1e36 cap, window from zero to 2^31 - 1. */
 typedef struct chord_b200_scores {
   double scale, cap;
   const float* slopes;
@@ -513,9 +513,12 @@ int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t gro
  *  out      bf16 [tokens, heads, head_dim], not overlapping q;  lse fp32 [tokens, heads] or null
  *  workspace  chord_b200_prompt_attention_workspace_bytes(...) bytes, 16-byte aligned
  * A token that sees nothing, or whose scores are all minus infinity, gets zeros and an lse of minus infinity.  Rows of
- * tokens of no sequence are not written.  What a token does not see, infinities and NaN too, does not change its
- * result.  Weights are rounded to BF16 before they multiply values; sums are FP32 and, where a sequence is cut over the
- * device, joined in their order: the same inputs give the same bits.  Three launches; no kernel waits for another CTA. */
+ * tokens of no sequence are not written.  What a token does not see does not change its bits; infinities and NaN there
+ * change no more than the rounding of its weights.  These are rounded to BF16 before they multiply values (of a step in which
+ * some row of the tile sees an infinity or a NaN among values, and another does not, they are not); sums are FP32 and,
+ * where a sequence is cut over the device, joined in their order: the same inputs give the same bits.  One launch, one more to
+ * join where something may be cut, and one more to plan for over 1,024 sequences or items; no kernel waits for another CTA.
+ * Strides of a BF16 cache must be from 16 to 2^40 - 16 bytes; those of heads and pages may be zero. */
 int chord_b200_prompt_attention(const void* q, int64_t q_token, int64_t q_head,
                                 const chord_b200_kv_cache* cache, const int32_t* tables,
                                 int64_t table_stride, int64_t max_pages, const int32_t* lengths,
