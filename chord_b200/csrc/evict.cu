@@ -613,7 +613,7 @@ __device__ __forceinline__ float load_ordered(const float* p) {
 
 // Rows forward within their pages.  A kept token never moves back, so rows are moved in order, a round of them at a time,
 // read whole before any of it is written; a CTA has some columns of a head's rows of its own (64 bytes or, of rows that
-// do not divide so, 32), so that no two have to wait for each other.  One more takes the scales.
+// do not divide so, 32 or 16), so that no two have to wait for each other.  One more takes the scales.
 __global__ void __launch_bounds__(kShiftThreads) evict_shift_kernel(const EvictParams p, int32_t slice_bytes) {
   __shared__ int32_t first_moved;
   ptx::grid_dependency_wait();
@@ -801,7 +801,7 @@ int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tabl
   if (rc) return rc;
   if (new_tables != nullptr) {
     const int rows = kCopyThreads / (p.row_bytes / 16);
-    const int64_t rounds = (keep + rows - 1) / rows;
+    const int64_t rounds = ((keep < most ? keep : most) + rows - 1) / rows;
     CHORD_CUDA(launch_kernel(evict_copy_kernel, dim3(static_cast<unsigned>((rounds + 3) / 4), heads, sequences), dim3(kCopyThreads), 0, s, kEarlyLaunch, p));
   } else {
     const int32_t slice = p.row_bytes % 64 == 0 ? 64 : p.row_bytes % 32 == 0 ? 32 : 16;
