@@ -8,7 +8,7 @@ import torch
 
 import chord_b200
 from tests import attention_cases as A
-from tests.prompt_cases import Prompt
+from tests.prompt_cases import Prompt, close
 from tests.test_gpu_eviction import check_eviction
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +113,12 @@ def test_offsets_beyond_32_bits(device, bits):
         got.append(out + [x[-used:] for x in parts(cache)])
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+def test_few_tokens_over_codes(device, dim):
+    """Rows that see few tokens do not average the rounding of weights: two BF16 numbers each, off by 2^-16, and sums of
+    at most 512 terms in FP32, each of which may be cut off at 2^-23 of the sum, in the result and in the weights' sum: 2^-13."""
+    case = Prompt(device, [(0, 40), (3, 200), (150, 60), (0, 1)], 8, 2, dim, 16, 8, seed=31)
+    close(case.run(), case.want(), weights=2.0 ** -16 + 2.0 ** -13)
+    close(case.run(window=3, cap=8.0), case.want(window=3, cap=8.0), weights=2.0 ** -16 + 2.0 ** -13)
