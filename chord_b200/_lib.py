@@ -179,7 +179,7 @@ def native():
 def direct():
     """The ``_torch_call`` module with the library's entry points, or None where it was not built.  Its
     functions answer None to a call that they leave to the wrapper."""
-    if _torch_call is None:
+    if _torch_call is None or not hasattr(_torch_call, "more_entries"):  # (or is of an earlier library)
         return None
     names = ("gemv", "qk_norm_rope", "qk_norm_rope_write", "cache_write", "cache_read", "paged_attention",
              "paged_attention_workspace_bytes")

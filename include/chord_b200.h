@@ -514,10 +514,11 @@ int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t gro
  *  workspace  chord_b200_prompt_attention_workspace_bytes(...) bytes, 16-byte aligned
  * A token that sees nothing, or whose scores are all minus infinity, gets zeros and an lse of minus infinity.  Rows of
  * tokens of no sequence are not written.  What a token does not see does not change its bits; infinities and NaN there
- * change no more than the rounding of its weights.  These are rounded to BF16 before they multiply values (over codes, where rows
- * of a tile see no more than some hundred tokens, to two BF16 numbers; of a step in which some row of the tile sees an infinity or a NaN among values, and another does not, they are not); sums are FP32 and,
- * where a sequence is cut over the device, joined in their order: the same inputs give the same bits.  One launch, one more to
- * join where something may be cut, and one more to plan for over 1,024 sequences or items; no kernel waits for another CTA.
+ * change no more than the rounding of its weights.  These are rounded to BF16 before they multiply values; to two BF16 numbers
+ * over codes where the rows of a tile see some hundred tokens or fewer, and not at all in a step in which some row of the
+ * tile sees an infinity or a NaN among values and another does not.  Sums are FP32 and, where a sequence is cut over the
+ * device, joined in their order: the same inputs give the same bits.  One launch, one more to join where something may be cut,
+ * and one more to plan for over 1,024 sequences or items; no kernel waits for another CTA.
  * Strides of a BF16 cache must be from 16 to 2^40 - 16 bytes; those of heads and pages may be zero. */
 int chord_b200_prompt_attention(const void* q, int64_t q_token, int64_t q_head,
                                 const chord_b200_kv_cache* cache, const int32_t* tables,
