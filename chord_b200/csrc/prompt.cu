@@ -171,6 +171,7 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
   p.extra = c.extra;
   p.extra_lse = c.extra_lse;
   p.out = static_cast<__nv_bfloat16*>(c.out);
+  p.out_32 = (reinterpret_cast<uintptr_t>(c.out) & 31u) == 0;
   p.lse = c.lse;
   p.status = c.status;
   constexpr double kLog2E = 1.4426950408889634074;

@@ -203,7 +203,8 @@ __device__ __forceinline__ void exchange4(uint32_t (&w)[4], int q) {
 
 // Writes 64 or 32 values, from `dim` on, of a warp's 32 rows as BF16.  Rows are spread over four lanes each (with a row to a
 // lane, every store touches 32 lines of memory: 6500 cycles for two tiles of 128 values, as long as two steps), which
-// then write 128 or 64 bytes of it in one go.  `row`, `mine` and `other` are those of the lane's own row; row < 0: none.
+// then write 128 or 64 bytes of it in one go, 32 bytes at a time where the results lie on 32 bytes, which a caller's need not.
+// `row`, `mine` and `other` are those of the lane's own row; row < 0: none.
 template <int kCount>
 __device__ __forceinline__ void write_rows(const PromptParams& p, uint32_t from, int dims, int dim, int64_t row, float mine, float other, int lane) {
   constexpr int kGroups = kCount / 8;
@@ -246,7 +247,14 @@ __device__ __forceinline__ void write_rows(const PromptParams& p, uint32_t from,
       for (int i = 0; i < kGroups / 4; ++i) exchange4(w[i], q);
       __nv_bfloat16* const at = p.out + to * dims + dim + q * (2 * kGroups);
       if (to >= 0) {
-        if constexpr (kGroups == 8) store_32_bytes(at, &w[0][0]);
+        if constexpr (kGroups == 8) {
+          if (p.out_32) {
+            store_32_bytes(at, &w[0][0]);
+          } else {
+            reinterpret_cast<uint4*>(at)[0] = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+            reinterpret_cast<uint4*>(at)[1] = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+          }
+        }
         if constexpr (kGroups == 4) *reinterpret_cast<uint4*>(at) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
       }
     }

@@ -65,6 +65,7 @@ struct PromptParams {
   int32_t head_step;   // from head to head in k_map and v_map: zero where all heads are one
   int32_t page_step;   // the same of pages
   bool q_boxes;        // queries by TMA
+  bool out_32;         // out lies on 32 bytes
   bool self;           // the main kernel's CTAs make the plan, each for itself
   Divisor group;
 };
