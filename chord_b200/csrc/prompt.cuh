@@ -554,6 +554,12 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     auto free_slot = [&](uint32_t number) {
       if (leader) ptx::mma_commit(bar(c.kv_empty[number % kRing]));
     };
+    // Of two tiles over codes, a step's scores are made when its scales are there.  The rows of the second tile go past items
+    // that have none, so they may come to a step while what has been looked at is items behind, of which the parity of
+    // `looked` tells nothing; s_full does, and scales_empty, which waits for them, holds back what comes after.
+    auto wait_scales = [&](uint32_t step) {
+      if constexpr (kCodes && L::kTwo) wait_to_issue(bar(c.looked[step % 8]), step / 8 & 1);
+    };
     // Scores go where weights were that the product before has read.  Products with other accumulators or of another
     // shape are not bound to run in order, so that one has to have ended.
     auto ended = [&](int tile) {  // the last one
@@ -609,6 +615,7 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
       wait_to_issue(bar(c.q_full), q_phase);
       q_phase ^= 1;
       wait_slot(taken);
+      wait_scales(taken / 2);
       if (bad != 0) break;
       for (int t = 0; t < tiles; ++t) scores(t, t, taken);
       free_slot(taken);
@@ -617,7 +624,10 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
       for (int32_t j = 0; j < n && bad == 0; ++j) {
         const uint32_t v = taken + 2 * j + 1, k = v + 1;
         const bool more = j + 1 < n;
-        if (more) wait_slot(k);
+        if (more) {
+          wait_slot(k);
+          wait_scales(k / 2);
+        }
         if constexpr (!L::kTwo) {
           if (j != 0) ended(0);
           if (bad != 0) break;
@@ -913,13 +923,14 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
           const uint32_t v_number = taken + 2 * j + 1, v_slot = v_number % kRing;
           const bool partial = any_masked(it, first);
           bool odd = false;
-          if (kCodes || partial) wait(bar(c.looked[v_number / 2 % 8]), v_number / 16 & 1);
           if (!kCodes && partial) {
+            wait(bar(c.looked[v_number / 2 % 8]), v_number / 16 & 1);
             odd = *const_cast<volatile uint32_t*>(&c.odd[v_number / 2 % 8]) == v_number + 1;
           }
           wait(bar(c.s_full[buffer]), s_phase >> buffer & 1);
           s_phase ^= 1u << buffer;
           ptx::tc_fence_after();
+          if constexpr (kCodes) wait(bar(c.looked[v_number / 2 % 8]), v_number / 16 & 1);  // (the scales)
           const float of_scores = kBent || kCodes ? 1.0f : p.scale;
           const bool changed = kBent || kCodes || partial;  // scores are kept as they become
 
