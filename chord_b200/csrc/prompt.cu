@@ -140,8 +140,10 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
   p.cache = cache;
   const int64_t group = c.heads / c.cache->heads;
   const bool codes = c.cache->k_scale != nullptr;
-  // (the plain kernels find the largest score before they scale it)
-  const bool bent = c.scores->cap > 0.0 || c.scores->slopes != nullptr || c.scores->scale <= 0.0;
+  constexpr double kLog2E = 1.4426950408889634074;
+  p.scale = static_cast<float>(c.scores->scale * kLog2E);
+  // (the plain kernels find the largest score before they scale it, so what they multiply with is above zero, in FP32 too)
+  const bool bent = c.scores->cap > 0.0 || c.scores->slopes != nullptr || p.scale <= 0.0f;
   PromptVariant v;
   CHORD_REQUIRE(prompt_variant_of(c.cache->head_dim, codes, bent, &v), "head_dim must be 64, 96, 128, 192 or 256, got %lld",
                 static_cast<long long>(c.cache->head_dim));
@@ -174,8 +176,6 @@ int launch_prompt(const PromptCall& c, const Cache& cache, const DeviceInfo& dev
   p.out_32 = (reinterpret_cast<uintptr_t>(c.out) & 31u) == 0;
   p.lse = c.lse;
   p.status = c.status;
-  constexpr double kLog2E = 1.4426950408889634074;
-  p.scale = static_cast<float>(c.scores->scale * kLog2E);
   p.cap = static_cast<float>(c.scores->cap * kLog2E);
   p.cap_scale = c.scores->cap > 0.0 ? static_cast<float>(c.scores->scale / c.scores->cap) : 0.0f;
   p.batch = static_cast<int32_t>(c.batch);
