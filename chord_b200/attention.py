@@ -376,7 +376,7 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     ``slopes[h]`` times a token's distance to the new one is then taken off.  Returns BF16 ``[batch, heads, head_dim]``
     (``outputs``, where given, must not overlap ``q``); ``lse``, if given, FP32 ``[batch,
     heads]``, receives the logarithm of each softmax's sum, with which results over parts of a
-    sequence can be joined.  A sequence of length zero gives zeros and minus infinity; a head whose query
+    sequence can be joined, and overlaps neither ``q`` nor ``outputs``.  A sequence of length zero gives zeros and minus infinity; a head whose query
     holds an infinity gives NaN over an 8-bit cache.
 
     Page ids outside the cache count as keys and values of zero and, like lengths beyond the
@@ -405,6 +405,10 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor,
     if given:
         _checks.apart("outputs", outputs, "q", q)
     sums = _sums(lse, batch, heads, device)
+    if lse is not None:
+        _checks.apart("lse", lse, "q", q)
+        if given:
+            _checks.apart("lse", lse, "outputs", outputs)
     if batch == 0:
         return outputs
     with _lib.on_device(device):

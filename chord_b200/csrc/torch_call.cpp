@@ -353,7 +353,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
   float* lse = nullptr;
   if (a[5] != Py_None) {
     const at::Tensor* t = tensor(a[5], at::kFloat, 2);
-    if (t == nullptr || t->get_device() != device || t->size(0) != batch || t->size(1) != heads || !t->is_contiguous()) return none();
+    if (t == nullptr || t->get_device() != device || t->size(0) != batch || t->size(1) != heads || !t->is_contiguous() || overlap(*t, *q)) return none();
     lse = t->mutable_data_ptr<float>();
   }
   void* const stream = stream_of(device);
@@ -436,6 +436,7 @@ PyObject* paged_attention_shaped(PyObject*, PyObject* const* a, Py_ssize_t count
   if (lengths == nullptr || !table_of(a[3], device, batch, &table) || !sums_of(a[5], device, batch, heads, &lse) ||
       !scores_of(a + 6, device, heads, &scores))
     return none();
+  if (lse != nullptr && overlap(THPVariable_Unpack(a[5]), *q)) return none();
   void* const stream = stream_of(device);
   int64_t word_count = 0;
   int32_t* const words = locks_of(device, stream, &word_count);

@@ -475,7 +475,7 @@ typedef struct chord_b200_scores {
  *  cache    head_dim 64, 96, 128, 192 or 256; heads % cache->heads == 0
  *  tables, table_stride, max_pages  as above; lengths int32 [batch], at most
  *           max_pages * page_size (more: cut, status bit 32)
- *  out      bf16 [batch, heads, head_dim], not overlapping q;  lse fp32 [batch, heads]
+ *  out      bf16 [batch, heads, head_dim], not overlapping q;  lse fp32 [batch, heads], overlapping neither
  *  locks    int32, chord_b200_paged_attention_lock_words() words, zero on entry and on exit
  *  workspace  chord_b200_paged_attention_workspace_bytes(head_dim, heads / cache->heads) bytes,
  *           16-byte aligned
@@ -510,7 +510,7 @@ int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t gro
  *  tables, table_stride, max_pages, lengths, cache   as above
  *  starts   int32 [tokens] or null: the first token of a query token's document
  *  prefixes int32 [batch] or null: so many first tokens are seen by all of the sequence's
- *  out      bf16 [tokens, heads, head_dim], not overlapping q;  lse fp32 [tokens, heads] or null
+ *  out      bf16 [tokens, heads, head_dim], not overlapping q;  lse fp32 [tokens, heads], overlapping neither, or null
  *  workspace  chord_b200_prompt_attention_workspace_bytes(...) bytes, 16-byte aligned
  * A token that sees nothing, or whose scores are all minus infinity, gets zeros and an lse of minus infinity.  Rows of
  * tokens of no sequence are not written.  What a token does not see does not change its bits; infinities and NaN there
@@ -554,7 +554,8 @@ int64_t chord_b200_shared_prefix_attention_workspace_bytes(int64_t groups, int64
  * What each token of sequence b got of its new token's attention:
  *   w[b, g, j] = sum of exp(x_h,j - lse[b, h]) over the heads h that share key-value head g
  * for the tokens j that it sees, with x as of `scores` and lse fp32 [batch, heads] as paged attention gives it (a head whose
- * lse is minus infinity gives nothing).  weights is fp32 [batch, kv_heads, width], rows contiguous, strides in elements;
+ * lse is minus infinity gives nothing).  weights is fp32 [batch, kv_heads, width], rows contiguous and apart from
+ * each other, q and lse, strides in elements;
  * add == 0: written whole, zeros for tokens that are not seen; else added to what is there.  lengths beyond the table or
  * width: cut, status bit 32; a page outside the cache counts as keys of zero.  batch <= 65535. */
 int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
