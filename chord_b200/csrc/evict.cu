@@ -342,9 +342,9 @@ struct EvictParams {
   int64_t weight_batch, weight_head;
   int32_t* new_lengths;  // [batch]
   float* new_weights;    // [batch, kv_heads, new_width], contiguous
-  int32_t* kept;         // [batch, kv_heads, keep]
+  int32_t* kept;         // [batch, kv_heads, places], as many as can be kept
   int32_t* status;
-  int32_t capacity, new_capacity, width, new_width, keep, first, recent, row_bytes;
+  int32_t capacity, new_capacity, width, new_width, keep, places, first, recent, row_bytes;
 };
 
 constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
   const float* const weights = p.weights + b * p.weight_batch + head * p.weight_head;
   const int64_t row = static_cast<int64_t>(b) * gridDim.x + head;
   float* const out = p.new_weights + row * p.new_width;
-  int32_t* const kept = p.kept + row * p.keep;
+  int32_t* const kept = p.kept + row * p.places;
   if (length <= p.keep) {
     for (int32_t i = threadIdx.x; i < p.new_width; i += kSelectThreads) {
       if (i < count) kept[i] = i;
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictPar
   ptx::grid_dependency_wait();
   const int32_t b = blockIdx.z, head = blockIdx.y, pieces = p.row_bytes / 16;
   const int32_t count = p.new_lengths[b];
-  const int32_t* const kept = p.kept + (static_cast<int64_t>(b) * gridDim.y + head) * p.keep;
+  const int32_t* const kept = p.kept + (static_cast<int64_t>(b) * gridDim.y + head) * p.places;
   const int32_t* const from_table = p.tables + b * p.table_stride;
   const int32_t* const to_table = p.new_tables + b * p.new_stride;
   const int32_t rows = kCopyThreads / pieces;  // of a round
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kShiftThreads) evict_shift_kernel(const EvictP
   ptx::grid_dependency_wait();
   const int32_t b = blockIdx.z, head = blockIdx.y, slices = p.row_bytes / slice_bytes;
   const int32_t count = p.new_lengths[b];
-  const int32_t* const kept = p.kept + (static_cast<int64_t>(b) * gridDim.y + head) * p.keep;
+  const int32_t* const kept = p.kept + (static_cast<int64_t>(b) * gridDim.y + head) * p.places;
   const int32_t* const table = p.tables + b * p.table_stride;
   if (threadIdx.x == 0) {  // (kept[i] - i never falls)
     int32_t low = 0, high = count;
@@ -757,9 +757,10 @@ int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tabl
   CHORD_REQUIRE(width > 0 && width < (1ll << 31) - 65536 && new_width > 0 && new_width < (1ll << 31) - 65536 && keep <= new_width &&
                     weight_batch >= 0 && weight_head >= 0,
                 "sizes of the weights out of range");
-  CHORD_REQUIRE(workspace_bytes >= chord_b200_cache_evict_workspace_bytes(batch, cache->heads, keep) && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0,
+  const int64_t places = keep < width ? keep : width, needed = chord_b200_cache_evict_workspace_bytes(batch, cache->heads, places);
+  CHORD_REQUIRE(needed >= 0 && workspace_bytes >= needed && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0,
                 "the workspace has %lld bytes, this launch needs %lld", static_cast<long long>(workspace_bytes),
-                static_cast<long long>(chord_b200_cache_evict_workspace_bytes(batch, cache->heads, keep)));
+                static_cast<long long>(needed));
   DeviceInfo device;
   if (int rc = current_device_info(&device)) return rc;
   if (int rc = require_blackwell(device)) return rc;
@@ -784,6 +785,7 @@ int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tabl
   p.width = static_cast<int32_t>(width);
   p.new_width = static_cast<int32_t>(new_width);
   p.keep = static_cast<int32_t>(keep);
+  p.places = static_cast<int32_t>(places);
   p.first = static_cast<int32_t>(first);
   p.recent = static_cast<int32_t>(recent);
   p.row_bytes = static_cast<int32_t>(cache->head_dim * (cache->k_scale != nullptr ? 1 : 2));

@@ -594,7 +594,7 @@ PyObject* cache_evict(PyObject*, PyObject* const* a, Py_ssize_t count) {
   {
     const Unlocked unlocked;
     new_lengths = empty({batch}, *lengths, at::kInt), new_weights = empty({batch, cache->heads, new_width}, *lengths, at::kFloat);
-    const int64_t size = batch * cache->heads * keep * 4;
+    const int64_t size = batch * cache->heads * std::min(keep, width) * 4;
     const at::Tensor workspace = empty({size}, *lengths, at::kByte);
     rc = more.cache_evict(cache, table.at, table.stride, table.pages, new_table.at, new_table.stride, new_table.pages,
                           lengths->const_data_ptr<int32_t>(), weights->const_data_ptr<float>(), cache->heads * width, width, width,

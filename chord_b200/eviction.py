@@ -115,7 +115,7 @@ def cache_evict(cache: KVCache, block_tables: torch.Tensor, lengths: torch.Tenso
     if batch == 0:
         return new_lengths, new_weights
     with _lib.on_device(device):
-        size = batch * cache.heads * keep * 4
+        size = batch * cache.heads * min(keep, width) * 4
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         _lib.check(_lib.native().chord_b200_cache_evict(
             cache.address, *table, *new_table, at, *held, width, new_lengths.data_ptr(), new_weights.data_ptr(),

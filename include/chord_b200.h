@@ -574,7 +574,7 @@ int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
  *  weights      fp32 [batch, kv_heads, width], rows contiguous; lengths beyond width or the table: cut, status bit 32
  *  new_lengths  int32 [batch]: min(lengths, keep)
  *  new_weights  fp32 [batch, kv_heads, new_width >= keep], contiguous: the kept tokens' weights, then zeros
- *  workspace    chord_b200_cache_evict_workspace_bytes(batch, kv_heads, keep) bytes, 4-byte aligned
+ *  workspace    chord_b200_cache_evict_workspace_bytes(batch, kv_heads, min(keep, width)) bytes, 4-byte aligned
  * first + recent <= keep.  A row whose page lies outside the cache moves as zeros, or is not written. */
 int chord_b200_cache_evict(const chord_b200_kv_cache* cache, const int32_t* tables,
                            int64_t table_stride, int64_t max_pages, const int32_t* new_tables,
