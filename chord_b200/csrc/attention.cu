@@ -348,7 +348,8 @@ __device__ __forceinline__ void join_parts(const AttentionParams& p, const Row& 
 //
 // kShaped: scores may be capped and leaned on by distance, and the results may stay in FP32.  Kernels of their own: the plain
 // ones keep their registers, and the cap is only paid for there.  16 ragged sequences of up to 4096 tokens, 16 + 8 heads of 256 in
-// BF16, capped, 75 us of 52 at the copy rate; 37 of 3000 of 12 heads of 64 in 8 bits, leaning, 38 of 17.
+// BF16, capped, 75 us of 52 at the copy rate (one warp a scheduler, whose own latency nothing covers); 37 of 3000 of 12 heads of 64 in 8 bits, leaning, 38 of 17
+// (some 15 steps of a warp one after another).
 template <int kDim, bool kCodes, int kTiles, bool kShaped>
 __global__ void __launch_bounds__(kThreads, (Layout<kDim, kCodes, kTiles>::kCtas))
 paged_attention_kernel(const AttentionParams p) {

@@ -16,12 +16,13 @@
 // P is rounded to BF16 (by 2^-8 of each weight at most, as the values that it multiplies were; a second BF16 number for the
 // rest would be a third product; see kFineSteps), its sum is added up before that in FP32.
 //
-// What bounds it: one prompt of 16,384 tokens, 64 + 8 heads of 128, 4.4 ms, 1.0 PFLOP/s of 1.4 that the library's products
-// sustain, the board at its power limit (1.5 GHz); the four-lane unit's exponentials take 1024 of a step's some 2300
-// cycles.  With queries, keys and values by cp.async 5.6 ms.  Over codes with capped scores, 4 x 1,024 queries of
+// What bounds it: one prompt of 16,384 tokens, 64 + 8 heads of 128, 4.1 to 4.5 ms, 1.0 PFLOP/s of 1.4 that the library's products
+// sustain.  At 4.45 ms and 1.72 GHz (the power limit; 1.965 without) a step of 256 rows and 128 tokens takes some 4300 cycles,
+// of which its products take 2048 and its exponentials, on the four-lane units, 2048 others: what is left is the chain of a tile, maximum,
+// weights, product, next scores, which the other tile covers in part.  With queries, keys and values by cp.async 5.6 ms.  Over codes with capped scores, 4 x 1,024 queries of
 // 16 + 8 heads of 256 after 30,000 tokens, 1.9 to 2.2 ms: the rows' arithmetic on scores (scales, cap, maximum) and the turning of
-// codes, 64 % of issue slots.  Short documents, 9 prompts of up to 2,048 tokens, 260 us for a floor of 72: an item's first step waits
-// for its queries and keys, its last one writes the rows (184 MB), and products make up a quarter of the time.
+// codes, 64 % of issue slots.  Short documents, 9 prompts of up to 2,048 tokens, 260 us for a floor of 72: 3,192 items of 1 to 4 steps, whose first step waits
+// for its queries and keys and whose last one writes the rows (184 MB); products make up a quarter of the time.
 #pragma once
 
 #include "prompt_plan.cuh"
@@ -203,7 +204,8 @@ __device__ __forceinline__ void exchange4(uint32_t (&w)[4], int q) {
 
 // Writes 64 or 32 values, from `dim` on, of a warp's 32 rows as BF16.  Rows are spread over four lanes each (with a row to a
 // lane, every store touches 32 lines of memory: 6500 cycles for two tiles of 128 values, as long as two steps), which
-// then write 128 or 64 bytes of it in one go, 32 bytes at a time where the results lie on 32 bytes, which a caller's need not.
+// then write 128 or 64 bytes of it in one go, 32 bytes at a time where the results lie on 32 bytes, which a caller's need not
+// (9 prompts of packed documents 257 us; 16 bytes at a time 271).
 // `row`, `mine` and `other` are those of the lane's own row; row < 0: none.
 template <int kCount>
 __device__ __forceinline__ void write_rows(const PromptParams& p, uint32_t from, int dims, int dim, int64_t row, float mine, float other, int lane) {
@@ -873,7 +875,8 @@ __global__ void __launch_bounds__((PromptLayout<kDim, kCodes>::kThreads), 1) pro
     // ---- rows: two threads each, which have half of a step's tokens and, at an item's end, half of the values ----
     // Scores are taken 32 at a time; of all but the last 32, the highest one is found first and they are read from
     // tensor memory again for their weights: with all of them in registers some 150 bytes were spilled, to the
-    // memory whose bandwidth the products use up.
+    // memory whose bandwidth the products use up.  (What the compiler still reports: none for heads of 192 and 256 and the plain
+    // kernel of 64, 28 to 72 bytes for the other BF16 ones, 48 to 144 over codes.)
     // A wait that gives up does not take a warp out of its loops: both warps of 32 rows meet at their named barrier as often
     // as the item asks for, whatever has failed.
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kRowRegs));  // (the host has checked that they are there)

@@ -454,7 +454,8 @@ int chord_b200_cache_read(const chord_b200_kv_cache* cache, const int32_t* table
 
 /* How a query's scores come about: x = scale q . k; with cap > 0 x = cap tanh(x / cap); with slopes (fp32 [heads], on the
  * device) x -= slopes[h] |p - j| for a query at position p and the token at j; with window > 0 only tokens j > p - window
- * are seen.  scale is finite, cap zero or from 1e-30 to 1e30 with |scale| <= 1e36 cap, window from zero to 2^31 - 1. */
+ * are seen.  All of it is held in FP32, the scale times log2(e) (over codes 64 times that): what leaves its range is an
+ * infinity there.  scale is finite, cap zero or from 1e-30 to 1e30 with |scale| <= 1e36 cap, window from zero to 2^31 - 1. */
 typedef struct chord_b200_scores {
   double scale, cap;
   const float* slopes;
@@ -510,15 +511,18 @@ int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t gro
  *  tables, table_stride, max_pages, lengths, cache   as above
  *  starts   int32 [tokens] or null: the first token of a query token's document
  *  prefixes int32 [batch] or null: so many first tokens are seen by all of the sequence's
- *  out      bf16 [tokens, heads, head_dim], not overlapping q;  lse fp32 [tokens, heads], overlapping neither, or null
+ *  out      bf16 [tokens, heads, head_dim] on a 16-byte boundary, not overlapping q;  lse fp32 [tokens, heads], overlapping
+ *           neither, or null
  *  workspace  chord_b200_prompt_attention_workspace_bytes(...) bytes, 16-byte aligned
  * A token that sees nothing, or whose scores are all minus infinity, gets zeros and an lse of minus infinity.  Rows of
- * tokens of no sequence are not written.  What a token does not see does not change its bits; infinities and NaN there
- * change no more than the rounding of its weights.  These are rounded to BF16 before they multiply values; to two BF16 numbers
- * over codes where the rows of a tile see some hundred tokens or fewer, and not at all in a step in which some row of the
- * tile sees an infinity or a NaN among values and another does not.  Sums are FP32 and, where a sequence is cut over the
- * device, joined in their order: the same inputs give the same bits.  One launch, one more to join where something may be cut,
- * and one more to plan for over 1,024 sequences or items; no kernel waits for another CTA.
+ * tokens of no sequence are not written.  In a call of the same lengths and offsets, the values of what a token does not see do
+ * not change its bits; infinities and NaN there change no more than the rounding of its weights.  (Other lengths, of later tokens
+ * or of other sequences, may change where sums are cut and joined, and that rounding.)  Weights are rounded to BF16 before
+ * they multiply values; to two BF16 numbers over codes where the 256 rows of an item (128 of heads above 128) see up to
+ * four steps of 128 (64) tokens; and not at all in a step in which some row of the item sees an infinity or a NaN among
+ * values and another does not.  Sums are FP32 and, where a sequence is cut over the device, joined in their order: the same
+ * inputs give the same bits.  One launch, one more to join where something may be cut, and one more to plan for over 1,024
+ * sequences or items; no kernel waits for another CTA.
  * Strides of a BF16 cache must be from 16 to 2^40 - 16 bytes; those of heads and pages may be zero. */
 int chord_b200_prompt_attention(const void* q, int64_t q_token, int64_t q_head,
                                 const chord_b200_kv_cache* cache, const int32_t* tables,
