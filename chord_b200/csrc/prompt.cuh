@@ -16,7 +16,7 @@
 // P is rounded to BF16 (by 2^-8 of each weight at most, as the values that it multiplies were; a second BF16 number for the
 // rest would be a third product; see kFineSteps), its sum is added up before that in FP32.
 //
-// What bounds it: one prompt of 16,384 tokens, 64 + 8 heads of 128, 4.1 to 4.5 ms, 1.0 PFLOP/s of 1.4 that the library's products
+// What bounds it: one prompt of 16,384 tokens, 64 + 8 heads of 128, 4.1 to 4.55 ms, 1.0 PFLOP/s of 1.4 that the library's products
 // sustain.  At 4.45 ms and 1.72 GHz (the power limit; 1.965 without) a step of 256 rows and 128 tokens takes some 4300 cycles,
 // of which its products take 2048 and its exponentials, on the four-lane units, 2048 others: what is left is the chain of a tile, maximum,
 // weights, product, next scores, which the other tile covers in part.  With queries, keys and values by cp.async 5.6 ms.  Over codes with capped scores, 4 x 1,024 queries of

@@ -40,10 +40,10 @@ def prompt_attention(q: torch.Tensor, cache: KVCache, block_tables: torch.Tensor
 
     ``slopes`` take the distance either way.  Returns BF16 ``[tokens, heads, head_dim]``; ``lse`` as for
     :func:`paged_attention`.  A token that sees nothing gives zeros and minus infinity.  Rows of tokens of no sequence
-    are left as they are.  In a call of the same lengths and offsets, the values of what a token does not see do not change its
+    are left as they are.  In calls that are alike in all else, the values of what a token does not see do not change its
     bits; infinities and NaN there change no more than how its weights are rounded (where neighbours see such a value, weights of
-    that step are not rounded to BF16).  Other lengths, of later tokens or of other sequences, may change where sums are cut and joined,
-    and over codes how weights are rounded.
+    that step are not rounded to BF16).  Other lengths, ``starts`` or ``prefixes``, of other tokens too, may change where sums are cut and
+    joined, and over codes how weights are rounded.
     Offsets that fall or lie outside ``q``, lengths beyond the table and pages outside the cache are reported by
     :func:`chord_b200.check_status`; nothing outside is read or written.  The same inputs give the same bits."""
     _cache(cache)

@@ -515,9 +515,9 @@ int64_t chord_b200_paged_attention_workspace_bytes(int64_t head_dim, int64_t gro
  *           neither, or null
  *  workspace  chord_b200_prompt_attention_workspace_bytes(...) bytes, 16-byte aligned
  * A token that sees nothing, or whose scores are all minus infinity, gets zeros and an lse of minus infinity.  Rows of
- * tokens of no sequence are not written.  In a call of the same lengths and offsets, the values of what a token does not see do
- * not change its bits; infinities and NaN there change no more than the rounding of its weights.  (Other lengths, of later tokens
- * or of other sequences, may change where sums are cut and joined, and that rounding.)  Weights are rounded to BF16 before
+ * tokens of no sequence are not written.  In calls that are alike in all else, the values of what a token does not see do not
+ * change its bits; infinities and NaN there change no more than the rounding of its weights.  (Other lengths, starts or
+ * prefixes, of other tokens too, may change where sums are cut and joined, and that rounding.)  Weights are rounded to BF16 before
  * they multiply values; to two BF16 numbers over codes where the 256 rows of an item (128 of heads above 128) see up to
  * four steps of 128 (64) tokens; and not at all in a step in which some row of the item sees an infinity or a NaN among
  * values and another does not.  Sums are FP32 and, where a sequence is cut over the device, joined in their order: the same
@@ -558,10 +558,10 @@ int64_t chord_b200_shared_prefix_attention_workspace_bytes(int64_t groups, int64
  * What each token of sequence b got of its new token's attention:
  *   w[b, g, j] = sum of exp(x_h,j - lse[b, h]) over the heads h that share key-value head g
  * for the tokens j that it sees, with x as of `scores` and lse fp32 [batch, heads] as paged attention gives it (a head whose
- * lse is minus infinity gives nothing).  weights is fp32 [batch, kv_heads, width], rows contiguous and apart from
- * each other, q and lse, strides in elements;
- * add == 0: written whole, zeros for tokens that are not seen; else added to what is there.  lengths beyond the table or
- * width: cut, status bit 32; a page outside the cache counts as keys of zero.  batch <= 65535. */
+ * lse is minus infinity gives nothing).  weights is fp32 [batch, kv_heads, width], strides in elements, rows contiguous and
+ * apart from each other, q and lse; add == 0: written whole, zeros for tokens that are not seen; else added to what is
+ * there.  lengths beyond the table or width: cut, status bit 32; a page outside the cache counts as keys of zero.
+ * batch <= 65535. */
 int chord_b200_attention_weights(const void* q, int64_t q_batch, int64_t q_head,
                                  const chord_b200_kv_cache* cache, const int32_t* tables,
                                  int64_t table_stride, int64_t max_pages, const int32_t* lengths,

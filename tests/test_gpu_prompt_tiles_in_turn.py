@@ -15,10 +15,10 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("heads", [24, 32])
 @pytest.mark.parametrize("dim,page", [(64, 25), (96, 25), (96, 26), (128, 25)])
 def test_scales_of_the_second_tile(device, dim, page, heads, cap):
-    """24 heads: queries by the warps that bring the scales as well; 32: by TMA.  Some 22 steps for a CTA, of 17 in a pair of
-    sequences: every run crosses items of either kind.  (Pages of 25 are not divided by boxes of 2; of heads of 128 they are
+    """24 heads: queries by the warps that bring the scales as well; 32: by TMA.  30 new tokens of three or four heads are one tile of 9
+    steps.  Some 22 steps for a CTA, of 17 or 18 in a pair of sequences: every run crosses items of either kind.  (Pages of 25 are not divided by boxes of 2; of heads of 128 they are
     loaded in boxes of one.)"""
-    case = Prompt(device, [(1100, 40), (0, 300)] * 24, heads, 8, dim, page, 8, seed=dim + heads)
+    case = Prompt(device, [(1100, 30), (0, 300)] * 24, heads, 8, dim, page, 8, seed=dim + heads)
     out, lse = case.check(cap=cap)
     different = torch.zeros((), dtype=torch.int64, device=device)
     for _ in range(50):
